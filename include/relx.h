@@ -570,6 +570,143 @@ double relx_measure_d2h(int device, size_t bytes, int iters, int rounds);
  * Returns -1 on failure. */
 double relx_measure_copy(int device, size_t bytes, int iters, int rounds);
 
+/* --------------------------------------------- paged-cache attention
+ *
+ * Operators of a program that attends over the key-value caches it lays out
+ * on the GPU: tables of a paged cache, norms and rotation of queries and
+ * keys, attention over the cache. No counterpart in the reference, whose
+ * programs leave these to the framework above it.
+ *
+ * Every buffer is in device memory. Calls enqueue on `stream` (a hipStream_t,
+ * 0: the legacy null stream) and return at once; they allocate nothing, copy
+ * nothing to the host and can be captured into a graph. Lengths, tables and
+ * slots are read on the device: what they say that does not fit (a page
+ * outside the cache, a row outside the operands) is left out there, never
+ * followed. Element types are (kind, bits) as in relx_param: (0, 32) f32,
+ * (0, 16) f16, (1, 16) bf16, (2, 8) int8. Strides are in elements; the last
+ * dimension is contiguous. Errors of all: "invalid_argument",
+ * "unsupported_layout" (a type, size or head layout that no kernel takes),
+ * "insufficient_capacity" (workspace), "resources_closed",
+ * "backend_failure". */
+
+/* [rows, heads, dim] */
+typedef struct relx_heads {
+  void *data;
+  int64_t row, head; /* strides */
+} relx_heads;
+
+/* A paged cache: keys and values [pages, page, kv_heads, dim] each, of any
+ * order in memory ([pages, kv_heads, page, dim], C5's result, is the same
+ * with other strides). int8 values stand for value * scale[head]. */
+typedef struct relx_cache {
+  void *keys;
+  int64_t key_page, key_slot, key_head; /* strides */
+  void *values;
+  int64_t value_page, value_slot, value_head;
+  const float *key_scale, *value_scale; /* [kv_heads], int8 caches only */
+  int64_t pages, page, kv_heads, dim, kind, bits;
+} relx_cache;
+
+/* Where the step's new tokens go. Request b has cached[b] tokens in the cache
+ * and adds fresh[b] (negative: 0). Row t, the j-th new token of its request,
+ * has position cached + j, and its slot is page id * page + position % page.
+ * Pages that a request has are read from its row of the table; the further
+ * ones it needs are taken from `free_pages` in request order and written to
+ * the table. A position past the table's columns, or a page that the list has
+ * none for, gives slot -1. With `parents` (the new token of the same request
+ * that each one follows, -1: the context; any other value outside [0, j)
+ * counts as -1) the position is cached + the token's depth in its tree, and
+ * mask[t] has the bits of its ancestors and its own (bit i of word w: new
+ * token 64 w + i). Rows past the last request's get slot -1, position 0 and
+ * an empty mask. */
+typedef struct relx_block_tables_args {
+  const int32_t *cached, *fresh; /* [requests] */
+  int32_t *table;                /* [requests, columns], row stride table_row */
+  int64_t table_row;
+  const int32_t *free_pages; /* [free_count] */
+  int64_t free_count;
+  const int32_t *parents; /* [rows], optional */
+  int32_t *starts;        /* [requests + 1]: each request's first row, and their number */
+  int64_t *slots;         /* [rows] */
+  int32_t *positions;     /* [rows] */
+  int64_t *mask;          /* [rows, words], with parents */
+  int32_t *taken;         /* [1]: pages wanted from the list (more than it has: it ran out) */
+  int64_t requests, columns, page, rows, words;
+} relx_block_tables_args;
+int relx_block_tables(relx_ctx *ctx, const relx_block_tables_args *args, uint64_t stream,
+                      relx_err *err);
+
+/* Root-mean-square norm of each head of queries and keys, times a weight of
+ * the head's elements, then the rotation of the first `rotary` elements by
+ * their row's position, in one pass: n = x / sqrt(mean x^2 + eps), y = n w,
+ * (z_i, z_j) = (y_i cos - y_j sin, y_j cos + y_i sin) with (i, j) =
+ * (i, i + rotary / 2), or with `pairs` (2 i, 2 i + 1). cos and sin are
+ * [angles, rotary / 2]; a position outside [0, angles) makes its rotated
+ * elements NaN. Sums and products are in 32 bits, rounded once. */
+typedef struct relx_rotation {
+  const int32_t *positions; /* [rows] */
+  const float *cos, *sin;
+  const void *q_weight, *k_weight; /* [dim], optional (1) */
+  int64_t weight_kind, weight_bits;
+  int64_t rows, heads, kv_heads, dim, rotary, pairs, angles, kind, bits;
+  double eps;
+} relx_rotation;
+int relx_norm_rotate(relx_ctx *ctx, const relx_rotation *rot, const relx_heads *q,
+                     const relx_heads *k, const relx_heads *q_out, const relx_heads *k_out,
+                     uint64_t stream, relx_err *err);
+
+/* Its gradients: those of the queries and keys in their type, those of the
+ * weights (where the weights are given) in f32, summed over rows and heads in
+ * an order that depends on the sizes alone. `workspace`: at least the bytes that
+ * relx_norm_rotate_workspace says. */
+int relx_norm_rotate_backward(relx_ctx *ctx, const relx_rotation *rot, const relx_heads *dq,
+                              const relx_heads *dk, const relx_heads *q, const relx_heads *k,
+                              const relx_heads *q_grad, const relx_heads *k_grad,
+                              float *q_weight_grad, float *k_weight_grad, void *workspace,
+                              size_t workspace_bytes, uint64_t stream, relx_err *err);
+int relx_norm_rotate_workspace(const relx_rotation *rot, size_t *bytes, relx_err *err);
+
+/* The serving form: queries to q_out (which may be the queries), keys and the
+ * values as they are into the cache at their row's slot (page * page size +
+ * offset; a slot outside the cache is skipped). An int8 cache takes
+ * clamp(round_half_even(x * fl32(1 / scale[head])), -128, 127), as the
+ * quantize stage does (NaN: -128). */
+int relx_norm_rotate_append(relx_ctx *ctx, const relx_rotation *rot, const relx_heads *q,
+                            const relx_heads *k, const relx_heads *v, const relx_heads *q_out,
+                            const int64_t *slots, const relx_cache *cache, uint64_t stream,
+                            relx_err *err);
+
+/* Attention of the step's rows over the cache. Request b's rows are
+ * [starts[b], starts[b + 1]), its tokens the cached[b] first ones of its table
+ * row and its rows' own after them. Row j sees every cached token, and of the
+ * request's own the i-th where bit i of its mask is set (without a mask those
+ * with i <= j). out = sum of softmax(scale q.k) v per head, head h reading key
+ * head h / (heads / kv_heads); a row that sees nothing, or of no request, is 0
+ * with lse -inf. A token that no row sees is not read into any sum, whatever it holds, and one
+ * that only some rows see touches only those. `lse` (optional): natural
+ * logarithm of the sum of exponentials, [rows, heads]. `workspace`: at least
+ * the bytes that relx_tree_attention_workspace says, any contents. Head sizes
+ * are multiples of 8 up to 256; q and out share a type, f16 or bf16, and the
+ * cache has it too or int8. */
+typedef struct relx_tree_attention_args {
+  relx_heads q, out;
+  relx_cache cache;
+  const int32_t *table; /* [requests, columns] */
+  int64_t table_row;
+  const int32_t *cached; /* [requests] */
+  const int32_t *starts; /* [requests + 1] */
+  const int64_t *mask;   /* [rows, words], optional */
+  float *lse;            /* optional */
+  void *workspace;
+  int64_t workspace_bytes;
+  int64_t rows, requests, heads, columns, words, kind, bits;
+  double scale;
+} relx_tree_attention_args;
+int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uint64_t stream,
+                        relx_err *err);
+int relx_tree_attention_workspace(const relx_tree_attention_args *args, size_t *bytes,
+                                  relx_err *err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -106,6 +106,31 @@ class relx_kernel_times(ctypes.Structure):
                 ("launches", ctypes.c_int64), ("ms", ctypes.c_double)]
 
 
+# the paged-cache operators' arguments: every field is eight bytes wide
+def _record(name, *fields):
+    return type(name, (ctypes.Structure,), {"_fields_": [
+        (f, t) for t, names in zip(fields[::2], fields[1::2]) for f in names.split()]})
+
+
+_P8, _I8, _D8 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_double
+relx_heads = _record("relx_heads", _P8, "data", _I8, "row head")
+relx_cache = _record(
+    "relx_cache", _P8, "keys", _I8, "key_page key_slot key_head", _P8, "values",
+    _I8, "value_page value_slot value_head", _P8, "key_scale value_scale",
+    _I8, "pages page kv_heads dim kind bits")
+relx_block_tables_args = _record(
+    "relx_block_tables_args", _P8, "cached fresh table", _I8, "table_row", _P8, "free_pages",
+    _I8, "free_count", _P8, "parents starts slots positions mask taken",
+    _I8, "requests columns page rows words")
+relx_rotation = _record(
+    "relx_rotation", _P8, "positions cos sin q_weight k_weight",
+    _I8, "weight_kind weight_bits rows heads kv_heads dim rotary pairs angles kind bits",
+    _D8, "eps")
+relx_tree_attention_args = _record(
+    "relx_tree_attention_args", relx_heads, "q out", relx_cache, "cache", _P8, "table",
+    _I8, "table_row", _P8, "cached starts mask lse workspace",
+    _I8, "workspace_bytes rows requests heads columns words kind bits", _D8, "scale")
+
 # every entry point include/relx.h declares, with its ctypes signature
 _VP, _SZ, _I, _I64, _U64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64
 _E = ctypes.POINTER(relx_err)
@@ -167,6 +192,15 @@ SIGNATURES = {
     "relx_host_stage": (_I, [_VP, _I, _VP, _VP, _I, _E]),
     "relx_verify_launches": (_I, [_VP, _I, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64), _E]),
     "relx_launch_kernels": (_I, [_VP, _I, ctypes.c_char_p, _SZ, _E]),
+    # argument records cross as packed bytes
+    "relx_block_tables": (_I, [_VP, _VP, _U64, _E]),
+    "relx_norm_rotate": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _U64, _E]),
+    "relx_norm_rotate_backward": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ,
+                                       _U64, _E]),
+    "relx_norm_rotate_workspace": (_I, [_VP, ctypes.POINTER(_SZ), _E]),
+    "relx_norm_rotate_append": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _U64, _E]),
+    "relx_tree_attention": (_I, [_VP, _VP, _U64, _E]),
+    "relx_tree_attention_workspace": (_I, [_VP, ctypes.POINTER(_SZ), _E]),
     "relx_ctx_synchronize": (_I, [_VP, _E]),
     "relx_ctx_time_kernels": (_I, [_VP, _I, _E]),
     "relx_ctx_kernel_times": (_I, [_VP, ctypes.POINTER(relx_kernel_times), _E]),

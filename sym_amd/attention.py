@@ -1,0 +1,389 @@
+"""Operators over paged key-value caches, on torch tensors.
+
+A program that lays key-value caches out on the GPU with relocation plans
+then attends over them. The calls of its step, in order:
+
+  block_tables          where the step's tokens go: slots, positions, pages
+                        taken from the free list, masks of drafted trees
+  norm_rotate_append    norm and rotation of the step's queries and keys; keys
+                        and values into the cache (int8 by a scale a head)
+  tree_attention        attention of the step's rows over the cache
+
+and, in training, `norm_rotate` (a differentiable function of its queries, keys
+and weights) with `norm_rotate_backward` beneath it.
+
+Calls take a `pyreloc.Context`, run on torch's current stream of its device,
+return at once and never wait for the GPU, so they can be captured into a
+graph; results are fresh tensors unless `out` is given. The package's own
+plans write caches that these calls read as they are: the int8 result
+[requests, heads, tokens, dim] of the C5 plan is the cache
+`result.transpose(1, 2)`, with one page a request. Bad arguments raise
+ValueError, what the library refuses TransferError("<code>: <detail>").
+"""
+import ctypes
+import struct
+from collections import namedtuple
+from functools import lru_cache
+
+import torch
+
+from . import _native as N
+from .transfer import _fail
+
+_KINDS = {torch.float32: (0, 32), torch.float16: (0, 16), torch.bfloat16: (1, 16), torch.int8: (2, 8)}
+
+Tables = namedtuple("Tables", "starts slots positions taken mask")
+Tables.__doc__ = """Where a step's tokens go (see `block_tables`): each request's first row
+[requests + 1], and per row its slot (int64, -1: none) and position; the pages
+wanted from the free list [1]; the trees' ancestor masks [rows, words] or None."""
+
+
+def _format(record):
+    """A record's fields as one struct format: all are eight bytes wide."""
+    out = ""
+    for _, t in record._fields_:
+        out += _format(t) if issubclass(t, ctypes.Structure) else \
+            "d" if t is ctypes.c_double else "Q" if t is ctypes.c_void_p else "q"
+    return out
+
+
+_HEADS = struct.Struct(_format(N.relx_heads))
+_CACHE = struct.Struct(_format(N.relx_cache))
+_TABLES = struct.Struct(_format(N.relx_block_tables_args))
+_ROTATION = struct.Struct(_format(N.relx_rotation))
+_ATTENTION = struct.Struct(_format(N.relx_tree_attention_args))
+
+
+def _bad(message):
+    raise ValueError(message)
+
+
+def _call(name, ctx, *args):
+    err = N.relx_err()
+    if getattr(N.lib(), name)(ctx._h, *args, ctypes.byref(err)):
+        _fail(err)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _device(ctx, like):
+    d = like.device
+    if d.type != "cuda" or d.index != ctx.device:
+        _bad("the tensors are on %s, the context on device %d" % (d, ctx.device))
+    return d
+
+
+def _row(t, name, dtype, n, device):
+    """A contiguous vector of `n` (None: any number)."""
+    if t.dtype is not dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != device or \
+            (t.shape[0] > 1 and t.stride(0) != 1):
+        _bad("%s: %s [%s] on %s, contiguous; got %s %s on %s"
+             % (name, dtype, "n" if n is None else n, device, t.dtype, list(t.shape), t.device))
+    return t.data_ptr()
+
+
+def _heads(t, name, shape, dtype, device):
+    """[rows, heads, dim] with a contiguous last dimension."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        _bad("%s: %s %s on %s; got %s %s on %s"
+             % (name, dtype, list(shape), device, t.dtype, list(t.shape), t.device))
+    row, head, one = t.stride()
+    if one != 1 and shape[2] > 1 and t.numel():
+        _bad("%s: the last dimension must be contiguous" % name)
+    return t.data_ptr(), row, head
+
+
+def _table(t, device):
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.device != device or (t.numel() > 1 and t.stride(1) != 1 and t.shape[1] > 1):
+        _bad("block table: int32 [requests, columns] on %s with contiguous rows; got %s %s on %s"
+             % (device, t.dtype, list(t.shape), t.device))
+    return t.shape[0], t.shape[1], t.data_ptr(), t.stride(0)
+
+
+def _cache(keys, values, k_scale, v_scale, device):
+    """The cache's record fields: keys and values [pages, page, kv_heads, dim]."""
+    shape = keys.shape
+    kind = _KINDS.get(keys.dtype)
+    if len(shape) != 4 or values.shape != shape or values.dtype is not keys.dtype or kind is None or \
+            keys.device != device or values.device != device:
+        _bad("cache: keys and values [pages, page, kv_heads, dim] of one type on %s; got %s %s on %s and %s %s on %s"
+             % (device, keys.dtype, list(shape), keys.device, values.dtype, list(values.shape), values.device))
+    kp, ks, kh, ko = keys.stride()
+    vp, vs, vh, vo = values.stride()
+    if shape[3] > 1 and (ko != 1 or vo != 1) and keys.numel():
+        _bad("cache: the last dimension must be contiguous")
+    scales = (0, 0)
+    if keys.dtype is torch.int8:
+        if k_scale is None or v_scale is None:
+            _bad("an int8 cache takes k_scale and v_scale")
+        scales = (_row(k_scale, "k_scale", torch.float32, shape[2], device),
+                  _row(v_scale, "v_scale", torch.float32, shape[2], device))
+    elif k_scale is not None or v_scale is not None:
+        _bad("scales go with an int8 cache")
+    return (keys.data_ptr(), kp, ks, kh, values.data_ptr(), vp, vs, vh, *scales, shape[0], shape[1], shape[2],
+            shape[3], *kind)
+
+
+# ------------------------------------------------------------ block tables
+
+def block_tables(ctx, cached, fresh, table, free_pages, page, rows, *, parents=None, words=1, out=None):
+    """Slots, positions and pages of a step's new tokens, on the GPU.
+
+    Request b has `cached[b]` tokens in the cache and adds `fresh[b]` (int32
+    [requests]). Pages of `page` slots are listed in `table` (int32
+    [requests, columns]); the further ones that a request needs are taken from
+    `free_pages` (int32) in request order and written into `table`. The step
+    has `rows` rows at most (rows past the requests' get slot -1). `parents`
+    (int32 [rows]) makes each request's new tokens a drafted tree: the one of
+    the same request that a token follows, always an earlier one, or -1; then
+    positions are those in the tree and `mask` (int64 [rows, words]) has each
+    token's ancestors and itself. Returns `Tables`; `out`: such a tuple to
+    write into. `taken` past len(free_pages) says that the list ran out, and
+    the slots without a page are -1."""
+    device = _device(ctx, table)
+    requests, columns, t_ptr, t_row = _table(table, device)
+    rows, page = int(rows), int(page)
+    if rows < 0 or page < 1:
+        _bad("block tables: rows = %d, page = %d" % (rows, page))
+    c_ptr = _row(cached, "cached", torch.int32, requests, device)
+    f_ptr = _row(fresh, "fresh", torch.int32, requests, device)
+    l_ptr = _row(free_pages, "free_pages", torch.int32, None, device)
+    if parents is None:
+        words = p_ptr = 0
+    else:
+        words = int(words)
+        p_ptr = _row(parents, "parents", torch.int32, rows, device)
+        if words < 1:
+            _bad("block tables: words = %d" % words)
+    if out is None:
+        i32 = torch.empty(requests + 2 + rows, dtype=torch.int32, device=device)
+        i64 = torch.empty(rows * (1 + words), dtype=torch.int64, device=device)
+        out = Tables(i32[:requests + 1], i64[:rows], i32[requests + 2:], i32[requests + 1:requests + 2],
+                     i64[rows:].view(rows, words) if words else None)
+        i32_ptr, i64_ptr = i32.data_ptr(), i64.data_ptr()
+        ptrs = (i32_ptr, i64_ptr, i32_ptr + 4 * (requests + 2), i64_ptr + 8 * rows if words else 0,
+                i32_ptr + 4 * (requests + 1))
+    else:
+        ptrs = (_row(out.starts, "starts", torch.int32, requests + 1, device),
+                _row(out.slots, "slots", torch.int64, rows, device),
+                _row(out.positions, "positions", torch.int32, rows, device), 0,
+                _row(out.taken, "taken", torch.int32, 1, device))
+        if words:
+            m = out.mask
+            if m is None or m.dtype is not torch.int64 or m.shape != (rows, words) or m.device != device or \
+                    not m.is_contiguous():
+                _bad("mask: contiguous int64 [%d, %d]" % (rows, words))
+            ptrs = ptrs[:3] + (m.data_ptr(), ptrs[4])
+    _call("relx_block_tables", ctx,
+          _TABLES.pack(c_ptr, f_ptr, t_ptr, t_row, l_ptr, free_pages.shape[0], p_ptr, *ptrs, requests, columns, page,
+                       rows, words), _stream(device))
+    return out
+
+
+# --------------------------------------------------------- norm and rotation
+
+def _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs):
+    """(packed rotation, query and key shapes, device)."""
+    device = _device(ctx, q)
+    qs, ks = q.shape, k.shape
+    kind = _KINDS.get(q.dtype)
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or kind is None or kind[1] == 8:
+        _bad("queries [rows, heads, dim] and keys [rows, kv_heads, dim] of one floating type; got %s %s and %s %s"
+             % (q.dtype, list(qs), k.dtype, list(ks)))
+    rows, dim = qs[0], qs[2]
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
+            cos.device != device or sin.device != device or not (cos.is_contiguous() and sin.is_contiguous()):
+        _bad("cos and sin: contiguous float32 [angles, rotary / 2] on %s; got %s %s and %s %s"
+             % (device, cos.dtype, list(cos.shape), sin.dtype, list(sin.shape)))
+    w_kind, w_ptr = (0, 32), [0, 0]
+    given = [w for w in (q_weight, k_weight) if w is not None]
+    if given:
+        w_kind = _KINDS.get(given[0].dtype)
+        if w_kind is None or w_kind[1] == 8 or given[0].dtype is not given[-1].dtype:
+            _bad("weights: one floating type; got %s" % [w.dtype for w in given])
+        w_ptr = [0 if w is None else _row(w, "weight", w.dtype, dim, device) for w in (q_weight, k_weight)]
+    p_ptr = _row(positions, "positions", torch.int32, rows, device)
+    return (_ROTATION.pack(p_ptr, cos.data_ptr(), sin.data_ptr(), *w_ptr, *w_kind, rows, qs[1], ks[1], dim,
+                           2 * cos.shape[1], 1 if pairs else 0, cos.shape[0], *kind, float(eps)), qs, ks, device)
+
+
+def _pack_heads(t, name, shape, dtype, device):
+    return _HEADS.pack(*_heads(t, name, shape, dtype, device))
+
+
+class _NormRotate(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, q, k, q_weight, k_weight, ctx, positions, cos, sin, eps, pairs):
+        fn.save_for_backward(q, k, q_weight, k_weight, positions, cos, sin)
+        fn.rest = ctx, eps, pairs
+        return _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, None)
+
+    @staticmethod
+    def backward(fn, dq, dk):
+        q, k, q_weight, k_weight, positions, cos, sin = fn.saved_tensors
+        ctx, eps, pairs = fn.rest
+        gq, gk, gqw, gkw = norm_rotate_backward(ctx, dq.contiguous(), dk.contiguous(), q, k, positions, cos, sin,
+                                                q_weight, k_weight, eps, pairs=pairs)
+        return (gq, gk, None if gqw is None else gqw.to(q_weight.dtype),
+                None if gkw is None else gkw.to(k_weight.dtype), None, None, None, None, None, None)
+
+
+def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pairs=False, out=None):
+    """Root-mean-square norm of each head, times a weight [dim] (None: 1), then
+    the rotation by position, in one pass over the queries [rows, heads, dim]
+    and keys [rows, kv_heads, dim] (f32, f16 or bf16; any row and head strides,
+    so views of a fused projection do).
+
+    `positions` (int32 [rows]) index `cos` and `sin` (float32
+    [angles, rotary / 2]), which turn the first `rotary` elements: halves
+    (i, i + rotary / 2), or neighbours (2 i, 2 i + 1) with `pairs`. A position
+    outside the table gives NaN. Returns (queries, keys); `out`: a pair of
+    tensors to write into. Differentiable in q, k and the weights (without
+    `out`)."""
+    if out is None and torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or
+            (k_weight is not None and k_weight.requires_grad)):
+        return _NormRotate.apply(q, k, q_weight, k_weight, ctx, positions, cos, sin, eps, pairs)
+    return _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out)
+
+
+def _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out):
+    rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
+    dtype = q.dtype
+    zq, zk = out if out is not None else (torch.empty(qs, dtype=dtype, device=device),
+                                          torch.empty(ks, dtype=dtype, device=device))
+    _call("relx_norm_rotate", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
+          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(zq, "query result", qs, dtype, device),
+          _pack_heads(zk, "key result", ks, dtype, device), _stream(device))
+    return zq, zk
+
+
+def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pairs=False):
+    """Gradients of `norm_rotate` for its results' gradients `dq` and `dk`:
+    (queries', keys', query weight's, key weight's). The weights' are float32
+    [dim], summed over rows and heads in a fixed order (None where the weight
+    is); the others have the operands' type."""
+    rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
+    dtype = q.dtype
+    gq, gk = torch.empty(qs, dtype=dtype, device=device), torch.empty(ks, dtype=dtype, device=device)
+    gw = [None if w is None else torch.empty(qs[2], dtype=torch.float32, device=device) for w in (q_weight, k_weight)]
+    room = None
+    if q_weight is not None or k_weight is not None:
+        room = torch.empty(_rotate_room(rot, qs, ks, dtype) // 4, dtype=torch.float32, device=device)
+    _call("relx_norm_rotate_backward", ctx, rot, _pack_heads(dq, "query gradient", qs, dtype, device),
+          _pack_heads(dk, "key gradient", ks, dtype, device), _pack_heads(q, "queries", qs, dtype, device),
+          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(gq, "query gradient", qs, dtype, device),
+          _pack_heads(gk, "key gradient", ks, dtype, device), 0 if gw[0] is None else gw[0].data_ptr(),
+          0 if gw[1] is None else gw[1].data_ptr(), 0 if room is None else room.data_ptr(),
+          0 if room is None else room.numel() * 4, _stream(device))
+    return gq, gk, gw[0], gw[1]
+
+
+_rooms = {}
+
+
+def _rotate_room(rot, qs, ks, dtype):
+    key = (qs, ks[1], dtype)
+    if key not in _rooms:
+        if len(_rooms) >= 1024:
+            _rooms.clear()
+        size, err = ctypes.c_size_t(), N.relx_err()
+        if N.lib().relx_norm_rotate_workspace(rot, ctypes.byref(size), ctypes.byref(err)):
+            _fail(err)
+        _rooms[key] = size.value
+    return _rooms[key]
+
+
+def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, sin, q_weight, k_weight, eps, *,
+                       pairs=False, k_scale=None, v_scale=None, out=None):
+    """The serving form of `norm_rotate`: returns the queries (in `out`, which
+    may be `q` itself), and puts the keys, and the values `v` [rows, kv_heads,
+    dim] as they are, into the cache at each row's slot (int64 [rows]; a slot
+    outside the cache is skipped, and rows have slots of their own). The cache
+    is [pages, page, kv_heads, dim] of any strides, of the operands' type, or
+    int8 with a scale a head (float32 [kv_heads] each), quantized as the
+    package's plans quantize."""
+    rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
+    dtype = q.dtype
+    if out is None:
+        out = torch.empty(qs, dtype=dtype, device=device)
+    cache = _CACHE.pack(*_cache(cache_k, cache_v, k_scale, v_scale, device))
+    _call("relx_norm_rotate_append", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
+          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(v, "values", ks, dtype, device),
+          _pack_heads(out, "query result", qs, dtype, device), _row(slots, "slots", torch.int64, qs[0], device),
+          cache, _stream(device))
+    return out
+
+
+# ------------------------------------------------------------ attention
+
+@lru_cache(maxsize=4096)
+def tree_attention_workspace(rows, requests, heads, kv_heads, dim, page):
+    """Bytes of device memory that a `tree_attention` call of these sizes
+    works in."""
+    size, err = ctypes.c_size_t(), N.relx_err()
+    args = N.relx_tree_attention_args()
+    args.rows, args.requests, args.heads = rows, requests, heads
+    args.cache.kv_heads, args.cache.dim, args.cache.page = kv_heads, dim, page
+    if N.lib().relx_tree_attention_workspace(bytes(args), ctypes.byref(size), ctypes.byref(err)):
+        _fail(err)
+    return size.value
+
+
+def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None, scale=None, k_scale=None,
+                   v_scale=None, out=None, lse=None, workspace=None):
+    """Attention of a step's rows q [rows, heads, dim] (f16, bf16) over a paged
+    cache [pages, page, kv_heads, dim] of any strides, of the same type or
+    int8 with scales [kv_heads].
+
+    Request b has the rows [starts[b], starts[b + 1]) and sees the `cached[b]`
+    first tokens of its row of `table`, and of its own new ones, which are
+    already in the cache after them, those whose bit its row of `mask` (int64
+    [rows, words], as `block_tables` makes it) has; without a mask, those up to
+    itself (one row a request: plain decoding). Head h reads key head
+    h // (heads // kv_heads). A row that sees nothing, or of no request, is 0.
+
+    `scale`: of the scores, by default dim ** -0.5. `lse`: float32 [rows,
+    heads] for the logarithm of each row's sum of exponentials. `workspace`: a
+    uint8 tensor of `tree_attention_workspace` bytes, for programs that keep
+    one a stream; by default torch's allocator gives it."""
+    device = _device(ctx, q)
+    shape, dtype = q.shape, q.dtype
+    kind = _KINDS.get(dtype)
+    if len(shape) != 3 or kind is None or kind[1] != 16:
+        _bad("queries: f16 or bf16 [rows, heads, dim]; got %s %s" % (dtype, list(shape)))
+    rows, heads, dim = shape
+    cache = _cache(cache_k, cache_v, k_scale, v_scale, device)
+    kv_heads = cache[12]
+    if cache[13] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or \
+            (cache_k.dtype is not dtype and cache_k.dtype is not torch.int8):
+        _bad("cache: %s or int8 [pages, page, kv_heads, %d] with kv_heads dividing %d; got %s %s"
+             % (dtype, dim, heads, cache_k.dtype, list(cache_k.shape)))
+    requests, columns, t_ptr, t_row = _table(table, device)
+    words = m_ptr = 0
+    if mask is not None:
+        if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != rows or mask.device != device or \
+                not mask.is_contiguous() or mask.shape[1] < 1:
+            _bad("mask: contiguous int64 [%d, words] on %s; got %s %s" % (rows, device, mask.dtype, list(mask.shape)))
+        words, m_ptr = mask.shape[1], mask.data_ptr()
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    l_ptr = 0
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != shape[:2] or lse.device != device or not lse.is_contiguous():
+            _bad("lse: contiguous float32 [%d, %d]" % (rows, heads))
+        l_ptr = lse.data_ptr()
+    if workspace is None:
+        workspace = torch.empty(tree_attention_workspace(rows, requests, heads, kv_heads, dim, cache[11]),
+                                dtype=torch.uint8, device=device)
+    elif workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+        _bad("workspace: contiguous uint8 on %s" % device)
+    _call("relx_tree_attention", ctx,
+          _ATTENTION.pack(*_heads(q, "queries", shape, dtype, device), *_heads(out, "result", shape, dtype, device),
+                          *cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
+                          _row(starts, "starts", torch.int32, requests + 1, device), m_ptr, l_ptr,
+                          workspace.data_ptr(), workspace.numel(), rows, requests, heads, columns, words, *kind,
+                          dim ** -0.5 if scale is None else float(scale)), _stream(device))
+    return out

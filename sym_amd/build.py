@@ -27,12 +27,17 @@ SOURCES = ["plan.cpp", "program.cpp", "runtime.cpp", "workers.cpp", "indexed.cpp
            "capi.cpp",
            "kernels.hip",
            "k_stream_fast.hip", "k_stream_generic.hip", "k_transpose.hip", "k_transpose_ragged.hip", "k_rows.hip", "k_interleave.hip",
-           "k_interleave_generic.hip", "k_interleave_ragged.hip", "k_permute.hip", "k_gather.hip", "k_copy.hip", "noalloc.hip"]
+           "k_interleave_generic.hip", "k_interleave_ragged.hip", "k_permute.hip", "k_gather.hip", "k_copy.hip", "noalloc.hip",
+           "attention.cpp", "k_tables.hip", "k_rotate.hip", "k_attend_f16.hip", "k_attend_bf16.hip"]
 
 
 # The one-level interleave takes its hot arguments as leading scalars that
 # the dispatch preloads into scalar registers.
-EXTRA = {"k_interleave.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"]}
+# The paged-cache operators have no bit contract: products and sums contract.
+EXTRA = {"k_interleave.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
+         "k_rotate.hip": ["-ffp-contract=fast"],
+         "k_attend_f16.hip": ["-ffp-contract=fast"],
+         "k_attend_bf16.hip": ["-ffp-contract=fast"]}
 
 
 def _compile(src):

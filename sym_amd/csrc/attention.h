@@ -1,0 +1,111 @@
+// attention.h - arguments and launches of the paged-cache operators
+// (k_tables.hip, k_rotate.hip, k_attend.h), checked and filled by
+// attention.cpp. Strides are in elements unless a name says bytes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "program.h"
+
+namespace relx {
+
+enum ElementType : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI8 = 3 };
+
+// ------------------------------------------------------------ block tables
+
+struct TablesArgs {
+  const int32_t *cached, *fresh;
+  int32_t *table;
+  int64_t table_row;
+  const int32_t *free_pages;
+  int64_t free_count;
+  const int32_t *parents;
+  int32_t *starts;
+  int64_t *slots;
+  int32_t *positions;
+  int64_t *mask;
+  int32_t *taken;
+  FastDiv page;
+  int32_t requests, columns, rows, words;
+  int32_t block_rows; // rows of a block
+};
+hipError_t tables_launch(TablesArgs a, hipStream_t s);
+
+// --------------------------------------------------------- norm and rotation
+
+struct Heads {
+  char *data;
+  int64_t row, head;
+};
+
+struct RotateArgs {
+  Heads x[3];   // queries, keys, values (values: the serving form)
+  Heads y[3];   // results (serving: y[0] only); backward: the operands' gradients
+  Heads dz[2];  // backward: the results' gradients
+  const void *weight[2];
+  const int32_t *positions;
+  const float *cos, *sin;
+  const int64_t *slots; // serving
+  const float *scale[2];
+  int64_t cache_page[2], cache_slot[2], cache_head[2];
+  char *cache[2];
+  float *partial; // backward: [parts, dim] per kind, queries' first
+  float *weight_grad[2];
+  FastDiv page;
+  int64_t pages_slots; // pages * page
+  int32_t weight_type;
+  int32_t rows, heads[2], dim, rotary, angles, pairs;
+  int32_t chunks[3]; // blocks of heads of each kind
+  int32_t chunk_heads;
+  float eps, inv_dim;
+};
+enum RotateForm : int { kRotateForward, kRotateBackward, kRotateAppend, kRotateAppendI8 };
+// Blocks over the rows that a launch of `rows` rows in `chunks` blocks of
+// heads takes (the backward's parts per chunk).
+int rotate_blocks(int form, int64_t rows, int64_t chunks);
+// Lanes that hold one head, each eight elements.
+int rotate_lanes(int dim);
+hipError_t rotate_launch(const RotateArgs &a, int form, int type, hipStream_t s);
+
+// ------------------------------------------------------------ tree attention
+
+struct AttendArgs {
+  const char *q;
+  int64_t q_row, q_head;
+  char *out;
+  int64_t out_row, out_head;
+  const char *keys, *values;
+  int64_t key_page, key_slot, key_head, value_page, value_slot, value_head; // bytes
+  const float *key_scale, *value_scale;
+  const int32_t *table;
+  int64_t table_row;
+  const int32_t *cached, *starts;
+  const int64_t *mask;
+  float *lse;
+  float *partial;    // [workgroups][2][tile rows][width] sums, unnormalised
+  float *stats;      // [workgroups][2][tile rows][2] maximum, sum of weights
+  int64_t *schedule; // [requests + 1] first unit of each request, and their number
+  FastDiv page, group;
+  int32_t rows, requests, heads, kv_heads, dim, pages, columns, words;
+  int32_t workgroups;
+  float scale; // of a score, times log2 e
+};
+
+// How a call runs: rows of query tiles per wave and workgroups.
+struct AttendPlan {
+  int width;      // head size, rounded up to a kernel's
+  int row_tiles;  // tiles of 16 query rows a wave keeps
+  bool fast;      // whole heads, and pages of whole token tiles
+  int workgroups;
+};
+AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
+                       int64_t page);
+size_t attend_workspace(const AttendPlan &p, int64_t requests);
+hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8,
+                         hipStream_t s);
+hipError_t attend_launch_f16(const AttendArgs &a, const AttendPlan &p, bool i8, hipStream_t s);
+hipError_t attend_launch_bf16(const AttendArgs &a, const AttendPlan &p, bool i8, hipStream_t s);
+
+} // namespace relx

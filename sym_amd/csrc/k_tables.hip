@@ -1,0 +1,184 @@
+// k_tables.hip - block tables and slot maps of a paged cache, built from the
+// requests' lengths.
+//
+// Two running sums over the requests (new rows, new pages) say where a
+// request's rows and pages begin. They are short beside the rows, so every
+// block computes them for itself, which makes the whole step one launch with
+// nothing to wait for between blocks; a block then fills its own run of rows,
+// a row per thread. A row finds its request by bisection over the sums of 256
+// runs of requests in shared memory, then inside the run.
+#include "attention.h"
+#include "index.h"
+
+namespace relx {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Sums of a run of requests.
+struct Sums {
+  int64_t rows, pages;
+};
+
+__device__ __forceinline__ int32_t ceil_pages(int64_t tokens, const TablesArgs &a) {
+  // tokens < 2^32
+  const uint32_t t = static_cast<uint32_t>(tokens);
+  const uint32_t q = fdiv(t, a.page);
+  const uint32_t n = q + (q * a.page.d != t);
+  return n < static_cast<uint32_t>(a.columns) ? static_cast<int32_t>(n) : a.columns;
+}
+
+struct Request {
+  int64_t cached, fresh;
+  int32_t have, need; // pages
+};
+
+__device__ __forceinline__ Request request(const TablesArgs &a, int b) {
+  Request r;
+  const int32_t c = a.cached[b], f = a.fresh[b];
+  r.cached = c > 0 ? c : 0;
+  r.fresh = f > 0 ? f : 0;
+  r.have = ceil_pages(r.cached, a);
+  r.need = ceil_pages(r.cached + r.fresh, a) - r.have;
+  return r;
+}
+
+__global__ __launch_bounds__(kThreads) void k_tables(TablesArgs a) {
+  __shared__ Sums before[kThreads + 1]; // sums of the runs before each
+  __shared__ Sums wave_sum[kThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int run = (a.requests + kThreads - 1) / kThreads;
+  const int b0 = min(tid * run, a.requests), b1 = min(b0 + run, a.requests);
+
+  Sums mine = {0, 0};
+  for (int b = b0; b < b1; ++b) {
+    const Request r = request(a, b);
+    mine.rows += r.fresh;
+    mine.pages += r.need;
+  }
+  Sums upto = mine; // inclusive over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t r = __shfl_up(upto.rows, o), p = __shfl_up(upto.pages, o);
+    if (lane >= o) {
+      upto.rows += r;
+      upto.pages += p;
+    }
+  }
+  if (lane == 63)
+    wave_sum[wave] = upto;
+  __syncthreads();
+  Sums first = {upto.rows - mine.rows, upto.pages - mine.pages};
+  for (int w = 0; w < wave; ++w) {
+    first.rows += wave_sum[w].rows;
+    first.pages += wave_sum[w].pages;
+  }
+  before[tid] = first;
+  if (tid == kThreads - 1)
+    before[kThreads] = {first.rows + mine.rows, first.pages + mine.pages};
+  __syncthreads();
+  const int64_t total = before[kThreads].rows;
+
+  if (blockIdx.x == 0) { // the sums themselves
+    Sums at = first;
+    for (int b = b0; b < b1; ++b) {
+      a.starts[b] = static_cast<int32_t>(min(at.rows, static_cast<int64_t>(INT32_MAX)));
+      at.rows += request(a, b).fresh;
+    }
+    if (tid == 0) {
+      a.starts[a.requests] = static_cast<int32_t>(min(total, static_cast<int64_t>(INT32_MAX)));
+      a.taken[0] = static_cast<int32_t>(min(before[kThreads].pages, static_cast<int64_t>(INT32_MAX)));
+    }
+  }
+
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.block_rows;
+  const int64_t t1 = min(t0 + a.block_rows, static_cast<int64_t>(a.rows));
+  Request r = {0, 0, 0, 0};
+  int64_t start = 0, end = 0, base = 0; // the request's rows, and its first page in the list
+  int b = -1;
+  for (int64_t t = t0 + tid; t < t1; t += kThreads) {
+    if (t >= total) {
+      a.slots[t] = -1;
+      a.positions[t] = 0;
+      for (int w = 0; w < a.words; ++w)
+        a.mask[t * a.words + w] = 0;
+      continue;
+    }
+    if (t >= end) { // the last run that begins at or before t, then its requests
+      int lo = 0, hi = kThreads;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (before[mid].rows <= t ? lo : hi) = mid;
+      }
+      b = lo * run;
+      start = before[lo].rows;
+      base = before[lo].pages;
+      r = request(a, b);
+      while (start + r.fresh <= t) {
+        start += r.fresh;
+        base += r.need;
+        r = request(a, ++b);
+      }
+      end = start + r.fresh;
+    }
+    const int64_t j = t - start;
+    const uint32_t x = static_cast<uint32_t>(r.cached + j);
+    const uint32_t g = fdiv(x, a.page), off = x - g * a.page.d;
+    int32_t id = -1;
+    if (g < static_cast<uint32_t>(r.have)) {
+      id = a.table[b * a.table_row + g];
+    } else if (g < static_cast<uint32_t>(a.columns)) {
+      const int64_t at = base + g - r.have;
+      if (at < a.free_count)
+        id = a.free_pages[at];
+      // the page's first token puts it into the table; each page that the
+      // request gains has one, since it begins where the others end
+      if (off == 0)
+        a.table[b * a.table_row + g] = id;
+    }
+    a.slots[t] = id >= 0 ? static_cast<int64_t>(id) * a.page.d + off : -1;
+
+    if (!a.parents) {
+      a.positions[t] = static_cast<int32_t>(x);
+      continue;
+    }
+    // Up the tree. A parent comes before its child, so the words of the mask
+    // fill from the highest down, each written once.
+    int64_t cur = j;
+    int32_t depth = -1;
+    int word = a.words - 1;
+    uint64_t bits = 0;
+    while (cur >= 0) {
+      const int w = static_cast<int>(cur >> 6);
+      for (; word > w; --word) {
+        a.mask[t * a.words + word] = static_cast<int64_t>(bits);
+        bits = 0;
+      }
+      if (w == word) // else: a token past the mask's words
+        bits |= uint64_t{1} << (cur & 63);
+      ++depth;
+      const int64_t up = a.parents[start + cur];
+      cur = up < cur ? up : -1;
+    }
+    for (; word >= 0; --word) {
+      a.mask[t * a.words + word] = static_cast<int64_t>(bits);
+      bits = 0;
+    }
+    a.positions[t] = static_cast<int32_t>(r.cached + depth);
+  }
+}
+
+} // namespace
+
+hipError_t tables_launch(TablesArgs a, hipStream_t s) {
+  // At most 1024 blocks: each one sums every request's lengths.
+  const int64_t runs = (static_cast<int64_t>(a.rows) + kThreads - 1) / kThreads;
+  const int64_t per = (runs + 1023) / 1024 > 0 ? (runs + 1023) / 1024 : 1;
+  const int64_t blocks = runs > 0 ? (runs + per - 1) / per : 1;
+  a.block_rows = static_cast<int32_t>(per * kThreads);
+  void *args[] = {&a};
+  return hipLaunchKernel(reinterpret_cast<const void *>(k_tables), dim3(static_cast<uint32_t>(blocks)),
+                         dim3(kThreads), args, 0, s);
+}
+
+} // namespace relx
