@@ -22,6 +22,7 @@ ValueError, what the library refuses TransferError("<code>: <detail>").
 """
 import ctypes
 import struct
+import threading
 from collections import namedtuple
 from functools import lru_cache
 
@@ -58,36 +59,53 @@ def _bad(message):
     raise ValueError(message)
 
 
+_functions = {}
+_errors = threading.local()
+
+
 def _call(name, ctx, *args):
-    err = N.relx_err()
-    if getattr(N.lib(), name)(ctx._h, *args, ctypes.byref(err)):
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(N.lib(), name)
+    try:
+        err = _errors.err
+    except AttributeError:
+        err = _errors.err = N.relx_err()
+        _errors.ref = ctypes.byref(err)
+    if fn(ctx._h, *args, _errors.ref):
         _fail(err)
 
 
+# torch's current stream as a handle; the plain query costs as much as a launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device):
+    if _raw_stream is not None:
+        return _raw_stream(device)
     return torch.cuda.current_stream(device).cuda_stream
 
 
 def _device(ctx, like):
-    d = like.device
-    if d.type != "cuda" or d.index != ctx.device:
-        _bad("the tensors are on %s, the context on device %d" % (d, ctx.device))
-    return d
+    """The context's device, which every tensor of the call is on."""
+    if like.get_device() != ctx.device:
+        _bad("the tensors are on %s, the context on device %d" % (like.device, ctx.device))
+    return ctx.device
 
 
 def _row(t, name, dtype, n, device):
     """A contiguous vector of `n` (None: any number)."""
-    if t.dtype is not dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != device or \
-            (t.shape[0] > 1 and t.stride(0) != 1):
-        _bad("%s: %s [%s] on %s, contiguous; got %s %s on %s"
+    if t.dtype is not dtype or t.dim() != 1 or t.get_device() != device or (n is not None and t.shape[0] != n) or \
+            not t.is_contiguous():
+        _bad("%s: %s [%s] on device %d, contiguous; got %s %s on %s"
              % (name, dtype, "n" if n is None else n, device, t.dtype, list(t.shape), t.device))
     return t.data_ptr()
 
 
 def _heads(t, name, shape, dtype, device):
     """[rows, heads, dim] with a contiguous last dimension."""
-    if t.shape != shape or t.dtype is not dtype or t.device != device:
-        _bad("%s: %s %s on %s; got %s %s on %s"
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
+        _bad("%s: %s %s on device %d; got %s %s on %s"
              % (name, dtype, list(shape), device, t.dtype, list(t.shape), t.device))
     row, head, one = t.stride()
     if one != 1 and shape[2] > 1 and t.numel():
@@ -96,34 +114,35 @@ def _heads(t, name, shape, dtype, device):
 
 
 def _table(t, device):
-    if t.dtype is not torch.int32 or t.dim() != 2 or t.device != device or (t.numel() > 1 and t.stride(1) != 1 and t.shape[1] > 1):
-        _bad("block table: int32 [requests, columns] on %s with contiguous rows; got %s %s on %s"
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != device or \
+            (t.stride(1) != 1 and t.numel() > 1 and t.shape[1] > 1):
+        _bad("block table: int32 [requests, columns] on device %d with contiguous rows; got %s %s on %s"
              % (device, t.dtype, list(t.shape), t.device))
-    return t.shape[0], t.shape[1], t.data_ptr(), t.stride(0)
+    requests, columns = t.shape
+    return requests, columns, t.data_ptr(), t.stride(0)
 
 
 def _cache(keys, values, k_scale, v_scale, device):
     """The cache's record fields: keys and values [pages, page, kv_heads, dim]."""
-    shape = keys.shape
-    kind = _KINDS.get(keys.dtype)
-    if len(shape) != 4 or values.shape != shape or values.dtype is not keys.dtype or kind is None or \
-            keys.device != device or values.device != device:
-        _bad("cache: keys and values [pages, page, kv_heads, dim] of one type on %s; got %s %s on %s and %s %s on %s"
-             % (device, keys.dtype, list(shape), keys.device, values.dtype, list(values.shape), values.device))
+    shape, dtype = keys.shape, keys.dtype
+    kind = _KINDS.get(dtype)
+    if len(shape) != 4 or values.shape != shape or values.dtype is not dtype or kind is None or \
+            keys.get_device() != device or values.get_device() != device:
+        _bad("cache: keys and values [pages, page, kv_heads, dim] of one type on device %d; got %s %s on %s and %s %s on %s"
+             % (device, dtype, list(shape), keys.device, values.dtype, list(values.shape), values.device))
     kp, ks, kh, ko = keys.stride()
     vp, vs, vh, vo = values.stride()
-    if shape[3] > 1 and (ko != 1 or vo != 1) and keys.numel():
+    if (ko != 1 or vo != 1) and shape[3] > 1 and keys.numel():
         _bad("cache: the last dimension must be contiguous")
-    scales = (0, 0)
-    if keys.dtype is torch.int8:
+    k_ptr = v_ptr = 0
+    if dtype is torch.int8:
         if k_scale is None or v_scale is None:
             _bad("an int8 cache takes k_scale and v_scale")
-        scales = (_row(k_scale, "k_scale", torch.float32, shape[2], device),
-                  _row(v_scale, "v_scale", torch.float32, shape[2], device))
+        k_ptr = _row(k_scale, "k_scale", torch.float32, shape[2], device)
+        v_ptr = _row(v_scale, "v_scale", torch.float32, shape[2], device)
     elif k_scale is not None or v_scale is not None:
         _bad("scales go with an int8 cache")
-    return (keys.data_ptr(), kp, ks, kh, values.data_ptr(), vp, vs, vh, *scales, shape[0], shape[1], shape[2],
-            shape[3], *kind)
+    return (keys.data_ptr(), kp, ks, kh, values.data_ptr(), vp, vs, vh, k_ptr, v_ptr, *shape, *kind)
 
 
 # ------------------------------------------------------------ block tables
@@ -158,13 +177,16 @@ def block_tables(ctx, cached, fresh, table, free_pages, page, rows, *, parents=N
         if words < 1:
             _bad("block tables: words = %d" % words)
     if out is None:
-        i32 = torch.empty(requests + 2 + rows, dtype=torch.int32, device=device)
-        i64 = torch.empty(rows * (1 + words), dtype=torch.int64, device=device)
-        out = Tables(i32[:requests + 1], i64[:rows], i32[requests + 2:], i32[requests + 1:requests + 2],
-                     i64[rows:].view(rows, words) if words else None)
-        i32_ptr, i64_ptr = i32.data_ptr(), i64.data_ptr()
-        ptrs = (i32_ptr, i64_ptr, i32_ptr + 4 * (requests + 2), i64_ptr + 8 * rows if words else 0,
-                i32_ptr + 4 * (requests + 1))
+        i32 = torch.empty(requests + 2 + rows, dtype=torch.int32, device=table.device)
+        i64 = torch.empty(rows * (1 + words), dtype=torch.int64, device=table.device)
+        p32, p64 = i32.data_ptr(), i64.data_ptr()
+        starts, taken, positions = i32.split((requests + 1, 1, rows))
+        ptrs = p32, p64, p32 + 4 * (requests + 2), p64 + 8 * rows if words else 0, p32 + 4 * (requests + 1)
+        mask = None
+        if words:
+            i64, mask = i64.split((rows, rows * words))
+            mask = mask.view(rows, words)
+        out = Tables(starts, i64, positions, taken, mask)
     else:
         ptrs = (_row(out.starts, "starts", torch.int32, requests + 1, device),
                 _row(out.slots, "slots", torch.int64, rows, device),
@@ -172,7 +194,7 @@ def block_tables(ctx, cached, fresh, table, free_pages, page, rows, *, parents=N
                 _row(out.taken, "taken", torch.int32, 1, device))
         if words:
             m = out.mask
-            if m is None or m.dtype is not torch.int64 or m.shape != (rows, words) or m.device != device or \
+            if m is None or m.dtype is not torch.int64 or m.shape != (rows, words) or m.get_device() != device or \
                     not m.is_contiguous():
                 _bad("mask: contiguous int64 [%d, %d]" % (rows, words))
             ptrs = ptrs[:3] + (m.data_ptr(), ptrs[4])
@@ -194,8 +216,8 @@ def _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs):
              % (q.dtype, list(qs), k.dtype, list(ks)))
     rows, dim = qs[0], qs[2]
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or \
-            cos.device != device or sin.device != device or not (cos.is_contiguous() and sin.is_contiguous()):
-        _bad("cos and sin: contiguous float32 [angles, rotary / 2] on %s; got %s %s and %s %s"
+            cos.get_device() != device or sin.get_device() != device or not (cos.is_contiguous() and sin.is_contiguous()):
+        _bad("cos and sin: contiguous float32 [angles, rotary / 2] on device %d; got %s %s and %s %s"
              % (device, cos.dtype, list(cos.shape), sin.dtype, list(sin.shape)))
     w_kind, w_ptr = (0, 32), [0, 0]
     given = [w for w in (q_weight, k_weight) if w is not None]
@@ -252,8 +274,8 @@ def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pair
 def _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out):
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
-    zq, zk = out if out is not None else (torch.empty(qs, dtype=dtype, device=device),
-                                          torch.empty(ks, dtype=dtype, device=device))
+    zq, zk = out if out is not None else (torch.empty(qs, dtype=dtype, device=q.device),
+                                          torch.empty(ks, dtype=dtype, device=q.device))
     _call("relx_norm_rotate", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
           _pack_heads(k, "keys", ks, dtype, device), _pack_heads(zq, "query result", qs, dtype, device),
           _pack_heads(zk, "key result", ks, dtype, device), _stream(device))
@@ -267,11 +289,11 @@ def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_wei
     is); the others have the operands' type."""
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
-    gq, gk = torch.empty(qs, dtype=dtype, device=device), torch.empty(ks, dtype=dtype, device=device)
-    gw = [None if w is None else torch.empty(qs[2], dtype=torch.float32, device=device) for w in (q_weight, k_weight)]
+    gq, gk = torch.empty(qs, dtype=dtype, device=q.device), torch.empty(ks, dtype=dtype, device=q.device)
+    gw = [None if w is None else torch.empty(qs[2], dtype=torch.float32, device=q.device) for w in (q_weight, k_weight)]
     room = None
     if q_weight is not None or k_weight is not None:
-        room = torch.empty(_rotate_room(rot, qs, ks, dtype) // 4, dtype=torch.float32, device=device)
+        room = torch.empty(_rotate_room(rot, qs, ks, dtype) // 4, dtype=torch.float32, device=q.device)
     _call("relx_norm_rotate_backward", ctx, rot, _pack_heads(dq, "query gradient", qs, dtype, device),
           _pack_heads(dk, "key gradient", ks, dtype, device), _pack_heads(q, "queries", qs, dtype, device),
           _pack_heads(k, "keys", ks, dtype, device), _pack_heads(gq, "query gradient", qs, dtype, device),
@@ -308,7 +330,7 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
     if out is None:
-        out = torch.empty(qs, dtype=dtype, device=device)
+        out = torch.empty(qs, dtype=dtype, device=q.device)
     cache = _CACHE.pack(*_cache(cache_k, cache_v, k_scale, v_scale, device))
     _call("relx_norm_rotate_append", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
           _pack_heads(k, "keys", ks, dtype, device), _pack_heads(v, "values", ks, dtype, device),
@@ -364,22 +386,22 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     requests, columns, t_ptr, t_row = _table(table, device)
     words = m_ptr = 0
     if mask is not None:
-        if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != rows or mask.device != device or \
+        if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != rows or mask.get_device() != device or \
                 not mask.is_contiguous() or mask.shape[1] < 1:
-            _bad("mask: contiguous int64 [%d, words] on %s; got %s %s" % (rows, device, mask.dtype, list(mask.shape)))
+            _bad("mask: contiguous int64 [%d, words] on device %d; got %s %s" % (rows, device, mask.dtype, list(mask.shape)))
         words, m_ptr = mask.shape[1], mask.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=q.device)
     l_ptr = 0
     if lse is not None:
-        if lse.dtype is not torch.float32 or lse.shape != shape[:2] or lse.device != device or not lse.is_contiguous():
+        if lse.dtype is not torch.float32 or lse.shape != shape[:2] or lse.get_device() != device or not lse.is_contiguous():
             _bad("lse: contiguous float32 [%d, %d]" % (rows, heads))
         l_ptr = lse.data_ptr()
     if workspace is None:
         workspace = torch.empty(tree_attention_workspace(rows, requests, heads, kv_heads, dim, cache[11]),
-                                dtype=torch.uint8, device=device)
-    elif workspace.dtype is not torch.uint8 or workspace.device != device or not workspace.is_contiguous():
-        _bad("workspace: contiguous uint8 on %s" % device)
+                                dtype=torch.uint8, device=q.device)
+    elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
+        _bad("workspace: contiguous uint8 on device %d" % device)
     _call("relx_tree_attention", ctx,
           _ATTENTION.pack(*_heads(q, "queries", shape, dtype, device), *_heads(out, "result", shape, dtype, device),
                           *cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),

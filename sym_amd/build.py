@@ -28,7 +28,8 @@ SOURCES = ["plan.cpp", "program.cpp", "runtime.cpp", "workers.cpp", "indexed.cpp
            "kernels.hip",
            "k_stream_fast.hip", "k_stream_generic.hip", "k_transpose.hip", "k_transpose_ragged.hip", "k_rows.hip", "k_interleave.hip",
            "k_interleave_generic.hip", "k_interleave_ragged.hip", "k_permute.hip", "k_gather.hip", "k_copy.hip", "noalloc.hip",
-           "attention.cpp", "k_tables.hip", "k_rotate.hip", "k_attend_f16.hip", "k_attend_bf16.hip"]
+           "attention.cpp", "k_tables.hip", "k_rotate.hip",
+           "k_attend_f16.hip", "k_attend_f16_i8.hip", "k_attend_bf16.hip", "k_attend_bf16_i8.hip"]
 
 
 # The one-level interleave takes its hot arguments as leading scalars that
@@ -37,7 +38,9 @@ SOURCES = ["plan.cpp", "program.cpp", "runtime.cpp", "workers.cpp", "indexed.cpp
 EXTRA = {"k_interleave.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
          "k_rotate.hip": ["-ffp-contract=fast"],
          "k_attend_f16.hip": ["-ffp-contract=fast"],
-         "k_attend_bf16.hip": ["-ffp-contract=fast"]}
+         "k_attend_f16_i8.hip": ["-ffp-contract=fast"],
+         "k_attend_bf16.hip": ["-ffp-contract=fast"],
+         "k_attend_bf16_i8.hip": ["-ffp-contract=fast"]}
 
 
 def _compile(src):

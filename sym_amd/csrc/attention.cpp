@@ -160,6 +160,9 @@ CacheBytes cache_bytes(const relx_cache &c) {
   layout(c.page * c.pages <= INT32_MAX, "cache: more than 2^31 - 1 slots");
   need(c.pages == 0 || (c.keys && c.values), "cache: null keys or values");
   need(b.type != kI8 || c.kv_heads == 0 || (c.key_scale && c.value_scale), "cache: an int8 cache has a scale a head");
+  need(c.key_page >= 0 && c.key_slot >= 0 && c.key_head >= 0 && c.value_page >= 0 && c.value_slot >= 0 &&
+           c.value_head >= 0,
+       "cache: negative strides");
   const int64_t w = b.type == kI8 ? 1 : b.type == kF32 ? 4 : 2;
   b.key_page = c.key_page * w;
   b.key_slot = c.key_slot * w;
@@ -184,7 +187,7 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   need(p.heads >= 1 && kv >= 1 && p.heads % kv == 0, "attention: query heads are a multiple of the key heads");
   layout(p.heads <= 65535, "attention: more than 65535 heads");
   layout(dim >= 8 && dim <= 256 && dim % 8 == 0, "attention: head sizes are multiples of 8 up to 256");
-  layout(p.columns == 0 || p.columns <= INT32_MAX / p.cache.page, "attention: a table of more than 2^31 - 1 tokens");
+  layout(p.columns == 0 || p.columns <= (int64_t{1} << 30) / p.cache.page, "attention: a table of more than 2^30 tokens");
   layout(p.rows <= INT32_MAX / p.heads, "attention: more than 2^31 - 1 rows of heads");
   need(std::isfinite(p.scale), "attention: scale");
   need(p.rows == 0 || (p.q.data && p.out.data), "attention: null queries or result");
@@ -227,8 +230,11 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   a.scale = static_cast<float>(p.scale * 1.4426950408889634);
   plan = attend_plan(p.rows, p.requests, kv, p.heads / kv, dim, p.cache.page);
   // a lane's distance inside a tile of 16 tokens is held in 32 bits
-  if (std::abs(a.key_slot) > INT32_MAX / 32 || std::abs(a.value_slot) > INT32_MAX / 32)
-    plan.fast = false;
+  if (a.key_slot > INT32_MAX / 32 || a.value_slot > INT32_MAX / 32)
+    plan.even = false;
+  const int64_t at = reinterpret_cast<int64_t>(a.keys) | reinterpret_cast<int64_t>(a.values) | a.key_page | a.key_slot |
+                     a.key_head | a.value_page | a.value_slot | a.value_head;
+  plan.aligned = at % 16 == 0;
   a.workgroups = plan.workgroups;
   return a;
 }
@@ -239,23 +245,25 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
                        int64_t page) {
   AttendPlan p{};
   p.width = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  p.fast = dim == p.width && page % 16 == 0;
+  p.even = page % 16 == 0;
   // query rows of a key head in an even batch
   const int64_t q = requests > 0 ? (rows + requests - 1) / requests * group : 0;
-  p.row_tiles = q <= 16 ? 1 : q <= 32 || p.width == 256 ? 2 : 4;
-  p.workgroups = p.row_tiles == 1 ? 512 : 256;
+  p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : 128;
+  p.workgroups = 512;
   (void)kv_heads;
   return p;
 }
 
 size_t attend_workspace(const AttendPlan &p, int64_t requests) {
-  const size_t rows = static_cast<size_t>(p.workgroups) * 2 * 16 * static_cast<size_t>(p.row_tiles);
+  const size_t rows = static_cast<size_t>(p.workgroups) * 2 * static_cast<size_t>(p.rows);
   return rows * static_cast<size_t>(p.width + 2) * sizeof(float) +
          (static_cast<size_t>(requests) + 1) * sizeof(int64_t);
 }
 
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8, hipStream_t s) {
-  return type == kF16 ? attend_launch_f16(a, p, i8, s) : attend_launch_bf16(a, p, i8, s);
+  if (type == kF16)
+    return i8 ? attend_launch_f16_i8(a, p, s) : attend_launch_f16(a, p, s);
+  return i8 ? attend_launch_bf16_i8(a, p, s) : attend_launch_bf16(a, p, s);
 }
 
 } // namespace relx
@@ -406,7 +414,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
       if (args->workspace_bytes < 0 || static_cast<size_t>(args->workspace_bytes) < want || !args->workspace)
         throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(args->workspace_bytes) +
                                                        " bytes, the call takes " + std::to_string(want));
-      const size_t rows = static_cast<size_t>(plan.workgroups) * 2 * 16 * static_cast<size_t>(plan.row_tiles);
+      const size_t rows = static_cast<size_t>(plan.workgroups) * 2 * static_cast<size_t>(plan.rows);
       relx::need(reinterpret_cast<uintptr_t>(args->workspace) % 16 == 0, "attention: workspace alignment");
       a.partial = static_cast<float *>(args->workspace);
       a.stats = a.partial + rows * static_cast<size_t>(plan.width);

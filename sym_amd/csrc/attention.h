@@ -93,11 +93,12 @@ struct AttendArgs {
   float scale; // of a score, times log2 e
 };
 
-// How a call runs: rows of query tiles per wave and workgroups.
+// How a call runs.
 struct AttendPlan {
   int width;      // head size, rounded up to a kernel's
-  int row_tiles;  // tiles of 16 query rows a wave keeps
-  bool fast;      // whole heads, and pages of whole token tiles
+  int rows;       // query rows of an item
+  bool even;      // pages of whole tiles of 16 tokens
+  bool aligned;   // cache rows at 16-byte addresses
   int workgroups;
 };
 AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
@@ -105,7 +106,9 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
 size_t attend_workspace(const AttendPlan &p, int64_t requests);
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8,
                          hipStream_t s);
-hipError_t attend_launch_f16(const AttendArgs &a, const AttendPlan &p, bool i8, hipStream_t s);
-hipError_t attend_launch_bf16(const AttendArgs &a, const AttendPlan &p, bool i8, hipStream_t s);
+hipError_t attend_launch_f16(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_f16_i8(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_bf16(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_bf16_i8(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
 
 } // namespace relx

@@ -4,8 +4,7 @@
 // One pass over the keys and values with the running maximum and sum of the
 // softmax. The query rows of a request that share a key head (its new tokens
 // times the heads of the group) are the columns of matrix products; a wave
-// keeps 16, 32 or 64 of them with their sums in registers and takes 32 tokens
-// at a time:
+// keeps 16 or 32 of them with their sums in registers:
 //
 //   S^T = K Q^T    16 tokens x 16 rows per product, dims contracted
 //   O^T += V^T P^T 16 dims x 16 rows per product, 32 tokens contracted
@@ -14,19 +13,28 @@
 // 4 (lane / 16) + 0..3 of each of two token tiles) is the layout of the
 // second product's operand if its contracted tokens are numbered
 // 8 (lane / 16) + 4 tile + 0..3, so the weights go from one product to the
-// next without leaving their lane. Keys and values come from the cache
-// straight into registers: a lane's 16 bytes of a key row are its operand, and
-// of values it loads 16 bytes (for a head of 128) from each of its eight
-// tokens and transposes the 8 x 8 block in place with byte permutes; the
-// dims that a product's rows stand for are numbered to suit. No shared memory
-// is touched between the products.
+// next without leaving their lane. Keys and values pass through shared memory, 32 tokens at a time:
+// a lane reads its 16 bytes of a key row as they are, and values transposed
+// (ds_read_b64_tr_b16: four tokens of one dim from four lanes' rows).
 //
-// The tokens of a wave's tiles lie `kUnit` apart: four waves take 128 tokens
-// in turn and add up at the end. The work of a call is the list of these
-// units over (request, key head, tile of query rows), cut into equal runs, one
-// per workgroup; an item that lies in several runs leaves partial sums that
-// k_attend_join adds up. So one long context fills the card as well as many
-// short ones do, and uneven lengths cost nothing.
+// How tokens get there (Source):
+//   kAsync   16-bit caches whose pages hold whole tiles of 16 tokens, rows at
+//            16-byte addresses: loads that write shared memory themselves, a
+//            ring of tiles ahead
+//   kStaged  everything else: through registers, where int8 is widened and
+//            what is no token becomes zero
+// and who works on them:
+//   up to 16 query rows share a key head (decoding): bound by the cache's
+//     bytes. The waves of a workgroup take turns at the tiles, each with a ring
+//     of its own and no barrier, and add up at the end.
+//   more (trees, chunks): the waves have rows of their own, 16 or 32 each, and
+//     share the tiles.
+//
+// The work of a call is the list of its units of tokens over (request, key
+// head, tile of query rows), cut into equal runs, one per workgroup; an item
+// that lies in several runs leaves partial sums that k_attend_join adds up. So
+// one long context fills the card as well as many short ones do, and uneven
+// lengths cost nothing.
 #pragma once
 
 #include <algorithm>
@@ -48,10 +56,15 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kAttendWaves = 4;
-constexpr int kStep = 32;                       // tokens of a wave at a time
-constexpr int kUnit = kStep * kAttendWaves;     // tokens of a workgroup at a time
-constexpr int kScan = 64 * kAttendWaves;        // threads
+constexpr int kScan = 128;    // runs of requests whose units a workgroup (of at least as many threads) adds up
+constexpr int kTile = 32;     // tokens of a tile
+constexpr int kSharedWaves = 4;
+constexpr int kSharedUnit = 64;
+// Waves that take turns: as many as their rings fit shared memory.
+constexpr int turn_waves(int dp) { return dp == 256 ? 2 : 4; }
+constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
+
+enum Source : int { kAsync, kStaged, kStagedEven };
 // Where a row's running maximum starts: finite, so that a difference with a
 // masked score's -inf stays -inf.
 constexpr float kNone = -1e30f;
@@ -65,6 +78,12 @@ template <class T> __device__ __forceinline__ T load(const char *p) {
 }
 template <class T> __device__ __forceinline__ void store(char *p, const T &v) {
   reinterpret_cast<Loose<T> *>(p)->v = v;
+}
+
+// Reads that are the same for the whole wave, through the scalar cache: they
+// do not queue behind the vector loads in flight.
+__device__ __forceinline__ int32_t scalar_load(const int32_t *p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uint64_t>(p));
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -81,6 +100,20 @@ template <int T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The same number, of which the compiler no longer knows what it is: what is
+// worked out from it in a loop stays there instead of filling registers outside.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <int T> __device__ __forceinline__ float widen16(uint32_t h) {
+  if constexpr (T == kF16)
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+  else
+    return __uint_as_float(h << 16);
 }
 
 // Two values rounded to nearest even. The weights of the second product are
@@ -114,103 +147,61 @@ template <int T> __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t h
 
 __device__ __forceinline__ float max_over_groups(float x) {
   // the four lanes that hold a row's other tokens: 16 and 32 lanes away
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-
-// acc += weights times values, dims e, e + 1, ... of each lane's.
-template <int T, int E, class F, class V, int... I>
-__device__ __forceinline__ void add_dims(f32x4 (&acc)[E], u32x4 weights, const F &operand, const V &v,
-                                         std::integer_sequence<int, I...>) {
-  ((acc[I] = mfma<T>(operand(v, std::integral_constant<int, I>{}), weights, acc[I])), ...);
-}
-template <int T, int E, class F, class V>
-__device__ __forceinline__ void add_values(f32x4 (&acc)[E], u32x4 weights, const F &operand, const V &v) {
-  add_dims<T, E>(acc, weights, operand, v, std::make_integer_sequence<int, E>{});
-}
-
-// The same for one row (the lanes that are `mine`), of the tokens that `sees`
-// has: the others' values do not enter.
-template <int T, int E, int I, class F, class V>
-__device__ __forceinline__ void add_row_dim(f32x4 (&acc)[E], u32x4 weights, const F &operand, const V &v,
-                                            u32x4 sees, bool mine) {
-  const u32x4 o = operand(v, std::integral_constant<int, I>{}) & sees;
-  const f32x4 one = mfma<T>(o, weights, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    acc[I][i] += mine ? one[i] : 0.0f;
-}
-template <int T, int E, class F, class V, int... I>
-__device__ __forceinline__ void add_row_dims(f32x4 (&acc)[E], u32x4 weights, const F &operand, const V &v,
-                                             u32x4 sees, bool mine, std::integer_sequence<int, I...>) {
-  (add_row_dim<T, E, I>(acc, weights, operand, v, sees, mine), ...);
-}
-template <int T, int E, class F, class V>
-__device__ __forceinline__ void add_row(f32x4 (&acc)[E], u32x4 weights, const F &operand, const V &v,
-                                        u32x4 sees, bool mine) {
-  add_row_dims<T, E>(acc, weights, operand, v, sees, mine, std::make_integer_sequence<int, E>{});
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // ------------------------------------------------------------ the schedule
 
 struct Request {
-  int64_t cached, length; // tokens in the cache before the step, and with it
-  int start, fresh;       // its rows
-  int tiles;              // tiles of query rows
-  int64_t units;          // of one item
+  int cached, length; // tokens in the cache before the step, and with it: at most 2^30
+  int start, fresh;   // its rows
+  int tiles;          // tiles of query rows
+  int units;          // of one item
 };
 
-template <int ROWS>
+// ROWS: query rows of an item, UNIT: tokens of a unit.
+template <int ROWS, int UNIT>
 __device__ __forceinline__ Request attend_request(const AttendArgs &a, int b) {
   Request r;
   const int s = min(max(a.starts[b], 0), a.rows), e = min(max(a.starts[b + 1], s), a.rows);
   r.start = s;
   r.fresh = e - s;
-  const int64_t room = a.pages > 0 ? static_cast<int64_t>(a.columns) * a.page.d : 0;
-  const int64_t c = max(a.cached[b], 0);
-  r.cached = min(c, room);
-  r.length = min(c + r.fresh, room);
+  const int room = a.pages > 0 ? a.columns * static_cast<int>(a.page.d) : 0;
+  r.cached = min(max(a.cached[b], 0), room);
+  r.length = r.fresh < room - r.cached ? r.cached + r.fresh : room;
   const int64_t q = static_cast<int64_t>(r.fresh) * a.group.d;
   r.tiles = static_cast<int>((q + ROWS - 1) / ROWS);
-  r.units = max((r.length + kUnit - 1) / kUnit, int64_t{1});
+  r.units = max((r.length + UNIT - 1) / UNIT, 1);
   return r;
 }
 
-template <int ROWS>
+template <int ROWS, int UNIT>
 __device__ __forceinline__ int64_t request_units(const AttendArgs &a, int b) {
-  const Request r = attend_request<ROWS>(a, b);
+  const Request r = attend_request<ROWS, UNIT>(a, b);
   return static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
 }
 
-// ------------------------------------------------------------ the kernel
+// The units before each run of requests, which every workgroup adds up for
+// itself.
+struct Schedule {
+  int64_t before[kScan + 1];
+  int64_t waves[kScan / 64];
+};
 
-template <int T, bool I8, int DP, int RT, bool FAST>
-__global__ __launch_bounds__(kScan, RT <= 2 && DP <= 128 ? 2 : 1) void k_attend(AttendArgs a) {
-  constexpr int ROWS = 16 * RT;
-  constexpr int E = DP / 16;              // dims of a lane's values
-  constexpr int CELL = I8 ? 1 : 2;        // bytes of a cache element
-  constexpr int KB = 16 / CELL;           // dims of a key load
-  constexpr int KS = DP / (4 * KB);       // key loads of a token
-  constexpr int QS = DP / 32;             // contraction steps
-  constexpr int VW = E * CELL / 4;        // words of a lane's values of a token
-  constexpr float kBias = T == kF16 ? 6.0f : 0.0f; // weights up to 2^14 in f16: small ones keep their bits
-
-  __shared__ int64_t before[kScan + 1];
-  __shared__ int64_t wave_units[kAttendWaves];
-  __shared__ float sums[kAttendWaves][16][DP + 4];
-  __shared__ float row_max[kAttendWaves][ROWS], row_sum[kAttendWaves][ROWS];
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
-
-  // every workgroup adds up the requests' units for itself
+template <int ROWS, int UNIT>
+__device__ __forceinline__ void add_up(const AttendArgs &a, Schedule &sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.requests + kScan - 1) / kScan;
-  {
-    const int b0 = min(tid * run, a.requests), b1 = min(b0 + run, a.requests);
-    int64_t mine = 0;
+  const int b0 = min(tid * run, a.requests), b1 = min(b0 + run, a.requests);
+  const bool in = tid < kScan;
+  int64_t mine = 0, upto = 0;
+  if (in) {
     for (int b = b0; b < b1; ++b)
-      mine += request_units<ROWS>(a, b);
-    int64_t upto = mine;
+      mine += request_units<ROWS, UNIT>(a, b);
+    upto = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int64_t v = __shfl_up(upto, o);
@@ -218,463 +209,856 @@ __global__ __launch_bounds__(kScan, RT <= 2 && DP <= 128 ? 2 : 1) void k_attend(
         upto += v;
     }
     if (lane == 63)
-      wave_units[wave] = upto;
-    __syncthreads();
+      sh.waves[wave] = upto;
+  }
+  __syncthreads();
+  if (in) {
     int64_t first = upto - mine;
     for (int w = 0; w < wave; ++w)
-      first += wave_units[w];
-    before[tid] = first;
+      first += sh.waves[w];
+    sh.before[tid] = first;
     if (tid == kScan - 1)
-      before[kScan] = first + mine;
+      sh.before[kScan] = first + mine;
     if (blockIdx.x == 0) { // for the join
       int64_t at = first;
       for (int b = b0; b < b1; ++b) {
         a.schedule[b] = at;
-        at += request_units<ROWS>(a, b);
+        at += request_units<ROWS, UNIT>(a, b);
       }
       if (tid == kScan - 1)
         a.schedule[a.requests] = first + mine;
     }
-    __syncthreads();
   }
-  const int64_t total = uniform64(before[kScan]);
+  __syncthreads();
+}
+
+// A workgroup's run of units. Workgroups go round the eight dies; neighbouring
+// runs share a die, whose cache serves the tiles of query rows that read the
+// same keys.
+struct Run {
+  int64_t wg, unit, end;
+};
+__device__ __forceinline__ Run my_run(const Schedule &sh) {
+  const int64_t total = uniform64(sh.before[kScan]);
   const int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  // Workgroups go round the eight dies; neighbouring runs share a die, whose
-  // cache serves the tiles of query rows that read the same keys.
-  const uint32_t die = blockIdx.x & 7u;
-  const int64_t wg = static_cast<int64_t>(die) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-  int64_t unit = wg * per;
-  const int64_t unit_end = min(total, unit + per);
+  Run r;
+  r.wg = static_cast<int64_t>(blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  r.wg = uniform64(r.wg);
+  r.unit = uniform64(r.wg * per);
+  r.end = uniform64(min(total, r.unit + per));
+  return r;
+}
 
-  while (unit < unit_end) {
-    // the item that holds `unit`
-    int lo = 0, hi = kScan;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (uniform64(before[mid]) <= unit)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    int b = lo * run;
-    int64_t at = uniform64(before[lo]);
-    Request r = attend_request<ROWS>(a, b);
-    for (;;) {
-      const int64_t n = static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
-      if (unit < at + n)
-        break;
-      at += n;
-      r = attend_request<ROWS>(a, ++b);
-    }
-    b = uniform(b);
-    at = uniform64(at);
-    const int64_t cached = uniform64(r.cached), length = uniform64(r.length);
-    const int start = uniform(r.start), fresh = uniform(r.fresh), tiles = uniform(r.tiles);
-    const int64_t units = uniform64(r.units);
-    const int64_t item = (unit - at) / units;
-    const int64_t s0 = unit - at - item * units;
-    const int64_t s1 = min(units, s0 + (unit_end - unit));
-    const int head = static_cast<int>(item / tiles);
-    const int tile = static_cast<int>(item - static_cast<int64_t>(head) * tiles);
-    unit += s1 - s0;
+// The part of an item that lies in a run: the units [s0, s1) of its `units`.
+struct Item {
+  int b, start, fresh, head, tile, cached, length, s0, s1, units;
+};
+template <int ROWS, int UNIT>
+__device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Run &run) {
+  int lo = 0, hi = kScan;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (uniform64(sh.before[mid]) <= run.unit)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int b = lo * ((a.requests + kScan - 1) / kScan);
+  int64_t at = uniform64(sh.before[lo]);
+  Request r = attend_request<ROWS, UNIT>(a, b);
+  for (;;) {
+    const int64_t n = static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
+    if (run.unit < at + n)
+      break;
+    at += n;
+    r = attend_request<ROWS, UNIT>(a, ++b);
+  }
+  Item i;
+  i.b = uniform(b);
+  at = uniform64(at);
+  i.cached = uniform(r.cached);
+  i.length = uniform(r.length);
+  i.start = uniform(r.start);
+  i.fresh = uniform(r.fresh);
+  i.units = uniform(r.units);
+  const int tiles = uniform(r.tiles);
+  const int64_t item = uniform64((run.unit - at) / i.units);
+  i.s0 = uniform(static_cast<int>(run.unit - at - item * i.units));
+  i.s1 = uniform(static_cast<int>(min(static_cast<int64_t>(i.units), i.s0 + (run.end - run.unit))));
+  i.head = uniform(static_cast<int>(item / tiles));
+  i.tile = static_cast<int>(item - static_cast<int64_t>(i.head) * tiles);
+  run.unit = uniform64(run.unit + i.s1 - i.s0);
+  return i;
+}
 
-    // ---- queries: this lane's row of each tile
-    const int rows = fresh * static_cast<int>(a.group.d) - tile * ROWS; // of this tile and later ones
-    u32x4 q[RT][QS];
-    int row_j[RT]; // the row's token among the new ones
+// What the p-th query row of the item's request and key head sees of the 32
+// tokens from `x`, as bits.
+__device__ __forceinline__ uint32_t row_sees(const AttendArgs &a, const Item &it, int p, int x) {
+  const int d = x - it.cached; // the first token's place among the new ones
+  if (d + 32 <= 0)
+    return 0xffffffffu;
+  const int j = static_cast<int>(fdiv(static_cast<uint32_t>(p), a.group)); // the row's own place there
+  if (!a.mask) {
+    const int n = j - d + 1;
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+  }
+  if (j >= it.fresh)
+    return 0u;
+  const int64_t *mask = a.mask + (it.start + static_cast<int64_t>(j)) * a.words;
+  const int from = d > 0 ? d : 0, word = from >> 6, sh = from & 63;
+  uint64_t m = 0;
+  if (word < a.words)
+    m = static_cast<uint64_t>(mask[word]) >> sh;
+  if (sh > 32 && word + 1 < a.words)
+    m |= static_cast<uint64_t>(mask[word + 1]) << (64 - sh);
+  const int old = d < 0 ? -d : 0; // cached tokens among the 32
+  return static_cast<uint32_t>(m << old) | ((1u << old) - 1u);
+}
+
+template <int T> constexpr float weight_bias() {
+  return T == kF16 ? 6.0f : 0.0f; // weights up to 2^14 in f16: small ones keep their bits
+}
+
+// One over a row's sum of weights, with the values' scale; 0 for a row that
+// saw nothing.
+__device__ __forceinline__ float finish(float sum, float scale) {
+  return sum > 0.0f ? scale / sum : sum == 0.0f ? 0.0f : sum;
+}
+__device__ __forceinline__ float log_sum(float top, float sum) {
+  return sum == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+}
+
+// ------------------------------------------------------------ tiles
+
+// Where the n-th 16-byte piece of a token's row lies in a tile ([kTile][DP] of
+// T): pieces are swapped by the token's number, so that sixteen lanes that read
+// the same piece of sixteen tokens, or all pieces of one, meet no bank twice.
+template <int DP> __device__ __forceinline__ int swap_of(int token) {
+  constexpr int P = DP / 8;
+  return P >= 16 ? token & 15 : (token >> 1) & (P - 1);
+}
+template <int DP> __device__ __forceinline__ int piece(int token, int n) {
+  return (token * (DP / 8) + (n ^ swap_of<DP>(token))) * 16;
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// Four tokens of one dim, a pair of words: lane i of sixteen gives the address
+// of four dims of token i / 4, and gets dim i.
+__device__ __forceinline__ u32x2 read_transposed(const char *p) {
+  typedef __attribute__((address_space(3))) i16x4 *at;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (at)(lds_char *)const_cast<char *>(p)));
+}
+
+// A shared array's place.
+__device__ __forceinline__ uint32_t place(const char *p) {
+  return uniform(static_cast<int>(reinterpret_cast<uintptr_t>((lds_char *)const_cast<char *>(p))));
+}
+
+// 16 bytes per lane from base + at into shared memory, lane after lane from
+// `to`. The compiler does not count it: arrived<N>() waits until at most the N
+// latest are on their way.
+__device__ __forceinline__ void load_async(const char *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(uniform(static_cast<int>(to))), "v"(at), "s"(uniform64(reinterpret_cast<int64_t>(base)))
+               : "memory");
+}
+template <int N> __device__ __forceinline__ void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// Waits for the wave's own reads and writes of shared memory.
+__device__ __forceinline__ void shared_done() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// The values of a tile at the 16 dims from 16 e, as an operand: dim 16 e +
+// lane % 16 of the lane's eight tokens.
+template <int DP> __device__ __forceinline__ u32x4 values_at(const char *tv, int e, int lane) {
+  const int c = lane & 15, g = lane >> 4;
+  const int token = 4 * g + (c >> 2), half = (c & 3) >> 1, byte = (c & 1) * 8;
+  const u32x2 lo = read_transposed(tv + piece<DP>(token, e * 2 + half) + byte);
+  const u32x2 hi = read_transposed(tv + piece<DP>(token + 16, e * 2 + half) + byte);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+template <int T> __device__ __forceinline__ bool finite16(uint32_t h) {
+  constexpr uint32_t kExp = T == kF16 ? 0x7c00u : 0x7f80u;
+  return (h & kExp) != kExp;
+}
+
+// Makes the values of a tile that no product may touch zero: of the tokens that
+// are not `seen` everything, which may be anything, and, where the rows see
+// different tokens (`mixed`), what is not finite: a product with a weight of
+// zero would carry it over to rows that do not see it (Rows::add_odd puts it
+// where it belongs). The NT tokens from `first`, by one wave; true if a token
+// that is seen had such a value.
+template <int T, int DP, int NT>
+__device__ __forceinline__ bool clean(char *tv, int first, uint32_t seen, bool mixed, int lane) {
+  constexpr int P = DP / 8;
+  bool odd = false;
+#pragma clang loop unroll(disable)
+  for (int i = lane; i < NT * P; i += 64) {
+    const int token = first + i / P;
+    u32x4 *at = reinterpret_cast<u32x4 *>(tv + token * DP * 2 + (i % P) * 16);
+    u32x4 v = *at;
+    if (!(seen >> token & 1u)) {
+      v = u32x4{0u, 0u, 0u, 0u};
+    } else if (mixed) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int i = t * 16 + c;
-      const uint32_t p = static_cast<uint32_t>(tile * ROWS + i);
-      const uint32_t j = fdiv(p, a.group);
-      row_j[t] = static_cast<int>(j);
-      const char *src = a.q + ((start + static_cast<int64_t>(j)) * a.q_row +
-                               (static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
-#pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        // the dims of contraction step s: those of this lane's keys
-        const int d = I8 ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
-        q[t][s] = u32x4{0u, 0u, 0u, 0u};
-        if (i < rows && d < a.dim)
-          q[t][s] = load<u32x4>(src + d * 2);
+      for (int n = 0; n < 4; ++n) {
+        const bool lo = finite16<T>(v[n]), hi = finite16<T>(v[n] >> 16);
+        odd |= !lo || !hi;
+        v[n] &= (lo ? 0xffffu : 0u) | (hi ? 0xffff0000u : 0u);
       }
     }
+    *at = v;
+  }
+  return __any(odd);
+}
 
-    const float scale = I8 ? a.scale * a.key_scale[head] : a.scale;
-    float top[RT], weight[RT];
-    f32x4 acc[RT][E];
+// A wave's query rows and their sums.
+template <int T, int DP, int RT> struct Rows {
+  static constexpr int E = DP / 16, QS = DP / 32;
+  u32x4 q[RT][QS];
+  float top[RT];     // reference maximum of a row's scaled scores
+  float sum[RT];     // of its weights, over this lane's tokens; total(): over all
+  f32x4 acc[RT][E];  // dims 16 e + 4 (lane / 16) + 0..3
+  float scale;
+
+  __device__ __forceinline__ void start(const AttendArgs &a, const Item &it, int row0, int rows, float score_scale,
+                                        int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    scale = score_scale;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
+      const uint32_t j = fdiv(p, a.group);
+      const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
+                               (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        const int d = s * 32 + g * 8;
+        q[t][s] = u32x4{0u, 0u, 0u, 0u};
+        if (t * 16 + c < rows && d < a.dim)
+          q[t][s] = load<u32x4>(src + d * 2);
+      }
       top[t] = kNone;
-      weight[t] = 0.0f;
+      sum[t] = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; ++e)
         acc[t][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // Here, once: else the compiler, which cannot know in the loop whether the
+    // queries have arrived, waits there for all loads in flight, every time.
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int s = 0; s < QS; ++s)
+        asm volatile("" : "+v"(q[t][s]));
+  }
 
-    const char *keys = a.keys + head * a.key_head;
-    const char *values = a.values + head * a.value_head;
-    const int32_t *table = a.table + b * a.table_row;
-    const int key_lane = FAST ? c * static_cast<int>(a.key_slot) + g * 16 : 0;
-    int value_lane[4];
+  // Takes in the tile's 32 tokens from `x`; `cut`: not every row sees all of
+  // them, and the values are clean; `seen`: those inside the request and on a
+  // page of the cache. One path, with little beside it that touches the sums:
+  // where several meet, the compiler keeps the sums in several places.
+  __device__ __forceinline__ void step(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
+                                       const char *tk, const char *tv, int lane_) {
+    constexpr float kBias = weight_bias<T>();
+    const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
+    f32x4 s[RT][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      value_lane[i] = FAST ? (4 * g + i) * static_cast<int>(a.value_slot) + c * E * CELL : 0;
-    const int value_dim = c * E < a.dim ? c * E : 0; // dims past the head's: any of its bytes
-
-    // Where the 32 tokens from `x` lie. FAST: pages hold whole tiles of 16
-    // tokens, so a tile's page is the same for all lanes; else lane l knows
-    // token l's. `seen`: tokens inside the request and on a page of the cache.
-    struct Where {
-      const char *k[2], *v[2];
-      int64_t k_off, v_off;
-      uint32_t seen;
-    };
-    auto find = [&](int64_t x) {
-      Where w;
-      w.seen = 0u;
-      if constexpr (FAST) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int64_t x0 = x + t * 16;
-          const int n = static_cast<int>(min(max(length - x0, int64_t{0}), int64_t{16}));
-          int id = 0;
-          uint32_t off = 0;
-          if (n > 0) {
-            const uint32_t p = fdiv(static_cast<uint32_t>(x0), a.page);
-            off = static_cast<uint32_t>(x0) - p * a.page.d;
-            id = uniform(table[p]);
-            if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages))
-              w.seen |= ((1u << n) - 1u) << (16 * t);
-            else
-              id = 0;
-          }
-          w.k[t] = keys + id * a.key_page + off * a.key_slot;
-          w.v[t] = values + id * a.value_page + off * a.value_slot;
-        }
-      } else {
-        const int64_t x0 = x + (lane & 31);
-        w.k_off = w.v_off = 0;
-        bool ok = x0 < length;
-        if (ok) {
-          const uint32_t p = fdiv(static_cast<uint32_t>(x0), a.page);
-          const uint32_t off = static_cast<uint32_t>(x0) - p * a.page.d;
-          const int id = table[p];
-          ok = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages);
-          if (ok) {
-            w.k_off = id * a.key_page + off * a.key_slot;
-            w.v_off = id * a.value_page + off * a.value_slot;
-          }
-        }
-        w.seen = static_cast<uint32_t>(__ballot(ok));
-      }
-      return w;
-    };
-    auto load_keys = [&](const Where &w, u32x4 (&k)[2][KS]) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const char *p = FAST ? w.k[t] + key_lane : keys + __shfl(w.k_off, t * 16 + c);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          if constexpr (FAST) {
-            k[t][s] = load<u32x4>(p + s * 64);
-          } else {
-            const int d = s * 4 * KB + g * KB;
-            if (d + KB <= a.dim) {
-              k[t][s] = load<u32x4>(p + d * CELL);
-            } else { // past the head's end (an int8 head may end inside a load)
-              k[t][s] = u32x4{0u, 0u, 0u, 0u};
-              if (I8 && d < a.dim) {
-                const u32x2 h = load<u32x2>(p + d);
-                k[t][s].x = h.x;
-                k[t][s].y = h.y;
-              }
-            }
-          }
-        }
-      }
-    };
-    auto load_values = [&](const Where &w, uint32_t (&v)[8][VW]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const char *p = FAST ? w.v[i >> 2] + value_lane[i & 3]
-                             : values + __shfl(w.v_off, (i >> 2) * 16 + 4 * g + (i & 3)) + value_dim * CELL;
-        if constexpr (VW == 1) {
-          v[i][0] = load<uint32_t>(p);
-        } else if constexpr (VW == 2) {
-          const u32x2 h = load<u32x2>(p);
-          v[i][0] = h.x;
-          v[i][1] = h.y;
-        } else {
-          // a head of fewer than DP dims may end inside a lane's sixteen
-          const bool in = FAST || value_dim + 8 < a.dim;
-          if (I8 && !in) {
-            const u32x2 h = load<u32x2>(p);
-            v[i][0] = h.x;
-            v[i][1] = h.y;
-            v[i][2] = v[i][3] = 0u;
-            continue;
-          }
-#pragma unroll
-          for (int n = 0; n < VW; n += 4) {
-            const u32x4 h = load<u32x4>(p + (in ? n * 4 : 0));
-            v[i][n] = h.x;
-            v[i][n + 1] = h.y;
-            v[i][n + 2] = h.z;
-            v[i][n + 3] = h.w;
-          }
-        }
-      }
-    };
-    // The values of the lane's eight tokens at its dim e, as an operand.
-    auto operand = [&](const uint32_t (&v)[8][VW], auto ec) {
-      constexpr int e = decltype(ec)::value;
-      u32x4 o;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        if constexpr (I8)
-          o[p] = pair8<T, e & 3, e & 3>(v[2 * p][e >> 2], v[2 * p + 1][e >> 2]);
-        else
-          o[p] = __builtin_amdgcn_perm(v[2 * p + 1][e >> 1], v[2 * p][e >> 1],
-                                       e & 1 ? 0x07060302u : 0x05040100u);
-      }
-      return o;
-    };
-
-    auto step = [&](int64_t x, const Where &w, const u32x4 (&k)[2][KS], uint32_t (&v)[8][VW]) {
-      f32x4 s[RT][2];
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-        s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        s[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < QS; ++i) {
-          u32x4 ka;
-          if constexpr (I8)
-            ka = widen8<T>(k[n][i >> 1][(i & 1) * 2], k[n][i >> 1][(i & 1) * 2 + 1]);
-          else
-            ka = k[n][i];
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-            s[t][n] = mfma<T>(ka, q[t][i], s[t][n]);
-        }
-
-      // what a row sees of these tokens, as bits
-      const bool cut = w.seen != 0xffffffffu || x + kStep > cached;
-      uint32_t bits[RT];
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-        bits[t] = 0xffffffffu;
-      bool odd = false; // a value that is not finite, in tokens that not every row sees
-      if (cut) {
-        const int64_t d = x - cached; // the first token's place among the new ones
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          if (d + kStep > 0) {
-            if (a.mask) {
-              const int64_t from = d > 0 ? d : 0;
-              const int word = static_cast<int>(from >> 6), sh = static_cast<int>(from & 63);
-              uint64_t m = 0;
-              if (t * 16 + c < rows) {
-                const int64_t *mp = a.mask + (start + static_cast<int64_t>(row_j[t])) * a.words;
-                if (word < a.words)
-                  m = static_cast<uint64_t>(mp[word]) >> sh;
-                if (sh > 32 && word + 1 < a.words)
-                  m |= static_cast<uint64_t>(mp[word + 1]) << (64 - sh);
-              }
-              const int old = d < 0 ? static_cast<int>(-d) : 0; // cached tokens of the step
-              bits[t] = static_cast<uint32_t>(m << old) | ((1u << old) - 1u);
-            } else {
-              const int64_t n = row_j[t] - d + 1;
-              bits[t] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-            }
-          }
-          bits[t] &= w.seen;
-        }
-        // tokens that no row may read hold anything: out of the products
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool in = w.seen >> ((i >> 2) * 16 + 4 * g + (i & 3)) & 1u;
-#pragma unroll
-          for (int n = 0; n < VW; ++n)
-            v[i][n] = in ? v[i][n] : 0u;
-        }
-        if constexpr (!I8) {
-          constexpr uint32_t kExp = T == kF16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int n = 0; n < VW; ++n)
-              odd |= (v[i][n] & kExp) == kExp || (v[i][n] >> 16 & kExp) == kExp;
-          odd = __any(odd);
-        }
+      for (int i = 0; i < QS; ++i) {
+        const u32x4 k = *reinterpret_cast<const u32x4 *>(tk + piece<DP>(n * 16 + c, i * 4 + g));
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!(bits[t] >> (n * 16 + 4 * g + i) & 1u))
-                s[t][n][i] = -__builtin_inff();
+          s[t][n] = mfma<T>(k, q[t][i], s[t][n]);
       }
-
+    }
+    if (__builtin_expect(cut, 0)) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        float most = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                           fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-        most = max_over_groups(most) * scale;
-        if (__any(most > top[t] + (kBias + kSlack))) {
-          const float next = fmaxf(top[t], most - kBias);
-          const float shrink = __builtin_amdgcn_exp2f(top[t] - next);
-          top[t] = next;
-          weight[t] *= shrink;
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            acc[t][e] *= shrink;
-        }
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(s[t][i >> 2][i & 3] * scale - top[t]);
-          weight[t] += p[i];
-        }
-        const u32x4 pb = {pack16<T>(p[0], p[1]), pack16<T>(p[2], p[3]), pack16<T>(p[4], p[5]),
-                          pack16<T>(p[6], p[7])};
-        if (!odd) {
-          add_values<T, E>(acc[t], pb, operand, v);
-        } else {
-          // A product with a weight of zero would carry the value over: row by
-          // row, without the tokens that the row does not see.
-#pragma clang loop unroll(disable)
-          for (int n = 0; n < 16; ++n) {
-            // keeps the operands of all sixteen rounds from being made at once
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-              for (int m = 0; m < VW; ++m)
-                asm volatile("" : "+v"(v[i][m]));
-            const uint32_t mine = __shfl(bits[t], n);
-            u32x4 sees;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t two = mine >> ((i >> 1) * 16 + 4 * g + (i & 1) * 2);
-              sees[i] = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-            }
-            add_row<T, E>(acc[t], pb, operand, v, sees, c == n);
-          }
-        }
-      }
-    };
-
-    // ---- the tokens of this run: the next step's keys are on their way
-    // while this one's are used
-    const int64_t x_end = min(s1 * kUnit, length);
-    int64_t x = s0 * kUnit + wave * kStep;
-    if (x < x_end) {
-      Where w = find(x);
-      u32x4 k[2][KS];
-      load_keys(w, k);
-      for (;;) {
-        uint32_t v[8][VW];
-        load_values(w, v);
-        const int64_t next = x + kUnit;
-        Where wn = w;
-        u32x4 kn[2][KS];
-        if (next < x_end) {
-          wn = find(next);
-          load_keys(wn, kn);
-        }
-        step(x, w, k, v);
-        if (next >= x_end)
-          break;
-        x = next;
-        w = wn;
+        const uint32_t bits = seen & row_sees(a, it, row0 + t * 16 + c, x);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
-            k[n][s] = kn[n][s];
+          for (int i = 0; i < 4; ++i)
+            if (!(bits >> (n * 16 + 4 * g + i) & 1u))
+              s[t][n][i] = -__builtin_inff();
       }
     }
 
-    // ---- the four waves' sums
+    float most[RT];
+    bool above = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      weight[t] += __shfl_xor(weight[t], 16);
-      weight[t] += __shfl_xor(weight[t], 32);
-      if (g == 0) {
-        row_max[wave][t * 16 + c] = top[t];
-        row_sum[wave][t * 16 + c] = weight[t];
+      most[t] = s[t][0][0];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          most[t] = fmaxf(most[t], s[t][n][i]);
+      most[t] = max_over_groups(most[t]) * scale;
+      above |= most[t] > top[t] + (kBias + kSlack);
+    }
+    if (__builtin_expect(__any(above), 0)) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float next = fmaxf(top[t], most[t] - kBias);
+        const float shrink = __builtin_amdgcn_exp2f(top[t] - next);
+        top[t] = next;
+        sum[t] *= shrink;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          acc[t][e] *= shrink;
+      }
+    }
+
+    u32x4 weights[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(s[t][n][i] * scale - top[t]);
+          sum[t] += p[i];
+        }
+        weights[t][n * 2] = pack16<T>(p[0], p[1]);
+        weights[t][n * 2 + 1] = pack16<T>(p[2], p[3]);
+      }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const u32x4 v = values_at<DP>(tv, e, lane);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        acc[t][e] = mfma<T>(v, weights[t], acc[t][e]);
+    }
+  }
+
+  __device__ __forceinline__ float total(int t) const {
+    const float x = sum[t] + __shfl_xor(sum[t], 16);
+    return x + __shfl_xor(x, 32);
+  }
+
+  // Adds what clean() took out of the tiles at x0, x0 + pace, ... before x_end:
+  // values that are not finite, of tokens that some rows see, to those rows.
+  // Hardly ever; a dim at a time, from the cache.
+  __device__ void add_odd(const AttendArgs &a, const Item &it, int row0, int rows, int x0, int x_end, int pace, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const int32_t *table = a.table + it.b * a.table_row;
+#pragma clang loop unroll(disable)
+    for (int x = x0; x < x_end; x += pace) {
+      if (x + kTile <= it.cached)
+        continue;
+#pragma clang loop unroll(disable)
+      for (int y = x; y < min(x + kTile, it.length); ++y) {
+        const uint32_t at = fdiv(static_cast<uint32_t>(y), a.page), off = static_cast<uint32_t>(y) - at * a.page.d;
+        const int id = table[at];
+        if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages))
+          continue;
+        const char *k = a.keys + it.head * a.key_head + id * a.key_page + off * a.key_slot;
+        const char *v = a.values + it.head * a.value_head + id * a.value_page + off * a.value_slot;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const int p = row0 + t * 16 + c;
+          if (t * 16 + c >= rows || !(row_sees(a, it, p, x) >> (y - x) & 1u))
+            continue;
+          const uint32_t j = fdiv(static_cast<uint32_t>(p), a.group);
+          const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
+                                   (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
+          float score = 0.0f;
+#pragma clang loop unroll(disable)
+          for (int d = 0; d < a.dim; ++d)
+            score += widen16<T>(load<uint16_t>(src + d * 2)) * widen16<T>(load<uint16_t>(k + d * 2));
+          const float weight = __builtin_amdgcn_exp2f(score * scale - top[t]);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (e * 16 + 4 * g + i < a.dim) {
+                const uint32_t h = load<uint16_t>(v + (e * 16 + 4 * g + i) * 2);
+                acc[t][e][i] += finite16<T>(h) ? 0.0f : weight * widen16<T>(h);
+              }
+        }
+      }
+    }
+  }
+};
+
+// How a wave brings its tokens of a tile into shared memory: NT tokens from
+// `first`, of every tile.
+template <int T, bool I8, int DP, int SRC, int NT> struct Loader {
+  static constexpr int CELL = I8 ? 1 : 2;
+  static constexpr int LB = 16 / CELL;                     // dims of a lane's load
+  static constexpr int TL = DP / LB;                       // lanes of a token
+  static constexpr int TPI = 64 / TL;                      // tokens of a load
+  static constexpr int LOADS = NT > TPI ? NT / TPI : 1;
+  static constexpr bool EVEN = SRC != kStaged;             // pages of whole tiles of 16 tokens
+
+  const char *keys, *values;
+  const int32_t *table;
+  int64_t key_page, value_page;
+  uint32_t key_slot, value_slot;
+  int64_t key_slot64, value_slot64; // kStaged: of any size
+  int length, pages, first, token, dim, cell_at, head_dims;
+  bool full; // the head fills the tile's rows
+  FastDiv page;
+  bool has;    // the lane's dims are the head's (all, or eight of an int8 load's)
+  bool whole;  // all of them
+  u32x4 stage[2][SRC == kAsync ? 1 : LOADS];
+  uint32_t there; // loads that are a token's, by bit
+
+  __device__ __forceinline__ Loader(const AttendArgs &a, int lane, int first_) {
+    first = first_;
+    token = lane / TL;
+    dim = (lane % TL) * LB;
+    key_page = a.key_page;
+    key_slot = static_cast<uint32_t>(a.key_slot);
+    value_page = a.value_page;
+    value_slot = static_cast<uint32_t>(a.value_slot);
+    key_slot64 = a.key_slot;
+    value_slot64 = a.value_slot;
+    head_dims = a.dim;
+    full = a.dim == DP;
+    pages = a.pages;
+    page = a.page;
+    has = dim < a.dim && token < NT;
+    whole = dim + LB <= a.dim;
+    cell_at = has ? dim * CELL : 0;
+    there = 0u;
+  }
+  __device__ __forceinline__ void item(const AttendArgs &a, const Item &it) {
+    keys = a.keys + it.head * a.key_head;
+    values = a.values + it.head * a.value_head;
+    table = a.table + it.b * a.table_row;
+    length = it.length;
+  }
+
+  // What the table says of the 16 tokens from x0 (past the length: -1); EVEN.
+  // Nothing waits for it here.
+  __device__ __forceinline__ int entry(int x0) const {
+    return x0 < length ? scalar_load(table + fdiv(static_cast<uint32_t>(x0), page)) : -1;
+  }
+  __device__ __forceinline__ bool is_page(int id) const {
+    return static_cast<uint32_t>(id) < static_cast<uint32_t>(pages);
+  }
+  // Which of the 32 tokens from x are there, by their two entries; EVEN.
+  __device__ __forceinline__ uint32_t seen(int x, int id0, int id1) const {
+    const int n = max(length - x, 0);
+    const uint32_t in = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    return in & ((is_page(id0) ? 0xffffu : 0u) | (is_page(id1) ? 0xffff0000u : 0u));
+  }
+
+  // kAsync: the wave's tokens of the tile at x, whose 16-token entries are
+  // id0 and id1 (no page: the first one's tokens, which nothing will see).
+  __device__ __forceinline__ void send(int x, int id0, int id1, uint32_t to_k, uint32_t to_v) const {
+    constexpr int GROUPS = NT > 16 ? 2 : 1; // of 16 tokens
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h) {
+      const int t0 = GROUPS == 2 ? h * 16 : first; // the group's part's first token
+      const int id = t0 < 16 ? id0 : id1;
+      const uint32_t x0 = static_cast<uint32_t>(x) + t0;
+      const uint32_t off = is_page(id) ? x0 - fdiv(x0, page) * page.d : 0u;
+      const uint32_t at = is_page(id) ? id : 0u;
+      const char *k = keys + static_cast<uint64_t>(at) * key_page + static_cast<uint64_t>(off) * key_slot;
+      const char *v = values + static_cast<uint64_t>(at) * value_page + static_cast<uint64_t>(off) * value_slot;
+#pragma unroll
+      for (int i = 0; i < LOADS / GROUPS; ++i) {
+        const int t = t0 + i * TPI;
+        const int n = (dim / 8) ^ swap_of<DP>(t + token); // the piece that lies at this lane's place
+        const uint32_t ko = token * key_slot + n * 16, vo = token * value_slot + n * 16;
+        const char *ki = k + static_cast<uint64_t>(i * TPI) * key_slot, *vi = v + static_cast<uint64_t>(i * TPI) * value_slot;
+        if (full || n * 8 < head_dims) {
+          load_async(ki, ko, to_k + t * DP * 2);
+          load_async(vi, vo, to_v + t * DP * 2);
+        }
+      }
+    }
+  }
+
+  // Through registers: the wave's tokens of the tile at x.
+  __device__ __forceinline__ void fetch(int x) {
+    there = 0u;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t0 = first + i * TPI;
+      const int x0 = x + t0 + (EVEN ? 0 : token);
+      int64_t id = -1;
+      if constexpr (EVEN) {
+        id = entry(x + (t0 & ~15));
+      } else if (x0 < length && has) {
+        id = table[fdiv(static_cast<uint32_t>(x0), page)];
+      }
+      id = is_page(static_cast<int>(id)) ? id : -1;
+      if (id >= 0 && has && x + t0 + token < length)
+        there |= 1u << i;
+      const uint32_t off = id >= 0 ? static_cast<uint32_t>(x0) - fdiv(static_cast<uint32_t>(x0), page) * page.d : 0u;
+      id = id >= 0 ? id : 0; // none: the first page, and zeros in its place
+      const char *k = keys + id * key_page + off * key_slot64, *v = values + id * value_page + off * value_slot64;
+      if constexpr (EVEN) {
+        k += token * key_slot + cell_at;
+        v += token * value_slot + cell_at;
+      } else {
+        k += cell_at;
+        v += cell_at;
+      }
+      if (I8 && !whole) { // eight dims, or none
+        const u32x2 hk = load<u32x2>(k), hv = load<u32x2>(v);
+        stage[0][i] = u32x4{hk.x, hk.y, 0u, 0u};
+        stage[1][i] = u32x4{hv.x, hv.y, 0u, 0u};
+      } else {
+        stage[0][i] = load<u32x4>(k);
+        stage[1][i] = load<u32x4>(v);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(char *tk, char *tv) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t = first + i * TPI + token;
+      const bool in = there >> i & 1u;
+      if (NT >= TPI || token < NT)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          char *to = kv ? tv : tk;
+          const u32x4 b = in ? stage[kv][i] : u32x4{0u, 0u, 0u, 0u};
+          if constexpr (I8) {
+            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8)) = widen8<T>(b.x, b.y);
+            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8 + 1)) = widen8<T>(b.z, b.w);
+          } else {
+            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8)) = b;
+          }
+        }
+    }
+  }
+  // The wave's tokens that are there, by their place among its NT.
+  __device__ __forceinline__ uint32_t tokens_there() const {
+    uint32_t bits = 0u;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      uint64_t b = __ballot(dim == 0 && (there >> i & 1u)); // a lane of each token
+#pragma unroll
+      for (int t = 0; t < (TPI < NT ? TPI : NT); ++t)
+        bits |= static_cast<uint32_t>(b >> (t * TL) & 1u) << (i * TPI + t);
+    }
+    return bits;
+  }
+};
+
+// ---------------------------------------------------------- up to 16 rows
+
+template <int T, bool I8, int DP, int SRC>
+__global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1 : 2) void k_attend_turns(AttendArgs a) {
+  constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
+  constexpr int RING = SRC != kAsync ? 1 : DP == 64 ? 4 : 2; // tiles of a wave
+  constexpr int TILE = kTile * DP * 2;
+  using Load = Loader<T, I8, DP, SRC, kTile>;
+
+  __shared__ Schedule schedule;
+  __shared__ __attribute__((aligned(16))) char tiles[W][RING][2][TILE];
+  __shared__ float row_max[W][ROWS], row_sum[W][ROWS];
+  static_assert(sizeof(tiles) >= W * 16 * (DP + 4) * sizeof(float), "the waves' sums fit the tiles");
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  Load load(a, lane, 0);
+  Rows<T, DP, 1> r;
+  add_up<ROWS, UNIT>(a, schedule);
+  Run run = my_run(schedule);
+
+  while (run.unit < run.end) {
+    const Item it = take<ROWS, UNIT>(a, schedule, run);
+    const int row0 = it.tile * ROWS;
+    const int rows = it.fresh * static_cast<int>(a.group.d) - row0; // of this tile and later ones
+    load.item(a, it);
+    const int x_end = min(it.s1 * UNIT, it.length), x0 = it.s0 * UNIT + wave * kTile;
+    const int count = x0 < x_end ? (x_end - x0 + UNIT - 1) / UNIT : 0; // this wave's tiles
+    bool odd = false;
+    auto take_in = [&](int x, uint32_t seen, int slot) {
+      const bool mixed = x + kTile > it.cached, cut = seen != 0xffffffffu || mixed;
+      if (__builtin_expect(cut, 0))
+        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, mixed && !I8, lane);
+      r.step(a, it, row0, x, seen, cut, tiles[wave][slot][0], tiles[wave][slot][1], lane);
+    };
+
+    if constexpr (SRC == kAsync) {
+      if (a.dim < DP) // places past the head's dims: no load writes them
+        for (int i = lane * 16; i < RING * 2 * TILE; i += 64 * 16)
+          *reinterpret_cast<u32x4 *>(&tiles[wave][0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
+      shared_done();
+      int id0 = load.entry(x0), id1 = load.entry(x0 + 16); // of the next tile to send
+      uint32_t seen[RING];                                     // of the tiles on their way
+      int xs = x0;
+      const uint32_t at = place(tiles[wave][0][0]);
+      auto send = [&](int slot) {
+        load.send(xs, id0, id1, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        const uint32_t s = load.seen(xs, id0, id1);
+        xs += UNIT;
+        id0 = load.entry(xs);
+        id1 = load.entry(xs + 16);
+        return s;
+      };
+#pragma unroll
+      for (int i = 0; i < RING; ++i)
+        seen[i] = i < count ? send(i) : 0u;
+      r.start(a, it, row0, rows, a.scale, lane);
+      int x = x0;
+      int slot = 0;
+#pragma clang loop unroll(disable)
+      for (int n = 0; n < count; ++n, x += UNIT) {
+        if (n + RING <= count)
+          arrived<(RING - 1) * 2 * Load::LOADS>();
+        else
+          arrived<0>();
+        take_in(x, seen[0], slot);
+        shared_done(); // its place is free
+#pragma unroll
+        for (int i = 0; i + 1 < RING; ++i)
+          seen[i] = seen[i + 1];
+        if (n + RING < count)
+          seen[RING - 1] = send(slot);
+        slot = slot + 1 == RING ? 0 : slot + 1;
+      }
+    } else {
+      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
+      char *tk = tiles[wave][0][0], *tv = tiles[wave][0][1];
+      int x = x0;
+      if (count > 0)
+        load.fetch(x);
+      for (int n = 0; n < count; ++n, x += UNIT) {
+        load.put(tk, tv);
+        const uint32_t seen = load.tokens_there();
+        if (n + 1 < count)
+          load.fetch(x + UNIT);
+        take_in(x, seen, 0);
+      }
+    }
+
+    if (!I8 && __builtin_expect(odd, 0))
+      r.add_odd(a, it, row0, rows, x0, x_end, UNIT, lane);
+
+    // ---- the waves' sums, where their tiles were
+    float(*sums)[16][DP + 4] = reinterpret_cast<float(*)[16][DP + 4]>(&tiles[0][0][0][0]);
+    const float sum = r.total(0);
+    if (g == 0) {
+      row_max[wave][c] = r.top[0];
+      row_sum[wave][c] = sum;
+    }
+    __syncthreads();
+    {
+      float most = kNone;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        most = fmaxf(most, row_max[w][c]);
+      const float f = __builtin_amdgcn_exp2f(r.top[0] - most);
+      if (c < rows)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          *reinterpret_cast<f32x4 *>(&sums[wave][c][e * 16 + 4 * g]) = r.acc[0][e] * f;
+    }
+    __syncthreads();
+    constexpr int DIMS = 16 * DP / (64 * W); // of a thread: sixteen rows over the workgroup
+    const int i = tid / (DP / DIMS), d0 = (tid % (DP / DIMS)) * DIMS;
+    if (i < rows) {
+      float m = kNone, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        m = fmaxf(m, row_max[w][i]);
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        l += row_sum[w][i] * __builtin_amdgcn_exp2f(row_max[w][i] - m);
+      const bool all = it.s0 == 0 && it.s1 == it.units;
+      const uint32_t p = static_cast<uint32_t>(row0 + i);
+      const uint32_t j = fdiv(p, a.group);
+      const int64_t row = it.start + static_cast<int64_t>(j);
+      const int64_t qh = static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d);
+      const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + i;
+      const float f = finish(l, I8 ? a.value_scale[it.head] : 1.0f);
+#pragma unroll
+      for (int d = 0; d < DIMS; d += 4) {
+        f32x4 o = *reinterpret_cast<const f32x4 *>(&sums[0][i][d0 + d]);
+#pragma unroll
+        for (int w = 1; w < W; ++w)
+          o += *reinterpret_cast<const f32x4 *>(&sums[w][i][d0 + d]);
+        if (!all) {
+          *reinterpret_cast<f32x4 *>(a.partial + part * DP + d0 + d) = o;
+        } else if (d0 + d < a.dim) {
+          o *= f;
+          store(a.out + (row * a.out_row + qh * a.out_head + d0 + d) * 2,
+                u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
+        }
+      }
+      if (d0 == 0) {
+        if (!all) {
+          a.stats[part * 2] = m;
+          a.stats[part * 2 + 1] = l;
+        } else if (a.lse) {
+          a.lse[row * a.heads + qh] = log_sum(m, l);
+        }
       }
     }
     __syncthreads();
-    const bool whole = s0 == 0 && s1 == units;
-    const int64_t part = (wg * 2 + (s0 == 0 ? 1 : 0)) * ROWS;
+  }
+}
+
+// ---------------------------------------------------------- more rows
+
+template <int T, bool I8, int DP, int RT, int SRC>
+__global__ __launch_bounds__(64 * kSharedWaves, 2) void k_attend_shared(AttendArgs a) {
+  constexpr int W = kSharedWaves, ROWS = 16 * RT * W, E = DP / 16, UNIT = kSharedUnit;
+  constexpr int RING = SRC != kAsync || DP == 256 ? 2 : 4;
+  constexpr int TILE = kTile * DP * 2;
+  using Load = Loader<T, I8, DP, SRC, kTile / W>;
+
+  __shared__ Schedule schedule;
+  __shared__ __attribute__((aligned(16))) char tiles[RING][2][TILE];
+  __shared__ uint8_t tokens[2][W]; // kStaged: each wave's tokens that are there
+  __shared__ int odd;              // clean() found something
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  Load load(a, lane, wave * (kTile / W));
+  Rows<T, DP, RT> r;
+  add_up<ROWS, UNIT>(a, schedule);
+  Run run = my_run(schedule);
+  if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
+    for (int i = tid * 16; i < RING * 2 * TILE; i += 64 * W * 16)
+      *reinterpret_cast<u32x4 *>(&tiles[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
+
+  while (run.unit < run.end) {
+    const Item it = take<ROWS, UNIT>(a, schedule, run);
+    const int row0 = (it.tile * W + wave) * 16 * RT;                // the wave's first
+    const int rows = it.fresh * static_cast<int>(a.group.d) - row0; // and how many from there
+    load.item(a, it);
+    const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.length);
+    const int count = x0 < x_end ? (x_end - x0 + kTile - 1) / kTile : 0;
+    auto take_in = [&](int x, uint32_t seen, int slot) {
+      const bool mixed = x + kTile > it.cached, cut = seen != 0xffffffffu || mixed;
+      if (__builtin_expect(cut, 0)) {
+        if (clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, mixed && !I8, lane) && lane == 0)
+          odd = 1;
+        __syncthreads();
+      }
+      if (rows > 0) // the same for the whole wave
+        r.step(a, it, row0, x, seen, cut, tiles[slot][0], tiles[slot][1], lane);
+    };
+    __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
+    if (tid == 0)
+      odd = 0; // before the barrier of the first tile
+
+    if constexpr (SRC == kAsync) {
+      int id0 = load.entry(x0), id1 = load.entry(x0 + 16); // of the next tile to send
+      uint32_t seen[RING - 1];                                 // of the tiles on their way
+      int xs = x0;
+      const uint32_t at = place(tiles[0][0]);
+      auto send = [&](int slot) {
+        load.send(xs, id0, id1, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        const uint32_t s = load.seen(xs, id0, id1);
+        xs += kTile;
+        id0 = load.entry(xs);
+        id1 = load.entry(xs + 16);
+        return s;
+      };
+#pragma unroll
+      for (int i = 0; i < RING - 1; ++i)
+        seen[i] = i < count ? send(i) : 0u;
+      r.start(a, it, row0, rows, a.scale, lane);
+      int x = x0;
+      int slot = 0;
+#pragma clang loop unroll(disable)
+      for (int n = 0; n < count; ++n, x += kTile) {
+        // this wave's part of the tile has arrived, then everybody's; and
+        // everybody is done with the tile before, whose place the next takes
+        if (n + RING - 1 <= count)
+          arrived<(RING - 2) * 2 * Load::LOADS>();
+        else
+          arrived<0>();
+        __syncthreads();
+        const uint32_t now = seen[0];
+#pragma unroll
+        for (int i = 0; i + 1 < RING - 1; ++i)
+          seen[i] = seen[i + 1];
+        if (n + RING - 1 < count)
+          seen[RING - 2] = send(slot == 0 ? RING - 1 : slot - 1);
+        take_in(x, now, slot);
+        slot = slot + 1 == RING ? 0 : slot + 1;
+      }
+    } else {
+      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
+      int x = x0;
+      auto put = [&](int slot) {
+        load.put(tiles[slot][0], tiles[slot][1]);
+        const uint32_t t = load.tokens_there();
+        if (lane == 0)
+          tokens[slot][wave] = static_cast<uint8_t>(t);
+      };
+      if (count > 0) {
+        load.fetch(x);
+        put(0);
+      }
+      if (count > 1)
+        load.fetch(x + kTile);
+      for (int n = 0; n < count; ++n, x += kTile) {
+        const int slot = n & 1;
+        __syncthreads();
+        uint32_t seen = 0u;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          seen |= static_cast<uint32_t>(tokens[slot][w]) << (w * (kTile / W));
+        seen = static_cast<uint32_t>(uniform(static_cast<int>(seen)));
+        if (n + 1 < count)
+          put(slot ^ 1);
+        if (n + 2 < count)
+          load.fetch(x + 2 * kTile);
+        take_in(x, seen, slot);
+      }
+    }
+
+    __syncthreads();
+    if (!I8 && __builtin_expect(odd, 0))
+      r.add_odd(a, it, row0, rows, x0, x_end, kTile, lane);
+
+    // ---- every wave's rows are its own
+    const bool whole = it.s0 == 0 && it.s1 == it.units;
+    const int ln = anew(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      float most = kNone;
-      {
-        const int i = t * 16 + c;
+      const float sum = r.total(t);
+      if (t * 16 + c >= rows)
+        continue;
+      if (whole) {
+        const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
+        const uint32_t j = fdiv(p, a.group);
+        const int64_t row = it.start + static_cast<int64_t>(j);
+        const int64_t qh = static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d);
+        const float f = finish(sum, I8 ? a.value_scale[it.head] : 1.0f);
+        char *dst = a.out + (row * a.out_row + qh * a.out_head + 4 * g) * 2;
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w)
-          most = fmaxf(most, row_max[w][i]);
-        const float f = __builtin_amdgcn_exp2f(top[t] - most);
-        if (i < rows)
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4)
-#pragma unroll
-            for (int e = 0; e < E; e += 4)
-              *reinterpret_cast<f32x4 *>(&sums[wave][c][(4 * g + i4) * E + e]) =
-                  f32x4{acc[t][e][i4] * f, acc[t][e + 1][i4] * f, acc[t][e + 2][i4] * f,
-                        acc[t][e + 3][i4] * f};
-      }
-      __syncthreads();
-      {
-        const int r16 = tid >> 4, i = t * 16 + r16, d0 = (tid & 15) * E;
-        if (i < rows) {
-          float m = kNone, l = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kAttendWaves; ++w)
-            m = fmaxf(m, row_max[w][i]);
-#pragma unroll
-          for (int w = 0; w < kAttendWaves; ++w)
-            l += row_sum[w][i] * __builtin_amdgcn_exp2f(row_max[w][i] - m);
-          float o[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            o[e] = sums[0][r16][d0 + e];
-#pragma unroll
-            for (int w = 1; w < kAttendWaves; ++w)
-              o[e] += sums[w][r16][d0 + e];
+        for (int e = 0; e < E; ++e)
+          if (e * 16 + 4 * g < a.dim) {
+            const f32x4 o = r.acc[t][e] * f;
+            store(dst + e * 32, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
           }
-          if (whole) {
-            const uint32_t p = static_cast<uint32_t>(tile * ROWS + i);
-            const uint32_t j = fdiv(p, a.group);
-            const int64_t row = start + static_cast<int64_t>(j);
-            const int64_t qh = static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d);
-            const float f = l > 0.0f ? (I8 ? a.value_scale[head] : 1.0f) / l : l == 0.0f ? 0.0f : l;
-            char *dst = a.out + (row * a.out_row + qh * a.out_head + d0) * 2;
+        if (a.lse && g == 0)
+          a.lse[row * a.heads + qh] = log_sum(r.top[t], sum);
+      } else {
+        const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
+        float *dst = a.partial + part * DP + 4 * g;
 #pragma unroll
-            for (int e = 0; e < E; e += 4)
-              if (d0 + e < a.dim)
-                store(dst + e * 2, u32x2{pack16<T>(o[e] * f, o[e + 1] * f), pack16<T>(o[e + 2] * f, o[e + 3] * f)});
-            if (a.lse && d0 == 0)
-              a.lse[row * a.heads + qh] =
-                  l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.693147180559945309f;
-          } else {
-            float *dst = a.partial + (part + i) * DP + d0;
-#pragma unroll
-            for (int e = 0; e < E; e += 4)
-              *reinterpret_cast<f32x4 *>(dst + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
-            if (d0 == 0) {
-              a.stats[(part + i) * 2] = m;
-              a.stats[(part + i) * 2 + 1] = l;
-            }
-          }
+        for (int e = 0; e < E; ++e)
+          *reinterpret_cast<f32x4 *>(dst + e * 16) = r.acc[t][e];
+        if (g == 0) {
+          a.stats[part * 2] = r.top[t];
+          a.stats[part * 2 + 1] = sum;
         }
       }
-      __syncthreads();
     }
   }
 }
@@ -682,9 +1066,8 @@ __global__ __launch_bounds__(kScan, RT <= 2 && DP <= 128 ? 2 : 1) void k_attend(
 // The rows of items that lie in several workgroups' runs: their partial sums,
 // added up; and zeros for the rows of no request. A wave takes an output row at
 // a time, a column of blocks the rows of a request.
-template <int T, bool I8, int DP, int RT>
+template <int T, bool I8, int DP, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
-  constexpr int ROWS = 16 * RT;
   constexpr int N = DP / 64; // dims of a lane
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int b = blockIdx.x;
@@ -702,7 +1085,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     }
     return;
   }
-  const Request r = attend_request<ROWS>(a, b);
+  const Request r = attend_request<ROWS, UNIT>(a, b);
   const int64_t total = a.schedule[a.requests], first = a.schedule[b];
   const int64_t per = (total + a.workgroups - 1) / a.workgroups;
   const int64_t count = static_cast<int64_t>(r.fresh) * a.heads;
@@ -737,7 +1120,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
       for (int n = 0; n < N; ++n)
         out[n] += a.partial[k * DP + lane * N + n] * f;
     }
-    const float f = sum > 0.0f ? (I8 ? a.value_scale[head] : 1.0f) / sum : sum == 0.0f ? 0.0f : sum;
+    const float f = finish(sum, I8 ? a.value_scale[head] : 1.0f);
     const int64_t orow = r.start + static_cast<int64_t>(j);
     char *dst = a.out + (orow * a.out_row + qh * a.out_head + lane * N) * 2;
     if (lane * N < a.dim) {
@@ -750,50 +1133,56 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
       }
     }
     if (a.lse && lane == 0)
-      a.lse[orow * a.heads + qh] =
-          sum == 0.0f ? -__builtin_inff() : (most + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+      a.lse[orow * a.heads + qh] = log_sum(most, sum);
   }
 }
 
-template <int T, bool I8, int DP, int RT>
-hipError_t attend_start(const AttendArgs &args, const AttendPlan &p, hipStream_t s) {
+template <int T, bool I8, int DP, int ROWS, int UNIT>
+hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args, const AttendPlan &p,
+                        hipStream_t s) {
   AttendArgs a = args;
   void *pa[] = {&a};
-  const void *k = p.fast ? reinterpret_cast<const void *>(k_attend<T, I8, DP, RT, true>)
-                         : reinterpret_cast<const void *>(k_attend<T, I8, DP, RT, false>);
-  hipError_t e = hipLaunchKernel(k, dim3(static_cast<uint32_t>(p.workgroups)), dim3(kScan), pa, 0, s);
+  hipError_t e = hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(p.workgroups)),
+                                 dim3(static_cast<uint32_t>(threads)), pa, 0, s);
   if (e != hipSuccess)
     return e;
   // a wave for every output row of an even batch, within 2^16 blocks a request
   const int64_t rows = (static_cast<int64_t>(a.rows) * a.heads + a.requests - 1) / a.requests;
   const int64_t y = std::min<int64_t>((rows + 3) / 4, 65535);
-  return hipLaunchKernel(reinterpret_cast<const void *>(k_attend_join<T, I8, DP, RT>),
+  return hipLaunchKernel(reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT>),
                          dim3(static_cast<uint32_t>(a.requests) + 1, static_cast<uint32_t>(y)), dim3(256), pa, 0, s);
 }
 
+template <int T, bool I8, int DP, int SRC>
+hipError_t attend_rows(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  if (p.rows == 16)
+    return attend_start<T, I8, DP, 16, turn_unit(DP)>(reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, SRC>),
+                                                      64 * turn_waves(DP), a, p, s);
+  if constexpr (DP < 256) // 32 rows of a wave with a head of 256 would not fit its registers
+    if (p.rows == 128)
+      return attend_start<T, I8, DP, 128, kSharedUnit>(
+          reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, 2, SRC>), 64 * kSharedWaves, a, p, s);
+  return attend_start<T, I8, DP, 64, kSharedUnit>(reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, 1, SRC>),
+                                                  64 * kSharedWaves, a, p, s);
+}
+
 template <int T, bool I8, int DP>
-hipError_t attend_tiles(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  switch (p.row_tiles) {
-  case 1:
-    return attend_start<T, I8, DP, 1>(a, p, s);
-  case 2:
-    return attend_start<T, I8, DP, 2>(a, p, s);
-  default:
-    if constexpr (DP <= 128)
-      return attend_start<T, I8, DP, 4>(a, p, s);
-    return hipErrorInvalidValue;
-  }
+hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  if constexpr (I8)
+    return p.even ? attend_rows<T, I8, DP, kStagedEven>(a, p, s) : attend_rows<T, I8, DP, kStaged>(a, p, s);
+  else
+    return p.even && p.aligned ? attend_rows<T, I8, DP, kAsync>(a, p, s) : attend_rows<T, I8, DP, kStaged>(a, p, s);
 }
 
 template <int T, bool I8>
 hipError_t attend_width(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   switch (p.width) {
   case 64:
-    return attend_tiles<T, I8, 64>(a, p, s);
+    return attend_source<T, I8, 64>(a, p, s);
   case 128:
-    return attend_tiles<T, I8, 128>(a, p, s);
+    return attend_source<T, I8, 128>(a, p, s);
   default:
-    return attend_tiles<T, I8, 256>(a, p, s);
+    return attend_source<T, I8, 256>(a, p, s);
   }
 }
 
