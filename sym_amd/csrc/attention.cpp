@@ -234,7 +234,9 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
     plan.even = false;
   const int64_t at = reinterpret_cast<int64_t>(a.keys) | reinterpret_cast<int64_t>(a.values) | a.key_page | a.key_slot |
                      a.key_head | a.value_page | a.value_slot | a.value_head;
-  plan.aligned = at % 16 == 0;
+  plan.async = plan.even && (at | dim * (i8 ? 1 : 2)) % 16 == 0;
+  if (plan.rows == 16)
+    plan.workgroups = turn_workgroups(plan.width, i8, plan.async);
   a.workgroups = plan.workgroups;
   return a;
 }
@@ -248,14 +250,14 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
   p.even = page % 16 == 0;
   // query rows of a key head in an even batch
   const int64_t q = requests > 0 ? (rows + requests - 1) / requests * group : 0;
-  p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : 128;
-  p.workgroups = 512;
+  p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : q <= 128 ? 128 : 256;
+  p.workgroups = p.rows == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;
   (void)kv_heads;
   return p;
 }
 
 size_t attend_workspace(const AttendPlan &p, int64_t requests) {
-  const size_t rows = static_cast<size_t>(p.workgroups) * 2 * static_cast<size_t>(p.rows);
+  const size_t rows = static_cast<size_t>(kMostWorkgroups) * 2 * static_cast<size_t>(p.rows);
   return rows * static_cast<size_t>(p.width + 2) * sizeof(float) +
          (static_cast<size_t>(requests) + 1) * sizeof(int64_t);
 }
@@ -414,7 +416,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
       if (args->workspace_bytes < 0 || static_cast<size_t>(args->workspace_bytes) < want || !args->workspace)
         throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(args->workspace_bytes) +
                                                        " bytes, the call takes " + std::to_string(want));
-      const size_t rows = static_cast<size_t>(plan.workgroups) * 2 * static_cast<size_t>(plan.rows);
+      const size_t rows = static_cast<size_t>(relx::kMostWorkgroups) * 2 * static_cast<size_t>(plan.rows);
       relx::need(reinterpret_cast<uintptr_t>(args->workspace) % 16 == 0, "attention: workspace alignment");
       a.partial = static_cast<float *>(args->workspace);
       a.stats = a.partial + rows * static_cast<size_t>(plan.width);

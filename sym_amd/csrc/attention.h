@@ -98,11 +98,24 @@ struct AttendPlan {
   int width;      // head size, rounded up to a kernel's
   int rows;       // query rows of an item
   bool even;      // pages of whole tiles of 16 tokens
-  bool aligned;   // cache rows at 16-byte addresses
+  bool async;     // and rows of whole 16-byte pieces at 16-byte addresses
   int workgroups;
 };
+constexpr int kMostWorkgroups = 512; // two to a compute unit
+
+// Waves that take turns, and workgroups of them that the card holds at once: a
+// ring of two tiles a wave, in 64 KiB (int8 heads of 128, say) or 128 KiB of a
+// compute unit's 160. More waves with less on its way each were slower: (64
+// requests of 2304 tokens on average, 8 key heads of 128, f16).
+constexpr int turn_waves(int width) { return width == 256 ? 2 : 4; }
+constexpr int turn_workgroups(int width, bool i8, bool async) {
+  const int ring = 2 * 2 * 32 * width * (i8 ? 1 : 2) * turn_waves(width);
+  return async ? (ring > 64 * 1024 ? kMostWorkgroups / 2 : kMostWorkgroups)
+               : width == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;
+}
 AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
                        int64_t page);
+// Bytes of a call's workspace, whatever its cache's addresses.
 size_t attend_workspace(const AttendPlan &p, int64_t requests);
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8,
                          hipStream_t s);

@@ -18,17 +18,17 @@
 // (ds_read_b64_tr_b16: four tokens of one dim from four lanes' rows).
 //
 // How tokens get there (Source):
-//   kAsync   16-bit caches whose pages hold whole tiles of 16 tokens, rows at
-//            16-byte addresses: loads that write shared memory themselves, a
-//            ring of tiles ahead
-//   kStaged  everything else: through registers, where int8 is widened and
-//            what is no token becomes zero
+//   kAsync   pages of whole tiles of 16 tokens and rows at 16-byte addresses:
+//            loads that write shared memory themselves, a ring of tiles ahead
+//   kStaged  everything else: through registers, where what is no token
+//            becomes zero
 // and who works on them:
 //   up to 16 query rows share a key head (decoding): bound by the cache's
 //     bytes. The waves of a workgroup take turns at the tiles, each with a ring
-//     of its own and no barrier, and add up at the end.
+//     of its own and no barrier, and add up at the end. int8 is widened in the
+//     registers.
 //   more (trees, chunks): the waves have rows of their own, 16 or 32 each, and
-//     share the tiles.
+//     share the tiles. int8 is widened on its way there, once for all of them.
 //
 // The work of a call is the list of its units of tokens over (request, key
 // head, tile of query rows), cut into equal runs, one per workgroup; an item
@@ -58,10 +58,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kScan = 128;    // runs of requests whose units a workgroup (of at least as many threads) adds up
 constexpr int kTile = 32;     // tokens of a tile
-constexpr int kSharedWaves = 4;
 constexpr int kSharedUnit = 64;
-// Waves that take turns: as many as their rings fit shared memory.
-constexpr int turn_waves(int dp) { return dp == 256 ? 2 : 4; }
 constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
 
 enum Source : int { kAsync, kStaged, kStagedEven };
@@ -101,6 +98,9 @@ template <int T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+
+// Keeps the scheduler from moving anything across.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // The same number, of which the compiler no longer knows what it is: what is
 // worked out from it in a loop stays there instead of filling registers outside.
@@ -330,15 +330,16 @@ __device__ __forceinline__ float log_sum(float top, float sum) {
 
 // ------------------------------------------------------------ tiles
 
-// Where the n-th 16-byte piece of a token's row lies in a tile ([kTile][DP] of
-// T): pieces are swapped by the token's number, so that sixteen lanes that read
-// the same piece of sixteen tokens, or all pieces of one, meet no bank twice.
-template <int DP> __device__ __forceinline__ int swap_of(int token) {
-  constexpr int P = DP / 8;
-  return P >= 16 ? token & 15 : (token >> 1) & (P - 1);
+// Where the n-th 16-byte piece of a token's row lies in a tile of kTile rows of
+// RB bytes: pieces are swapped by the token's number, so that sixteen lanes that
+// read the same piece of sixteen tokens, or all pieces of one, meet no bank
+// twice.
+template <int RB> __device__ __forceinline__ int swap_of(int token) {
+  constexpr int P = RB / 16;
+  return P >= 16 ? token & 15 : (token / (16 / P)) & (P - 1);
 }
-template <int DP> __device__ __forceinline__ int piece(int token, int n) {
-  return (token * (DP / 8) + (n ^ swap_of<DP>(token))) * 16;
+template <int RB> __device__ __forceinline__ int piece(int token, int n) {
+  return token * RB + (n ^ swap_of<RB>(token)) * 16;
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -357,6 +358,15 @@ __device__ __forceinline__ uint32_t place(const char *p) {
   return uniform(static_cast<int>(reinterpret_cast<uintptr_t>((lds_char *)const_cast<char *>(p))));
 }
 
+// Eight tokens of one int8 dim: lane i of sixteen gives the address of eight
+// dims of token i / 2, and gets dim i.
+__device__ __forceinline__ u32x2 read_transposed8(const char *p) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2 *at;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                       (at)(lds_char *)const_cast<char *>(p)));
+}
+
 // 16 bytes per lane from base + at into shared memory, lane after lane from
 // `to`. The compiler does not count it: arrived<N>() waits until at most the N
 // latest are on their way.
@@ -373,15 +383,44 @@ template <int N> __device__ __forceinline__ void arrived() {
 // Waits for the wave's own reads and writes of shared memory.
 __device__ __forceinline__ void shared_done() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
-// The values of a tile at the 16 dims from 16 e, as an operand: dim 16 e +
-// lane % 16 of the lane's eight tokens.
-template <int DP> __device__ __forceinline__ u32x4 values_at(const char *tv, int e, int lane) {
-  const int c = lane & 15, g = lane >> 4;
-  const int token = 4 * g + (c >> 2), half = (c & 3) >> 1, byte = (c & 1) * 8;
-  const u32x2 lo = read_transposed(tv + piece<DP>(token, e * 2 + half) + byte);
-  const u32x2 hi = read_transposed(tv + piece<DP>(token + 16, e * 2 + half) + byte);
-  return u32x4{lo.x, lo.y, hi.x, hi.y};
-}
+// A tile's values as operands: at(e) has dim 16 e + lane % 16 of the lane's eight
+// tokens. RAW: the tile holds int8. EARLY: all read at once, ahead of their use.
+template <int T, int DP, bool RAW, bool EARLY> struct Values {
+  static constexpr int E = DP / 16;
+  const char *tv;
+  int lane;
+  u32x2 lo[EARLY ? E : 1], hi[EARLY && !RAW ? E : 1];
+  __device__ __forceinline__ u32x2 part(int e, int tile) const {
+    const int c = lane & 15, g = lane >> 4;
+    if constexpr (RAW) {
+      const int token = 4 * g + ((c >> 1) & 3) + (c >> 3) * 16;
+      return read_transposed8(tv + piece<DP>(token, e) + (c & 1) * 8);
+    } else {
+      const int token = 4 * g + (c >> 2) + tile * 16, half = (c & 3) >> 1;
+      return read_transposed(tv + piece<DP * 2>(token, e * 2 + half) + (c & 1) * 8);
+    }
+  }
+  __device__ __forceinline__ Values(const char *tv_, int lane_) : tv(tv_), lane(lane_) {
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lo[e] = part(e, 0);
+        if constexpr (!RAW)
+          hi[e] = part(e, 1);
+      }
+      keep_order();
+    }
+  }
+  __device__ __forceinline__ u32x4 at(int e) const {
+    const u32x2 a = EARLY ? lo[e] : part(e, 0);
+    if constexpr (RAW) {
+      return widen8<T>(a.x, a.y);
+    } else {
+      const u32x2 b = EARLY ? hi[e] : part(e, 1);
+      return u32x4{a.x, a.y, b.x, b.y};
+    }
+  }
+};
 
 template <int T> __device__ __forceinline__ bool finite16(uint32_t h) {
   constexpr uint32_t kExp = T == kF16 ? 0x7c00u : 0x7f80u;
@@ -419,7 +458,7 @@ __device__ __forceinline__ bool clean(char *tv, int first, uint32_t seen, bool m
 }
 
 // A wave's query rows and their sums.
-template <int T, int DP, int RT> struct Rows {
+template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   static constexpr int E = DP / 16, QS = DP / 32;
   u32x4 q[RT][QS];
   float top[RT];     // reference maximum of a row's scaled scores
@@ -439,7 +478,8 @@ template <int T, int DP, int RT> struct Rows {
                                (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma unroll
       for (int s = 0; s < QS; ++s) {
-        const int d = s * 32 + g * 8;
+        // the dims of contraction step s: those of a lane's piece of a key
+        const int d = RAW ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
         q[t][s] = u32x4{0u, 0u, 0u, 0u};
         if (t * 16 + c < rows && d < a.dim)
           q[t][s] = load<u32x4>(src + d * 2);
@@ -468,6 +508,14 @@ template <int T, int DP, int RT> struct Rows {
     constexpr float kBias = weight_bias<T>();
     const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
     f32x4 s[RT][2];
+    constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
+    u32x4 k[2][KR];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < KR; ++i)
+        k[n][i] = *reinterpret_cast<const u32x4 *>(tk + piece<RAW ? DP : DP * 2>(n * 16 + c, i * 4 + g));
+    keep_order(); // all reads on their way before the first is waited for
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -475,12 +523,18 @@ template <int T, int DP, int RT> struct Rows {
         s[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < QS; ++i) {
-        const u32x4 k = *reinterpret_cast<const u32x4 *>(tk + piece<DP>(n * 16 + c, i * 4 + g));
+        u32x4 ki;
+        if constexpr (RAW)
+          ki = i & 1 ? widen8<T>(k[n][i >> 1].z, k[n][i >> 1].w) : widen8<T>(k[n][i >> 1].x, k[n][i >> 1].y);
+        else
+          ki = k[n][i];
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-          s[t][n] = mfma<T>(k, q[t][i], s[t][n]);
+          s[t][n] = mfma<T>(ki, q[t][i], s[t][n]);
       }
     }
+    // and (EARLY) the values', which arrive during the softmax
+    const Values<T, DP, RAW, EARLY> v(tv, lane);
     if (__builtin_expect(cut, 0)) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
@@ -536,10 +590,10 @@ template <int T, int DP, int RT> struct Rows {
       }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const u32x4 v = values_at<DP>(tv, e, lane);
+      const u32x4 ve = v.at(e);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-        acc[t][e] = mfma<T>(v, weights[t], acc[t][e]);
+        acc[t][e] = mfma<T>(ve, weights[t], acc[t][e]);
     }
   }
 
@@ -595,13 +649,14 @@ template <int T, int DP, int RT> struct Rows {
 
 // How a wave brings its tokens of a tile into shared memory: NT tokens from
 // `first`, of every tile.
-template <int T, bool I8, int DP, int SRC, int NT> struct Loader {
+template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
   static constexpr int CELL = I8 ? 1 : 2;
   static constexpr int LB = 16 / CELL;                     // dims of a lane's load
   static constexpr int TL = DP / LB;                       // lanes of a token
   static constexpr int TPI = 64 / TL;                      // tokens of a load
   static constexpr int LOADS = NT > TPI ? NT / TPI : 1;
   static constexpr bool EVEN = SRC != kStaged;             // pages of whole tiles of 16 tokens
+  static constexpr int RB = DP * (RAW ? 1 : 2);            // bytes of a token in the tile
 
   const char *keys, *values;
   const int32_t *table;
@@ -673,12 +728,12 @@ template <int T, bool I8, int DP, int SRC, int NT> struct Loader {
 #pragma unroll
       for (int i = 0; i < LOADS / GROUPS; ++i) {
         const int t = t0 + i * TPI;
-        const int n = (dim / 8) ^ swap_of<DP>(t + token); // the piece that lies at this lane's place
+        const int n = (dim / LB) ^ swap_of<RB>(t + token); // the piece that lies at this lane's place
         const uint32_t ko = token * key_slot + n * 16, vo = token * value_slot + n * 16;
         const char *ki = k + static_cast<uint64_t>(i * TPI) * key_slot, *vi = v + static_cast<uint64_t>(i * TPI) * value_slot;
-        if (full || n * 8 < head_dims) {
-          load_async(ki, ko, to_k + t * DP * 2);
-          load_async(vi, vo, to_v + t * DP * 2);
+        if ((NT >= TPI || token < NT) && (full || n * LB < head_dims)) {
+          load_async(ki, ko, to_k + t * RB);
+          load_async(vi, vo, to_v + t * RB);
         }
       }
     }
@@ -730,11 +785,11 @@ template <int T, bool I8, int DP, int SRC, int NT> struct Loader {
         for (int kv = 0; kv < 2; ++kv) {
           char *to = kv ? tv : tk;
           const u32x4 b = in ? stage[kv][i] : u32x4{0u, 0u, 0u, 0u};
-          if constexpr (I8) {
-            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8)) = widen8<T>(b.x, b.y);
-            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8 + 1)) = widen8<T>(b.z, b.w);
+          if constexpr (I8 && !RAW) {
+            *reinterpret_cast<u32x4 *>(to + piece<RB>(t, dim / 8)) = widen8<T>(b.x, b.y);
+            *reinterpret_cast<u32x4 *>(to + piece<RB>(t, dim / 8 + 1)) = widen8<T>(b.z, b.w);
           } else {
-            *reinterpret_cast<u32x4 *>(to + piece<DP>(t, dim / 8)) = b;
+            *reinterpret_cast<u32x4 *>(to + piece<RB>(t, dim / LB)) = b;
           }
         }
     }
@@ -756,21 +811,22 @@ template <int T, bool I8, int DP, int SRC, int NT> struct Loader {
 // ---------------------------------------------------------- up to 16 rows
 
 template <int T, bool I8, int DP, int SRC>
-__global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1 : 2) void k_attend_turns(AttendArgs a) {
+__global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC == kAsync) == kMostWorkgroups ? 2 : 1) void k_attend_turns(AttendArgs a) {
   constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
-  constexpr int RING = SRC != kAsync ? 1 : DP == 64 ? 4 : 2; // tiles of a wave
-  constexpr int TILE = kTile * DP * 2;
-  using Load = Loader<T, I8, DP, SRC, kTile>;
+  constexpr int TILE = kTile * DP * (I8 ? 1 : 2);
+  constexpr int RING = SRC == kAsync ? 2 : 1; // tiles of a wave
+  using Load = Loader<T, I8, DP, SRC, kTile, I8>;
 
   __shared__ Schedule schedule;
-  __shared__ __attribute__((aligned(16))) char tiles[W][RING][2][TILE];
+  constexpr int SUMS = W * 16 * (DP + 4) * sizeof(float); // the waves', at the end
+  __shared__ __attribute__((aligned(16))) char room[W * RING * 2 * TILE > SUMS ? W * RING * 2 * TILE : SUMS];
+  char(*tiles)[RING][2][TILE] = reinterpret_cast<char(*)[RING][2][TILE]>(room);
   __shared__ float row_max[W][ROWS], row_sum[W][ROWS];
-  static_assert(sizeof(tiles) >= W * 16 * (DP + 4) * sizeof(float), "the waves' sums fit the tiles");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   Load load(a, lane, 0);
-  Rows<T, DP, 1> r;
+  Rows<T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
   add_up<ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
 
@@ -784,8 +840,8 @@ __global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1
     bool odd = false;
     auto take_in = [&](int x, uint32_t seen, int slot) {
       const bool mixed = x + kTile > it.cached, cut = seen != 0xffffffffu || mixed;
-      if (__builtin_expect(cut, 0))
-        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, mixed && !I8, lane);
+      if (!I8 && __builtin_expect(cut, 0)) // what int8 holds is finite
+        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, mixed, lane);
       r.step(a, it, row0, x, seen, cut, tiles[wave][slot][0], tiles[wave][slot][1], lane);
     };
 
@@ -809,7 +865,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1
 #pragma unroll
       for (int i = 0; i < RING; ++i)
         seen[i] = i < count ? send(i) : 0u;
-      r.start(a, it, row0, rows, a.scale, lane);
+      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
       int x = x0;
       int slot = 0;
 #pragma clang loop unroll(disable)
@@ -846,7 +902,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1
       r.add_odd(a, it, row0, rows, x0, x_end, UNIT, lane);
 
     // ---- the waves' sums, where their tiles were
-    float(*sums)[16][DP + 4] = reinterpret_cast<float(*)[16][DP + 4]>(&tiles[0][0][0][0]);
+    float(*sums)[16][DP + 4] = reinterpret_cast<float(*)[16][DP + 4]>(room);
     const float sum = r.total(0);
     if (g == 0) {
       row_max[wave][c] = r.top[0];
@@ -911,12 +967,13 @@ __global__ __launch_bounds__(64 * turn_waves(DP), SRC == kAsync || DP == 256 ? 1
 
 // ---------------------------------------------------------- more rows
 
-template <int T, bool I8, int DP, int RT, int SRC>
-__global__ __launch_bounds__(64 * kSharedWaves, 2) void k_attend_shared(AttendArgs a) {
-  constexpr int W = kSharedWaves, ROWS = 16 * RT * W, E = DP / 16, UNIT = kSharedUnit;
-  constexpr int RING = SRC != kAsync || DP == 256 ? 2 : 4;
+template <int T, bool I8, int DP, int RT, int W, int SRC>
+__global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
+  constexpr int ROWS = 16 * RT * W, E = DP / 16, UNIT = kSharedUnit;
   constexpr int TILE = kTile * DP * 2;
-  using Load = Loader<T, I8, DP, SRC, kTile / W>;
+  // tiles at a time: 64 KiB for each four waves
+  constexpr int RING = SRC != kAsync ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
+  using Load = Loader<T, I8, DP, SRC, kTile / W, false>;
 
   __shared__ Schedule schedule;
   __shared__ __attribute__((aligned(16))) char tiles[RING][2][TILE];
@@ -925,7 +982,7 @@ __global__ __launch_bounds__(64 * kSharedWaves, 2) void k_attend_shared(AttendAr
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Load load(a, lane, wave * (kTile / W));
-  Rows<T, DP, RT> r;
+  Rows<T, DP, RT, false, DP <= 128 && (I8 || SRC == kAsync)> r; // where the registers hold them
   add_up<ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
   if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
@@ -1153,25 +1210,35 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
                          dim3(static_cast<uint32_t>(a.requests) + 1, static_cast<uint32_t>(y)), dim3(256), pa, 0, s);
 }
 
+template <int T, bool I8, int DP, int RT, int W, int SRC>
+hipError_t attend_start_shared(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  return attend_start<T, I8, DP, 16 * RT * W, kSharedUnit>(
+      reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, RT, W, SRC>), 64 * W, a, p, s);
+}
+
 template <int T, bool I8, int DP, int SRC>
-hipError_t attend_rows(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  if (p.rows == 16)
-    return attend_start<T, I8, DP, 16, turn_unit(DP)>(reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, SRC>),
-                                                      64 * turn_waves(DP), a, p, s);
-  if constexpr (DP < 256) // 32 rows of a wave with a head of 256 would not fit its registers
+hipError_t attend_shared(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  if constexpr (DP < 256) { // 32 rows of a wave with a head of 256 would not fit its registers
     if (p.rows == 128)
-      return attend_start<T, I8, DP, 128, kSharedUnit>(
-          reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, 2, SRC>), 64 * kSharedWaves, a, p, s);
-  return attend_start<T, I8, DP, 64, kSharedUnit>(reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, 1, SRC>),
-                                                  64 * kSharedWaves, a, p, s);
+      return attend_start_shared<T, I8, DP, 2, 4, SRC>(a, p, s);
+    if (p.rows == 256)
+      return attend_start_shared<T, I8, DP, 2, 8, SRC>(a, p, s);
+  }
+  return attend_start_shared<T, I8, DP, 1, 4, SRC>(a, p, s);
 }
 
 template <int T, bool I8, int DP>
 hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  if (p.rows == 16)
+    return attend_start<T, I8, DP, 16, turn_unit(DP)>(
+        p.async ? reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, kAsync>)
+                : reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, kStaged>),
+        64 * turn_waves(DP), a, p, s);
+  // int8 is widened once for all waves, on its way through registers
   if constexpr (I8)
-    return p.even ? attend_rows<T, I8, DP, kStagedEven>(a, p, s) : attend_rows<T, I8, DP, kStaged>(a, p, s);
+    return p.even ? attend_shared<T, I8, DP, kStagedEven>(a, p, s) : attend_shared<T, I8, DP, kStaged>(a, p, s);
   else
-    return p.even && p.aligned ? attend_rows<T, I8, DP, kAsync>(a, p, s) : attend_rows<T, I8, DP, kStaged>(a, p, s);
+    return p.async ? attend_shared<T, I8, DP, kAsync>(a, p, s) : attend_shared<T, I8, DP, kStaged>(a, p, s);
 }
 
 template <int T, bool I8>
