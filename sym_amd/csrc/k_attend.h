@@ -499,15 +499,15 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
         asm volatile("" : "+v"(q[t][s]));
   }
 
-  // Takes in the tile's 32 tokens from `x`; `cut`: not every row sees all of
-  // them, and the values are clean; `seen`: those inside the request and on a
-  // page of the cache. One path, with little beside it that touches the sums:
-  // where several meet, the compiler keeps the sums in several places.
-  __device__ __forceinline__ void step(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
-                                       const char *tk, const char *tv, int lane_) {
-    constexpr float kBias = weight_bias<T>();
+  // Taking in a tile's 32 tokens from `x`, in three parts. `cut`: not every row
+  // sees all of them, and the values are clean; `seen`: those inside the request
+  // and on a page of the cache. One path, with little beside it that touches
+  // the sums: where several meet, the compiler keeps the sums in several places.
+  f32x4 s[RT][2];     // scores, unscaled
+  u32x4 weights[RT];
+
+  __device__ __forceinline__ void scores(const char *tk, int lane_) {
     const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
-    f32x4 s[RT][2];
     constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
     u32x4 k[2][KR];
 #pragma unroll
@@ -533,9 +533,13 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
           s[t][n] = mfma<T>(ki, q[t][i], s[t][n]);
       }
     }
-    // and (EARLY) the values', which arrive during the softmax
-    const Values<T, DP, RAW, EARLY> v(tv, lane);
+  }
+
+  __device__ __forceinline__ void soften(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
+                                         int lane_) {
+    constexpr float kBias = weight_bias<T>();
     if (__builtin_expect(cut, 0)) {
+      const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         const uint32_t bits = seen & row_sees(a, it, row0 + t * 16 + c, x);
@@ -574,7 +578,6 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       }
     }
 
-    u32x4 weights[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -588,6 +591,9 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
         weights[t][n * 2] = pack16<T>(p[0], p[1]);
         weights[t][n * 2 + 1] = pack16<T>(p[2], p[3]);
       }
+  }
+
+  __device__ __forceinline__ void add(const Values<T, DP, RAW, EARLY> &v) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const u32x4 ve = v.at(e);
@@ -595,6 +601,14 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       for (int t = 0; t < RT; ++t)
         acc[t][e] = mfma<T>(ve, weights[t], acc[t][e]);
     }
+  }
+
+  __device__ __forceinline__ void step(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
+                                       const char *tk, const char *tv, int lane) {
+    scores(tk, lane);
+    const Values<T, DP, RAW, EARLY> v(tv, anew(lane)); // EARLY: they arrive during the softmax
+    soften(a, it, row0, x, seen, cut, lane);
+    add(v);
   }
 
   __device__ __forceinline__ float total(int t) const {
@@ -978,41 +992,45 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   __shared__ Schedule schedule;
   __shared__ __attribute__((aligned(16))) char tiles[RING][2][TILE];
   __shared__ uint8_t tokens[2][W]; // kStaged: each wave's tokens that are there
-  __shared__ int odd;              // clean() found something
+  __shared__ int odd_of[2];        // clean() found something, in every other item
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Load load(a, lane, wave * (kTile / W));
-  Rows<T, DP, RT, false, DP <= 128 && (I8 || SRC == kAsync)> r; // where the registers hold them
+  constexpr bool EARLY = DP <= 128 && (I8 || SRC == kAsync); // where the registers hold them
+  Rows<T, DP, RT, false, EARLY> r;
+  if (tid < 2)
+    odd_of[tid] = 0;
   add_up<ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
   if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
     for (int i = tid * 16; i < RING * 2 * TILE; i += 64 * W * 16)
       *reinterpret_cast<u32x4 *>(&tiles[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
 
-  while (run.unit < run.end) {
+  for (int turn = 0; run.unit < run.end; turn ^= 1) {
     const Item it = take<ROWS, UNIT>(a, schedule, run);
+    int &odd = odd_of[turn];
     const int row0 = (it.tile * W + wave) * 16 * RT;                // the wave's first
     const int rows = it.fresh * static_cast<int>(a.group.d) - row0; // and how many from there
     load.item(a, it);
     const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.length);
     const int count = x0 < x_end ? (x_end - x0 + kTile - 1) / kTile : 0;
+    auto is_cut = [&](int x, uint32_t seen) { return seen != 0xffffffffu || x + kTile > it.cached; };
+    // this wave's tokens of a tile that it has brought, before the others may read them
+    auto clean_own = [&](int x, uint32_t seen, int slot) {
+      if (!I8 && __builtin_expect(is_cut(x, seen), 0) &&
+          clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, x + kTile > it.cached, lane) && lane == 0)
+        odd = 1;
+    };
     auto take_in = [&](int x, uint32_t seen, int slot) {
-      const bool mixed = x + kTile > it.cached, cut = seen != 0xffffffffu || mixed;
-      if (__builtin_expect(cut, 0)) {
-        if (clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, mixed && !I8, lane) && lane == 0)
-          odd = 1;
-        __syncthreads();
-      }
       if (rows > 0) // the same for the whole wave
-        r.step(a, it, row0, x, seen, cut, tiles[slot][0], tiles[slot][1], lane);
+        r.step(a, it, row0, x, seen, is_cut(x, seen), tiles[slot][0], tiles[slot][1], lane);
     };
     __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
     if (tid == 0)
-      odd = 0; // before the barrier of the first tile
+      odd_of[turn ^ 1] = 0;
 
     if constexpr (SRC == kAsync) {
       int id0 = load.entry(x0), id1 = load.entry(x0 + 16); // of the next tile to send
-      uint32_t seen[RING - 1];                                 // of the tiles on their way
       int xs = x0;
       const uint32_t at = place(tiles[0][0]);
       auto send = [&](int slot) {
@@ -1023,12 +1041,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         id1 = load.entry(xs + 16);
         return s;
       };
+      uint32_t seen[RING - 1]; // of the tiles on their way
 #pragma unroll
       for (int i = 0; i < RING - 1; ++i)
         seen[i] = i < count ? send(i) : 0u;
       r.start(a, it, row0, rows, a.scale, lane);
-      int x = x0;
-      int slot = 0;
+      int x = x0, slot = 0;
 #pragma clang loop unroll(disable)
       for (int n = 0; n < count; ++n, x += kTile) {
         // this wave's part of the tile has arrived, then everybody's; and
@@ -1037,8 +1055,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           arrived<(RING - 2) * 2 * Load::LOADS>();
         else
           arrived<0>();
-        __syncthreads();
         const uint32_t now = seen[0];
+        clean_own(x, now, slot);
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i + 1 < RING - 1; ++i)
           seen[i] = seen[i + 1];
@@ -1055,6 +1074,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         const uint32_t t = load.tokens_there();
         if (lane == 0)
           tokens[slot][wave] = static_cast<uint8_t>(t);
+        const int xp = x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile); // the tile put: this one or the next
+        clean_own(xp, t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W))), slot);
       };
       if (count > 0) {
         load.fetch(x);
