@@ -33,6 +33,16 @@ template <class T> __device__ __forceinline__ void store(void *p, const T &v) {
   static_cast<Loose<T> *>(p)->v = v;
 }
 
+template <class T> __device__ __forceinline__ void store_past(void *p, const T &v) {
+  __builtin_nontemporal_store(v, &static_cast<Loose<T> *>(p)->v);
+}
+
+// The same for the whole wave: through the scalar cache, which does not queue
+// behind the vector loads in flight.
+template <class T> __device__ __forceinline__ T scalar_load(const T *p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uint64_t>(p));
+}
+
 template <int T> constexpr int width() { return T == kF32 ? 4 : 2; }
 
 template <int T> __device__ __forceinline__ float widen16(uint32_t h) {
@@ -51,44 +61,51 @@ template <int T> __device__ __forceinline__ uint32_t pack16(float x, float y) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
-// Up to eight elements at `p`, of which the first `n` are the head's.
-template <int T> __device__ __forceinline__ void load8(const char *p, int n, float *v) {
+// Eight elements as they lie in memory, of which the first `n` are the head's
+// (the others zero). Loads are nothing but loads, so they can be on their way
+// while the row before is worked on. Everything is read once: past the caches.
+template <int T> struct Raw {
+  u32x4 v[T == kF32 ? 2 : 1];
+};
+template <int T> __device__ __forceinline__ Raw<T> load_raw(const char *p, int n) {
+  Raw<T> r;
   if (n >= kV) {
-    if constexpr (T == kF32) {
-      const f32x4 a = load<f32x4>(p), b = load<f32x4>(p + 16);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
-    } else {
-      const u32x4 a = load<u32x4>(p);
-#pragma unroll
-      for (int e = 0; e < kV; ++e)
-        v[e] = widen16<T>((a[e >> 1] >> ((e & 1) * 16)) & 0xffffu);
-    }
-    return;
+    for (int i = 0; i < (T == kF32 ? 2 : 1); ++i)
+      r.v[i] = __builtin_nontemporal_load(&reinterpret_cast<const Loose<u32x4> *>(p + i * 16)->v);
+    return r;
   }
+  uint32_t b[T == kF32 ? kV : kV / 2] = {};
 #pragma unroll
   for (int e = 0; e < kV; ++e) {
-    v[e] = 0.0f;
-    if (e < n) {
-      if constexpr (T == kF32)
-        v[e] = load<float>(p + e * 4);
-      else
-        v[e] = widen16<T>(load<uint16_t>(p + e * 2));
-    }
+    if constexpr (T == kF32)
+      b[e] = e < n ? load<uint32_t>(p + e * 4) : 0u;
+    else
+      b[e >> 1] |= (e < n ? load<uint16_t>(p + e * 2) : 0u) << ((e & 1) * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < (T == kF32 ? 2 : 1); ++i)
+    r.v[i] = u32x4{b[i * 4], b[i * 4 + 1], b[i * 4 + 2], b[i * 4 + 3]};
+  return r;
+}
+template <int T> __device__ __forceinline__ void widen(const Raw<T> &r, float *v) {
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    if constexpr (T == kF32)
+      v[e] = __uint_as_float(r.v[e >> 2][e & 3]);
+    else
+      v[e] = widen16<T>((r.v[0][e >> 1] >> ((e & 1) * 16)) & 0xffffu);
   }
 }
 
 template <int T> __device__ __forceinline__ void store8(char *p, int n, const float *v) {
   if (n >= kV) {
     if constexpr (T == kF32) {
-      store(p, f32x4{v[0], v[1], v[2], v[3]});
-      store(p + 16, f32x4{v[4], v[5], v[6], v[7]});
+      store_past(p, f32x4{v[0], v[1], v[2], v[3]});
+      store_past(p + 16, f32x4{v[4], v[5], v[6], v[7]});
     } else {
-      store(p, u32x4{pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]),
-                     pack16<T>(v[6], v[7])});
+      store_past(p, u32x4{pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]),
+                          pack16<T>(v[6], v[7])});
     }
     return;
   }
@@ -110,11 +127,11 @@ __device__ __forceinline__ void load_weight(const void *w, int type, int at, int
     return;
   const char *p = static_cast<const char *>(w) + static_cast<int64_t>(at) * (type == kF32 ? 4 : 2);
   if (type == kF32)
-    load8<kF32>(p, n, v);
+    widen(load_raw<kF32>(p, n), v);
   else if (type == kF16)
-    load8<kF16>(p, n, v);
+    widen(load_raw<kF16>(p, n), v);
   else
-    load8<kBF16>(p, n, v);
+    widen(load_raw<kBF16>(p, n), v);
 }
 
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
@@ -158,55 +175,59 @@ __device__ __forceinline__ Turn make_turn(const RotateArgs &a, int lane, int fir
   return t;
 }
 
-// cos and sin of the lane's elements at a row's position, sin with the sign
-// that its element's product takes: z = y * cos + partner * sin. Elements that
-// do not turn have (1, 0).
-__device__ __forceinline__ void angles(const RotateArgs &a, const Turn &t, int64_t position,
-                                       float *co, float *si) {
-#pragma unroll
-  for (int e = 0; e < kV; ++e) {
-    co[e] = 1.0f;
-    si[e] = 0.0f;
+// The angles of the lane's elements at a row's position (kPairs: four, of two
+// elements each).
+struct Angles {
+  f32x4 c[2], s[2];
+};
+__device__ __forceinline__ Angles load_angles(const RotateArgs &a, const Turn &t, int64_t position) {
+  Angles r = {};
+  if (position < 0 || position >= a.angles) { // loud, and nothing read
+    const float nan = __builtin_nanf("");
+    r.c[0] = r.c[1] = f32x4{nan, nan, nan, nan};
+    return r;
   }
   if (t.first >= t.rotary)
-    return;
-  if (position < 0 || position >= a.angles) { // no such angle: loud, and nothing read
-#pragma unroll
-    for (int e = 0; e < kV; ++e)
-      if (t.first + e < t.rotary)
-        co[e] = __builtin_nanf("");
-    return;
-  }
+    return r;
   const float *c = a.cos + position * t.half, *s = a.sin + position * t.half;
   if (t.how == kPairs && t.first + kV <= t.rotary) {
-    const f32x4 vc = load<f32x4>(c + (t.first >> 1)), vs = load<f32x4>(s + (t.first >> 1));
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      co[e] = vc[e >> 1];
-      si[e] = e & 1 ? vs[e >> 1] : -vs[e >> 1];
-    }
+    r.c[0] = load<f32x4>(c + (t.first >> 1));
+    r.s[0] = load<f32x4>(s + (t.first >> 1));
   } else if (t.how == kLanes) {
-    const bool low = t.first < t.half;
-    const int at = low ? t.first : t.first - t.half;
-#pragma unroll
-    for (int v = 0; v < kV; v += 4) {
-      const f32x4 vc = load<f32x4>(c + at + v), vs = load<f32x4>(s + at + v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        co[v + e] = vc[e];
-        si[v + e] = low ? -vs[e] : vs[e];
-      }
-    }
+    const int at = t.first < t.half ? t.first : t.first - t.half;
+    r.c[0] = load<f32x4>(c + at);
+    r.c[1] = load<f32x4>(c + at + 4);
+    r.s[0] = load<f32x4>(s + at);
+    r.s[1] = load<f32x4>(s + at + 4);
   } else {
+    float vc[kV], vs[kV];
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       const int i = t.first + e;
-      if (i < t.rotary) {
-        const bool low = t.how == kPairs ? !(i & 1) : i < t.half;
-        const int at = t.how == kPairs ? i >> 1 : low ? i : i - t.half;
-        co[e] = c[at];
-        si[e] = low ? -s[at] : s[at];
-      }
+      const int at = t.how == kPairs ? (t.first >> 1) + e : i < t.half ? i : i - t.half;
+      const bool in = t.how == kPairs ? at < t.half : i < t.rotary;
+      vc[e] = in ? c[at] : 0.0f;
+      vs[e] = in ? s[at] : 0.0f;
+    }
+    r.c[0] = f32x4{vc[0], vc[1], vc[2], vc[3]};
+    r.c[1] = f32x4{vc[4], vc[5], vc[6], vc[7]};
+    r.s[0] = f32x4{vs[0], vs[1], vs[2], vs[3]};
+    r.s[1] = f32x4{vs[4], vs[5], vs[6], vs[7]};
+  }
+  return r;
+}
+
+// cos and sin of each of the lane's elements, sin with the sign that its
+// partner's product takes: z = y * cos + partner * sin.
+__device__ __forceinline__ void angles(const Turn &t, const Angles &r, float *co, float *si) {
+#pragma unroll
+  for (int e = 0; e < kV; ++e) {
+    if (t.how == kPairs) {
+      co[e] = r.c[0][e >> 1];
+      si[e] = e & 1 ? r.s[0][e >> 1] : -r.s[0][e >> 1];
+    } else {
+      co[e] = r.c[e >> 2][e & 3];
+      si[e] = t.first + e < t.half ? -r.s[e >> 2][e & 3] : r.s[e >> 2][e & 3];
     }
   }
 }
@@ -287,27 +308,49 @@ __global__ __launch_bounds__(64 * kWaves) void k_rotate(RotateArgs a) {
   }
   const Heads xs = a.x[kind];
 
+  // The next row's elements and angles are on their way while a row is worked
+  // on, and the position of the one after it.
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWaves;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave; row < a.rows; row += step) {
-    float x[U][kV], dz[U][kV];
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(wave);
+  int64_t position = turns && row < a.rows ? scalar_load(a.positions + row) : 0;
+  Raw<T> next_x[U] = {}, next_dz[kBack ? U : 1] = {};
+  Angles next_angles = {};
+  int64_t next_slot = -1;
+  auto fetch = [&](int64_t r) {
+    if (r >= a.rows)
+      return;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t head = head0 + u * H;
       if (live[u]) {
-        load8<T>(xs.data + (row * xs.row + head * xs.head + first) * W, n, x[u]);
+        next_x[u] = load_raw<T>(xs.data + (r * xs.row + head * xs.head + first) * W, n);
         if constexpr (kBack)
-          load8<T>(a.dz[kind].data + (row * a.dz[kind].row + head * a.dz[kind].head + first) * W, n,
-                   dz[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kV; ++e)
-          x[u][e] = dz[u][e] = 0.0f;
+          next_dz[u] = load_raw<T>(a.dz[kind].data + (r * a.dz[kind].row + head * a.dz[kind].head + first) * W, n);
       }
     }
-    int64_t slot = -1, cache_at = 0;
+    if (turns) {
+      next_angles = load_angles(a, t, position);
+      if (r + step < a.rows)
+        position = scalar_load(a.positions + r + step);
+    }
+    if (kServe && kind > 0)
+      next_slot = scalar_load(a.slots + r);
+  };
+  fetch(row);
+  for (; row < a.rows; row += step) {
+    Raw<T> now_x[U], now_dz[kBack ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now_x[u] = next_x[u];
+      if constexpr (kBack)
+        now_dz[u] = next_dz[u];
+    }
+    const Angles now_angles = next_angles;
+    const int64_t slot = next_slot;
+    fetch(row + step);
+    int64_t cache_at = 0;
     if constexpr (kServe) {
       if (kind > 0) {
-        slot = a.slots[row];
         if (slot < 0 || slot >= a.pages_slots)
           continue;
         const uint32_t page = fdiv(static_cast<uint32_t>(slot), a.page);
@@ -317,27 +360,31 @@ __global__ __launch_bounds__(64 * kWaves) void k_rotate(RotateArgs a) {
     }
     float co[kV], si[kV];
     if (turns)
-      angles(a, t, a.positions[row], co, si);
+      angles(t, now_angles, co, si);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (chunk * a.chunk_heads + u * H >= heads || u * H >= a.chunk_heads)
         break; // no heads left: the same for the whole wave
       const int64_t head = head0 + u * H;
+      float x[kV], dz[kV];
+      widen(now_x[u], x);
+      if constexpr (kBack)
+        widen(now_dz[u], dz);
       float z[kV];
       if (kServe && !turns) {
 #pragma unroll
         for (int e = 0; e < kV; ++e)
-          z[e] = x[u][e];
+          z[e] = x[e];
       } else if constexpr (!kBack) {
         float ss = 0.0f;
 #pragma unroll
         for (int e = 0; e < kV; ++e)
-          ss += x[u][e] * x[u][e];
+          ss += x[e] * x[e];
         const float r = rsqrtf(head_sum<L>(ss) * a.inv_dim + a.eps);
         float y[kV], p[kV];
 #pragma unroll
         for (int e = 0; e < kV; ++e)
-          y[e] = x[u][e] * r * w[e];
+          y[e] = x[e] * r * w[e];
         partners<L>(t, lane, y, p, room[wave]);
 #pragma unroll
         for (int e = 0; e < kV; ++e)
@@ -345,18 +392,18 @@ __global__ __launch_bounds__(64 * kWaves) void k_rotate(RotateArgs a) {
       } else {
         // the transposed rotation: the partner's product with the other sign
         float g[kV], p[kV], ss = 0.0f, ux = 0.0f;
-        partners<L>(t, lane, dz[u], p, room[wave]);
+        partners<L>(t, lane, dz, p, room[wave]);
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          g[e] = first + e < a.rotary ? dz[u][e] * co[e] - p[e] * si[e] : dz[u][e];
-          ss += x[u][e] * x[u][e];
-          ux += g[e] * w[e] * x[u][e];
+          g[e] = first + e < a.rotary ? dz[e] * co[e] - p[e] * si[e] : dz[e];
+          ss += x[e] * x[e];
+          ux += g[e] * w[e] * x[e];
         }
         const float r = rsqrtf(head_sum<L>(ss) * a.inv_dim + a.eps);
         const float m = head_sum<L>(ux) * r * a.inv_dim; // mean(u n)
 #pragma unroll
         for (int e = 0; e < kV; ++e) {
-          const float nx = x[u][e] * r;
+          const float nx = x[e] * r;
           dw[e] += g[e] * nx;
           z[e] = r * (g[e] * w[e] - nx * m);
         }
