@@ -200,14 +200,15 @@ __device__ __forceinline__ Angles load_angles(const RotateArgs &a, const Turn &t
     r.s[0] = load<f32x4>(s + at);
     r.s[1] = load<f32x4>(s + at + 4);
   } else {
+    // some of the lane's elements do not turn, or turn in the other half:
+    // what they load is not used
     float vc[kV], vs[kV];
 #pragma unroll
     for (int e = 0; e < kV; ++e) {
       const int i = t.first + e;
-      const int at = t.how == kPairs ? (t.first >> 1) + e : i < t.half ? i : i - t.half;
-      const bool in = t.how == kPairs ? at < t.half : i < t.rotary;
-      vc[e] = in ? c[at] : 0.0f;
-      vs[e] = in ? s[at] : 0.0f;
+      const int at = min(t.how == kPairs ? (t.first >> 1) + e : i < t.half ? i : i - t.half, t.half - 1);
+      vc[e] = c[at];
+      vs[e] = s[at];
     }
     r.c[0] = f32x4{vc[0], vc[1], vc[2], vc[3]};
     r.c[1] = f32x4{vc[4], vc[5], vc[6], vc[7]};
@@ -527,8 +528,9 @@ int rotate_lanes(int dim) {
 
 int rotate_blocks(int form, int64_t rows, int64_t chunks) {
   const int64_t blocks = (rows + kWaves - 1) / kWaves;
-  // enough waves to fill the card several times over
-  const int64_t most = 256 * (form == kRotateBackward ? 8 : 16);
+  // As many waves as the card holds at once (three on a SIMD), or twice that
+  // where no block leaves a part of a sum: TODO
+  const int64_t most = 256 * (form == kRotateBackward ? 3 : 8);
   const int64_t cap = most / chunks > 0 ? most / chunks : 1;
   return static_cast<int>(blocks < cap ? blocks : cap);
 }
