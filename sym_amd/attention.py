@@ -52,7 +52,7 @@ _HEADS = struct.Struct(_format(N.relx_heads))
 _CACHE = struct.Struct(_format(N.relx_cache))
 _TABLES = struct.Struct(_format(N.relx_block_tables_args))
 _ROTATION = struct.Struct(_format(N.relx_rotation))
-_ATTENTION = struct.Struct(_format(N.relx_tree_attention_args))
+_ATTENTION = struct.Struct(_format(N.relx_tree_attention_args)[6:])  # after its two relx_heads
 
 
 def _bad(message):
@@ -77,6 +77,7 @@ def _call(name, ctx, *args):
 
 
 # torch's current stream as a handle; the plain query costs as much as a launch
+_split = torch.unsafe_split_with_sizes  # of buffers that nobody else has
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -95,7 +96,7 @@ def _device(ctx, like):
 
 def _row(t, name, dtype, n, device):
     """A contiguous vector of `n` (None: any number)."""
-    if t.dtype is not dtype or t.dim() != 1 or t.get_device() != device or (n is not None and t.shape[0] != n) or \
+    if t.dtype is not dtype or t.get_device() != device or (t.dim() != 1 if n is None else t.shape != (n,)) or \
             not t.is_contiguous():
         _bad("%s: %s [%s] on device %d, contiguous; got %s %s on %s"
              % (name, dtype, "n" if n is None else n, device, t.dtype, list(t.shape), t.device))
@@ -103,14 +104,14 @@ def _row(t, name, dtype, n, device):
 
 
 def _heads(t, name, shape, dtype, device):
-    """[rows, heads, dim] with a contiguous last dimension."""
+    """[rows, heads, dim] with a contiguous last dimension, packed."""
     if t.shape != shape or t.dtype is not dtype or t.get_device() != device:
         _bad("%s: %s %s on device %d; got %s %s on %s"
              % (name, dtype, list(shape), device, t.dtype, list(t.shape), t.device))
     row, head, one = t.stride()
     if one != 1 and shape[2] > 1 and t.numel():
         _bad("%s: the last dimension must be contiguous" % name)
-    return t.data_ptr(), row, head
+    return _HEADS.pack(t.data_ptr(), row, head)
 
 
 def _table(t, device):
@@ -177,14 +178,14 @@ def block_tables(ctx, cached, fresh, table, free_pages, page, rows, *, parents=N
         if words < 1:
             _bad("block tables: words = %d" % words)
     if out is None:
-        i32 = torch.empty(requests + 2 + rows, dtype=torch.int32, device=table.device)
-        i64 = torch.empty(rows * (1 + words), dtype=torch.int64, device=table.device)
+        i32 = table.new_empty(requests + 2 + rows)
+        i64 = table.new_empty(rows * (1 + words), dtype=torch.int64)
         p32, p64 = i32.data_ptr(), i64.data_ptr()
-        starts, taken, positions = i32.split((requests + 1, 1, rows))
+        starts, taken, positions = _split(i32, (requests + 1, 1, rows))
         ptrs = p32, p64, p32 + 4 * (requests + 2), p64 + 8 * rows if words else 0, p32 + 4 * (requests + 1)
         mask = None
         if words:
-            i64, mask = i64.split((rows, rows * words))
+            i64, mask = _split(i64, (rows, rows * words))
             mask = mask.view(rows, words)
         out = Tables(starts, i64, positions, taken, mask)
     else:
@@ -219,20 +220,21 @@ def _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs):
             cos.get_device() != device or sin.get_device() != device or not (cos.is_contiguous() and sin.is_contiguous()):
         _bad("cos and sin: contiguous float32 [angles, rotary / 2] on device %d; got %s %s and %s %s"
              % (device, cos.dtype, list(cos.shape), sin.dtype, list(sin.shape)))
-    w_kind, w_ptr = (0, 32), [0, 0]
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    if given:
-        w_kind = _KINDS.get(given[0].dtype)
-        if w_kind is None or w_kind[1] == 8 or given[0].dtype is not given[-1].dtype:
-            _bad("weights: one floating type; got %s" % [w.dtype for w in given])
-        w_ptr = [0 if w is None else _row(w, "weight", w.dtype, dim, device) for w in (q_weight, k_weight)]
+    qw_ptr = kw_ptr = 0
+    given = k_weight if q_weight is None else q_weight
+    if given is None:
+        w_kind = 0, 32
+    else:
+        w_kind = _KINDS.get(given.dtype)
+        if w_kind is None or w_kind[1] == 8:
+            _bad("weights: a floating type; got %s" % given.dtype)
+        if q_weight is not None:
+            qw_ptr = _row(q_weight, "weight", given.dtype, dim, device)
+        if k_weight is not None:
+            kw_ptr = _row(k_weight, "weight", given.dtype, dim, device)
     p_ptr = _row(positions, "positions", torch.int32, rows, device)
-    return (_ROTATION.pack(p_ptr, cos.data_ptr(), sin.data_ptr(), *w_ptr, *w_kind, rows, qs[1], ks[1], dim,
+    return (_ROTATION.pack(p_ptr, cos.data_ptr(), sin.data_ptr(), qw_ptr, kw_ptr, *w_kind, rows, qs[1], ks[1], dim,
                            2 * cos.shape[1], 1 if pairs else 0, cos.shape[0], *kind, float(eps)), qs, ks, device)
-
-
-def _pack_heads(t, name, shape, dtype, device):
-    return _HEADS.pack(*_heads(t, name, shape, dtype, device))
 
 
 class _NormRotate(torch.autograd.Function):
@@ -274,11 +276,10 @@ def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pair
 def _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out):
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
-    zq, zk = out if out is not None else (torch.empty(qs, dtype=dtype, device=q.device),
-                                          torch.empty(ks, dtype=dtype, device=q.device))
-    _call("relx_norm_rotate", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
-          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(zq, "query result", qs, dtype, device),
-          _pack_heads(zk, "key result", ks, dtype, device), _stream(device))
+    zq, zk = out if out is not None else (q.new_empty(qs), k.new_empty(ks))
+    _call("relx_norm_rotate", ctx, rot, _heads(q, "queries", qs, dtype, device),
+          _heads(k, "keys", ks, dtype, device), _heads(zq, "query result", qs, dtype, device),
+          _heads(zk, "key result", ks, dtype, device), _stream(device))
     return zq, zk
 
 
@@ -289,18 +290,24 @@ def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_wei
     is); the others have the operands' type."""
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
-    gq, gk = torch.empty(qs, dtype=dtype, device=q.device), torch.empty(ks, dtype=dtype, device=q.device)
-    gw = [None if w is None else torch.empty(qs[2], dtype=torch.float32, device=q.device) for w in (q_weight, k_weight)]
-    room = None
-    if q_weight is not None or k_weight is not None:
-        room = torch.empty(_rotate_room(rot, qs, ks, dtype) // 4, dtype=torch.float32, device=q.device)
-    _call("relx_norm_rotate_backward", ctx, rot, _pack_heads(dq, "query gradient", qs, dtype, device),
-          _pack_heads(dk, "key gradient", ks, dtype, device), _pack_heads(q, "queries", qs, dtype, device),
-          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(gq, "query gradient", qs, dtype, device),
-          _pack_heads(gk, "key gradient", ks, dtype, device), 0 if gw[0] is None else gw[0].data_ptr(),
-          0 if gw[1] is None else gw[1].data_ptr(), 0 if room is None else room.data_ptr(),
-          0 if room is None else room.numel() * 4, _stream(device))
-    return gq, gk, gw[0], gw[1]
+    gq, gk = q.new_empty(qs), k.new_empty(ks)
+    gqw = gkw = None
+    gqw_ptr = gkw_ptr = room_ptr = size = 0
+    if q_weight is not None:
+        gqw = cos.new_empty(qs[2])
+        gqw_ptr = gqw.data_ptr()
+    if k_weight is not None:
+        gkw = cos.new_empty(qs[2])
+        gkw_ptr = gkw.data_ptr()
+    if gqw_ptr or gkw_ptr:
+        size = _rotate_room(rot, qs, ks, dtype)
+        room = cos.new_empty(size // 4)
+        room_ptr = room.data_ptr()
+    _call("relx_norm_rotate_backward", ctx, rot, _heads(dq, "query gradient", qs, dtype, device),
+          _heads(dk, "key gradient", ks, dtype, device), _heads(q, "queries", qs, dtype, device),
+          _heads(k, "keys", ks, dtype, device), _heads(gq, "query gradient", qs, dtype, device),
+          _heads(gk, "key gradient", ks, dtype, device), gqw_ptr, gkw_ptr, room_ptr, size, _stream(device))
+    return gq, gk, gqw, gkw
 
 
 _rooms = {}
@@ -330,11 +337,11 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
     if out is None:
-        out = torch.empty(qs, dtype=dtype, device=q.device)
+        out = q.new_empty(qs)
     cache = _CACHE.pack(*_cache(cache_k, cache_v, k_scale, v_scale, device))
-    _call("relx_norm_rotate_append", ctx, rot, _pack_heads(q, "queries", qs, dtype, device),
-          _pack_heads(k, "keys", ks, dtype, device), _pack_heads(v, "values", ks, dtype, device),
-          _pack_heads(out, "query result", qs, dtype, device), _row(slots, "slots", torch.int64, qs[0], device),
+    _call("relx_norm_rotate_append", ctx, rot, _heads(q, "queries", qs, dtype, device),
+          _heads(k, "keys", ks, dtype, device), _heads(v, "values", ks, dtype, device),
+          _heads(out, "query result", qs, dtype, device), _row(slots, "slots", torch.int64, qs[0], device),
           cache, _stream(device))
     return out
 
@@ -391,20 +398,20 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
             _bad("mask: contiguous int64 [%d, words] on device %d; got %s %s" % (rows, device, mask.dtype, list(mask.shape)))
         words, m_ptr = mask.shape[1], mask.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = q.new_empty(shape)
     l_ptr = 0
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != shape[:2] or lse.get_device() != device or not lse.is_contiguous():
             _bad("lse: contiguous float32 [%d, %d]" % (rows, heads))
         l_ptr = lse.data_ptr()
     if workspace is None:
-        workspace = torch.empty(tree_attention_workspace(rows, requests, heads, kv_heads, dim, cache[11]),
-                                dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(tree_attention_workspace(rows, requests, heads, kv_heads, dim, cache[11]),
+                                dtype=torch.uint8)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _bad("workspace: contiguous uint8 on device %d" % device)
     _call("relx_tree_attention", ctx,
-          _ATTENTION.pack(*_heads(q, "queries", shape, dtype, device), *_heads(out, "result", shape, dtype, device),
-                          *cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
+          _heads(q, "queries", shape, dtype, device) + _heads(out, "result", shape, dtype, device) +
+          _ATTENTION.pack(*cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
                           _row(starts, "starts", torch.int32, requests + 1, device), m_ptr, l_ptr,
                           workspace.data_ptr(), workspace.numel(), rows, requests, heads, columns, words, *kind,
                           dim ** -0.5 if scale is None else float(scale)), _stream(device))
