@@ -62,11 +62,11 @@ constexpr int kSharedUnit = 64;
 constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
 
 enum Source : int { kAsync, kStaged, kStagedEven };
-// Where a row's running maximum starts: finite, so that a difference with a
+// Where a row's reference maximum starts: finite, so that a difference with a
 // masked score's -inf stays -inf.
-constexpr float kNone = -1e30f;
-// A row's reference maximum moves only once a score exceeds it by this many
-// powers of two; until then weights up to 2^8 are summed as they are.
+constexpr float kNone = -3.402823466e38f;
+// A row's reference maximum moves only once a lane's weights of a tile add up
+// to more than two to this; until then they are summed as they are.
 constexpr float kSlack = 8.0f;
 
 template <class T> struct __attribute__((packed)) Loose { T v; };
@@ -97,6 +97,14 @@ template <int T> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The kernel's arguments, read anew: what needs them now and then does not
+// hold scalar registers through the loops.
+__device__ __forceinline__ const AttendArgs &args_again() {
+  uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const AttendArgs *)reinterpret_cast<const __attribute__((address_space(4))) AttendArgs *>(p);
 }
 
 // Keeps the scheduler from moving anything across.
@@ -345,26 +353,27 @@ template <int RB> __device__ __forceinline__ int piece(int token, int n) {
 typedef __attribute__((address_space(3))) char lds_char;
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// Four tokens of one dim, a pair of words: lane i of sixteen gives the address
-// of four dims of token i / 4, and gets dim i.
-__device__ __forceinline__ u32x2 read_transposed(const char *p) {
-  typedef __attribute__((address_space(3))) i16x4 *at;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (at)(lds_char *)const_cast<char *>(p)));
-}
-
 // A shared array's place.
 __device__ __forceinline__ uint32_t place(const char *p) {
   return uniform(static_cast<int>(reinterpret_cast<uintptr_t>((lds_char *)const_cast<char *>(p))));
 }
+__device__ __forceinline__ u32x4 read16(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>(at);
+}
+
+// Four tokens of one dim, a pair of words: lane i of sixteen gives the address
+// of four dims of token i / 4, and gets dim i.
+__device__ __forceinline__ u32x2 read_transposed(uint32_t at) {
+  typedef __attribute__((address_space(3))) i16x4 *From;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<From>(at)));
+}
 
 // Eight tokens of one int8 dim: lane i of sixteen gives the address of eight
 // dims of token i / 2, and gets dim i.
-__device__ __forceinline__ u32x2 read_transposed8(const char *p) {
+__device__ __forceinline__ u32x2 read_transposed8(uint32_t at) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
-  typedef __attribute__((address_space(3))) i32x2 *at;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                       (at)(lds_char *)const_cast<char *>(p)));
+  typedef __attribute__((address_space(3))) i32x2 *From;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<From>(at)));
 }
 
 // 16 bytes per lane from base + at into shared memory, lane after lane from
@@ -383,24 +392,37 @@ template <int N> __device__ __forceinline__ void arrived() {
 // Waits for the wave's own reads and writes of shared memory.
 __device__ __forceinline__ void shared_done() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
+// Where a lane's reads of a tile begin: its first piece of a key, and of the
+// values. Piece n + k of a token lies at the place of piece n with the bits of
+// 16 k turned over (tiles lie at multiples of their tokens' bytes), and sixteen
+// tokens on is the same piece: so all reads of a tile have one address each in
+// registers outside the loop.
+template <int DP, bool RAW> struct Reads {
+  static constexpr int RB = DP * (RAW ? 1 : 2);
+  uint32_t key, value;
+  __device__ __forceinline__ explicit Reads(int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    key = piece<RB>(c, g);
+    if constexpr (RAW)
+      value = piece<RB>(4 * g + ((c >> 1) & 3) + (c >> 3) * 16, 0) + (c & 1) * 8;
+    else
+      value = piece<RB>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8;
+  }
+};
+
 // A tile's values as operands: at(e) has dim 16 e + lane % 16 of the lane's eight
 // tokens. RAW: the tile holds int8. EARLY: all read at once, ahead of their use.
 template <int T, int DP, bool RAW, bool EARLY> struct Values {
   static constexpr int E = DP / 16;
-  const char *tv;
-  int lane;
+  uint32_t from;
   u32x2 lo[EARLY ? E : 1], hi[EARLY && !RAW ? E : 1];
   __device__ __forceinline__ u32x2 part(int e, int tile) const {
-    const int c = lane & 15, g = lane >> 4;
-    if constexpr (RAW) {
-      const int token = 4 * g + ((c >> 1) & 3) + (c >> 3) * 16;
-      return read_transposed8(tv + piece<DP>(token, e) + (c & 1) * 8);
-    } else {
-      const int token = 4 * g + (c >> 2) + tile * 16, half = (c & 3) >> 1;
-      return read_transposed(tv + piece<DP * 2>(token, e * 2 + half) + (c & 1) * 8);
-    }
+    if constexpr (RAW)
+      return read_transposed8(from ^ (e * 16));
+    else
+      return read_transposed((from ^ (e * 32)) + tile * 16 * DP * 2);
   }
-  __device__ __forceinline__ Values(const char *tv_, int lane_) : tv(tv_), lane(lane_) {
+  __device__ __forceinline__ explicit Values(uint32_t from_) : from(from_) {
     if constexpr (EARLY) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -506,15 +528,15 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   f32x4 s[RT][2];     // scores, unscaled
   u32x4 weights[RT];
 
-  __device__ __forceinline__ void scores(const char *tk, int lane_) {
-    const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
+  // from: the tile's place and the lane's first piece in it
+  __device__ __forceinline__ void scores(uint32_t from) {
     constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
     u32x4 k[2][KR];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < KR; ++i)
-        k[n][i] = *reinterpret_cast<const u32x4 *>(tk + piece<RAW ? DP : DP * 2>(n * 16 + c, i * 4 + g));
+        k[n][i] = read16((from ^ (i * 64)) + n * 16 * DP * (RAW ? 1 : 2));
     keep_order(); // all reads on their way before the first is waited for
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -535,10 +557,27 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     }
   }
 
-  __device__ __forceinline__ void soften(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
-                                         int lane_) {
+  // The weights of a row, and their sum over the lane's tokens.
+  __device__ __forceinline__ float weigh(int t) {
+    float p[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[n][i] = __builtin_amdgcn_exp2f(s[t][n][i] * scale - top[t]);
+      weights[t][n * 2] = pack16<T>(p[n][0], p[n][1]);
+      weights[t][n * 2 + 1] = pack16<T>(p[n][2], p[n][3]);
+    }
+    return ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+  }
+
+  // Weights go by the maximum so far. Whether that still does shows in their
+  // own sum, so a tile's maximum is looked for only where it does not: in a
+  // row's first tile and a few later ones.
+  __device__ __forceinline__ void soften(const Item &it, int row0, int x, uint32_t seen, bool cut, int lane_) {
     constexpr float kBias = weight_bias<T>();
     if (__builtin_expect(cut, 0)) {
+      const AttendArgs &a = args_again();
       const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
@@ -577,20 +616,9 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
           acc[t][e] *= shrink;
       }
     }
-
 #pragma unroll
     for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(s[t][n][i] * scale - top[t]);
-          sum[t] += p[i];
-        }
-        weights[t][n * 2] = pack16<T>(p[0], p[1]);
-        weights[t][n * 2 + 1] = pack16<T>(p[2], p[3]);
-      }
+      sum[t] += weigh(t);
   }
 
   __device__ __forceinline__ void add(const Values<T, DP, RAW, EARLY> &v) {
@@ -603,11 +631,12 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     }
   }
 
-  __device__ __forceinline__ void step(const AttendArgs &a, const Item &it, int row0, int x, uint32_t seen, bool cut,
-                                       const char *tk, const char *tv, int lane) {
-    scores(tk, lane);
-    const Values<T, DP, RAW, EARLY> v(tv, anew(lane)); // EARLY: they arrive during the softmax
-    soften(a, it, row0, x, seen, cut, lane);
+  // tk, tv: the places of the tile's keys and values.
+  __device__ __forceinline__ void step(const Item &it, int row0, int x, uint32_t seen, bool cut, uint32_t tk, uint32_t tv,
+                                       const Reads<DP, RAW> &reads, int lane) {
+    scores(tk + reads.key);
+    const Values<T, DP, RAW, EARLY> v(tv + reads.value); // EARLY: they arrive during the softmax
+    soften(it, row0, x, seen, cut, lane);
     add(v);
   }
 
@@ -616,45 +645,48 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     return x + __shfl_xor(x, 32);
   }
 
-  // Adds what clean() took out of the tiles at x0, x0 + pace, ... before x_end:
-  // values that are not finite, of tokens that some rows see, to those rows.
-  // Hardly ever; a dim at a time, from the cache.
-  __device__ void add_odd(const AttendArgs &a, const Item &it, int row0, int rows, int x0, int x_end, int pace, int lane) {
+  // Gives `add` what clean() took out of the tiles at x0, x0 + pace, ... before
+  // x_end: values that are not finite, of tokens that some rows see, times their
+  // weights in those rows. Hardly ever; a dim at a time, from the cache, to
+  // where the sums have been stored: they are not in registers here.
+  template <class Add>
+  __device__ __forceinline__ void add_odd(const Item &it, int row0, int rows, int x0, int x_end, int pace, int lane,
+                                          Add add) const {
+    const AttendArgs &a = args_again();
     const int c = lane & 15, g = lane >> 4;
     const int32_t *table = a.table + it.b * a.table_row;
-#pragma clang loop unroll(disable)
-    for (int x = x0; x < x_end; x += pace) {
-      if (x + kTile <= it.cached)
-        continue;
-#pragma clang loop unroll(disable)
-      for (int y = x; y < min(x + kTile, it.length); ++y) {
-        const uint32_t at = fdiv(static_cast<uint32_t>(y), a.page), off = static_cast<uint32_t>(y) - at * a.page.d;
-        const int id = table[at];
-        if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages))
-          continue;
-        const char *k = a.keys + it.head * a.key_head + id * a.key_page + off * a.key_slot;
-        const char *v = a.values + it.head * a.value_head + id * a.value_page + off * a.value_slot;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int p = row0 + t * 16 + c;
-          if (t * 16 + c >= rows || !(row_sees(a, it, p, x) >> (y - x) & 1u))
+    for (int t = 0; t < RT; ++t) {
+      const int p = row0 + t * 16 + c;
+      if (t * 16 + c >= rows)
+        continue;
+      const uint32_t j = fdiv(static_cast<uint32_t>(p), a.group);
+      const char *q = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
+                             (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
+#pragma clang loop unroll(disable)
+      for (int x = x0; x < x_end; x += pace) {
+        if (x + kTile <= it.cached)
+          continue;
+        const uint32_t sees = row_sees(a, it, p, x);
+#pragma clang loop unroll(disable)
+        for (int y = x; y < min(x + kTile, it.length); ++y) {
+          const uint32_t at = fdiv(static_cast<uint32_t>(y), a.page), off = static_cast<uint32_t>(y) - at * a.page.d;
+          const int id = table[at];
+          if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages) || !(sees >> (y - x) & 1u))
             continue;
-          const uint32_t j = fdiv(static_cast<uint32_t>(p), a.group);
-          const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
-                                   (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
+          const char *k = a.keys + it.head * a.key_head + id * a.key_page + off * a.key_slot;
+          const char *v = a.values + it.head * a.value_head + id * a.value_page + off * a.value_slot;
           float score = 0.0f;
 #pragma clang loop unroll(disable)
           for (int d = 0; d < a.dim; ++d)
-            score += widen16<T>(load<uint16_t>(src + d * 2)) * widen16<T>(load<uint16_t>(k + d * 2));
+            score += widen16<T>(load<uint16_t>(q + d * 2)) * widen16<T>(load<uint16_t>(k + d * 2));
           const float weight = __builtin_amdgcn_exp2f(score * scale - top[t]);
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (e * 16 + 4 * g + i < a.dim) {
-                const uint32_t h = load<uint16_t>(v + (e * 16 + 4 * g + i) * 2);
-                acc[t][e][i] += finite16<T>(h) ? 0.0f : weight * widen16<T>(h);
-              }
+#pragma clang loop unroll(disable)
+          for (int d = 4 * g; d < a.dim; d += (d & 3) == 3 ? 13 : 1) {
+            const uint32_t h = load<uint16_t>(v + d * 2);
+            if (!finite16<T>(h))
+              add(t, d, weight * widen16<T>(h));
+          }
         }
       }
     }
@@ -684,6 +716,8 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
   bool whole;  // all of them
   u32x4 stage[2][SRC == kAsync ? 1 : LOADS];
   uint32_t there; // loads that are a token's, by bit
+  // kAsync: the lane's token in a load, and its piece in the first load
+  uint32_t key_lane, value_lane, place16;
 
   __device__ __forceinline__ Loader(const AttendArgs &a, int lane, int first_) {
     first = first_;
@@ -703,6 +737,9 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
     whole = dim + LB <= a.dim;
     cell_at = has ? dim * CELL : 0;
     there = 0u;
+    key_lane = token * key_slot;
+    value_lane = token * value_slot;
+    place16 = ((dim / LB) ^ swap_of<RB>(first + token)) * 16;
   }
   __device__ __forceinline__ void item(const AttendArgs &a, const Item &it) {
     keys = a.keys + it.head * a.key_head;
@@ -711,43 +748,62 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
     length = it.length;
   }
 
+  __device__ __forceinline__ bool is_page(int id) const {
+    return static_cast<uint32_t>(id) < static_cast<uint32_t>(pages);
+  }
   // What the table says of the 16 tokens from x0 (past the length: -1); EVEN.
   // Nothing waits for it here.
   __device__ __forceinline__ int entry(int x0) const {
     return x0 < length ? scalar_load(table + fdiv(static_cast<uint32_t>(x0), page)) : -1;
   }
-  __device__ __forceinline__ bool is_page(int id) const {
-    return static_cast<uint32_t>(id) < static_cast<uint32_t>(pages);
+  // The entries of a tile's two halves, and the places in their pages; kAsync.
+  struct Next {
+    int id[2];
+    uint32_t off[2];
+  };
+  __device__ __forceinline__ Next look(int x) const {
+    Next t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t x0 = static_cast<uint32_t>(x) + h * 16, n = fdiv(x0, page);
+      t.id[h] = static_cast<int>(x0) < length ? scalar_load(table + n) : -1;
+      t.off[h] = x0 - n * page.d;
+    }
+    return t;
   }
-  // Which of the 32 tokens from x are there, by their two entries; EVEN.
-  __device__ __forceinline__ uint32_t seen(int x, int id0, int id1) const {
+  // Which halves lie on a page.
+  __device__ __forceinline__ uint32_t halves(const Next &t) const {
+    return (is_page(t.id[0]) ? 1u : 0u) | (is_page(t.id[1]) ? 2u : 0u);
+  }
+  // Which of the 32 tokens from x are there.
+  __device__ __forceinline__ uint32_t seen(int x, uint32_t on) const {
     const int n = max(length - x, 0);
     const uint32_t in = n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-    return in & ((is_page(id0) ? 0xffffu : 0u) | (is_page(id1) ? 0xffff0000u : 0u));
+    return in & ((on & 1u ? 0xffffu : 0u) | (on & 2u ? 0xffff0000u : 0u));
   }
 
-  // kAsync: the wave's tokens of the tile at x, whose 16-token entries are
-  // id0 and id1 (no page: the first one's tokens, which nothing will see).
-  __device__ __forceinline__ void send(int x, int id0, int id1, uint32_t to_k, uint32_t to_v) const {
+  // kAsync: the wave's tokens of a tile (of no page: the first one's, which
+  // nothing will see).
+  __device__ __forceinline__ void send(const Next &next, uint32_t to_k, uint32_t to_v) const {
     constexpr int GROUPS = NT > 16 ? 2 : 1; // of 16 tokens
 #pragma unroll
     for (int h = 0; h < GROUPS; ++h) {
       const int t0 = GROUPS == 2 ? h * 16 : first; // the group's part's first token
-      const int id = t0 < 16 ? id0 : id1;
-      const uint32_t x0 = static_cast<uint32_t>(x) + t0;
-      const uint32_t off = is_page(id) ? x0 - fdiv(x0, page) * page.d : 0u;
+      const bool second = GROUPS == 2 ? h : t0 >= 16;
+      const int id = second ? next.id[1] : next.id[0];
+      const uint32_t off = is_page(id) ? (second ? next.off[1] : next.off[0]) + (t0 & 15) : 0u;
       const uint32_t at = is_page(id) ? id : 0u;
       const char *k = keys + static_cast<uint64_t>(at) * key_page + static_cast<uint64_t>(off) * key_slot;
       const char *v = values + static_cast<uint64_t>(at) * value_page + static_cast<uint64_t>(off) * value_slot;
 #pragma unroll
       for (int i = 0; i < LOADS / GROUPS; ++i) {
         const int t = t0 + i * TPI;
-        const int n = (dim / LB) ^ swap_of<RB>(t + token); // the piece that lies at this lane's place
-        const uint32_t ko = token * key_slot + n * 16, vo = token * value_slot + n * 16;
+        // the piece that lies at this lane's place
+        const uint32_t n16 = LOADS == 1 ? place16 : place16 ^ (swap_of<RB>((h * 16 + i * TPI) & 15) * 16);
         const char *ki = k + static_cast<uint64_t>(i * TPI) * key_slot, *vi = v + static_cast<uint64_t>(i * TPI) * value_slot;
-        if ((NT >= TPI || token < NT) && (full || n * LB < head_dims)) {
-          load_async(ki, ko, to_k + t * RB);
-          load_async(vi, vo, to_v + t * RB);
+        if ((NT >= TPI || token < NT) && (full || static_cast<int>(n16) < head_dims * CELL)) {
+          load_async(ki, key_lane + n16, to_k + t * RB);
+          load_async(vi, value_lane + n16, to_v + t * RB);
         }
       }
     }
@@ -841,45 +897,48 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
   const int c = lane & 15, g = lane >> 4;
   Load load(a, lane, 0);
   Rows<T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
+  const Reads<DP, I8> reads(lane);
   add_up<ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
 
   while (run.unit < run.end) {
-    const Item it = take<ROWS, UNIT>(a, schedule, run);
+    const Item it = take<ROWS, UNIT>(args_again(), schedule, run);
     const int row0 = it.tile * ROWS;
-    const int rows = it.fresh * static_cast<int>(a.group.d) - row0; // of this tile and later ones
-    load.item(a, it);
+    const int rows = it.fresh * static_cast<int>(args_again().group.d) - row0; // of this tile and later ones
+    load.item(args_again(), it);
     const int x_end = min(it.s1 * UNIT, it.length), x0 = it.s0 * UNIT + wave * kTile;
     const int count = x0 < x_end ? (x_end - x0 + UNIT - 1) / UNIT : 0; // this wave's tiles
     bool odd = false;
-    auto take_in = [&](int x, uint32_t seen, int slot) {
-      const bool mixed = x + kTile > it.cached, cut = seen != 0xffffffffu || mixed;
+    auto start = [&] {
+      const AttendArgs &b = args_again();
+      r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
+    };
+    const uint32_t at = place(tiles[wave][0][0]);
+    auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
       if (!I8 && __builtin_expect(cut, 0)) // what int8 holds is finite
-        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, mixed, lane);
-      r.step(a, it, row0, x, seen, cut, tiles[wave][slot][0], tiles[wave][slot][1], lane);
+        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, x + kTile > it.cached, lane);
+      r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
     };
 
     if constexpr (SRC == kAsync) {
-      if (a.dim < DP) // places past the head's dims: no load writes them
+      if (!load.full) // places past the head's dims: no load writes them
         for (int i = lane * 16; i < RING * 2 * TILE; i += 64 * 16)
           *reinterpret_cast<u32x4 *>(&tiles[wave][0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
       shared_done();
-      int id0 = load.entry(x0), id1 = load.entry(x0 + 16); // of the next tile to send
-      uint32_t seen[RING];                                     // of the tiles on their way
+      typename Load::Next next = load.look(x0); // the next tile to send
+      uint32_t on = 0u;                         // of the tiles on their way: their halves on a page
       int xs = x0;
-      const uint32_t at = place(tiles[wave][0][0]);
-      auto send = [&](int slot) {
-        load.send(xs, id0, id1, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
-        const uint32_t s = load.seen(xs, id0, id1);
+      auto send = [&](int slot, int place) {
+        load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        on |= load.halves(next) << (2 * place);
         xs += UNIT;
-        id0 = load.entry(xs);
-        id1 = load.entry(xs + 16);
-        return s;
+        next = load.look(xs);
       };
 #pragma unroll
       for (int i = 0; i < RING; ++i)
-        seen[i] = i < count ? send(i) : 0u;
-      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
+        if (i < count)
+          send(i, i);
+      start();
       int x = x0;
       int slot = 0;
 #pragma clang loop unroll(disable)
@@ -888,17 +947,16 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
           arrived<(RING - 1) * 2 * Load::LOADS>();
         else
           arrived<0>();
-        take_in(x, seen[0], slot);
+        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
+        take_in(x, cut ? load.seen(x, on) : 0xffffffffu, cut, slot);
         shared_done(); // its place is free
-#pragma unroll
-        for (int i = 0; i + 1 < RING; ++i)
-          seen[i] = seen[i + 1];
+        on >>= 2;
         if (n + RING < count)
-          seen[RING - 1] = send(slot);
+          send(slot, RING - 1);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
     } else {
-      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
+      start();
       char *tk = tiles[wave][0][0], *tv = tiles[wave][0][1];
       int x = x0;
       if (count > 0)
@@ -908,12 +966,9 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         const uint32_t seen = load.tokens_there();
         if (n + 1 < count)
           load.fetch(x + UNIT);
-        take_in(x, seen, 0);
+        take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, 0);
       }
     }
-
-    if (!I8 && __builtin_expect(odd, 0))
-      r.add_odd(a, it, row0, rows, x0, x_end, UNIT, lane);
 
     // ---- the waves' sums, where their tiles were
     float(*sums)[16][DP + 4] = reinterpret_cast<float(*)[16][DP + 4]>(room);
@@ -933,11 +988,14 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
 #pragma unroll
         for (int e = 0; e < E; ++e)
           *reinterpret_cast<f32x4 *>(&sums[wave][c][e * 16 + 4 * g]) = r.acc[0][e] * f;
+      if (!I8 && __builtin_expect(odd, 0))
+        r.add_odd(it, row0, rows, x0, x_end, UNIT, lane, [&](int, int d, float v) { sums[wave][c][d] += v * f; });
     }
     __syncthreads();
     constexpr int DIMS = 16 * DP / (64 * W); // of a thread: sixteen rows over the workgroup
     const int i = tid / (DP / DIMS), d0 = (tid % (DP / DIMS)) * DIMS;
     if (i < rows) {
+      const AttendArgs &a = args_again();
       float m = kNone, l = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w)
@@ -1002,50 +1060,53 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
     odd_of[tid] = 0;
   add_up<ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
+  const Reads<DP, false> reads(lane);
   if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
     for (int i = tid * 16; i < RING * 2 * TILE; i += 64 * W * 16)
       *reinterpret_cast<u32x4 *>(&tiles[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
 
   for (int turn = 0; run.unit < run.end; turn ^= 1) {
-    const Item it = take<ROWS, UNIT>(a, schedule, run);
+    const Item it = take<ROWS, UNIT>(args_again(), schedule, run);
     int &odd = odd_of[turn];
     const int row0 = (it.tile * W + wave) * 16 * RT;                // the wave's first
-    const int rows = it.fresh * static_cast<int>(a.group.d) - row0; // and how many from there
-    load.item(a, it);
+    const int rows = it.fresh * static_cast<int>(args_again().group.d) - row0; // and how many from there
+    load.item(args_again(), it);
     const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.length);
     const int count = x0 < x_end ? (x_end - x0 + kTile - 1) / kTile : 0;
-    auto is_cut = [&](int x, uint32_t seen) { return seen != 0xffffffffu || x + kTile > it.cached; };
     // this wave's tokens of a tile that it has brought, before the others may read them
-    auto clean_own = [&](int x, uint32_t seen, int slot) {
-      if (!I8 && __builtin_expect(is_cut(x, seen), 0) &&
+    auto clean_own = [&](int x, uint32_t seen, bool cut, int slot) {
+      if (!I8 && __builtin_expect(cut, 0) &&
           clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, x + kTile > it.cached, lane) && lane == 0)
         odd = 1;
     };
-    auto take_in = [&](int x, uint32_t seen, int slot) {
+    const uint32_t at = place(tiles[0][0]);
+    auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
       if (rows > 0) // the same for the whole wave
-        r.step(a, it, row0, x, seen, is_cut(x, seen), tiles[slot][0], tiles[slot][1], lane);
+        r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
+    };
+    auto start = [&] {
+      const AttendArgs &b = args_again();
+      r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
     };
     __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
     if (tid == 0)
       odd_of[turn ^ 1] = 0;
 
     if constexpr (SRC == kAsync) {
-      int id0 = load.entry(x0), id1 = load.entry(x0 + 16); // of the next tile to send
+      typename Load::Next next = load.look(x0); // the next tile to send
+      uint32_t on = 0u;                         // of the tiles on their way: their halves on a page
       int xs = x0;
-      const uint32_t at = place(tiles[0][0]);
-      auto send = [&](int slot) {
-        load.send(xs, id0, id1, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
-        const uint32_t s = load.seen(xs, id0, id1);
+      auto send = [&](int slot, int place) {
+        load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        on |= load.halves(next) << (2 * place);
         xs += kTile;
-        id0 = load.entry(xs);
-        id1 = load.entry(xs + 16);
-        return s;
+        next = load.look(xs);
       };
-      uint32_t seen[RING - 1]; // of the tiles on their way
 #pragma unroll
       for (int i = 0; i < RING - 1; ++i)
-        seen[i] = i < count ? send(i) : 0u;
-      r.start(a, it, row0, rows, a.scale, lane);
+        if (i < count)
+          send(i, i);
+      start();
       int x = x0, slot = 0;
 #pragma clang loop unroll(disable)
       for (int n = 0; n < count; ++n, x += kTile) {
@@ -1055,19 +1116,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           arrived<(RING - 2) * 2 * Load::LOADS>();
         else
           arrived<0>();
-        const uint32_t now = seen[0];
-        clean_own(x, now, slot);
+        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
+        const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
+        clean_own(x, seen, cut, slot);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i + 1 < RING - 1; ++i)
-          seen[i] = seen[i + 1];
+        on >>= 2;
         if (n + RING - 1 < count)
-          seen[RING - 2] = send(slot == 0 ? RING - 1 : slot - 1);
-        take_in(x, now, slot);
+          send(slot == 0 ? RING - 1 : slot - 1, RING - 2);
+        take_in(x, seen, cut, slot);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
     } else {
-      r.start(a, it, row0, rows, I8 ? a.scale * a.key_scale[it.head] : a.scale, lane);
+      start();
       int x = x0;
       auto put = [&](int slot) {
         load.put(tiles[slot][0], tiles[slot][1]);
@@ -1075,7 +1135,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         if (lane == 0)
           tokens[slot][wave] = static_cast<uint8_t>(t);
         const int xp = x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile); // the tile put: this one or the next
-        clean_own(xp, t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W))), slot);
+        const uint32_t seen = t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W)));
+        clean_own(xp, seen, seen != 0xffffffffu || xp + kTile > it.cached, slot);
       };
       if (count > 0) {
         load.fetch(x);
@@ -1095,15 +1156,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           put(slot ^ 1);
         if (n + 2 < count)
           load.fetch(x + 2 * kTile);
-        take_in(x, seen, slot);
+        take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, slot);
       }
     }
 
     __syncthreads();
-    if (!I8 && __builtin_expect(odd, 0))
-      r.add_odd(a, it, row0, rows, x0, x_end, kTile, lane);
-
+    const bool any_odd = !I8 && odd;
     // ---- every wave's rows are its own
+    const AttendArgs &b = args_again();
     const bool whole = it.s0 == 0 && it.s1 == it.units;
     const int ln = anew(lane), c = ln & 15, g = ln >> 4;
 #pragma unroll
@@ -1113,30 +1173,46 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         continue;
       if (whole) {
         const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
-        const uint32_t j = fdiv(p, a.group);
+        const uint32_t j = fdiv(p, b.group);
         const int64_t row = it.start + static_cast<int64_t>(j);
-        const int64_t qh = static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d);
-        const float f = finish(sum, I8 ? a.value_scale[it.head] : 1.0f);
-        char *dst = a.out + (row * a.out_row + qh * a.out_head + 4 * g) * 2;
+        const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
+        const float f = finish(sum, I8 ? b.value_scale[it.head] : 1.0f);
+        char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (e * 16 + 4 * g < a.dim) {
+          if (e * 16 + 4 * g < b.dim) {
             const f32x4 o = r.acc[t][e] * f;
             store(dst + e * 32, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
           }
-        if (a.lse && g == 0)
-          a.lse[row * a.heads + qh] = log_sum(r.top[t], sum);
+        if (b.lse && g == 0)
+          b.lse[row * b.heads + qh] = log_sum(r.top[t], sum);
       } else {
         const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
-        float *dst = a.partial + part * DP + 4 * g;
+        float *dst = b.partial + part * DP + 4 * g;
 #pragma unroll
         for (int e = 0; e < E; ++e)
           *reinterpret_cast<f32x4 *>(dst + e * 16) = r.acc[t][e];
         if (g == 0) {
-          a.stats[part * 2] = r.top[t];
-          a.stats[part * 2 + 1] = sum;
+          b.stats[part * 2] = r.top[t];
+          b.stats[part * 2 + 1] = sum;
         }
       }
+    }
+    if (__builtin_expect(any_odd, 0)) {
+      r.add_odd(it, row0, rows, x0, x_end, kTile, lane, [&](int t, int d, float v) {
+        const AttendArgs &b = args_again();
+        const int i = wave * 16 * RT + t * 16 + c;
+        if (!whole) {
+          b.partial[((run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + i) * DP + d] += v;
+          return;
+        }
+        // what is rounded is finite, and what comes to it is not
+        const uint32_t p = static_cast<uint32_t>(it.tile * ROWS + i);
+        const uint32_t j = fdiv(p, b.group);
+        char *o = b.out + ((it.start + static_cast<int64_t>(j)) * b.out_row +
+                           (static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d)) * b.out_head + d) * 2;
+        store(o, static_cast<uint16_t>(pack16<T>(widen16<T>(relx::load<uint16_t>(o)) + v, 0.0f)));
+      });
     }
   }
 }
