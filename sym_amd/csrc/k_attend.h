@@ -756,7 +756,9 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
   __device__ __forceinline__ int entry(int x0) const {
     return x0 < length ? scalar_load(table + fdiv(static_cast<uint32_t>(x0), page)) : -1;
   }
-  // The entries of a tile's two halves, and the places in their pages; kAsync.
+  // The entries of a tile's two halves, and the places in their pages (past the
+  // length: the last page's first), where there are tokens; kAsync. No branch:
+  // what is loaded is not looked at before the tile is sent.
   struct Next {
     int id[2];
     uint32_t off[2];
@@ -765,9 +767,10 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
     Next t;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t x0 = static_cast<uint32_t>(x) + h * 16, n = fdiv(x0, page);
-      t.id[h] = static_cast<int>(x0) < length ? scalar_load(table + n) : -1;
-      t.off[h] = x0 - n * page.d;
+      const int x0 = x + h * 16;
+      const uint32_t at = static_cast<uint32_t>(min(x0, length - 1)), n = fdiv(at, page);
+      t.id[h] = scalar_load(table + n);
+      t.off[h] = x0 < length ? at - n * page.d : 0u;
     }
     return t;
   }
@@ -925,20 +928,23 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         for (int i = lane * 16; i < RING * 2 * TILE; i += 64 * 16)
           *reinterpret_cast<u32x4 *>(&tiles[wave][0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
       shared_done();
-      typename Load::Next next = load.look(x0); // the next tile to send
-      uint32_t on = 0u;                         // of the tiles on their way: their halves on a page
-      int xs = x0;
-      auto send = [&](int slot, int place) {
+      uint32_t on = 0u; // of the tiles on their way: their halves on a page
+      auto send = [&](const typename Load::Next &next, int slot, int place) {
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
         on |= load.halves(next) << (2 * place);
-        xs += UNIT;
-        next = load.look(xs);
       };
+      typename Load::Next next[RING + 1];
+      if (count > 0) {
 #pragma unroll
-      for (int i = 0; i < RING; ++i)
-        if (i < count)
-          send(i, i);
+        for (int i = 0; i <= RING; ++i)
+          next[i] = load.look(x0 + i * UNIT);
+#pragma unroll
+        for (int i = 0; i < RING; ++i)
+          if (i < count)
+            send(next[i], i, i);
+      }
       start();
+      typename Load::Next then = next[RING];
       int x = x0;
       int slot = 0;
 #pragma clang loop unroll(disable)
@@ -952,7 +958,8 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         shared_done(); // its place is free
         on >>= 2;
         if (n + RING < count)
-          send(slot, RING - 1);
+          send(then, slot, RING - 1);
+        then = load.look(x + (RING + 1) * UNIT);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
     } else {
@@ -1080,33 +1087,42 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         odd = 1;
     };
     const uint32_t at = place(tiles[0][0]);
+    __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
+    if (tid == 0)
+      odd_of[turn ^ 1] = 0;
+
+    // A wave without rows brings its tokens all the same. Two loops, so that
+    // in neither the sums meet a way round them.
+    auto work = [&](auto busy) {
+    constexpr bool BUSY = decltype(busy)::value;
     auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
-      if (rows > 0) // the same for the whole wave
+      if constexpr (BUSY)
         r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
     };
     auto start = [&] {
       const AttendArgs &b = args_again();
       r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
     };
-    __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
-    if (tid == 0)
-      odd_of[turn ^ 1] = 0;
 
     if constexpr (SRC == kAsync) {
-      typename Load::Next next = load.look(x0); // the next tile to send
-      uint32_t on = 0u;                         // of the tiles on their way: their halves on a page
-      int xs = x0;
-      auto send = [&](int slot, int place) {
+      uint32_t on = 0u; // of the tiles on their way: their halves on a page
+      auto send = [&](const typename Load::Next &next, int slot, int place) {
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
         on |= load.halves(next) << (2 * place);
-        xs += kTile;
-        next = load.look(xs);
       };
+      typename Load::Next next[RING];
+      if (count > 0) {
 #pragma unroll
-      for (int i = 0; i < RING - 1; ++i)
-        if (i < count)
-          send(i, i);
-      start();
+        for (int i = 0; i < RING; ++i)
+          next[i] = load.look(x0 + i * kTile);
+#pragma unroll
+        for (int i = 0; i < RING - 1; ++i)
+          if (i < count)
+            send(next[i], i, i);
+      }
+      if constexpr (BUSY)
+        start();
+      typename Load::Next then = next[RING - 1];
       int x = x0, slot = 0;
 #pragma clang loop unroll(disable)
       for (int n = 0; n < count; ++n, x += kTile) {
@@ -1122,12 +1138,17 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         __syncthreads();
         on >>= 2;
         if (n + RING - 1 < count)
-          send(slot == 0 ? RING - 1 : slot - 1, RING - 2);
+          send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
         take_in(x, seen, cut, slot);
+        // here, where no read of shared memory is waited for: scalar loads
+        // come in any order, so a wait beside them is one for all
+        keep_order();
+        then = load.look(x + RING * kTile);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
     } else {
-      start();
+      if constexpr (BUSY)
+        start();
       int x = x0;
       auto put = [&](int slot) {
         load.put(tiles[slot][0], tiles[slot][1]);
@@ -1161,6 +1182,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
     }
 
     __syncthreads();
+    if constexpr (!BUSY)
+      return;
     const bool any_odd = !I8 && odd;
     // ---- every wave's rows are its own
     const AttendArgs &b = args_again();
@@ -1214,6 +1237,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         store(o, static_cast<uint16_t>(pack16<T>(widen16<T>(relx::load<uint16_t>(o)) + v, 0.0f)));
       });
     }
+    };
+    if (rows > 0) // the same for the whole wave
+      work(std::true_type());
+    else
+      work(std::false_type());
   }
 }
 
