@@ -65,8 +65,8 @@ enum Source : int { kAsync, kStaged, kStagedEven };
 // Where a row's reference maximum starts: finite, so that a difference with a
 // masked score's -inf stays -inf.
 constexpr float kNone = -3.402823466e38f;
-// A row's reference maximum moves only once a lane's weights of a tile add up
-// to more than two to this; until then they are summed as they are.
+// A row's reference maximum moves only once a score exceeds it by this many
+// powers of two; until then weights up to 2^8 are summed as they are.
 constexpr float kSlack = 8.0f;
 
 template <class T> struct __attribute__((packed)) Loose { T v; };
@@ -571,9 +571,9 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     return ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
   }
 
-  // Weights go by the maximum so far. Whether that still does shows in their
-  // own sum, so a tile's maximum is looked for only where it does not: in a
-  // row's first tile and a few later ones.
+  // Weights go by the reference maximum, which moves only where some lane has
+  // seen a score far above it: in a row's first tile and a few later ones. So
+  // lanes compare theirs then and not at every tile.
   __device__ __forceinline__ void soften(const Item &it, int row0, int x, uint32_t seen, bool cut, int lane_) {
     constexpr float kBias = weight_bias<T>();
     if (__builtin_expect(cut, 0)) {
@@ -601,13 +601,12 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           most[t] = fmaxf(most[t], s[t][n][i]);
-      most[t] = max_over_groups(most[t]) * scale;
-      above |= most[t] > top[t] + (kBias + kSlack);
+      above |= most[t] * scale > top[t] + (kBias + kSlack);
     }
     if (__builtin_expect(__any(above), 0)) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const float next = fmaxf(top[t], most[t] - kBias);
+        const float next = fmaxf(top[t], max_over_groups(most[t]) * scale - kBias);
         const float shrink = __builtin_amdgcn_exp2f(top[t] - next);
         top[t] = next;
         sum[t] *= shrink;
