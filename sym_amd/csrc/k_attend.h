@@ -257,6 +257,12 @@ __device__ __forceinline__ Run my_run(const Schedule &sh) {
   return r;
 }
 
+// Partial sums of 16 rows lie as the lanes hold them: a store, and a load of the
+// join, is one piece of memory. Where dim d of row i of a part lies.
+template <int DP> __device__ __forceinline__ int part_at(int i, int d) {
+  return (i >> 4) * 16 * DP + (((d >> 4) * 4 + ((d >> 2) & 3)) * 16 + (i & 15)) * 4 + (d & 3);
+}
+
 // The part of an item that lies in a run: the units [s0, s1) of its `units`.
 struct Item {
   int b, start, fresh, head, tile, cached, length, s0, s1, units;
@@ -299,17 +305,28 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   return i;
 }
 
-// What the p-th query row of the item's request and key head sees of the 32
-// tokens from `x`, as bits.
-__device__ __forceinline__ uint32_t row_sees(const AttendArgs &a, const Item &it, int p, int x) {
+// What the j-th new token sees of the 32 tokens from `x`, as bits: all cached
+// ones, and of the new ones those in its `mask` or, without one, up to itself.
+__device__ __forceinline__ uint32_t sees(const Item &it, bool masked, int j, uint64_t mask, int x) {
   const int d = x - it.cached; // the first token's place among the new ones
   if (d + 32 <= 0)
     return 0xffffffffu;
-  const int j = static_cast<int>(fdiv(static_cast<uint32_t>(p), a.group)); // the row's own place there
-  if (!a.mask) {
+  if (!masked) {
     const int n = j - d + 1;
     return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
   }
+  const int old = d < 0 ? -d : 0; // cached tokens among the 32
+  const uint64_t m = d <= 0 ? mask : d < 64 ? mask >> d : 0u;
+  return static_cast<uint32_t>(m << old) | ((1u << old) - 1u);
+}
+
+// The same for the p-th query row of the item's request and key head, with a
+// mask of any length.
+__device__ __forceinline__ uint32_t row_sees(const AttendArgs &a, const Item &it, int p, int x) {
+  const int j = static_cast<int>(fdiv(static_cast<uint32_t>(p), a.group));
+  const int d = x - it.cached;
+  if (!a.mask || d + 32 <= 0)
+    return sees(it, false, j, 0u, x);
   if (j >= it.fresh)
     return 0u;
   const int64_t *mask = a.mask + (it.start + static_cast<int64_t>(j)) * a.words;
@@ -319,7 +336,7 @@ __device__ __forceinline__ uint32_t row_sees(const AttendArgs &a, const Item &it
     m = static_cast<uint64_t>(mask[word]) >> sh;
   if (sh > 32 && word + 1 < a.words)
     m |= static_cast<uint64_t>(mask[word + 1]) << (64 - sh);
-  const int old = d < 0 ? -d : 0; // cached tokens among the 32
+  const int old = d < 0 ? -d : 0;
   return static_cast<uint32_t>(m << old) | ((1u << old) - 1u);
 }
 
@@ -385,6 +402,13 @@ __device__ __forceinline__ void load_async(const char *base, uint32_t at, uint32
                : "s"(uniform(static_cast<int>(to))), "v"(at), "s"(uniform64(reinterpret_cast<int64_t>(base)))
                : "memory");
 }
+// The same for four bytes a lane.
+__device__ __forceinline__ void load_async4(const void *base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(uniform(static_cast<int>(to))), "v"(at), "s"(uniform64(reinterpret_cast<int64_t>(base)))
+               : "memory");
+}
 template <int N> __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
@@ -408,6 +432,17 @@ template <int DP, bool RAW> struct Reads {
     else
       value = piece<RB>(4 * g + (c >> 2), (c & 3) >> 1) + (c & 1) * 8;
   }
+};
+
+// Waits for the workgroup's other waves, and for no memory.
+__device__ __forceinline__ void meet() {
+  asm volatile("" : : : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
+}
+
+struct NoValues {
+  __device__ __forceinline__ explicit NoValues(uint32_t) {}
 };
 
 // A tile's values as operands: at(e) has dim 16 e + lane % 16 of the lane's eight
@@ -486,16 +521,24 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   float top[RT];     // reference maximum of a row's scaled scores
   float sum[RT];     // of its weights, over this lane's tokens; total(): over all
   f32x4 acc[RT][E];  // dims 16 e + 4 (lane / 16) + 0..3
+  int place[RT];     // among the request's new tokens
+  uint64_t mask[RT]; // of one word
   float scale;
+  int words;         // of a mask; 0: none
 
   __device__ __forceinline__ void start(const AttendArgs &a, const Item &it, int row0, int rows, float score_scale,
                                         int lane) {
     const int c = lane & 15, g = lane >> 4;
     scale = score_scale;
+    words = a.mask ? a.words : 0;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
       const uint32_t j = fdiv(p, a.group);
+      place[t] = static_cast<int>(j);
+      mask[t] = 0u;
+      if (words == 1 && place[t] < it.fresh)
+        mask[t] = static_cast<uint64_t>(a.mask[it.start + static_cast<int64_t>(j)]);
       const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
                                (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma unroll
@@ -528,16 +571,19 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   f32x4 s[RT][2];     // scores, unscaled
   u32x4 weights[RT];
 
+  static constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
+  u32x4 k[2][KR];
+
   // from: the tile's place and the lane's first piece in it
-  __device__ __forceinline__ void scores(uint32_t from) {
-    constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
-    u32x4 k[2][KR];
+  __device__ __forceinline__ void read_keys(uint32_t from) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < KR; ++i)
         k[n][i] = read16((from ^ (i * 64)) + n * 16 * DP * (RAW ? 1 : 2));
     keep_order(); // all reads on their way before the first is waited for
+  }
+  __device__ __forceinline__ void scores() {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -577,11 +623,11 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   __device__ __forceinline__ void soften(const Item &it, int row0, int x, uint32_t seen, bool cut, int lane_) {
     constexpr float kBias = weight_bias<T>();
     if (__builtin_expect(cut, 0)) {
-      const AttendArgs &a = args_again();
       const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const uint32_t bits = seen & row_sees(a, it, row0 + t * 16 + c, x);
+        const uint32_t bits = seen & (words > 1 ? row_sees(args_again(), it, row0 + t * 16 + c, x)
+                                                : sees(it, words == 1, place[t], mask[t], x));
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -633,7 +679,8 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   // tk, tv: the places of the tile's keys and values.
   __device__ __forceinline__ void step(const Item &it, int row0, int x, uint32_t seen, bool cut, uint32_t tk, uint32_t tv,
                                        const Reads<DP, RAW> &reads, int lane) {
-    scores(tk + reads.key);
+    read_keys(tk + reads.key);
+    scores();
     const Values<T, DP, RAW, EARLY> v(tv + reads.value); // EARLY: they arrive during the softmax
     soften(it, row0, x, seen, cut, lane);
     add(v);
@@ -693,8 +740,8 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 };
 
 // How a wave brings its tokens of a tile into shared memory: NT tokens from
-// `first`, of every tile.
-template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
+// `first`, of every tile. Its tiles are PACE tokens apart.
+template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Loader {
   static constexpr int CELL = I8 ? 1 : 2;
   static constexpr int LB = 16 / CELL;                     // dims of a lane's load
   static constexpr int TL = DP / LB;                       // lanes of a token
@@ -756,20 +803,40 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW> struct Loader {
     return x0 < length ? scalar_load(table + fdiv(static_cast<uint32_t>(x0), page)) : -1;
   }
   // The entries of a tile's two halves, and the places in their pages (past the
-  // length: the last page's first), where there are tokens; kAsync. No branch:
-  // what is loaded is not looked at before the tile is sent.
+  // length: the last page's first); kAsync, where there are tokens. A wave keeps
+  // the entries of kAhead tiles in its lanes, and brings the next ones through
+  // shared memory like the tiles: no wait, neither for them nor, as scalar loads
+  // would make it, for reads of shared memory.
+  static constexpr int kAhead = 32;
   struct Next {
     int id[2];
     uint32_t off[2];
   };
-  __device__ __forceinline__ Next look(int x) const {
+  int entries;   // of tile lane / 2, half lane % 2
+  uint32_t room; // [2][64] of this wave
+  __device__ __forceinline__ uint32_t entry_at(int x, int lane) const {
+    return fdiv(static_cast<uint32_t>(min(x + (lane >> 1) * PACE + (lane & 1) * 16, length - 1)), page) * 4u;
+  }
+  // The first entries, and the next on their way.
+  __device__ __forceinline__ void first_entries(int x, int count, int lane) {
+    entries = *reinterpret_cast<const int32_t *>(reinterpret_cast<const char *>(table) + entry_at(x, lane));
+    if (count > kAhead)
+      load_async4(table, entry_at(x + kAhead * PACE, lane), room + 256);
+  }
+  // The n-th tile, at x; called for one after the other.
+  __device__ __forceinline__ Next look(int n, int x, int lane) {
+    if (n > 0 && n % kAhead == 0) {
+      const uint32_t half = n / kAhead % 2 * 256;
+      entries = *reinterpret_cast<const __attribute__((address_space(3))) int *>(room + half + lane * 4);
+      load_async4(table, entry_at(x + kAhead * PACE, lane), room + (half ^ 256));
+    }
     Next t;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int x0 = x + h * 16;
-      const uint32_t at = static_cast<uint32_t>(min(x0, length - 1)), n = fdiv(at, page);
-      t.id[h] = scalar_load(table + n);
-      t.off[h] = x0 < length ? at - n * page.d : 0u;
+      t.id[h] = __builtin_amdgcn_readlane(entries, n % kAhead * 2 + h);
+      const uint32_t at = static_cast<uint32_t>(min(x0, length - 1));
+      t.off[h] = x0 < length ? at - fdiv(at, page) * page.d : 0u;
     }
     return t;
   }
@@ -887,7 +954,8 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
   constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
   constexpr int TILE = kTile * DP * (I8 ? 1 : 2);
   constexpr int RING = SRC == kAsync ? 2 : 1; // tiles of a wave
-  using Load = Loader<T, I8, DP, SRC, kTile, I8>;
+  using Load = Loader<T, I8, DP, SRC, kTile, I8, UNIT>;
+  __shared__ int entries[SRC == kAsync ? W : 1][2][64];
 
   __shared__ Schedule schedule;
   constexpr int SUMS = W * 16 * (DP + 4) * sizeof(float); // the waves', at the end
@@ -898,6 +966,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   Load load(a, lane, 0);
+  load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
   Rows<T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
   const Reads<DP, I8> reads(lane);
   add_up<ROWS, UNIT>(a, schedule);
@@ -934,9 +1003,10 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
       };
       typename Load::Next next[RING + 1];
       if (count > 0) {
+        load.first_entries(x0, count, lane);
 #pragma unroll
         for (int i = 0; i <= RING; ++i)
-          next[i] = load.look(x0 + i * UNIT);
+          next[i] = load.look(i, x0 + i * UNIT, lane);
 #pragma unroll
         for (int i = 0; i < RING; ++i)
           if (i < count)
@@ -958,9 +1028,10 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         on >>= 2;
         if (n + RING < count)
           send(then, slot, RING - 1);
-        then = load.look(x + (RING + 1) * UNIT);
+        then = load.look(n + RING + 1, x + (RING + 1) * UNIT, lane);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
+      arrived<0>(); // the last entries, wanted or not
     } else {
       start();
       char *tk = tiles[wave][0][0], *tv = tiles[wave][0][1];
@@ -1023,7 +1094,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         for (int w = 1; w < W; ++w)
           o += *reinterpret_cast<const f32x4 *>(&sums[w][i][d0 + d]);
         if (!all) {
-          *reinterpret_cast<f32x4 *>(a.partial + part * DP + d0 + d) = o;
+          *reinterpret_cast<f32x4 *>(a.partial + (part - i) * DP + part_at<DP>(i, d0 + d)) = o;
         } else if (d0 + d < a.dim) {
           o *= f;
           store(a.out + (row * a.out_row + qh * a.out_head + d0 + d) * 2,
@@ -1051,7 +1122,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   constexpr int TILE = kTile * DP * 2;
   // tiles at a time: 64 KiB for each four waves
   constexpr int RING = SRC != kAsync ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
-  using Load = Loader<T, I8, DP, SRC, kTile / W, false>;
+  // A tile's keys are read during the products of the one before.
+  constexpr bool AHEAD = SRC == kAsync && RING > 2;
+  using Load = Loader<T, I8, DP, SRC, kTile / W, false, kTile>;
+  __shared__ int entries[SRC == kAsync ? W : 1][2][64];
 
   __shared__ Schedule schedule;
   __shared__ __attribute__((aligned(16))) char tiles[RING][2][TILE];
@@ -1060,6 +1134,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Load load(a, lane, wave * (kTile / W));
+  load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
   constexpr bool EARLY = DP <= 128 && (I8 || SRC == kAsync); // where the registers hold them
   Rows<T, DP, RT, false, EARLY> r;
   if (tid < 2)
@@ -1084,14 +1159,16 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
       if (!I8 && __builtin_expect(cut, 0) &&
           clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, x + kTile > it.cached, lane) && lane == 0)
         odd = 1;
+      if (!I8 && __builtin_expect(cut, 0))
+        shared_done();
     };
     const uint32_t at = place(tiles[0][0]);
     __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`
     if (tid == 0)
       odd_of[turn ^ 1] = 0;
 
-    // A wave without rows brings its tokens all the same. Two loops, so that
-    // in neither the sums meet a way round them.
+    // A wave without rows brings its tokens all the same. Loops of their own, so
+    // that in none the sums meet a way round them.
     auto work = [&](auto busy) {
     constexpr bool BUSY = decltype(busy)::value;
     auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
@@ -1111,40 +1188,77 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
       };
       typename Load::Next next[RING];
       if (count > 0) {
+        load.first_entries(x0, count, lane);
 #pragma unroll
         for (int i = 0; i < RING; ++i)
-          next[i] = load.look(x0 + i * kTile);
+          next[i] = load.look(i, x0 + i * kTile, lane);
+      }
+      if constexpr (BUSY)
+        start(); // the queries arrive while the table does
+      if (count > 0) {
 #pragma unroll
         for (int i = 0; i < RING - 1; ++i)
           if (i < count)
             send(next[i], i, i);
       }
-      if constexpr (BUSY)
-        start();
       typename Load::Next then = next[RING - 1];
       int x = x0, slot = 0;
-#pragma clang loop unroll(disable)
-      for (int n = 0; n < count; ++n, x += kTile) {
-        // this wave's part of the tile has arrived, then everybody's; and
-        // everybody is done with the tile before, whose place the next takes
-        if (n + RING - 1 <= count)
-          arrived<(RING - 2) * 2 * Load::LOADS>();
+      const int last = x0 + (count - 1) * kTile;
+      uint32_t seen = 0xffffffffu;
+      bool cut = false;
+      // Waits for this wave's part of the tile at x, of which SENT later ones
+      // are on their way, and looks it over.
+      auto receive = [&](auto sent, int x, int slot) {
+        constexpr int SENT = decltype(sent)::value;
+        if (x + SENT * kTile <= last)
+          arrived<SENT * 2 * Load::LOADS>();
         else
           arrived<0>();
-        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
-        const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
+        cut = (on & 3u) != 3u || x + kTile > it.cached;
+        seen = cut ? load.seen(x, on) : 0xffffffffu;
         clean_own(x, seen, cut, slot);
-        __syncthreads();
         on >>= 2;
-        if (n + RING - 1 < count)
-          send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
-        take_in(x, seen, cut, slot);
-        // here, where no read of shared memory is waited for: scalar loads
-        // come in any order, so a wait beside them is one for all
-        keep_order();
-        then = load.look(x + RING * kTile);
-        slot = slot + 1 == RING ? 0 : slot + 1;
+      };
+      if constexpr (AHEAD) {
+        if (count > 0)
+          receive(std::integral_constant<int, RING - 2>(), x, 0);
+        meet();
+        if constexpr (BUSY)
+          r.read_keys(at + reads.key);
+#pragma clang loop unroll(disable)
+        for (int n = 0; x <= last; ++n, x += kTile) {
+          const uint32_t tile = at + slot * 2 * TILE;
+          if constexpr (BUSY)
+            r.scores();
+          const typename std::conditional<BUSY, Values<T, DP, false, EARLY>, NoValues>::type v(tile + TILE + reads.value);
+          if constexpr (BUSY)
+            r.soften(it, row0, x, seen, cut, lane);
+          const int free = slot == 0 ? RING - 1 : slot - 1;
+          slot = slot + 1 == RING ? 0 : slot + 1;
+          if (x < last)
+            receive(std::integral_constant<int, RING - 3>(), x + kTile, slot);
+          meet(); // everybody's part of the next tile is there, and the tile before has been read
+          if (x + (RING - 1) * kTile <= last)
+            send(then, free, RING - 2);
+          if constexpr (BUSY) {
+            r.read_keys(at + slot * 2 * TILE + reads.key); // after the last tile: not used
+            r.add(v);
+          }
+          then = load.look(n + RING, x + RING * kTile, lane);
+        }
+      } else {
+#pragma clang loop unroll(disable)
+        for (int n = 0; x <= last; ++n, x += kTile) {
+          receive(std::integral_constant<int, RING - 2>(), x, slot);
+          meet(); // everybody's part of the tile is there, and the tile before has been read
+          if (x + (RING - 1) * kTile <= last)
+            send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
+          take_in(x, seen, cut, slot);
+          then = load.look(n + RING, x + RING * kTile, lane);
+          slot = slot + 1 == RING ? 0 : slot + 1;
+        }
       }
+      arrived<0>(); // the last entries, wanted or not
     } else {
       if constexpr (BUSY)
         start();
@@ -1210,10 +1324,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           b.lse[row * b.heads + qh] = log_sum(r.top[t], sum);
       } else {
         const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
-        float *dst = b.partial + part * DP + 4 * g;
+        float *dst = b.partial + (part - c) * DP + part_at<DP>(c, 4 * g);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          *reinterpret_cast<f32x4 *>(dst + e * 16) = r.acc[t][e];
+          *reinterpret_cast<f32x4 *>(dst + e * 256) = r.acc[t][e];
         if (g == 0) {
           b.stats[part * 2] = r.top[t];
           b.stats[part * 2 + 1] = sum;
@@ -1225,7 +1339,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         const AttendArgs &b = args_again();
         const int i = wave * 16 * RT + t * 16 + c;
         if (!whole) {
-          b.partial[((run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + i) * DP + d] += v;
+          b.partial[(run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS * DP + part_at<DP>(i, d)] += v;
           return;
         }
         // what is rounded is finite, and what comes to it is not
@@ -1245,12 +1359,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
 }
 
 // The rows of items that lie in several workgroups' runs: their partial sums,
-// added up; and zeros for the rows of no request. A wave takes an output row at
-// a time, a column of blocks the rows of a request.
+// added up; and zeros for the rows of no request. A column of blocks takes the
+// rows of a request, a block sixteen of them at a time: its waves share their
+// parts, kParts on their way at once.
 template <int T, bool I8, int DP, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
-  constexpr int N = DP / 64; // dims of a lane
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  constexpr int E = DP / 16, kParts = DP > 128 ? 1 : 2;
+  __shared__ f32x4 sums[4][E][64];
+  __shared__ float tops[4][16], totals[4][16];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int b = blockIdx.x;
   if (b == a.requests) { // rows of no request
     const int r0 = min(max(a.starts[0], 0), a.rows), r1 = min(max(a.starts[a.requests], r0), a.rows);
@@ -1269,52 +1386,92 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
   const Request r = attend_request<ROWS, UNIT>(a, b);
   const int64_t total = a.schedule[a.requests], first = a.schedule[b];
   const int64_t per = (total + a.workgroups - 1) / a.workgroups;
-  const int64_t count = static_cast<int64_t>(r.fresh) * a.heads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.y) * 4 + wave; i < count; i += static_cast<int64_t>(gridDim.y) * 4) {
-    const int j = static_cast<int>(i / a.heads), qh = static_cast<int>(i - static_cast<int64_t>(j) * a.heads);
-    const int head = static_cast<int>(fdiv(static_cast<uint32_t>(qh), a.group));
-    const int p = j * static_cast<int>(a.group.d) + qh - head * static_cast<int>(a.group.d);
-    const int tile = p / ROWS, row = p % ROWS;
-    const int64_t u0 = first + (static_cast<int64_t>(head) * r.tiles + tile) * r.units;
-    const int64_t w0 = u0 / per, w1 = (u0 + r.units - 1) / per;
+  const int64_t rows = static_cast<int64_t>(r.fresh) * a.group.d, sixteens = (rows + 15) / 16;
+  for (int64_t i = blockIdx.y; i < sixteens * a.kv_heads; i += gridDim.y) {
+    const int head = static_cast<int>(i / sixteens), row0 = static_cast<int>(i - head * sixteens) * 16;
+    const int64_t u0 = first + (static_cast<int64_t>(head) * r.tiles + row0 / ROWS) * r.units;
+    const int64_t w0 = uniform64(u0 / per), w1 = uniform64((u0 + r.units - 1) / per);
     if (w0 == w1)
       continue; // written whole
-    // a run that begins inside the item left its part in its first place, the
-    // run in which the item begins in its second
-    auto at = [&](int64_t w) { return (w * 2 + (w == w0 ? 1 : 0)) * ROWS + row; };
-    float most = kNone;
-    for (int64_t w = w0 + lane; w <= w1; w += 64)
-      most = fmaxf(most, a.stats[at(w) * 2]);
+    float top = kNone, sum = 0.0f;
+    f32x4 acc[E];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-      most = fmaxf(most, __shfl_xor(most, o));
-    float sum = 0.0f, out[N];
+    for (int e = 0; e < E; ++e)
+      acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t w = w0 + wave; w <= w1; w += 4 * kParts) {
+      f32x4 o[kParts][E];
+      float m[kParts], l[kParts], most = top;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      out[n] = 0.0f;
-#pragma unroll 4
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t k = at(w);
-      const float f = __builtin_amdgcn_exp2f(a.stats[k * 2] - most);
-      sum += a.stats[k * 2 + 1] * f;
+      for (int k = 0; k < kParts; ++k) {
+        // a run that begins inside the item left its part in its first place,
+        // the run in which the item begins in its second
+        const bool is = w + 4 * k <= w1;
+        const int64_t at = ((is ? w + 4 * k : w) * 2 + (w == w0 && (k == 0 || !is) ? 1 : 0)) * ROWS + row0 % ROWS;
+        m[k] = is ? a.stats[(at + c) * 2] : kNone;
+        l[k] = is ? a.stats[(at + c) * 2 + 1] : 0.0f;
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        out[n] += a.partial[k * DP + lane * N + n] * f;
-    }
-    const float f = finish(sum, I8 ? a.value_scale[head] : 1.0f);
-    const int64_t orow = r.start + static_cast<int64_t>(j);
-    char *dst = a.out + (orow * a.out_row + qh * a.out_head + lane * N) * 2;
-    if (lane * N < a.dim) {
-      if constexpr (N == 1) {
-        store(dst, static_cast<uint16_t>(pack16<T>(out[0] * f, 0.0f)));
-      } else {
-#pragma unroll
-        for (int n = 0; n < N; n += 2)
-          store(dst + n * 2, pack16<T>(out[n] * f, out[n + 1] * f));
+        for (int e = 0; e < E; ++e)
+          o[k][e] = *reinterpret_cast<const f32x4 *>(a.partial + at * DP + (e * 64 + lane) * 4);
       }
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+        most = fmaxf(most, m[k]);
+      const float f = __builtin_amdgcn_exp2f(top - most);
+      top = most;
+      sum *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        acc[e] *= f;
+#pragma unroll
+      for (int k = 0; k < kParts; ++k)
+        if (w + 4 * k <= w1) {
+          const float fk = __builtin_amdgcn_exp2f(m[k] - top);
+          sum += l[k] * fk;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            acc[e] += o[k][e] * fk;
+        }
     }
-    if (a.lse && lane == 0)
-      a.lse[orow * a.heads + qh] = log_sum(most, sum);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      sums[wave][e][lane] = acc[e];
+    if (g == 0) {
+      tops[wave][c] = top;
+      totals[wave][c] = sum;
+    }
+    __syncthreads();
+    top = kNone;
+    sum = 0.0f;
+    float f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      top = fmaxf(top, tops[k][c]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[k] = __builtin_amdgcn_exp2f(tops[k][c] - top);
+      sum += totals[k][c] * f[k];
+    }
+    if (row0 + c < rows) {
+      const uint32_t p = static_cast<uint32_t>(row0 + c);
+      const uint32_t j = fdiv(p, a.group);
+      const int64_t row = r.start + static_cast<int64_t>(j);
+      const int64_t qh = static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d);
+      const float scale = finish(sum, I8 ? a.value_scale[head] : 1.0f);
+#pragma unroll
+      for (int n = 0; n < E / 4; ++n) {
+        const int e = wave * (E / 4) + n, d = e * 16 + 4 * g;
+        f32x4 o = sums[0][e][lane] * f[0];
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+          o += sums[k][e][lane] * f[k];
+        o *= scale;
+        if (d < a.dim)
+          store(a.out + (row * a.out_row + qh * a.out_head + d) * 2, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
+      }
+      if (a.lse && threadIdx.x < 16)
+        a.lse[row * a.heads + qh] = log_sum(top, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -1327,9 +1484,9 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
                                  dim3(static_cast<uint32_t>(threads)), pa, 0, s);
   if (e != hipSuccess)
     return e;
-  // a wave for every output row of an even batch, within 2^16 blocks a request
-  const int64_t rows = (static_cast<int64_t>(a.rows) * a.heads + a.requests - 1) / a.requests;
-  const int64_t y = std::min<int64_t>((rows + 3) / 4, 65535);
+  // a block for every sixteen output rows of an even batch, within 2^16 a request
+  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d;
+  const int64_t y = std::min<int64_t>((rows + 15) / 16 * a.kv_heads, 65535);
   return hipLaunchKernel(reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT>),
                          dim3(static_cast<uint32_t>(a.requests) + 1, static_cast<uint32_t>(y)), dim3(256), pa, 0, s);
 }
