@@ -161,6 +161,14 @@ __device__ __forceinline__ float max_over_groups(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// n / d for n that hardly ever needs more than 32 bits: short code, since a
+// kernel of a few microseconds waits for every line of it to be fetched.
+__device__ __forceinline__ int64_t divide(int64_t n, int d) {
+  if (__builtin_expect(n >> 32 == 0, 1))
+    return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+  return n / d;
+}
+
 // ------------------------------------------------------------ the schedule
 
 struct Request {
@@ -246,9 +254,12 @@ __device__ __forceinline__ void add_up(const AttendArgs &a, Schedule &sh) {
 struct Run {
   int64_t wg, unit, end;
 };
+__device__ __forceinline__ int64_t units_of_run(int64_t total, int workgroups) {
+  return (total + workgroups - 1) >> (31 - __builtin_clz(workgroups)); // a power of two
+}
 __device__ __forceinline__ Run my_run(const Schedule &sh) {
   const int64_t total = uniform64(sh.before[kScan]);
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t per = units_of_run(total, gridDim.x);
   Run r;
   r.wg = static_cast<int64_t>(blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   r.wg = uniform64(r.wg);
@@ -257,10 +268,14 @@ __device__ __forceinline__ Run my_run(const Schedule &sh) {
   return r;
 }
 
-// Partial sums of 16 rows lie as the lanes hold them: a store, and a load of the
-// join, is one piece of memory. Where dim d of row i of a part lies.
-template <int DP> __device__ __forceinline__ int part_at(int i, int d) {
-  return (i >> 4) * 16 * DP + (((d >> 4) * 4 + ((d >> 2) & 3)) * 16 + (i & 15)) * 4 + (d & 3);
+// Partial sums of a part's rows: where dim d of row i lies. The shared kernel's
+// lie as its lanes hold them, sixteen rows by sixteen dims, so that a store is
+// one piece of memory.
+template <int DP, int ROWS> __device__ __forceinline__ int part_at(int i, int d) {
+  if constexpr (ROWS == 16)
+    return i * DP + d;
+  else
+    return (i >> 4) * 16 * DP + (((d >> 4) * 4 + ((d >> 2) & 3)) * 16 + (i & 15)) * 4 + (d & 3);
 }
 
 // The part of an item that lies in a run: the units [s0, s1) of its `units`.
@@ -296,10 +311,10 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   i.fresh = uniform(r.fresh);
   i.units = uniform(r.units);
   const int tiles = uniform(r.tiles);
-  const int64_t item = uniform64((run.unit - at) / i.units);
+  const int64_t item = uniform64(divide(run.unit - at, i.units));
   i.s0 = uniform(static_cast<int>(run.unit - at - item * i.units));
   i.s1 = uniform(static_cast<int>(min(static_cast<int64_t>(i.units), i.s0 + (run.end - run.unit))));
-  i.head = uniform(static_cast<int>(item / tiles));
+  i.head = uniform(static_cast<int>(divide(item, tiles)));
   i.tile = static_cast<int>(item - static_cast<int64_t>(i.head) * tiles);
   run.unit = uniform64(run.unit + i.s1 - i.s0);
   return i;
@@ -1001,19 +1016,15 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
         on |= load.halves(next) << (2 * place);
       };
-      typename Load::Next next[RING + 1];
-      if (count > 0) {
+      if (count > 0)
         load.first_entries(x0, count, lane);
-#pragma unroll
-        for (int i = 0; i <= RING; ++i)
-          next[i] = load.look(i, x0 + i * UNIT, lane);
-#pragma unroll
-        for (int i = 0; i < RING; ++i)
-          if (i < count)
-            send(next[i], i, i);
-      }
-      start();
-      typename Load::Next then = next[RING];
+      start(); // the queries arrive while the table does
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < min(count, RING); ++i)
+        send(load.look(i, x0 + i * UNIT, lane), i, i);
+      typename Load::Next then = {}; // the next tile to send
+      if (count > 0)
+        then = load.look(RING, x0 + RING * UNIT, lane);
       int x = x0;
       int slot = 0;
 #pragma clang loop unroll(disable)
@@ -1094,7 +1105,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
         for (int w = 1; w < W; ++w)
           o += *reinterpret_cast<const f32x4 *>(&sums[w][i][d0 + d]);
         if (!all) {
-          *reinterpret_cast<f32x4 *>(a.partial + (part - i) * DP + part_at<DP>(i, d0 + d)) = o;
+          *reinterpret_cast<f32x4 *>(a.partial + (part - i) * DP + part_at<DP, ROWS>(i, d0 + d)) = o;
         } else if (d0 + d < a.dim) {
           o *= f;
           store(a.out + (row * a.out_row + qh * a.out_head + d0 + d) * 2,
@@ -1186,22 +1197,16 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
         on |= load.halves(next) << (2 * place);
       };
-      typename Load::Next next[RING];
-      if (count > 0) {
+      if (count > 0)
         load.first_entries(x0, count, lane);
-#pragma unroll
-        for (int i = 0; i < RING; ++i)
-          next[i] = load.look(i, x0 + i * kTile, lane);
-      }
       if constexpr (BUSY)
         start(); // the queries arrive while the table does
-      if (count > 0) {
-#pragma unroll
-        for (int i = 0; i < RING - 1; ++i)
-          if (i < count)
-            send(next[i], i, i);
-      }
-      typename Load::Next then = next[RING - 1];
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < min(count, RING - 1); ++i)
+        send(load.look(i, x0 + i * kTile, lane), i, i);
+      typename Load::Next then = {}; // the next tile to send
+      if (count > 0)
+        then = load.look(RING - 1, x0 + (RING - 1) * kTile, lane);
       int x = x0, slot = 0;
       const int last = x0 + (count - 1) * kTile;
       uint32_t seen = 0xffffffffu;
@@ -1324,7 +1329,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           b.lse[row * b.heads + qh] = log_sum(r.top[t], sum);
       } else {
         const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
-        float *dst = b.partial + (part - c) * DP + part_at<DP>(c, 4 * g);
+        float *dst = b.partial + (part - c) * DP + part_at<DP, ROWS>(c, 4 * g);
 #pragma unroll
         for (int e = 0; e < E; ++e)
           *reinterpret_cast<f32x4 *>(dst + e * 256) = r.acc[t][e];
@@ -1339,7 +1344,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         const AttendArgs &b = args_again();
         const int i = wave * 16 * RT + t * 16 + c;
         if (!whole) {
-          b.partial[(run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS * DP + part_at<DP>(i, d)] += v;
+          b.partial[(run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS * DP + part_at<DP, ROWS>(i, d)] += v;
           return;
         }
         // what is rounded is finite, and what comes to it is not
@@ -1360,19 +1365,25 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
 
 // The rows of items that lie in several workgroups' runs: their partial sums,
 // added up; and zeros for the rows of no request. A column of blocks takes the
-// rows of a request, a block sixteen of them at a time: its waves share their
-// parts, kParts on their way at once.
-template <int T, bool I8, int DP, int ROWS, int UNIT>
-__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
-  constexpr int E = DP / 16, kParts = DP > 128 ? 1 : 2;
-  __shared__ f32x4 sums[4][E][64];
-  __shared__ float tops[4][16], totals[4][16];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+// rows of a request, PHASES waves a piece of 64 times four dims at a time. It is
+// bound by how long a read takes of what other dies have written: so all parts
+// are on their way at once, where there are many by sharing them among waves.
+template <int T, bool I8, int DP, int ROWS, int UNIT, int PHASES>
+__global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join(AttendArgs a) {
+  constexpr bool LANED = ROWS > 16;                   // see part_at
+  constexpr int N = LANED ? 16 : 256 / DP;            // rows of a piece
+  constexpr int E = LANED ? DP / 16 : 1;              // pieces of N rows
+  constexpr int WAVES = PHASES == 1 ? 4 : PHASES;     // of a block
+  constexpr int PIECES = WAVES / PHASES;              // of a block
+  __shared__ f32x4 sums[PHASES][64];
+  __shared__ float tops[PHASES][64], totals[PHASES][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), phase = PHASES == 1 ? 0 : wave;
+  const int c = LANED ? lane & 15 : lane / (DP / 4);
   const int b = blockIdx.x;
   if (b == a.requests) { // rows of no request
     const int r0 = min(max(a.starts[0], 0), a.rows), r1 = min(max(a.starts[a.requests], r0), a.rows);
     const int64_t none = static_cast<int64_t>(r0 + a.rows - r1) * a.heads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.y) * 4 + wave; i < none; i += static_cast<int64_t>(gridDim.y) * 4) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.y) * WAVES + wave; i < none; i += static_cast<int64_t>(gridDim.y) * WAVES) {
       int64_t row = i / a.heads;
       const int64_t qh = i - row * a.heads;
       row += row < r0 ? 0 : r1 - r0;
@@ -1385,93 +1396,91 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
   }
   const Request r = attend_request<ROWS, UNIT>(a, b);
   const int64_t total = a.schedule[a.requests], first = a.schedule[b];
-  const int64_t per = (total + a.workgroups - 1) / a.workgroups;
-  const int64_t rows = static_cast<int64_t>(r.fresh) * a.group.d, sixteens = (rows + 15) / 16;
-  for (int64_t i = blockIdx.y; i < sixteens * a.kv_heads; i += gridDim.y) {
-    const int head = static_cast<int>(i / sixteens), row0 = static_cast<int>(i - head * sixteens) * 16;
+  const int64_t per = units_of_run(total, a.workgroups);
+  const int64_t rows = static_cast<int64_t>(r.fresh) * a.group.d;
+  const int groups = static_cast<int>((rows + N - 1) / N); // of a key head's rows
+  const int64_t count = static_cast<int64_t>(groups) * a.kv_heads * E;
+  for (int64_t i = static_cast<int64_t>(blockIdx.y) * PIECES + (PHASES == 1 ? wave : 0); i < count;
+       i += static_cast<int64_t>(gridDim.y) * PIECES) {
+    const int e = static_cast<int>(i % E), head = static_cast<int>(divide(i / E, groups));
+    const int row0 = static_cast<int>(i / E - static_cast<int64_t>(head) * groups) * N;
+    const int d = LANED ? e * 16 + (lane >> 4) * 4 : lane % (DP / 4) * 4;
     const int64_t u0 = first + (static_cast<int64_t>(head) * r.tiles + row0 / ROWS) * r.units;
-    const int64_t w0 = uniform64(u0 / per), w1 = uniform64((u0 + r.units - 1) / per);
+    const int64_t w0 = uniform64(divide(u0, static_cast<int>(per))), w1 = uniform64(divide(u0 + r.units - 1, static_cast<int>(per)));
     if (w0 == w1)
       continue; // written whole
+    const bool valid = row0 + c < rows;
     float top = kNone, sum = 0.0f;
-    f32x4 acc[E];
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    int64_t w = w0 + phase;
+    auto take = [&](auto many) { // the next parts of this phase
+      constexpr int MANY = decltype(many)::value;
+      f32x4 o[MANY];
+      f32x2 ml[MANY];
+      float most = top;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t w = w0 + wave; w <= w1; w += 4 * kParts) {
-      f32x4 o[kParts][E];
-      float m[kParts], l[kParts], most = top;
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) {
+      for (int k = 0; k < MANY; ++k) {
         // a run that begins inside the item left its part in its first place,
         // the run in which the item begins in its second
-        const bool is = w + 4 * k <= w1;
-        const int64_t at = ((is ? w + 4 * k : w) * 2 + (w == w0 && (k == 0 || !is) ? 1 : 0)) * ROWS + row0 % ROWS;
-        m[k] = is ? a.stats[(at + c) * 2] : kNone;
-        l[k] = is ? a.stats[(at + c) * 2 + 1] : 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          o[k][e] = *reinterpret_cast<const f32x4 *>(a.partial + at * DP + (e * 64 + lane) * 4);
+        const int64_t wk = min(w + k * PHASES, w1), at = (wk * 2 + (wk == w0 ? 1 : 0)) * ROWS + row0 % ROWS;
+        ml[k] = *reinterpret_cast<const f32x2 *>(a.stats + (at + c) * 2);
+        o[k] = *reinterpret_cast<const f32x4 *>(a.partial + at * DP + (e * 64 + lane) * 4);
       }
 #pragma unroll
-      for (int k = 0; k < kParts; ++k)
-        most = fmaxf(most, m[k]);
+      for (int k = 0; k < MANY; ++k)
+        most = fmaxf(most, ml[k].x);
       const float f = __builtin_amdgcn_exp2f(top - most);
       top = most;
       sum *= f;
+      acc *= f;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        acc[e] *= f;
-#pragma unroll
-      for (int k = 0; k < kParts; ++k)
-        if (w + 4 * k <= w1) {
-          const float fk = __builtin_amdgcn_exp2f(m[k] - top);
-          sum += l[k] * fk;
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            acc[e] += o[k][e] * fk;
+      for (int k = 0; k < MANY; ++k)
+        if (w + k * PHASES <= w1) {
+          const float fk = __builtin_amdgcn_exp2f(ml[k].x - top);
+          sum += ml[k].y * fk;
+          acc += o[k] * fk;
         }
+      w += MANY * PHASES;
+    };
+    if (valid) {
+      while (w + 4 * PHASES <= w1)
+        take(std::integral_constant<int, 8>());
+      if (w <= w1)
+        take(std::integral_constant<int, 4>());
     }
+    if constexpr (PHASES > 1) {
+      sums[phase][lane] = acc;
+      tops[phase][lane] = top;
+      totals[phase][lane] = sum;
+      __syncthreads();
+      if (phase == 0) {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      sums[wave][e][lane] = acc[e];
-    if (g == 0) {
-      tops[wave][c] = top;
-      totals[wave][c] = sum;
+        for (int k = 1; k < PHASES; ++k)
+          top = fmaxf(top, tops[k][lane]);
+        float f = __builtin_amdgcn_exp2f(tops[0][lane] - top);
+        sum *= f;
+        acc *= f;
+#pragma unroll
+        for (int k = 1; k < PHASES; ++k) {
+          f = __builtin_amdgcn_exp2f(tops[k][lane] - top);
+          sum += totals[k][lane] * f;
+          acc += sums[k][lane] * f;
+        }
+      }
     }
-    __syncthreads();
-    top = kNone;
-    sum = 0.0f;
-    float f[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      top = fmaxf(top, tops[k][c]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f[k] = __builtin_amdgcn_exp2f(tops[k][c] - top);
-      sum += totals[k][c] * f[k];
-    }
-    if (row0 + c < rows) {
+    if (valid && phase == 0) {
       const uint32_t p = static_cast<uint32_t>(row0 + c);
       const uint32_t j = fdiv(p, a.group);
       const int64_t row = r.start + static_cast<int64_t>(j);
       const int64_t qh = static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d);
-      const float scale = finish(sum, I8 ? a.value_scale[head] : 1.0f);
-#pragma unroll
-      for (int n = 0; n < E / 4; ++n) {
-        const int e = wave * (E / 4) + n, d = e * 16 + 4 * g;
-        f32x4 o = sums[0][e][lane] * f[0];
-#pragma unroll
-        for (int k = 1; k < 4; ++k)
-          o += sums[k][e][lane] * f[k];
-        o *= scale;
-        if (d < a.dim)
-          store(a.out + (row * a.out_row + qh * a.out_head + d) * 2, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
-      }
-      if (a.lse && threadIdx.x < 16)
+      acc *= finish(sum, I8 ? a.value_scale[head] : 1.0f);
+      if (d < a.dim)
+        store(a.out + (row * a.out_row + qh * a.out_head + d) * 2, u32x2{pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3])});
+      if (a.lse && d == 0)
         a.lse[row * a.heads + qh] = log_sum(top, sum);
     }
-    __syncthreads();
+    if constexpr (PHASES > 1)
+      __syncthreads();
   }
 }
 
@@ -1484,11 +1493,17 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
                                  dim3(static_cast<uint32_t>(threads)), pa, 0, s);
   if (e != hipSuccess)
     return e;
-  // a block for every sixteen output rows of an even batch, within 2^16 a request
-  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d;
-  const int64_t y = std::min<int64_t>((rows + 15) / 16 * a.kv_heads, 65535);
-  return hipLaunchKernel(reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT>),
-                         dim3(static_cast<uint32_t>(a.requests) + 1, static_cast<uint32_t>(y)), dim3(256), pa, 0, s);
+  // A wave for every piece of an even batch, within 2^16 blocks a request; eight
+  // where an item lies in more than eight runs, on average.
+  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d, n = ROWS > 16 ? 16 : 256 / DP;
+  const int64_t pieces = (rows + n - 1) / n * a.kv_heads * (ROWS > 16 ? DP / 16 : 1);
+  const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * a.requests;
+  const bool many = p.workgroups > 8 * items;
+  return hipLaunchKernel(many ? reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 8>)
+                              : reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 1>),
+                         dim3(static_cast<uint32_t>(a.requests) + 1,
+                              static_cast<uint32_t>(std::min<int64_t>(many ? pieces : (pieces + 3) / 4, 65535))),
+                         dim3(many ? 512 : 256), pa, 0, s);
 }
 
 template <int T, bool I8, int DP, int RT, int W, int SRC>
