@@ -1244,7 +1244,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
             receive(std::integral_constant<int, RING - 3>(), x + kTile, slot);
           meet(); // everybody's part of the next tile is there, and the tile before has been read
           if (x + (RING - 1) * kTile <= last)
-            send(then, free, RING - 2);
+            send(then, free, RING - 3); // the tile after the next is the lowest in `on`
           if constexpr (BUSY) {
             r.read_keys(at + slot * 2 * TILE + reads.key); // after the last tile: not used
             r.add(v);
