@@ -8,7 +8,20 @@
 // (or, where halves do not begin on a lane, through shared memory). A block
 // of heads belongs to one kind (queries, keys, values), so a wave keeps its
 // weights, and walks the rows of the batch: a row's angles are loaded once
-// for all heads of the block. Everything is read once and written once.
+// for all heads of the block.
+//
+//   forward   n = x / sqrt(mean(x^2) + eps), y = n w, z = R(position) y
+//   backward  g = R^T dz, u = g w, dx = (u - n mean(u n)) / sqrt(..),
+//             dw = sum over rows and heads of g n
+//
+// Bound by bytes: everything is read once and written once, past the caches.
+// What decides is how much is on its way, so a wave loads its next row before
+// it works on this one. 32768 rows of 32 + 8 heads of 128 in bf16, from views
+// of a fused projection: forward 124 us (5.4 TB/s; 177 without the next row
+// ahead, 155 with stores through the caches), backward with the weights'
+// gradients 186 us (5.4 TB/s; 310 before). 8192 rows into a cache 78 us
+// (5.2 TB/s; 113 before). The sums of the weights' gradients are added block
+// by block in a fixed order by a second launch (4 us): no atomics.
 #include "attention.h"
 #include "index.h"
 
@@ -529,7 +542,9 @@ int rotate_lanes(int dim) {
 int rotate_blocks(int form, int64_t rows, int64_t chunks) {
   const int64_t blocks = (rows + kWaves - 1) / kWaves;
   // As many waves as the card holds at once (three on a SIMD), or twice that
-  // where no block leaves a part of a sum: TODO
+  // where no block leaves a part of a sum. 32768 rows of 40 heads of 128, bf16,
+  // in a kernel trace: forward 135 us with 1024 or 2048 blocks, 141 with 4096, 158 with 8192;
+  // backward 188 with 768, 190 with 1536, 195 with 2048.
   const int64_t most = 256 * (form == kRotateBackward ? 3 : 8);
   const int64_t cap = most / chunks > 0 ? most / chunks : 1;
   return static_cast<int>(blocks < cap ? blocks : cap);
