@@ -94,6 +94,11 @@ __device__ __forceinline__ int32_t scalar_load(const int32_t *p) {
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(x) >> 32), lane);
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
 __device__ __forceinline__ int64_t uniform64(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
@@ -787,7 +792,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   bool whole;  // all of them
   u32x4 stage[2][SRC == kAsync ? 1 : LOADS];
   uint32_t there; // loads that are a token's, by bit
-  // kAsync: the lane's token in a load, and its piece in the first load
+  // kAsync: the lane's token of the first load in its group of sixteen, and its piece
   uint32_t key_lane, value_lane, place16;
 
   __device__ __forceinline__ Loader(const AttendArgs &a, int lane, int first_) {
@@ -808,8 +813,8 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     whole = dim + LB <= a.dim;
     cell_at = has ? dim * CELL : 0;
     there = 0u;
-    key_lane = token * key_slot;
-    value_lane = token * value_slot;
+    key_lane = (token + (first & 15)) * key_slot;
+    value_lane = (token + (first & 15)) * value_slot;
     place16 = ((dim / LB) ^ swap_of<RB>(first + token)) * 16;
   }
   __device__ __forceinline__ void item(const AttendArgs &a, const Item &it) {
@@ -827,47 +832,59 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   __device__ __forceinline__ int entry(int x0) const {
     return x0 < length ? scalar_load(table + fdiv(static_cast<uint32_t>(x0), page)) : -1;
   }
-  // The entries of a tile's two halves, and the places in their pages (past the
-  // length: the last page's first); kAsync, where there are tokens. A wave keeps
-  // the entries of kAhead tiles in its lanes, and brings the next ones through
-  // shared memory like the tiles: no wait, neither for them nor, as scalar loads
-  // would make it, for reads of shared memory.
+  // Where the 16-token groups of a wave's next kAhead tiles lie in the cache,
+  // group g of them in lane g: one wave's worth of arithmetic, and two reads of a
+  // lane a tile. The table's next entries come through shared memory like the
+  // tiles: no wait, neither for them nor, as scalar loads would make it, for reads
+  // of shared memory. kAsync, where there are tokens.
   static constexpr int kAhead = 32;
+  static constexpr int GROUPS = NT > 16 ? 2 : 1; // that this wave brings of a tile
   struct Next {
-    int id[2];
-    uint32_t off[2];
+    int64_t key[GROUPS], value[GROUPS];
+    uint32_t on; // which of the tile's halves lie on a page
   };
-  int entries;   // of tile lane / 2, half lane % 2
-  uint32_t room; // [2][64] of this wave
+  int64_t key_at, value_at;
+  uint64_t paged; // the groups that lie on a page
+  uint32_t room;  // [2][64] of this wave
+  __device__ __forceinline__ int group_at(int x, int lane) const { return x + (lane >> 1) * PACE + (lane & 1) * 16; }
   __device__ __forceinline__ uint32_t entry_at(int x, int lane) const {
-    return fdiv(static_cast<uint32_t>(min(x + (lane >> 1) * PACE + (lane & 1) * 16, length - 1)), page) * 4u;
+    return fdiv(static_cast<uint32_t>(min(group_at(x, lane), length - 1)), page);
+  }
+  // Past the length: the last page's first tokens; of no page: the first one's,
+  // which nothing will see.
+  __device__ __forceinline__ void take_entries(int id, int x, int lane) {
+    const bool is = is_page(id);
+    const int x0 = group_at(x, lane);
+    const uint32_t off = is && x0 < length ? static_cast<uint32_t>(x0) - fdiv(static_cast<uint32_t>(x0), page) * page.d : 0u;
+    const uint64_t at = is ? static_cast<uint32_t>(id) : 0u;
+    key_at = static_cast<int64_t>(at * key_page + static_cast<uint64_t>(off) * key_slot);
+    value_at = static_cast<int64_t>(at * value_page + static_cast<uint64_t>(off) * value_slot);
+    paged = __ballot(is);
   }
   // The first entries, and the next on their way.
   __device__ __forceinline__ void first_entries(int x, int count, int lane) {
-    entries = *reinterpret_cast<const int32_t *>(reinterpret_cast<const char *>(table) + entry_at(x, lane));
+    const int id = table[entry_at(x, lane)];
     if (count > kAhead)
-      load_async4(table, entry_at(x + kAhead * PACE, lane), room + 256);
+      load_async4(table, entry_at(x + kAhead * PACE, lane) * 4u, room + 256);
+    take_entries(id, x, lane);
   }
   // The n-th tile, at x; called for one after the other.
   __device__ __forceinline__ Next look(int n, int x, int lane) {
     if (n > 0 && n % kAhead == 0) {
       const uint32_t half = n / kAhead % 2 * 256;
-      entries = *reinterpret_cast<const __attribute__((address_space(3))) int *>(room + half + lane * 4);
-      load_async4(table, entry_at(x + kAhead * PACE, lane), room + (half ^ 256));
+      take_entries(*reinterpret_cast<const __attribute__((address_space(3))) int *>(room + half + lane * 4), x, lane);
+      load_async4(table, entry_at(x + kAhead * PACE, lane) * 4u, room + (half ^ 256));
     }
+    const int g = n % kAhead * 2;
     Next t;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int x0 = x + h * 16;
-      t.id[h] = __builtin_amdgcn_readlane(entries, n % kAhead * 2 + h);
-      const uint32_t at = static_cast<uint32_t>(min(x0, length - 1));
-      t.off[h] = x0 < length ? at - fdiv(at, page) * page.d : 0u;
+    for (int h = 0; h < GROUPS; ++h) {
+      const int from = g + (GROUPS == 2 ? h : first >> 4);
+      t.key[h] = of_lane(key_at, from);
+      t.value[h] = of_lane(value_at, from);
     }
+    t.on = static_cast<uint32_t>(paged >> g) & 3u;
     return t;
-  }
-  // Which halves lie on a page.
-  __device__ __forceinline__ uint32_t halves(const Next &t) const {
-    return (is_page(t.id[0]) ? 1u : 0u) | (is_page(t.id[1]) ? 2u : 0u);
   }
   // Which of the 32 tokens from x are there.
   __device__ __forceinline__ uint32_t seen(int x, uint32_t on) const {
@@ -876,22 +893,14 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     return in & ((on & 1u ? 0xffffu : 0u) | (on & 2u ? 0xffff0000u : 0u));
   }
 
-  // kAsync: the wave's tokens of a tile (of no page: the first one's, which
-  // nothing will see).
+  // kAsync: the wave's tokens of a tile.
   __device__ __forceinline__ void send(const Next &next, uint32_t to_k, uint32_t to_v) const {
-    constexpr int GROUPS = NT > 16 ? 2 : 1; // of 16 tokens
 #pragma unroll
     for (int h = 0; h < GROUPS; ++h) {
-      const int t0 = GROUPS == 2 ? h * 16 : first; // the group's part's first token
-      const bool second = GROUPS == 2 ? h : t0 >= 16;
-      const int id = second ? next.id[1] : next.id[0];
-      const uint32_t off = is_page(id) ? (second ? next.off[1] : next.off[0]) + (t0 & 15) : 0u;
-      const uint32_t at = is_page(id) ? id : 0u;
-      const char *k = keys + static_cast<uint64_t>(at) * key_page + static_cast<uint64_t>(off) * key_slot;
-      const char *v = values + static_cast<uint64_t>(at) * value_page + static_cast<uint64_t>(off) * value_slot;
+      const char *k = keys + next.key[h], *v = values + next.value[h];
 #pragma unroll
       for (int i = 0; i < LOADS / GROUPS; ++i) {
-        const int t = t0 + i * TPI;
+        const int t = (GROUPS == 2 ? h * 16 : first) + i * TPI;
         // the piece that lies at this lane's place
         const uint32_t n16 = LOADS == 1 ? place16 : place16 ^ (swap_of<RB>((h * 16 + i * TPI) & 15) * 16);
         const char *ki = k + static_cast<uint64_t>(i * TPI) * key_slot, *vi = v + static_cast<uint64_t>(i * TPI) * value_slot;
@@ -1024,7 +1033,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
       uint32_t on = 0u; // of the tiles on their way: their halves on a page
       auto send = [&](const typename Load::Next &next, int slot, int place) {
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
-        on |= load.halves(next) << (2 * place);
+        on |= next.on << (2 * place);
       };
       if (count > 0)
         load.first_entries(x0, count, lane);
@@ -1209,7 +1218,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
       uint32_t on = 0u; // of the tiles on their way: their halves on a page
       auto send = [&](const typename Load::Next &next, int slot, int place) {
         load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
-        on |= load.halves(next) << (2 * place);
+        on |= next.on << (2 * place);
       };
       if (count > 0)
         load.first_entries(x0, count, lane);
