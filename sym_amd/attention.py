@@ -76,15 +76,10 @@ def _call(name, ctx, *args):
         _fail(err)
 
 
-# torch's current stream as a handle; the plain query costs as much as a launch
 _split = torch.unsafe_split_with_sizes  # of buffers that nobody else has
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _stream(device):
-    if _raw_stream is not None:
-        return _raw_stream(device)
-    return torch.cuda.current_stream(device).cuda_stream
+# torch's current stream as a handle; the plain query costs as much as a launch
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _device(ctx, like):
@@ -112,6 +107,11 @@ def _heads(t, name, shape, dtype, device):
     if one != 1 and shape[2] > 1 and t.numel():
         _bad("%s: the last dimension must be contiguous" % name)
     return _HEADS.pack(t.data_ptr(), row, head)
+
+
+def _made(t, shape):
+    """A record of a tensor that the call has made, [rows, heads, dim]."""
+    return _HEADS.pack(t.data_ptr(), shape[1] * shape[2], shape[2])
 
 
 def _table(t, device):
@@ -276,10 +276,14 @@ def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pair
 def _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out):
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
-    zq, zk = out if out is not None else (q.new_empty(qs), k.new_empty(ks))
-    _call("relx_norm_rotate", ctx, rot, _heads(q, "queries", qs, dtype, device),
-          _heads(k, "keys", ks, dtype, device), _heads(zq, "query result", qs, dtype, device),
-          _heads(zk, "key result", ks, dtype, device), _stream(device))
+    if out is None:
+        zq, zk = q.new_empty(qs), k.new_empty(ks)
+        results = _made(zq, qs), _made(zk, ks)
+    else:
+        zq, zk = out
+        results = _heads(zq, "query result", qs, dtype, device), _heads(zk, "key result", ks, dtype, device)
+    _call("relx_norm_rotate", ctx, rot, _heads(q, "queries", qs, dtype, device), _heads(k, "keys", ks, dtype, device),
+          *results, _stream(device))
     return zq, zk
 
 
@@ -305,8 +309,7 @@ def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_wei
         room_ptr = room.data_ptr()
     _call("relx_norm_rotate_backward", ctx, rot, _heads(dq, "query gradient", qs, dtype, device),
           _heads(dk, "key gradient", ks, dtype, device), _heads(q, "queries", qs, dtype, device),
-          _heads(k, "keys", ks, dtype, device), _heads(gq, "query gradient", qs, dtype, device),
-          _heads(gk, "key gradient", ks, dtype, device), gqw_ptr, gkw_ptr, room_ptr, size, _stream(device))
+          _heads(k, "keys", ks, dtype, device), _made(gq, qs), _made(gk, ks), gqw_ptr, gkw_ptr, room_ptr, size, _stream(device))
     return gq, gk, gqw, gkw
 
 
@@ -338,10 +341,13 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     dtype = q.dtype
     if out is None:
         out = q.new_empty(qs)
+        result = _made(out, qs)
+    else:
+        result = _heads(out, "query result", qs, dtype, device)
     cache = _CACHE.pack(*_cache(cache_k, cache_v, k_scale, v_scale, device))
     _call("relx_norm_rotate_append", ctx, rot, _heads(q, "queries", qs, dtype, device),
           _heads(k, "keys", ks, dtype, device), _heads(v, "values", ks, dtype, device),
-          _heads(out, "query result", qs, dtype, device), _row(slots, "slots", torch.int64, qs[0], device),
+          result, _row(slots, "slots", torch.int64, qs[0], device),
           cache, _stream(device))
     return out
 
@@ -399,6 +405,9 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
         words, m_ptr = mask.shape[1], mask.data_ptr()
     if out is None:
         out = q.new_empty(shape)
+        result = _made(out, shape)
+    else:
+        result = _heads(out, "result", shape, dtype, device)
     l_ptr = 0
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != shape[:2] or lse.get_device() != device or not lse.is_contiguous():
@@ -410,7 +419,7 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _bad("workspace: contiguous uint8 on device %d" % device)
     _call("relx_tree_attention", ctx,
-          _heads(q, "queries", shape, dtype, device) + _heads(out, "result", shape, dtype, device) +
+          _heads(q, "queries", shape, dtype, device) + result +
           _ATTENTION.pack(*cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
                           _row(starts, "starts", torch.int32, requests + 1, device), m_ptr, l_ptr,
                           workspace.data_ptr(), workspace.numel(), rows, requests, heads, columns, words, *kind,

@@ -257,7 +257,8 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
   // of 128, bf16, us by rows of an item:
   //   256 rows each   64: 633   128: 377   256: 335
   //   128 rows        64: 338   128: 203   256: 261
-  //   16 rows         16: 185   64: 176; int8, 64 requests of one: 16: 279, 64: 441
+  //   64 rows         16: 454   64: 176
+  //   16 rows         16: 185   64: 176; 64 int8 requests of one row: 16: 279, 64: 441
   const int64_t q = requests > 0 ? (rows + requests - 1) / requests * group : 0;
   p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : q <= 128 ? 128 : 256;
   p.workgroups = p.rows == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;

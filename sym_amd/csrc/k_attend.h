@@ -40,11 +40,11 @@
 // Measured, with the join (8 key heads of 128 each, unless said):
 //   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 280 us,
 //     5.6 TB/s of cache. Bound by the reads.
-//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 113 us, 4.8 TB/s. Bound
+//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 111 us, 4.8 TB/s. Bound
 //     by the reads: without the products it takes 105.
-//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 85 us, 410 TFLOP/s; up to
-//     32768: 341 us, 530 TFLOP/s. Bound by the waves' own instructions: reads
-//     alone take 57 of 90, products without the softmax 70.
+//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 82 us, 430 TFLOP/s; up to
+//     32768: 329 us, 550 TFLOP/s. Bound by the waves' own instructions: reads
+//     alone take 57, products without the softmax 70.
 #pragma once
 
 #include <algorithm>
