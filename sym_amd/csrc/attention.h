@@ -91,6 +91,7 @@ struct AttendArgs {
   int32_t rows, requests, heads, kv_heads, dim, pages, columns, words;
   int32_t workgroups;
   float scale; // of a score, times log2 e
+  bool once;   // in an even batch, one tile of query rows reads a key head
 };
 
 // How a call runs.

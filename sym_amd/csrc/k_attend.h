@@ -425,12 +425,15 @@ __device__ __forceinline__ u32x2 read_transposed8(uint32_t at) {
 
 // 16 bytes per lane from base + at into shared memory, lane after lane from
 // `to`. The compiler does not count it: arrived<N>() waits until at most the N
-// latest are on their way.
-__device__ __forceinline__ void load_async(const char *base, uint32_t at, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(uniform(static_cast<int>(to))), "v"(at), "s"(uniform64(reinterpret_cast<int64_t>(base)))
-               : "memory");
+// latest are on their way. ONCE: past the caches, for what no other workgroup
+// reads.
+template <bool ONCE> __device__ __forceinline__ void load_async(const char *base, uint32_t at, uint32_t to) {
+  const int m0 = uniform(static_cast<int>(to));
+  const int64_t from = uniform64(reinterpret_cast<int64_t>(base));
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(m0), "v"(at), "s"(from) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(at), "s"(from) : "memory");
 }
 // The same for four bytes a lane.
 __device__ __forceinline__ void load_async4(const void *base, uint32_t at, uint32_t to) {
@@ -787,6 +790,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   int64_t key_slot64, value_slot64; // kStaged: of any size
   int length, pages, first, token, dim, cell_at, head_dims;
   bool full; // the head fills the tile's rows
+  bool once; // one tile of query rows reads a key head
   FastDiv page;
   bool has;    // the lane's dims are the head's (all, or eight of an int8 load's)
   bool whole;  // all of them
@@ -807,6 +811,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     value_slot64 = a.value_slot;
     head_dims = a.dim;
     full = a.dim == DP;
+    once = a.once;
     pages = a.pages;
     page = a.page;
     has = dim < a.dim && token < NT;
@@ -894,7 +899,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   }
 
   // kAsync: the wave's tokens of a tile.
-  __device__ __forceinline__ void send(const Next &next, uint32_t to_k, uint32_t to_v) const {
+  template <bool ONCE> __device__ __forceinline__ void send(const Next &next, uint32_t to_k, uint32_t to_v) const {
 #pragma unroll
     for (int h = 0; h < GROUPS; ++h) {
       const char *k = keys + next.key[h], *v = values + next.value[h];
@@ -905,8 +910,8 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
         const uint32_t n16 = LOADS == 1 ? place16 : place16 ^ (swap_of<RB>((h * 16 + i * TPI) & 15) * 16);
         const char *ki = k + static_cast<uint64_t>(i * TPI) * key_slot, *vi = v + static_cast<uint64_t>(i * TPI) * value_slot;
         if ((NT >= TPI || token < NT) && (full || static_cast<int>(n16) < head_dims * CELL)) {
-          load_async(ki, key_lane + n16, to_k + t * RB);
-          load_async(vi, value_lane + n16, to_v + t * RB);
+          load_async<ONCE>(ki, key_lane + n16, to_k + t * RB);
+          load_async<ONCE>(vi, value_lane + n16, to_v + t * RB);
         }
       }
     }
@@ -1032,7 +1037,7 @@ __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC ==
       shared_done();
       uint32_t on = 0u; // of the tiles on their way: their halves on a page
       auto send = [&](const typename Load::Next &next, int slot, int place) {
-        load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        load.template send<true>(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
         on |= next.on << (2 * place);
       };
       if (count > 0)
@@ -1217,7 +1222,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
     if constexpr (SRC == kAsync) {
       uint32_t on = 0u; // of the tiles on their way: their halves on a page
       auto send = [&](const typename Load::Next &next, int slot, int place) {
-        load.send(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+        const uint32_t to = at + slot * 2 * TILE;
+        if (load.once)
+          load.template send<true>(next, to, to + TILE);
+        else
+          load.template send<false>(next, to, to + TILE);
         on |= next.on << (2 * place);
       };
       if (count > 0)
