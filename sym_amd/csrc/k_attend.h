@@ -28,8 +28,7 @@
 //     of its own and no barrier, and add up at the end. int8 is widened in the
 //     registers.
 //   more (trees, chunks): the waves have rows of their own, 16 or 32 each, and
-//     share the tiles, whose keys they read during the products of the tile
-//     before. int8 is widened on its way there, once for all of them.
+//     share the tiles. int8 is widened on its way there, once for all of them.
 //
 // The work of a call is the list of its units of tokens over (request, key
 // head, tile of query rows), cut into equal runs, one per workgroup; an item
@@ -474,10 +473,6 @@ __device__ __forceinline__ void meet() {
   asm volatile("" : : : "memory");
 }
 
-struct NoValues {
-  __device__ __forceinline__ explicit NoValues(uint32_t) {}
-};
-
 // A tile's values as operands: at(e) has dim 16 e + lane % 16 of the lane's eight
 // tokens. RAW: the tile holds int8. EARLY: all read at once, ahead of their use.
 template <int T, int DP, bool RAW, bool EARLY> struct Values {
@@ -604,19 +599,16 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   f32x4 s[RT][2];     // scores, unscaled
   u32x4 weights[RT];
 
-  static constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
-  u32x4 k[2][KR];
-
   // from: the tile's place and the lane's first piece in it
-  __device__ __forceinline__ void read_keys(uint32_t from) {
+  __device__ __forceinline__ void scores(uint32_t from) {
+    constexpr int KR = RAW ? QS / 2 : QS; // reads of a token's key
+    u32x4 k[2][KR];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < KR; ++i)
         k[n][i] = read16((from ^ (i * 64)) + n * 16 * DP * (RAW ? 1 : 2));
     keep_order(); // all reads on their way before the first is waited for
-  }
-  __device__ __forceinline__ void scores() {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -712,8 +704,7 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   // tk, tv: the places of the tile's keys and values.
   __device__ __forceinline__ void step(const Item &it, int row0, int x, uint32_t seen, bool cut, uint32_t tk, uint32_t tv,
                                        const Reads<DP, RAW> &reads, int lane) {
-    read_keys(tk + reads.key);
-    scores();
+    scores(tk + reads.key);
     const Values<T, DP, RAW, EARLY> v(tv + reads.value); // EARLY: they arrive during the softmax
     soften(it, row0, x, seen, cut, lane);
     add(v);
@@ -1157,9 +1148,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   constexpr int TILE = kTile * DP * 2;
   // tiles at a time: 64 KiB for each four waves
   constexpr int RING = SRC != kAsync ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
-  // A tile's keys are read during the products of the one before: 109 us against
-  // 112 for 52 rows over 131072 tokens; nothing lost with 256 rows.
-  constexpr bool AHEAD = SRC == kAsync && RING > 2;
   using Load = Loader<T, I8, DP, SRC, kTile / W, false, kTile>;
   __shared__ int entries[SRC == kAsync ? W : 1][2][64];
 
@@ -1241,59 +1229,24 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         then = load.look(RING - 1, x0 + (RING - 1) * kTile, lane);
       int x = x0, slot = 0;
       const int last = x0 + (count - 1) * kTile;
-      uint32_t seen = 0xffffffffu;
-      bool cut = false;
-      // Waits for this wave's part of the tile at x, of which SENT later ones
-      // are on their way, and looks it over.
-      auto receive = [&](auto sent, int x, int slot) {
-        constexpr int SENT = decltype(sent)::value;
-        if (x + SENT * kTile <= last)
-          arrived<SENT * 2 * Load::LOADS>();
+#pragma clang loop unroll(disable)
+      for (int n = 0; x <= last; ++n, x += kTile) {
+        // this wave's part of the tile is there, then everybody's, and everybody
+        // has read the tile before, whose place the next takes
+        if (x + (RING - 2) * kTile <= last)
+          arrived<(RING - 2) * 2 * Load::LOADS>();
         else
           arrived<0>();
-        cut = (on & 3u) != 3u || x + kTile > it.cached;
-        seen = cut ? load.seen(x, on) : 0xffffffffu;
+        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
+        const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
         clean_own(x, seen, cut, slot);
-        on >>= 2;
-      };
-      if constexpr (AHEAD) {
-        if (count > 0)
-          receive(std::integral_constant<int, RING - 2>(), x, 0);
         meet();
-        if constexpr (BUSY)
-          r.read_keys(at + reads.key);
-#pragma clang loop unroll(disable)
-        for (int n = 0; x <= last; ++n, x += kTile) {
-          const uint32_t tile = at + slot * 2 * TILE;
-          if constexpr (BUSY)
-            r.scores();
-          const typename std::conditional<BUSY, Values<T, DP, false, EARLY>, NoValues>::type v(tile + TILE + reads.value);
-          if constexpr (BUSY)
-            r.soften(it, row0, x, seen, cut, lane);
-          const int free = slot == 0 ? RING - 1 : slot - 1;
-          slot = slot + 1 == RING ? 0 : slot + 1;
-          if (x < last)
-            receive(std::integral_constant<int, RING - 3>(), x + kTile, slot);
-          meet(); // everybody's part of the next tile is there, and the tile before has been read
-          if (x + (RING - 1) * kTile <= last)
-            send(then, free, RING - 3); // the tile after the next is the lowest in `on`
-          if constexpr (BUSY) {
-            r.read_keys(at + slot * 2 * TILE + reads.key); // after the last tile: not used
-            r.add(v);
-          }
-          then = load.look(n + RING, x + RING * kTile, lane);
-        }
-      } else {
-#pragma clang loop unroll(disable)
-        for (int n = 0; x <= last; ++n, x += kTile) {
-          receive(std::integral_constant<int, RING - 2>(), x, slot);
-          meet(); // everybody's part of the tile is there, and the tile before has been read
-          if (x + (RING - 1) * kTile <= last)
-            send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
-          take_in(x, seen, cut, slot);
-          then = load.look(n + RING, x + RING * kTile, lane);
-          slot = slot + 1 == RING ? 0 : slot + 1;
-        }
+        on >>= 2;
+        if (x + (RING - 1) * kTile <= last)
+          send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
+        take_in(x, seen, cut, slot);
+        then = load.look(n + RING, x + RING * kTile, lane);
+        slot = slot + 1 == RING ? 0 : slot + 1;
       }
       arrived<0>(); // the last entries, wanted or not
     } else {
