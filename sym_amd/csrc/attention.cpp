@@ -125,7 +125,9 @@ RotateArgs rotate_args(const relx_rotation &r, int &type) {
   a.pairs = r.pairs != 0;
   a.eps = static_cast<float>(r.eps);
   a.inv_dim = 1.0f / static_cast<float>(r.dim);
-  // a wave's heads at a time, twice where there are more of them
+  // A wave's heads at a time, twice where there are more of them: 32768 rows of 40
+  // heads of 128 forward took 136 us in a trace so, 167 without, 133 to 158 with
+  // four times.
   const int at_once = 64 / rotate_lanes(a.dim);
   a.chunk_heads = std::max(a.heads[0], a.heads[1]) > at_once ? 2 * at_once : at_once;
   for (int k = 0; k < 2; ++k)
@@ -235,15 +237,16 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   const int64_t at = reinterpret_cast<int64_t>(a.keys) | reinterpret_cast<int64_t>(a.values) | a.key_page | a.key_slot |
                      a.key_head | a.value_page | a.value_slot | a.value_head;
   // Tiles that go to shared memory by themselves against tiles through registers:
-  // 8 requests of 256 rows over up to 32768 tokens 335 us against 375, one of 52
-  // rows over 131072 109 against 166, 64 int8 requests of one 280 against 440.
+  // 8 requests of 256 rows over up to 32768 tokens 314 us against 366, one of 52
+  // rows over 131072 97 against 166, 64 int8 requests of one 250 against 434.
   plan.async = plan.even && (at | dim * (i8 ? 1 : 2)) % 16 == 0;
   if (plan.rows == 16)
     plan.workgroups = turn_workgroups(plan.width, i8, plan.async);
   a.workgroups = plan.workgroups;
-  // Then keys and values go past the caches: 64 int8 requests of one row 247 us
-  // against 278, 52 rows over 131072 tokens 97 against 107. Where other tiles
-  // read them too: 565 against 512 (512 tokens of 8 requests over up to 8192).
+  // Then keys and values go past the caches: 52 rows over 131072 tokens 97 us
+  // against 108, 128 rows of 8 requests over up to 32768 170 against 198, 64 int8
+  // requests of one row, whose kernel always does, 247 against 278. Where other
+  // tiles read them too: 528 against 480 (512 tokens of 8 requests, up to 8192).
   a.once = p.requests > 0 && (p.rows + p.requests - 1) / p.requests * (p.heads / kv) <= plan.rows;
   return a;
 }
@@ -259,10 +262,10 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
   // tile less often and leave fewer waves to read ahead; a row that is not there
   // costs what one that is does. 8 requests of up to 32768 tokens, 8 key heads
   // of 128, bf16, us by rows of an item:
-  //   256 rows each   64: 633   128: 377   256: 335
-  //   128 rows        64: 338   128: 203   256: 261
-  //   64 rows         16: 454   64: 176
-  //   16 rows         16: 185   64: 176; 64 int8 requests of one row: 16: 279, 64: 441
+  //   256 rows each   64: 586   128: 349   256: 314
+  //   128 rows        64: 333   128: 170   256: 193
+  //   64 rows         16: 445   64: 159
+  //   16 rows         16: 166   64: 171; 64 int8 requests of one row: 16: 250, 64: 434
   const int64_t q = requests > 0 ? (rows + requests - 1) / requests * group : 0;
   p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : q <= 128 ? 128 : 256;
   p.workgroups = p.rows == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;

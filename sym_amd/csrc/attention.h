@@ -107,8 +107,8 @@ constexpr int kMostWorkgroups = 512; // two to a compute unit
 // Waves that take turns, and workgroups of them that the card holds at once: a
 // ring of two tiles a wave, in 64 KiB (int8 heads of 128, say) or 128 KiB of a
 // compute unit's 160. Where two fit, two: 64 requests of 512 int8 tokens at most
-// with 32 key heads took 57 us with 512 workgroups, 77 with 256, and 86 with 256
-// whose rings hold four tiles; up to 4096 tokens 280, 270 to 300, and 290 to 330.
+// with 32 key heads take 53 us with 512 workgroups, 74 with 256; up to 4096 tokens
+// 250 and 290. Rings of four tiles in 256 workgroups were slower still.
 constexpr int turn_waves(int width) { return width == 256 ? 2 : 4; }
 constexpr int turn_workgroups(int width, bool i8, bool async) {
   const int ring = 2 * 2 * 32 * width * (i8 ? 1 : 2) * turn_waves(width);

@@ -37,13 +37,13 @@
 // lengths cost nothing.
 //
 // Measured, with the join (8 key heads of 128 each, unless said):
-//   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 280 us,
-//     5.6 TB/s of cache. Bound by the reads.
-//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 111 us, 4.8 TB/s. Bound
-//     by the reads: without the products it takes 105.
-//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 82 us, 430 TFLOP/s; up to
-//     32768: 329 us, 550 TFLOP/s. Bound by the waves' own instructions: reads
-//     alone take 57, products without the softmax 70.
+//   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 250 to 265
+//     us, 5.9 to 6.3 TB/s of cache. Bound by the reads.
+//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 103 us, 5.2 TB/s. Bound
+//     by the reads, but for the join's 6.
+//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 77 us, 456 TFLOP/s; up to
+//     32768: 323 us, 560 TFLOP/s. Bound by the waves' own instructions: an
+//     earlier form of 90 us took 57 for the reads alone, 70 without the softmax.
 #pragma once
 
 #include <algorithm>
@@ -1160,8 +1160,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   Load load(a, lane, wave * (kTile / W));
   load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
   // A tile's values are read ahead of the softmax, where the registers hold them:
-  // 81 us against 91 for 8 requests of 256 rows over up to 8192 tokens of 8 key
-  // heads of 128, 335 against 363 up to 32768.
+  // 77 us against 81 for 8 requests of 256 rows over up to 8192 tokens of 8 key
+  // heads of 128, 314 against 341 up to 32768. The same for the next tile's keys
+  // was slower (81).
   constexpr bool EARLY = DP <= 128 && (I8 || SRC == kAsync);
   Rows<T, DP, RT, false, EARLY> r;
   if (tid < 2)
@@ -1480,7 +1481,7 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
     return e;
   // A wave for every piece of an even batch, within 2^16 blocks a request; eight
   // where an item lies in more than eight runs, on average: 8.1 us against 11.8
-  // for 64 parts of 64 rows (17 MB), but 27 against 8.8 for five of 256 (42 MB).
+  // for 64 parts of 64 rows (14 MB), but 27 against 8.8 for five of 256 (31 MB).
   const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d, n = ROWS > 16 ? 16 : 256 / DP;
   const int64_t pieces = (rows + n - 1) / n * a.kv_heads * (ROWS > 16 ? DP / 16 : 1);
   const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * a.requests;
