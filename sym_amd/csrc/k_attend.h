@@ -430,9 +430,15 @@ template <bool ONCE> __device__ __forceinline__ void load_async(const char *base
   const int m0 = uniform(static_cast<int>(to));
   const int64_t from = uniform64(reinterpret_cast<int64_t>(base));
   if constexpr (ONCE)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(m0), "v"(at), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(m0), "v"(at), "s"(from)
+                 : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(at), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(m0), "v"(at), "s"(from)
+                 : "memory");
 }
 // The same for four bytes a lane.
 __device__ __forceinline__ void load_async4(const void *base, uint32_t at, uint32_t to) {
@@ -980,7 +986,8 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
 // ---------------------------------------------------------- up to 16 rows
 
 template <int T, bool I8, int DP, int SRC>
-__global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC == kAsync) == kMostWorkgroups ? 2 : 1) void k_attend_turns(AttendArgs a) {
+__global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC == kAsync) == kMostWorkgroups ? 2 : 1)
+void k_attend_turns(AttendArgs a) {
   constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
   constexpr int TILE = kTile * DP * (I8 ? 1 : 2);
   constexpr int RING = SRC == kAsync ? 2 : 1; // tiles of a wave
@@ -1198,149 +1205,149 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
     // A wave without rows brings its tokens all the same. Loops of their own, so
     // that in none the sums meet a way round them.
     auto work = [&](auto busy) {
-    constexpr bool BUSY = decltype(busy)::value;
-    auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
-      if constexpr (BUSY)
-        r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
-    };
-    auto start = [&] {
-      const AttendArgs &b = args_again();
-      r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
-    };
-
-    if constexpr (SRC == kAsync) {
-      uint32_t on = 0u; // of the tiles on their way: their halves on a page
-      auto send = [&](const typename Load::Next &next, int slot, int place) {
-        const uint32_t to = at + slot * 2 * TILE;
-        if (load.once)
-          load.template send<true>(next, to, to + TILE);
-        else
-          load.template send<false>(next, to, to + TILE);
-        on |= next.on << (2 * place);
+      constexpr bool BUSY = decltype(busy)::value;
+      auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
+        if constexpr (BUSY)
+          r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
       };
-      if (count > 0)
-        load.first_entries(x0, count, lane);
-      if constexpr (BUSY)
-        start(); // the queries arrive while the table does
-#pragma clang loop unroll(disable)
-      for (int i = 0; i < min(count, RING - 1); ++i)
-        send(load.look(i, x0 + i * kTile, lane), i, i);
-      typename Load::Next then = {}; // the next tile to send
-      if (count > 0)
-        then = load.look(RING - 1, x0 + (RING - 1) * kTile, lane);
-      int x = x0, slot = 0;
-      const int last = x0 + (count - 1) * kTile;
-#pragma clang loop unroll(disable)
-      for (int n = 0; x <= last; ++n, x += kTile) {
-        // this wave's part of the tile is there, then everybody's, and everybody
-        // has read the tile before, whose place the next takes
-        if (x + (RING - 2) * kTile <= last)
-          arrived<(RING - 2) * 2 * Load::LOADS>();
-        else
-          arrived<0>();
-        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
-        const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
-        clean_own(x, seen, cut, slot);
-        meet();
-        on >>= 2;
-        if (x + (RING - 1) * kTile <= last)
-          send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
-        take_in(x, seen, cut, slot);
-        then = load.look(n + RING, x + RING * kTile, lane);
-        slot = slot + 1 == RING ? 0 : slot + 1;
-      }
-      arrived<0>(); // the last entries, wanted or not
-    } else {
-      if constexpr (BUSY)
-        start();
-      int x = x0;
-      auto put = [&](int slot) {
-        load.put(tiles[slot][0], tiles[slot][1]);
-        const uint32_t t = load.tokens_there();
-        if (lane == 0)
-          tokens[slot][wave] = static_cast<uint8_t>(t);
-        const int xp = x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile); // the tile put: this one or the next
-        const uint32_t seen = t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W)));
-        clean_own(xp, seen, seen != 0xffffffffu || xp + kTile > it.cached, slot);
-      };
-      if (count > 0) {
-        load.fetch(x);
-        put(0);
-      }
-      if (count > 1)
-        load.fetch(x + kTile);
-      for (int n = 0; n < count; ++n, x += kTile) {
-        const int slot = n & 1;
-        __syncthreads();
-        uint32_t seen = 0u;
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-          seen |= static_cast<uint32_t>(tokens[slot][w]) << (w * (kTile / W));
-        seen = static_cast<uint32_t>(uniform(static_cast<int>(seen)));
-        if (n + 1 < count)
-          put(slot ^ 1);
-        if (n + 2 < count)
-          load.fetch(x + 2 * kTile);
-        take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, slot);
-      }
-    }
-
-    __syncthreads();
-    if constexpr (!BUSY)
-      return;
-    const bool any_odd = !I8 && odd;
-    // ---- every wave's rows are its own
-    const AttendArgs &b = args_again();
-    const bool whole = it.s0 == 0 && it.s1 == it.units;
-    const int ln = anew(lane), c = ln & 15, g = ln >> 4;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const float sum = r.total(t);
-      if (t * 16 + c >= rows)
-        continue;
-      if (whole) {
-        const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
-        const uint32_t j = fdiv(p, b.group);
-        const int64_t row = it.start + static_cast<int64_t>(j);
-        const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
-        const float f = finish(sum, I8 ? b.value_scale[it.head] : 1.0f);
-        char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (e * 16 + 4 * g < b.dim) {
-            const f32x4 o = r.acc[t][e] * f;
-            store(dst + e * 32, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
-          }
-        if (b.lse && g == 0)
-          b.lse[row * b.heads + qh] = log_sum(r.top[t], sum);
-      } else {
-        const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
-        float *dst = b.partial + (part - c) * DP + part_at<DP, ROWS>(c, 4 * g);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          *reinterpret_cast<f32x4 *>(dst + e * 256) = r.acc[t][e];
-        if (g == 0) {
-          b.stats[part * 2] = r.top[t];
-          b.stats[part * 2 + 1] = sum;
-        }
-      }
-    }
-    if (__builtin_expect(any_odd, 0)) {
-      r.add_odd(it, row0, rows, x0, x_end, kTile, lane, [&](int t, int d, float v) {
+      auto start = [&] {
         const AttendArgs &b = args_again();
-        const int i = wave * 16 * RT + t * 16 + c;
-        if (!whole) {
-          b.partial[(run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS * DP + part_at<DP, ROWS>(i, d)] += v;
-          return;
+        r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
+      };
+
+      if constexpr (SRC == kAsync) {
+        uint32_t on = 0u; // of the tiles on their way: their halves on a page
+        auto send = [&](const typename Load::Next &next, int slot, int place) {
+          const uint32_t to = at + slot * 2 * TILE;
+          if (load.once)
+            load.template send<true>(next, to, to + TILE);
+          else
+            load.template send<false>(next, to, to + TILE);
+          on |= next.on << (2 * place);
+        };
+        if (count > 0)
+          load.first_entries(x0, count, lane);
+        if constexpr (BUSY)
+          start(); // the queries arrive while the table does
+#pragma clang loop unroll(disable)
+        for (int i = 0; i < min(count, RING - 1); ++i)
+          send(load.look(i, x0 + i * kTile, lane), i, i);
+        typename Load::Next then = {}; // the next tile to send
+        if (count > 0)
+          then = load.look(RING - 1, x0 + (RING - 1) * kTile, lane);
+        int x = x0, slot = 0;
+        const int last = x0 + (count - 1) * kTile;
+#pragma clang loop unroll(disable)
+        for (int n = 0; x <= last; ++n, x += kTile) {
+          // this wave's part of the tile is there, then everybody's, and everybody
+          // has read the tile before, whose place the next takes
+          if (x + (RING - 2) * kTile <= last)
+            arrived<(RING - 2) * 2 * Load::LOADS>();
+          else
+            arrived<0>();
+          const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
+          const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
+          clean_own(x, seen, cut, slot);
+          meet();
+          on >>= 2;
+          if (x + (RING - 1) * kTile <= last)
+            send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
+          take_in(x, seen, cut, slot);
+          then = load.look(n + RING, x + RING * kTile, lane);
+          slot = slot + 1 == RING ? 0 : slot + 1;
         }
-        // what is rounded is finite, and what comes to it is not
-        const uint32_t p = static_cast<uint32_t>(it.tile * ROWS + i);
-        const uint32_t j = fdiv(p, b.group);
-        char *o = b.out + ((it.start + static_cast<int64_t>(j)) * b.out_row +
-                           (static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d)) * b.out_head + d) * 2;
-        store(o, static_cast<uint16_t>(pack16<T>(widen16<T>(relx::load<uint16_t>(o)) + v, 0.0f)));
-      });
-    }
+        arrived<0>(); // the last entries, wanted or not
+      } else {
+        if constexpr (BUSY)
+          start();
+        int x = x0;
+        auto put = [&](int slot) {
+          load.put(tiles[slot][0], tiles[slot][1]);
+          const uint32_t t = load.tokens_there();
+          if (lane == 0)
+            tokens[slot][wave] = static_cast<uint8_t>(t);
+          const int xp = x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile); // the tile put: this one or the next
+          const uint32_t seen = t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W)));
+          clean_own(xp, seen, seen != 0xffffffffu || xp + kTile > it.cached, slot);
+        };
+        if (count > 0) {
+          load.fetch(x);
+          put(0);
+        }
+        if (count > 1)
+          load.fetch(x + kTile);
+        for (int n = 0; n < count; ++n, x += kTile) {
+          const int slot = n & 1;
+          __syncthreads();
+          uint32_t seen = 0u;
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            seen |= static_cast<uint32_t>(tokens[slot][w]) << (w * (kTile / W));
+          seen = static_cast<uint32_t>(uniform(static_cast<int>(seen)));
+          if (n + 1 < count)
+            put(slot ^ 1);
+          if (n + 2 < count)
+            load.fetch(x + 2 * kTile);
+          take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, slot);
+        }
+      }
+
+      __syncthreads();
+      if constexpr (!BUSY)
+        return;
+      const bool any_odd = !I8 && odd;
+      // ---- every wave's rows are its own
+      const AttendArgs &b = args_again();
+      const bool whole = it.s0 == 0 && it.s1 == it.units;
+      const int ln = anew(lane), c = ln & 15, g = ln >> 4;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float sum = r.total(t);
+        if (t * 16 + c >= rows)
+          continue;
+        if (whole) {
+          const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
+          const uint32_t j = fdiv(p, b.group);
+          const int64_t row = it.start + static_cast<int64_t>(j);
+          const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
+          const float f = finish(sum, I8 ? b.value_scale[it.head] : 1.0f);
+          char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (e * 16 + 4 * g < b.dim) {
+              const f32x4 o = r.acc[t][e] * f;
+              store(dst + e * 32, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
+            }
+          if (b.lse && g == 0)
+            b.lse[row * b.heads + qh] = log_sum(r.top[t], sum);
+        } else {
+          const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + wave * 16 * RT + t * 16 + c;
+          float *dst = b.partial + (part - c) * DP + part_at<DP, ROWS>(c, 4 * g);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            *reinterpret_cast<f32x4 *>(dst + e * 256) = r.acc[t][e];
+          if (g == 0) {
+            b.stats[part * 2] = r.top[t];
+            b.stats[part * 2 + 1] = sum;
+          }
+        }
+      }
+      if (__builtin_expect(any_odd, 0)) {
+        r.add_odd(it, row0, rows, x0, x_end, kTile, lane, [&](int t, int d, float v) {
+          const AttendArgs &b = args_again();
+          const int i = wave * 16 * RT + t * 16 + c;
+          if (!whole) {
+            b.partial[(run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS * DP + part_at<DP, ROWS>(i, d)] += v;
+            return;
+          }
+          // what is rounded is finite, and what comes to it is not
+          const uint32_t p = static_cast<uint32_t>(it.tile * ROWS + i);
+          const uint32_t j = fdiv(p, b.group);
+          char *o = b.out + ((it.start + static_cast<int64_t>(j)) * b.out_row +
+                             (static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d)) * b.out_head + d) * 2;
+          store(o, static_cast<uint16_t>(pack16<T>(widen16<T>(relx::load<uint16_t>(o)) + v, 0.0f)));
+        });
+      }
     };
     if (rows > 0) // the same for the whole wave
       work(std::true_type());
@@ -1392,7 +1399,8 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
     const int row0 = static_cast<int>(i / E - static_cast<int64_t>(head) * groups) * N;
     const int d = LANED ? e * 16 + (lane >> 4) * 4 : lane % (DP / 4) * 4;
     const int64_t u0 = first + (static_cast<int64_t>(head) * r.tiles + row0 / ROWS) * r.units;
-    const int64_t w0 = uniform64(divide(u0, static_cast<int>(per))), w1 = uniform64(divide(u0 + r.units - 1, static_cast<int>(per)));
+    const int64_t w0 = uniform64(divide(u0, static_cast<int>(per)));
+    const int64_t w1 = uniform64(divide(u0 + r.units - 1, static_cast<int>(per)));
     if (w0 == w1)
       continue; // written whole
     const bool valid = row0 + c < rows;
@@ -1461,7 +1469,8 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
       const int64_t qh = static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d);
       acc *= finish(sum, I8 ? a.value_scale[head] : 1.0f);
       if (d < a.dim)
-        store(a.out + (row * a.out_row + qh * a.out_head + d) * 2, u32x2{pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3])});
+        store(a.out + (row * a.out_row + qh * a.out_head + d) * 2,
+              u32x2{pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3])});
       if (a.lse && d == 0)
         a.lse[row * a.heads + qh] = log_sum(top, sum);
     }
@@ -1482,7 +1491,8 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
   // A wave for every piece of an even batch, within 2^16 blocks a request; eight
   // where an item lies in more than eight runs, on average: 8.1 us against 11.8
   // for 64 parts of 64 rows (14 MB), but 27 against 8.8 for five of 256 (31 MB).
-  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d, n = ROWS > 16 ? 16 : 256 / DP;
+  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d;
+  const int64_t n = ROWS > 16 ? 16 : 256 / DP;
   const int64_t pieces = (rows + n - 1) / n * a.kv_heads * (ROWS > 16 ? DP / 16 : 1);
   const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * a.requests;
   const bool many = p.workgroups > 8 * items;
