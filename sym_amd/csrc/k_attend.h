@@ -50,6 +50,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "attend_share.h"
 #include "attention.h"
 #include "index.h"
 
@@ -773,10 +774,8 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 // `first`, of every tile. Its tiles are PACE tokens apart.
 template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Loader {
   static constexpr int CELL = I8 ? 1 : 2;
-  static constexpr int LB = 16 / CELL;                     // dims of a lane's load
-  static constexpr int TL = DP / LB;                       // lanes of a token
-  static constexpr int TPI = 64 / TL;                      // tokens of a load
-  static constexpr int LOADS = NT > TPI ? NT / TPI : 1;
+  using Lanes = Share<DP, CELL, NT>;
+  static constexpr int LB = Lanes::LB, TL = Lanes::TL, TPI = Lanes::TPI, LOADS = Lanes::LOADS;
   static constexpr bool EVEN = SRC != kStaged;             // pages of whole tiles of 16 tokens
   static constexpr int RB = DP * (RAW ? 1 : 2);            // bytes of a token in the tile
 
@@ -786,6 +785,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   uint32_t key_slot, value_slot;
   int64_t key_slot64, value_slot64; // kStaged: of any size
   int length, pages, first, token, dim, cell_at, head_dims;
+  uint32_t key_token, value_token; // kStagedEven: where the lane's token lies after the load's first
   bool full; // the head fills the tile's rows
   bool once; // one tile of query rows reads a key head
   FastDiv page;
@@ -811,10 +811,12 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     once = a.once;
     pages = a.pages;
     page = a.page;
-    has = dim < a.dim && token < NT;
+    has = dim < a.dim && Lanes::brings(lane);
     whole = dim + LB <= a.dim;
     cell_at = has ? dim * CELL : 0;
     there = 0u;
+    key_token = static_cast<uint32_t>(Lanes::token(lane)) * key_slot;
+    value_token = static_cast<uint32_t>(Lanes::token(lane)) * value_slot;
     key_lane = (token + (first & 15)) * key_slot;
     value_lane = (token + (first & 15)) * value_slot;
     place16 = ((dim / LB) ^ swap_of<RB>(first + token)) * 16;
@@ -934,8 +936,8 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
       id = id >= 0 ? id : 0; // none: the first page, and zeros in its place
       const char *k = keys + id * key_page + off * key_slot64, *v = values + id * value_page + off * value_slot64;
       if constexpr (EVEN) {
-        k += token * key_slot + cell_at;
-        v += token * value_slot + cell_at;
+        k += key_token + cell_at;
+        v += value_token + cell_at;
       } else {
         k += cell_at;
         v += cell_at;
