@@ -427,8 +427,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
     int type;
     bool i8;
     relx::AttendArgs a = relx::attend_args(*args, plan, type, i8);
-    const bool any = a.rows > 0 && a.requests > 0;
-    if (any) {
+    if (a.rows > 0 && a.requests > 0) {
       const size_t want = relx::attend_workspace(plan, a.requests);
       if (args->workspace_bytes < 0 || static_cast<size_t>(args->workspace_bytes) < want || !args->workspace)
         throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(args->workspace_bytes) +
@@ -440,7 +439,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
       a.schedule = reinterpret_cast<int64_t *>(a.stats + rows * 2);
     }
     relx::on_context(ctx, [&] {
-      if (any)
+      if (a.rows > 0)
         relx::launched(relx::attend_launch(a, plan, type, i8, relx::stream_of(stream)), "attention");
     });
   });

@@ -1375,8 +1375,12 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), phase = PHASES == 1 ? 0 : wave;
   const int c = LANED ? lane & 15 : lane / (DP / 4);
   const int b = blockIdx.x;
-  if (b == a.requests) { // rows of no request
-    const int r0 = min(max(a.starts[0], 0), a.rows), r1 = min(max(a.starts[a.requests], r0), a.rows);
+  if (b == a.requests) { // rows of no request: where there is none, all
+    int r0 = 0, r1 = 0;
+    if (a.requests > 0) {
+      r0 = min(max(a.starts[0], 0), a.rows);
+      r1 = min(max(a.starts[a.requests], r0), a.rows);
+    }
     const int64_t none = static_cast<int64_t>(r0 + a.rows - r1) * a.heads;
     for (int64_t i = static_cast<int64_t>(blockIdx.y) * WAVES + wave; i < none; i += static_cast<int64_t>(gridDim.y) * WAVES) {
       int64_t row = i / a.heads;
@@ -1486,17 +1490,19 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
                         hipStream_t s) {
   AttendArgs a = args;
   void *pa[] = {&a};
-  hipError_t e = hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(p.workgroups)),
-                                 dim3(static_cast<uint32_t>(threads)), pa, 0, s);
+  hipError_t e = hipSuccess;
+  if (a.requests > 0)
+    e = hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(p.workgroups)), dim3(static_cast<uint32_t>(threads)), pa, 0, s);
   if (e != hipSuccess)
     return e;
   // A wave for every piece of an even batch, within 2^16 blocks a request; eight
   // where an item lies in more than eight runs, on average: 8.1 us against 11.8
   // for 64 parts of 64 rows (14 MB), but 27 against 8.8 for five of 256 (31 MB).
-  const int64_t rows = (static_cast<int64_t>(a.rows) + a.requests - 1) / a.requests * a.group.d;
+  const int64_t requests = std::max(a.requests, 1);
+  const int64_t rows = (a.rows + requests - 1) / requests * a.group.d;
   const int64_t n = ROWS > 16 ? 16 : 256 / DP;
   const int64_t pieces = (rows + n - 1) / n * a.kv_heads * (ROWS > 16 ? DP / 16 : 1);
-  const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * a.requests;
+  const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * requests;
   const bool many = p.workgroups > 8 * items;
   return hipLaunchKernel(many ? reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 8>)
                               : reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 1>),
