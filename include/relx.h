@@ -685,7 +685,8 @@ int relx_norm_rotate_append(relx_ctx *ctx, const relx_rotation *rot, const relx_
  * with lse -inf. A token that no row sees is not read into any sum, whatever it holds, and one
  * that only some rows see touches only those. `lse` (optional): natural
  * logarithm of the sum of exponentials, [rows, heads]. `workspace`: at least
- * the bytes that relx_tree_attention_workspace says, any contents. Head sizes
+ * the bytes that relx_tree_attention_workspace says, any contents. `scale` and the
+ * cache's scales may have either sign or be zero. Head sizes
  * are multiples of 8 up to 256; q and out share a type, f16 or bf16, and the
  * cache has it too or int8. */
 typedef struct relx_tree_attention_args {

@@ -191,7 +191,8 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   layout(dim >= 8 && dim <= 256 && dim % 8 == 0, "attention: head sizes are multiples of 8 up to 256");
   layout(p.columns == 0 || p.columns <= (int64_t{1} << 30) / p.cache.page, "attention: a table of more than 2^30 tokens");
   layout(p.rows <= INT32_MAX / p.heads, "attention: more than 2^31 - 1 rows of heads");
-  need(std::isfinite(p.scale), "attention: scale");
+  const float scale = static_cast<float>(p.scale * 1.4426950408889634);
+  need(std::isfinite(scale), "attention: scale");
   need(p.rows == 0 || (p.q.data && p.out.data), "attention: null queries or result");
   need(p.requests == 0 || (p.cached && p.starts), "attention: null lengths");
   need(p.requests == 0 || p.columns == 0 || p.table, "attention: null table");
@@ -229,7 +230,7 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   a.pages = static_cast<int32_t>(p.cache.pages);
   a.columns = static_cast<int32_t>(p.columns);
   a.words = static_cast<int32_t>(p.words);
-  a.scale = static_cast<float>(p.scale * 1.4426950408889634);
+  a.scale = scale;
   plan = attend_plan(p.rows, p.requests, kv, p.heads / kv, dim, p.cache.page);
   // a lane's distance inside a tile of 16 tokens is held in 32 bits
   if (a.key_slot > INT32_MAX / 32 || a.value_slot > INT32_MAX / 32)

@@ -558,13 +558,18 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   f32x4 acc[RT][E];  // dims 16 e + 4 (lane / 16) + 0..3
   int place[RT];     // among the request's new tokens
   uint64_t mask[RT]; // of one word
-  float scale;
+  float scale;       // above zero: its sign is the queries'
   int words;         // of a mask; 0: none
 
   __device__ __forceinline__ void start(const AttendArgs &a, const Item &it, int row0, int rows, float score_scale,
                                         int lane) {
     const int c = lane & 15, g = lane >> 4;
-    scale = score_scale;
+    // The maximum and the mask's -inf are those of unscaled scores, which goes for
+    // a scale above zero alone: so a negative one turns the queries over, and zero
+    // is the least normal number, by which no finite score reaches a bit of a weight.
+    constexpr float kLeast = 1.17549435e-38f;
+    const uint32_t sign = score_scale < 0.0f ? 0x80008000u : 0u;
+    scale = fabsf(score_scale) < kLeast ? kLeast : fabsf(score_scale);
     words = a.mask ? a.words : 0;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -583,6 +588,7 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
         q[t][s] = u32x4{0u, 0u, 0u, 0u};
         if (t * 16 + c < rows && d < a.dim)
           q[t][s] = load<u32x4>(src + d * 2);
+        q[t][s] ^= sign;
       }
       top[t] = kNone;
       sum[t] = 0.0f;
@@ -757,7 +763,7 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 #pragma clang loop unroll(disable)
           for (int d = 0; d < a.dim; ++d)
             score += widen16<T>(load<uint16_t>(q + d * 2)) * widen16<T>(load<uint16_t>(k + d * 2));
-          const float weight = __builtin_amdgcn_exp2f(score * scale - top[t]);
+          const float weight = __builtin_amdgcn_exp2f(score * a.scale - top[t]);
 #pragma clang loop unroll(disable)
           for (int d = 4 * g; d < a.dim; d += (d & 3) == 3 ? 13 : 1) {
             const uint32_t h = load<uint16_t>(v + d * 2);

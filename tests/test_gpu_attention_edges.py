@@ -44,3 +44,71 @@ def test_rows_without_any_request_are_zero(ctx, dtype, cache, heads, dim, rows):
     assert not out.any() and (lse == -float("inf")).all()
     room[:, 1, :, :dim] = 7.0
     assert (room == 7.0).all()  # and nothing beside it
+
+
+# ------------------------------------------------------------ scales
+
+# heads, kv, dim, page, cached, fresh, words: one row a key head, up to 16, 64, 128, 256
+SCALED = [(4, 4, 128, 16, [70, 0, 33], [1, 1, 1], 0), (8, 2, 64, 24, [30, 3], [3, 2], 1), (8, 2, 128, 16, [40, 9], [12, 9], 1),
+          (4, 2, 136, 16, [50], [20], 1), (4, 1, 128, 16, [100], [25], 0), (4, 1, 64, 32, [90], [60], 1), (2, 1, 128, 8, [33], [70], 2)]
+
+
+def result(ctx, s, **more):
+    d = on_gpu(s)
+    lse = torch.full(s["q"].shape[:2], 7.0, device=DEV)
+    out = A.tree_attention(ctx, d["q"], d["cache_k"], d["cache_v"], d["table"], d["cached"], d["starts"], mask=d["mask"],
+                           scale=d["scale"], k_scale=d["k_scale"], v_scale=d["v_scale"], lse=lse, **more)
+    torch.cuda.synchronize()
+    return out.double().cpu(), lse.double().cpu()
+
+
+def check(ctx, s, what, positive=None):
+    """`positive`: the same step with a scale of zero or above, for the bound."""
+    p = dict(s, **(positive or {}))
+    say("attend", what)
+    out, lse = result(ctx, s)
+    want, want_lse, bound = C.attention(p["q"], p["cache_k"], p["cache_v"], p["table"], p["cached"], p["starts"], p["mask"],
+                                        p["scale"], p["k_scale"], p["v_scale"], p["q"].dtype)
+    assert not torch.isnan(out).any(), what
+    assert bool(((out - want).abs() <= bound + 2.0 ** -24).all()), what
+    empty = torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), empty), what
+    assert bool(((lse - want_lse)[~empty].abs() <= 2.0 ** -17 * (1 + want_lse[~empty].abs())).all()), what
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,cached,fresh,words", SCALED)
+@pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, I8)])
+def test_tree_attention_of_scales_that_are_not_positive(ctx, heads, kv, dim, page, cached, fresh, words, dtype, cache):
+    s = C.attention_case(dim + fresh[0], cached, fresh, heads, kv, dim, dtype, cache, page, tree_words=words)
+    if words:
+        s["mask"][1] = 0  # sees the context alone, which a request may not have
+    check(ctx, dict(s, scale=0.0), ("zero", heads, kv, dim, page, dtype, cache))
+    check(ctx, dict(s, scale=-0.1), ("negative", heads, kv, dim, page, dtype, cache), dict(q=-s["q"], scale=0.1))
+    check(ctx, dict(s, scale=1e-30), ("tiny", heads, kv, dim, page, dtype, cache))
+    if cache == I8:
+        k = s["k_scale"].clone()
+        k[0], k[-1] = -k[0], (0.0 if kv > 1 else -k[-1])
+        check(ctx, dict(s, k_scale=k, v_scale=-s["v_scale"]), ("key scales", heads, kv, dim, page, dtype))
+        check(ctx, dict(s, k_scale=k * 0), ("key scales of zero", heads, kv, dim, page, dtype))
+
+
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("fresh", [4, 40])
+def test_a_negative_scale_is_the_negative_queries_bit_for_bit(ctx, page, fresh):
+    """With infinities and NaN in values that only some rows see, too."""
+    s = C.attention_case(page, [50, 0], [fresh, fresh], 4, 2, 128, BF16, BF16, page, tree_words=1)
+    g, o = divmod(50 + 2, page)
+    s["cache_v"][int(s["table"][0, g]), o, 0, 5] = float("inf")
+    s["cache_v"][int(s["table"][0, g]), o, 1, 9] = float("nan")
+    out, lse = result(ctx, dict(s, scale=-0.125))
+    want, want_lse = result(ctx, dict(s, q=-s["q"], scale=0.125))
+    assert torch.isnan(want).any() and torch.isinf(want).any()
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
+    assert torch.equal(lse, want_lse)
+
+
+def test_a_scale_that_is_no_finite_number_is_refused(ctx):
+    s = C.attention_case(1, [20], [2], 4, 2, 64, F16, F16, 16)
+    for scale in (float("inf"), float("nan"), 3e38, -1e300):
+        with pytest.raises(P.TransferError, match="invalid_argument"):
+            result(ctx, dict(s, scale=scale))
