@@ -413,7 +413,10 @@ __global__ __launch_bounds__(64 * kWaves) void k_rotate(RotateArgs a) {
           ss += x[e] * x[e];
           ux += g[e] * w[e] * x[e];
         }
-        const float r = rsqrtf(head_sum<L>(ss) * a.inv_dim + a.eps);
+        // lanes without a head add nothing to the weight's gradient, also where
+        // eps = 0 makes their root infinite
+        const float mean = head_sum<L>(ss) * a.inv_dim;
+        const float r = live[u] ? rsqrtf(mean + a.eps) : 0.0f;
         const float m = head_sum<L>(ux) * r * a.inv_dim; // mean(u n)
 #pragma unroll
         for (int e = 0; e < kV; ++e) {

@@ -112,3 +112,29 @@ def test_a_scale_that_is_no_finite_number_is_refused(ctx):
     for scale in (float("inf"), float("nan"), 3e38, -1e300):
         with pytest.raises(P.TransferError, match="invalid_argument"):
             result(ctx, dict(s, scale=scale))
+
+
+# ------------------------------------------------------------ norms without eps
+
+@pytest.mark.parametrize("heads,kv,dim", [(3, 1, 128), (5, 2, 64), (9, 3, 256), (1, 1, 80), (4, 4, 512)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_weight_gradients_without_eps(ctx, heads, kv, dim, dtype):
+    """A wave has room for more heads than there are: what is not there adds nothing."""
+    say("eps 0", heads, kv, dim, dtype)
+    gen = torch.Generator().manual_seed(dim + heads)
+    rows, rotary = 23, dim // 2
+    x = {n: torch.randn((rows, h, dim), generator=gen).to(dtype) for n, h in (("q", heads), ("k", kv), ("dq", heads), ("dk", kv))}
+    w = [(1 + 0.3 * torch.randn(dim, generator=gen)).to(dtype) for _ in range(2)]
+    a = torch.rand((rows, rotary // 2), generator=gen, dtype=torch.float64) * 6
+    cos, sin = a.cos().float(), a.sin().float()
+    at = torch.arange(rows, dtype=torch.int32)
+    d = {n: t.to(DEV) for n, t in x.items()}
+    got = A.norm_rotate_backward(ctx, d["dq"], d["dk"], d["q"], d["k"], at.to(DEV), cos.to(DEV), sin.to(DEV), w[0].to(DEV),
+                                 w[1].to(DEV), 0.0)
+    torch.cuda.synchronize()
+    u = C.ROUND[dtype]
+    for i, n in enumerate("qk"):
+        want, bound, want_w, size_w = C.norm_rotate_back(x["d" + n], x[n], w[i], cos.double(), sin.double(), rotary, False, 0.0)
+        assert bool(((got[i].double().cpu() - want).abs() <= bound * (1 + u) + u * want.abs() + 2.0 ** -25).all()), n
+        # as where eps is not zero: a term has dim / 2 + 8 roundings, its sums fewer than 192
+        assert bool(((got[2 + i].double().cpu() - want_w).abs() <= (dim / 2 + 8 + 192) * C.F32 * size_w).all()), n
