@@ -24,9 +24,10 @@ import ctypes
 import struct
 import threading
 from collections import namedtuple
-from functools import lru_cache
+from functools import lru_cache, partial
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .transfer import _fail
@@ -146,6 +147,28 @@ def _cache(keys, values, k_scale, v_scale, device):
     return (keys.data_ptr(), kp, ks, kh, values.data_ptr(), vp, vs, vh, k_ptr, v_ptr, *shape, *kind)
 
 
+def _in_graph(*operands):
+    """Whether torch would follow a gradient through a call of these."""
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+class _NoGradient(torch.autograd.Function):
+    """A call that has no gradient, of operands that want one: its result says so
+    when a gradient reaches it, rather than end it in silence."""
+    @staticmethod
+    def forward(fn, name, call, *operands):
+        fn.name = name
+        return call()
+
+    @staticmethod
+    def backward(fn, *gradients):
+        raise RuntimeError("sym_amd.attention.%s has no gradient" % fn.name)
+
+
 # ------------------------------------------------------------ block tables
 
 def block_tables(ctx, cached, fresh, table, free_pages, page, rows, *, parents=None, words=1, out=None):
@@ -245,7 +268,10 @@ class _NormRotate(torch.autograd.Function):
         return _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, None)
 
     @staticmethod
+    @once_differentiable
     def backward(fn, dq, dk):
+        if fn.needs_input_grad[6] or fn.needs_input_grad[7]:
+            raise RuntimeError("sym_amd.attention.norm_rotate has no gradient for cos and sin")
         q, k, q_weight, k_weight, positions, cos, sin = fn.saved_tensors
         ctx, eps, pairs = fn.rest
         gq, gk, gqw, gkw = norm_rotate_backward(ctx, dq.contiguous(), dk.contiguous(), q, k, positions, cos, sin,
@@ -264,11 +290,9 @@ def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pair
     [angles, rotary / 2]), which turn the first `rotary` elements: halves
     (i, i + rotary / 2), or neighbours (2 i, 2 i + 1) with `pairs`. A position
     outside the table gives NaN. Returns (queries, keys); `out`: a pair of
-    tensors to write into. Differentiable in q, k and the weights (without
-    `out`)."""
-    if out is None and torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad) or
-            (k_weight is not None and k_weight.requires_grad)):
+    tensors to write into. Differentiable in q, k and the weights, once (without
+    `out`; a second derivative, or one by cos and sin, raises)."""
+    if out is None and _in_graph(q, k, q_weight, k_weight, cos, sin):
         return _NormRotate.apply(q, k, q_weight, k_weight, ctx, positions, cos, sin, eps, pairs)
     return _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out)
 
@@ -336,7 +360,13 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     outside the cache is skipped, and rows have slots of their own). The cache
     is [pages, page, kv_heads, dim] of any strides, of the operands' type, or
     int8 with a scale a head (float32 [kv_heads] each), quantized as the
-    package's plans quantize."""
+    package's plans quantize. There is no gradient: one that reaches the result
+    (without `out`) raises."""
+    if out is None and _in_graph(q, k, v, cos, sin, q_weight, k_weight):
+        return _NoGradient.apply(
+            "norm_rotate_append",
+            partial(norm_rotate_append, ctx, q, k, v, slots, cache_k, cache_v, positions, cos, sin, q_weight, k_weight, eps,
+                    pairs=pairs, k_scale=k_scale, v_scale=v_scale), q, k, v, cos, sin, q_weight, k_weight)
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
     if out is None:
@@ -383,7 +413,13 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     `scale`: of the scores, by default dim ** -0.5. `lse`: float32 [rows,
     heads] for the logarithm of each row's sum of exponentials. `workspace`: a
     uint8 tensor of `tree_attention_workspace` bytes, for programs that keep
-    one a stream; by default torch's allocator gives it."""
+    one a stream; by default torch's allocator gives it. There is no gradient:
+    one that reaches the result (without `out`) raises."""
+    if out is None and _in_graph(q, cache_k, cache_v, k_scale, v_scale):
+        return _NoGradient.apply(
+            "tree_attention",
+            partial(tree_attention, ctx, q, cache_k, cache_v, table, cached, starts, mask=mask, scale=scale, k_scale=k_scale,
+                    v_scale=v_scale, lse=lse, workspace=workspace), q, cache_k, cache_v, k_scale, v_scale)
     device = _device(ctx, q)
     shape, dtype = q.shape, q.dtype
     kind = _KINDS.get(dtype)

@@ -138,3 +138,16 @@ def test_weight_gradients_without_eps(ctx, heads, kv, dim, dtype):
         assert bool(((got[i].double().cpu() - want).abs() <= bound * (1 + u) + u * want.abs() + 2.0 ** -25).all()), n
         # as where eps is not zero: a term has dim / 2 + 8 roundings, its sums fewer than 192
         assert bool(((got[2 + i].double().cpu() - want_w).abs() <= (dim / 2 + 8 + 192) * C.F32 * size_w).all()), n
+
+
+def test_norm_rotate_is_differentiable_once(ctx):
+    say("second derivative")
+    gen = torch.Generator().manual_seed(2)
+    q, k = (torch.randn((3, 2, 64), generator=gen).to(DEV).requires_grad_() for _ in range(2))
+    cos, sin = torch.ones((3, 32), device=DEV), torch.zeros((3, 32), device=DEV)
+    at = torch.arange(3, dtype=torch.int32, device=DEV)
+    zq, _ = A.norm_rotate(ctx, q, k, at, cos, sin, None, None, 1e-6)
+    grad, = torch.autograd.grad((zq ** 3).sum(), q, create_graph=True)
+    assert torch.isfinite(grad).all()
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        ((q ** 2).sum() + (grad ** 2).sum()).backward()
