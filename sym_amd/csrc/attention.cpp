@@ -66,7 +66,8 @@ TablesArgs tables_args(const relx_block_tables_args &p) {
   need(p.table_row >= p.columns || p.requests <= 1, "block tables: table rows overlap");
   need(p.free_count == 0 || p.free_pages, "block tables: null page list");
   need(p.rows == 0 || (p.slots && p.positions), "block tables: null slots or positions");
-  need((p.parents != nullptr) == (p.words > 0), "block tables: a mask goes with parents");
+  // a list of no parents may have no address
+  need(p.rows == 0 || (p.parents != nullptr) == (p.words > 0), "block tables: a mask goes with parents");
   need(!p.parents || p.rows == 0 || p.mask, "block tables: null mask");
   TablesArgs a{};
   a.cached = p.cached;
@@ -160,7 +161,7 @@ CacheBytes cache_bytes(const relx_cache &c) {
   b.type = element_type(c.kind, c.bits);
   need(c.pages >= 0 && fits32(c.pages) && c.page >= 1 && fits32(c.page) && c.kv_heads >= 0, "cache: sizes");
   layout(c.page * c.pages <= INT32_MAX, "cache: more than 2^31 - 1 slots");
-  need(c.pages == 0 || (c.keys && c.values), "cache: null keys or values");
+  need(c.pages == 0 || c.kv_heads == 0 || (c.keys && c.values), "cache: null keys or values");
   need(b.type != kI8 || c.kv_heads == 0 || (c.key_scale && c.value_scale), "cache: an int8 cache has a scale a head");
   need(c.key_page >= 0 && c.key_slot >= 0 && c.key_head >= 0 && c.value_page >= 0 && c.value_slot >= 0 &&
            c.value_head >= 0,

@@ -46,6 +46,36 @@ def test_rows_without_any_request_are_zero(ctx, dtype, cache, heads, dim, rows):
     assert (room == 7.0).all()  # and nothing beside it
 
 
+# ------------------------------------------------------------ no rows
+
+@pytest.mark.parametrize("words", [1, 3])
+@pytest.mark.parametrize("given", [False, True])
+def test_block_tables_of_trees_without_rows(ctx, words, given):
+    say("trees without rows", words)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    out = A.Tables(torch.full((3,), -7, **i32), torch.empty(0, dtype=torch.int64, device=DEV), torch.empty(0, **i32),
+                   torch.full((1,), -7, **i32), torch.empty((0, words), dtype=torch.int64, device=DEV)) if given else None
+    t = A.block_tables(ctx, torch.tensor([4, 30], **i32), torch.zeros(2, **i32), torch.zeros((2, 4), **i32),
+                       torch.empty(0, **i32), 16, 0, parents=torch.empty(0, **i32), words=words, out=out)
+    torch.cuda.synchronize()
+    assert t.starts.tolist() == [0, 0, 0] and t.taken.tolist() == [0]
+    assert t.slots.shape == t.positions.shape == (0,) and t.mask.shape == (0, words)
+
+
+def test_append_without_key_heads(ctx):
+    """An empty cache tensor has no address either; the queries turn as ever."""
+    say("append without key heads")
+    gen = torch.Generator().manual_seed(1)
+    q = torch.randn((3, 4, 64), generator=gen).to(F16).to(DEV)
+    none, cache = torch.empty((3, 0, 64), dtype=F16, device=DEV), torch.empty((2, 16, 0, 64), dtype=F16, device=DEV)
+    turn = (torch.arange(3, dtype=torch.int32, device=DEV), torch.ones((3, 32), device=DEV), torch.zeros((3, 32), device=DEV),
+            None, None, 1e-6)
+    out = A.norm_rotate_append(ctx, q, none, none, torch.arange(3, device=DEV), cache, cache, *turn)
+    want, _ = A.norm_rotate(ctx, q, none, *turn)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 # ------------------------------------------------------------ scales
 
 # heads, kv, dim, page, cached, fresh, words: one row a key head, up to 16, 64, 128, 256
