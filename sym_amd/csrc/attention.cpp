@@ -4,7 +4,6 @@
 
 #include <climits>
 #include <cmath>
-#include <mutex>
 
 #include "capi.h"
 #include "runtime.h"
@@ -43,9 +42,10 @@ void launched(hipError_t e, const char *what) {
 }
 
 // Runs `fn` with the context's device current, if the context takes calls.
+// Not under its mutex, which transfers hold until the GPU has done them: these
+// calls use nothing that it guards.
 template <class F> void on_context(relx_ctx *ctx, F &&fn) {
   need(ctx != nullptr, "null context");
-  std::lock_guard<std::mutex> g(ctx->ctx->mu);
   if (ctx->ctx->closed || ctx->ctx->quarantined)
     throw Error("resources_closed", "context is closed or quarantined");
   DeviceScope scope(ctx->ctx->device);

@@ -353,8 +353,10 @@ struct Context {
   // arena orders its streams after it.
   bool unsynced = false;
   std::thread::id last_thread; // the thread of the previous pipeline call
-  bool quarantined = false;
-  bool closed = false;
+  // Written under `mu`; read without it by calls that take nothing of the
+  // context but its device.
+  std::atomic<bool> quarantined{false};
+  std::atomic<bool> closed{false};
   ~Context(); // frees the status flags (the rest goes in destroy_context)
 };
 
