@@ -341,15 +341,18 @@ _rooms = {}
 
 
 def _rotate_room(rot, qs, ks, dtype):
+    # other threads may clear the sizes at any time
     key = (qs, ks[1], dtype)
-    if key not in _rooms:
-        if len(_rooms) >= 1024:
-            _rooms.clear()
+    room = _rooms.get(key)
+    if room is None:
         size, err = ctypes.c_size_t(), N.relx_err()
         if N.lib().relx_norm_rotate_workspace(rot, ctypes.byref(size), ctypes.byref(err)):
             _fail(err)
-        _rooms[key] = size.value
-    return _rooms[key]
+        room = size.value
+        if len(_rooms) >= 1024:
+            _rooms.clear()
+        _rooms[key] = room
+    return room
 
 
 def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, sin, q_weight, k_weight, eps, *,

@@ -37,3 +37,41 @@ def test_calls_do_not_wait_for_transfers(results):
 
 def test_a_quarantined_context_takes_no_calls(results):
     assert results["tables of a quarantined context"] == "resources_closed"
+
+
+def test_workspace_sizes_while_others_clear_them(monkeypatch):
+    """Every size of the backward's workspace is found, also where it is cleared
+    between a thread's look and its answer."""
+    torch = pytest.importorskip("torch")
+    from sym_amd import _native as N
+    from sym_amd import attention as A
+
+    class Cleared(dict):
+        """As if another thread cleared it between any two steps of this one."""
+        def _clear(self):
+            dict.clear(self)
+
+        def __contains__(self, key):
+            found = dict.__contains__(self, key)
+            self._clear()
+            return found
+
+        def __setitem__(self, key, value):
+            dict.__setitem__(self, key, value)
+            self._clear()
+
+        def __len__(self):
+            n = dict.__len__(self)
+            self._clear()
+            return n
+
+        def get(self, key, default=None):
+            value = dict.get(self, key, default)
+            self._clear()
+            return value
+
+    monkeypatch.setattr(A, "_rooms", Cleared())
+    positions = (N.ctypes.c_int32 * 4)()
+    rot = A._ROTATION.pack(N.ctypes.addressof(positions), 0, 0, 0, 0, 0, 32, 4, 6, 2, 64, 0, 0, 0, 0, 16, 1e-6)
+    sizes = [A._rotate_room(rot, torch.Size((4, 6, 64)), torch.Size((4, 2, 64)), torch.float16) for _ in range(3)]
+    assert sizes[0] > 0 and len(set(sizes)) == 1
