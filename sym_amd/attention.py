@@ -275,7 +275,8 @@ class _NormRotate(torch.autograd.Function):
         q, k, q_weight, k_weight, positions, cos, sin = fn.saved_tensors
         ctx, eps, pairs = fn.rest
         gq, gk, gqw, gkw = norm_rotate_backward(ctx, dq.contiguous(), dk.contiguous(), q, k, positions, cos, sin,
-                                                q_weight, k_weight, eps, pairs=pairs)
+                                                q_weight, k_weight, eps, pairs=pairs,
+                                                weight_grads=fn.needs_input_grad[2:4])
         return (gq, gk, None if gqw is None else gqw.to(q_weight.dtype),
                 None if gkw is None else gkw.to(k_weight.dtype), None, None, None, None, None, None)
 
@@ -311,20 +312,22 @@ def _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs,
     return zq, zk
 
 
-def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pairs=False):
+def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pairs=False,
+                         weight_grads=(True, True)):
     """Gradients of `norm_rotate` for its results' gradients `dq` and `dk`:
     (queries', keys', query weight's, key weight's). The weights' are float32
     [dim], summed over rows and heads in a fixed order (None where the weight
-    is); the others have the operands' type."""
+    is, or where `weight_grads` says that it is not wanted); the others have the
+    operands' type."""
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
     gq, gk = q.new_empty(qs), k.new_empty(ks)
     gqw = gkw = None
     gqw_ptr = gkw_ptr = room_ptr = size = 0
-    if q_weight is not None:
+    if q_weight is not None and weight_grads[0]:
         gqw = cos.new_empty(qs[2])
         gqw_ptr = gqw.data_ptr()
-    if k_weight is not None:
+    if k_weight is not None and weight_grads[1]:
         gkw = cos.new_empty(qs[2])
         gkw_ptr = gkw.data_ptr()
     if gqw_ptr or gkw_ptr:

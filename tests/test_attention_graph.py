@@ -86,3 +86,18 @@ def test_calls_without_a_gradient_say_so(monkeypatch):
             given = torch.empty_like(h[0], requires_grad=False)
             assert call(out=given) is given and not given.requires_grad
             t.requires_grad_(False)
+
+
+@pytest.mark.parametrize("wanted", [(True, False), (False, True), (False, False), (True, True)])
+def test_gradients_of_frozen_weights_are_not_computed(squares, monkeypatch, wanted):
+    q, k, cos, sin, _ = squares
+    asked = []
+
+    def backward(ctx, dq, dk, *rest, weight_grads, **more):
+        asked.append(tuple(weight_grads))
+        return dq, dk, *(torch.ones(4) if w else None for w in weight_grads)
+    monkeypatch.setattr(A, "norm_rotate_backward", backward)
+    weights = [torch.ones(4).requires_grad_(w) for w in wanted]
+    zq, zk = A.norm_rotate(Ctx, q, k, None, cos, sin, *weights, 1e-6)
+    (zq.sum() + zk.sum()).backward()
+    assert asked == [wanted] and [w.grad is not None for w in weights] == list(wanted)

@@ -181,3 +181,19 @@ def test_norm_rotate_is_differentiable_once(ctx):
     assert torch.isfinite(grad).all()
     with pytest.raises(RuntimeError, match="once_differentiable"):
         ((q ** 2).sum() + (grad ** 2).sum()).backward()
+
+
+@pytest.mark.parametrize("wanted", [(True, False), (False, True), (False, False)])
+def test_gradients_without_those_of_frozen_weights(ctx, wanted):
+    say("frozen weights", wanted)
+    gen = torch.Generator().manual_seed(3)
+    q, k, dq, dk = (torch.randn((50, n, 80), generator=gen).to(BF16).to(DEV) for n in (5, 2, 5, 2))
+    w = [torch.rand(80, generator=gen).to(BF16).to(DEV) for _ in range(2)]
+    a = torch.rand((50, 40), generator=gen).to(DEV)
+    args = (dq, dk, q, k, torch.arange(50, dtype=torch.int32, device=DEV), a.cos(), a.sin(), *w, 1e-6)
+    every = A.norm_rotate_backward(ctx, *args)
+    some = A.norm_rotate_backward(ctx, *args, weight_grads=wanted)
+    torch.cuda.synchronize()
+    assert torch.equal(every[0], some[0]) and torch.equal(every[1], some[1])
+    for i in range(2):
+        assert torch.equal(every[2 + i], some[2 + i]) if wanted[i] else some[2 + i] is None
