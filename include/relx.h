@@ -584,7 +584,7 @@ double relx_measure_copy(int device, size_t bytes, int iters, int rounds);
  * outside the cache, a row outside the operands) is left out there, never
  * followed. Element types are (kind, bits) as in relx_param: (0, 32) f32,
  * (0, 16) f16, (1, 16) bf16, (2, 8) int8. Strides are in elements; the last
- * dimension is contiguous. Errors of all: "invalid_argument",
+ * dimension is contiguous, and the elements of a result lie apart. Errors of all: "invalid_argument",
  * "unsupported_layout" (a type, size or head layout that no kernel takes),
  * "insufficient_capacity" (workspace), "resources_closed",
  * "backend_failure". */

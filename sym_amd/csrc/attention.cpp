@@ -4,6 +4,8 @@
 
 #include <climits>
 #include <cmath>
+#include <cstdlib>
+#include <utility>
 
 #include "capi.h"
 #include "runtime.h"
@@ -53,6 +55,34 @@ template <class F> void on_context(relx_ctx *ctx, F &&fn) {
 }
 
 hipStream_t stream_of(uint64_t s) { return reinterpret_cast<hipStream_t>(s); }
+
+// Whether elements of [n1, n2, dim] with these strides share a place.
+bool overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t dim) {
+  using Wide = __int128;
+  s1 = n1 > 1 ? std::abs(s1) : 0;
+  s2 = n2 > 1 ? std::abs(s2) : 0;
+  if (s1 > s2) {
+    std::swap(n1, n2);
+    std::swap(s1, s2);
+  }
+  if ((n1 > 1 && s1 < dim) || (n2 > 1 && s2 < dim))
+    return true;
+  if (n1 <= 1 || n2 <= 1)
+    return false;
+  // the larger steps that end inside the smaller ones' reach: hardly ever any
+  const Wide reach = static_cast<Wide>(n1 - 1) * s1;
+  for (int64_t i = 1; i < n2 && static_cast<Wide>(i) * s2 < reach + dim; ++i) {
+    const Wide at = static_cast<Wide>(i) * s2, below = at / s1; // the steps next to it
+    if ((below < n1 && at - below * s1 < dim) || (below + 1 < n1 && (below + 1) * s1 - at < dim))
+      return true;
+  }
+  return false;
+}
+
+// A result that several threads would write in one place is refused.
+void writable(const relx_heads *h, int64_t rows, int64_t heads, int64_t dim) {
+  need(!h || rows == 0 || heads == 0 || !overlap(rows, h->row, heads, h->head, dim), "a result's elements overlap");
+}
 
 // ------------------------------------------------------------ block tables
 
@@ -195,6 +225,7 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   const float scale = static_cast<float>(p.scale * 1.4426950408889634);
   need(std::isfinite(scale), "attention: scale");
   need(p.rows == 0 || (p.q.data && p.out.data), "attention: null queries or result");
+  writable(&p.out, p.rows, p.heads, dim);
   need(p.requests == 0 || (p.cached && p.starts), "attention: null lengths");
   need(p.requests == 0 || p.columns == 0 || p.table, "attention: null table");
   need(!p.mask || p.words >= 1, "attention: a mask has words");
@@ -312,6 +343,8 @@ int relx_norm_rotate(relx_ctx *ctx, const relx_rotation *rot, const relx_heads *
     const bool uq = a.rows && a.heads[0], uk = a.rows && a.heads[1];
     a.x[0] = relx::heads_of(q, uq, "norm and rotation: null queries");
     a.x[1] = relx::heads_of(k, uk, "norm and rotation: null keys");
+    relx::writable(q_out, a.rows, a.heads[0], a.dim);
+    relx::writable(k_out, a.rows, a.heads[1], a.dim);
     a.y[0] = relx::heads_of(q_out, uq, "norm and rotation: null query result");
     a.y[1] = relx::heads_of(k_out, uk, "norm and rotation: null key result");
     relx::on_context(ctx, [&] {
@@ -344,6 +377,8 @@ int relx_norm_rotate_backward(relx_ctx *ctx, const relx_rotation *rot, const rel
     a.x[1] = relx::heads_of(k, uk, "norm and rotation: null keys");
     a.dz[0] = relx::heads_of(dq, uq, "norm and rotation: null query gradient");
     a.dz[1] = relx::heads_of(dk, uk, "norm and rotation: null key gradient");
+    relx::writable(q_grad, a.rows, a.heads[0], a.dim);
+    relx::writable(k_grad, a.rows, a.heads[1], a.dim);
     a.y[0] = relx::heads_of(q_grad, uq, "norm and rotation: null query gradient");
     a.y[1] = relx::heads_of(k_grad, uk, "norm and rotation: null key gradient");
     a.weight_grad[0] = q_weight_grad;
@@ -380,6 +415,15 @@ int relx_norm_rotate_append(relx_ctx *ctx, const relx_rotation *rot, const relx_
     a.x[0] = relx::heads_of(q, uq, "append: null queries");
     a.x[1] = relx::heads_of(k, uk, "append: null keys");
     a.x[2] = relx::heads_of(v, uk, "append: null values");
+    relx::writable(q_out, a.rows, a.heads[0], a.dim);
+    const auto apart = [&](int64_t page, int64_t slot, int64_t head) {
+      return !relx::overlap(cache->pages, page, cache->page, slot, cache->dim) &&
+             !relx::overlap(cache->pages, page, cache->kv_heads, head, cache->dim) &&
+             !relx::overlap(cache->page, slot, cache->kv_heads, head, cache->dim);
+    };
+    relx::need(!uk || cache->pages == 0 || (apart(cache->key_page, cache->key_slot, cache->key_head) &&
+                                            apart(cache->value_page, cache->value_slot, cache->value_head)),
+               "append: the cache's elements overlap");
     a.y[0] = relx::heads_of(q_out, uq, "append: null query result");
     relx::need(!uk || slots, "append: null slots");
     a.chunks[2] = a.chunks[1];

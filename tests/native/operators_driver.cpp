@@ -8,6 +8,8 @@
 #include <cstring>
 #include <functional>
 #include <mutex>
+#include <set>
+#include <string>
 #include <thread>
 
 #include "../../include/relx.h"
@@ -67,6 +69,73 @@ std::string beside_a_transfer(const std::function<std::string()> &call) {
   return returned ? result : "waited";
 }
 
+// norm and rotation into a result of these strides, dims of 8
+std::string rotate(int64_t rows, int64_t row, int64_t heads, int64_t head) {
+  relx_rotation r{};
+  r.positions = g_int;
+  r.rows = rows;
+  r.heads = heads;
+  r.dim = 8;
+  r.bits = 16;
+  relx_heads x{g_long, heads * 8, 8}, y{g_long, row, head};
+  relx_err err;
+  const std::string forward = relx_norm_rotate(g_ctx, &r, &x, nullptr, &y, nullptr, 0, &err) == RELX_OK ? "ok" : err.code;
+  const std::string back = relx_norm_rotate_backward(g_ctx, &r, &x, nullptr, &x, nullptr, &y, nullptr, nullptr, nullptr,
+                                                     nullptr, 0, 0, &err) == RELX_OK
+                               ? "ok"
+                               : err.code;
+  return forward == back ? forward : forward + " and " + back;
+}
+
+// and by brute force
+std::string rotate_walked(int64_t rows, int64_t row, int64_t heads, int64_t head) {
+  std::set<int64_t> seen;
+  for (int64_t r = 0; r < rows; ++r)
+    for (int64_t h = 0; h < heads; ++h)
+      for (int64_t d = 0; d < 8; ++d)
+        if (!seen.insert(r * row + h * head + d).second)
+          return "invalid_argument";
+  return "ok";
+}
+
+// the two over all small strides
+std::string rotate_everywhere() {
+  int wrong = 0;
+  for (int64_t rows = 1; rows < 6; ++rows)
+    for (int64_t heads = 1; heads < 6; ++heads)
+      for (int64_t row = 0; row < 60; row += 3)
+        for (int64_t head = 0; head < 60; ++head)
+          wrong += rotate(rows, row, heads, head) != rotate_walked(rows, row, heads, head);
+  return std::to_string(wrong);
+}
+
+// one row into a cache of two pages of four slots of three heads
+std::string append(int64_t page, int64_t slot, int64_t head) {
+  relx_rotation r{};
+  r.positions = g_int;
+  r.rows = 1;
+  r.kv_heads = 3;
+  r.dim = 8;
+  r.bits = 16;
+  relx_heads x{g_long, 24, 8};
+  relx_cache c{g_long, 96, 24, 8, g_long, page, slot, head, nullptr, nullptr, 2, 4, 3, 8, 0, 16};
+  relx_err err;
+  return relx_norm_rotate_append(g_ctx, &r, nullptr, &x, &x, nullptr, g_long, &c, 0, &err) == RELX_OK ? "ok" : err.code;
+}
+
+std::string attend(int64_t rows, int64_t row, int64_t heads, int64_t head) {
+  relx_tree_attention_args a{};
+  a.q = {g_long, heads * 8, 8};
+  a.out = {g_long, row, head};
+  a.cache = {g_long, 96, 24, 8, g_long, 96, 24, 8, nullptr, nullptr, 2, 4, heads, 8, 0, 16};
+  a.rows = rows;
+  a.heads = heads;
+  a.bits = 16;
+  a.scale = 1.0;
+  relx_err err;
+  return relx_tree_attention(g_ctx, &a, 0, &err) == RELX_OK ? "ok" : err.code;
+}
+
 void say(const char *what, const std::string &result) { std::printf("%s: %s\n", what, result.c_str()); }
 
 } // namespace
@@ -79,6 +148,16 @@ int main() {
   say("tables", tables());
   say("tables beside a transfer", beside_a_transfer(tables));
   say("launches", std::to_string(relx::g_launches));
+  say("results of any strides that are judged otherwise than by brute force", rotate_everywhere());
+  say("append", append(96, 24, 8));
+  say("append, head-major", append(96, 8, 32));
+  say("append, pages inside slots", append(24, 48, 8));
+  say("append, one page twice", append(0, 24, 8));
+  say("append, slots that share elements", append(96, 20, 8));
+  say("append, heads that share elements", append(96, 24, 4));
+  say("attend", attend(5, 16, 2, 8));
+  say("attend, one row for all", attend(5, 0, 2, 8));
+  say("attend, one head for all", attend(5, 16, 2, 0));
   g_ctx->ctx->quarantined = true;
   say("tables of a quarantined context", tables());
   g_ctx->ctx->quarantined = false;

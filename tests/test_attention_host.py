@@ -39,6 +39,17 @@ def test_a_quarantined_context_takes_no_calls(results):
     assert results["tables of a quarantined context"] == "resources_closed"
 
 
+def test_results_that_share_elements_are_refused(results):
+    """A result in which several rows or heads lie at one place would be written by
+    several threads; any other strides are taken."""
+    assert results["results of any strides that are judged otherwise than by brute force"] == "0"
+    for what in ("append", "append, head-major", "append, pages inside slots", "attend"):
+        assert results[what] == "ok", what
+    for what in ("append, one page twice", "append, slots that share elements", "append, heads that share elements",
+                 "attend, one row for all", "attend, one head for all"):
+        assert results[what] == "invalid_argument", what
+
+
 def test_workspace_sizes_while_others_clear_them(monkeypatch):
     """Every size of the backward's workspace is found, also where it is cleared
     between a thread's look and its answer."""

@@ -197,3 +197,22 @@ def test_gradients_without_those_of_frozen_weights(ctx, wanted):
     assert torch.equal(every[0], some[0]) and torch.equal(every[1], some[1])
     for i in range(2):
         assert torch.equal(every[2 + i], some[2 + i]) if wanted[i] else some[2 + i] is None
+
+
+def test_expanded_results_are_refused(ctx):
+    say("expanded results")
+    s = on_gpu(C.attention_case(1, [20], [3], 4, 2, 64, F16, F16, 16))
+    flat = torch.zeros((1, 4, 64), dtype=F16, device=DEV)
+    with pytest.raises(P.TransferError, match="invalid_argument.*overlap"):
+        A.tree_attention(ctx, s["q"], s["cache_k"], s["cache_v"], s["table"], s["cached"], s["starts"], out=flat.expand(3, 4, 64))
+    turn = (torch.zeros(3, dtype=torch.int32, device=DEV), torch.ones((1, 32), device=DEV), torch.zeros((1, 32), device=DEV))
+    with pytest.raises(P.TransferError, match="invalid_argument.*overlap"):
+        A.norm_rotate(ctx, s["q"], s["q"], *turn, None, None, 1e-6, out=(torch.empty_like(s["q"]), flat.expand(3, 4, 64)))
+    k = s["q"][:, :2]
+    with pytest.raises(P.TransferError, match="invalid_argument.*overlap"):
+        A.norm_rotate_append(ctx, s["q"], k, k, torch.arange(3, device=DEV), s["cache_k"][:1].expand(2, 16, 2, 64),
+                             s["cache_v"][:2], *turn, None, None, 1e-6)
+    # reading an expanded cache is no matter
+    A.tree_attention(ctx, s["q"], s["cache_k"][:1].expand(4, 16, 2, 64), s["cache_v"][:1].expand(4, 16, 2, 64), s["table"],
+                     s["cached"], s["starts"])
+    torch.cuda.synchronize()
