@@ -434,19 +434,19 @@ template <bool ONCE> __device__ __forceinline__ void load_async(const char *base
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
                  :
                  : "s"(m0), "v"(at), "s"(from)
-                 : "memory");
+                 : "memory", "m0");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(m0), "v"(at), "s"(from)
-                 : "memory");
+                 : "memory", "m0");
 }
 // The same for four bytes a lane.
 __device__ __forceinline__ void load_async4(const void *base, uint32_t at, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                :
                : "s"(uniform(static_cast<int>(to))), "v"(at), "s"(uniform64(reinterpret_cast<int64_t>(base)))
-               : "memory");
+               : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
