@@ -473,9 +473,10 @@ template <int DP, bool RAW> struct Reads {
   }
 };
 
-// Waits for the workgroup's other waves, and for no memory.
+// Waits for the workgroup's other waves, and for the wave's own reads of shared
+// memory, whose place another wave's load may take next; for no other memory.
 __device__ __forceinline__ void meet() {
-  asm volatile("" : : : "memory");
+  shared_done();
   __builtin_amdgcn_s_barrier();
   asm volatile("" : : : "memory");
 }
@@ -1202,8 +1203,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
       if (!I8 && __builtin_expect(cut, 0) &&
           clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, x + kTile > it.cached, lane) && lane == 0)
         odd = 1;
-      if (!I8 && __builtin_expect(cut, 0))
-        shared_done();
     };
     const uint32_t at = place(tiles[0][0]);
     __syncthreads(); // the tiles are free, and everybody has looked at the last item's `odd`

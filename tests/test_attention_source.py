@@ -28,3 +28,15 @@ def test_what_assembly_writes_is_named():
     assert len(writes) >= 3
     for f, s in writes:
         assert '"m0"' in s.split(":")[-1], (f, s)
+
+
+def test_a_bare_barrier_waits_for_shared_memory():
+    """A wave that passes it may have its loads take the place of what another reads."""
+    found = 0
+    for path in sorted(glob.glob(os.path.join(CSRC, "k_attend*")) + glob.glob(os.path.join(CSRC, "k_rotate*"))):
+        text = open(path).read()
+        for m in re.finditer(r"__builtin_amdgcn_s_barrier\(\)", text):
+            found += 1
+            before = text[text.rindex("{", 0, m.start()):m.start()]
+            assert "shared_done();" in before or "lgkmcnt(0)" in before, path
+    assert found >= 1
