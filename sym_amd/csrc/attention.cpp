@@ -166,6 +166,11 @@ RotateArgs rotate_args(const relx_rotation &r, int &type) {
   return a;
 }
 
+// Blocks of heads are the launch's second dimension.
+void fits_launch(const RotateArgs &a) {
+  layout(a.chunks[0] + a.chunks[1] + a.chunks[2] <= 65535, "norm and rotation: more than 65535 blocks of heads");
+}
+
 Heads heads_of(const relx_heads *h, bool used, const char *what) {
   need(!used || (h && h->data), what);
   return used ? Heads{static_cast<char *>(h->data), h->row, h->head} : Heads{};
@@ -216,6 +221,8 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   layout(i8 || c.type == type, "attention: a cache of the queries' type or int8");
   need(fits32(p.rows) && fits32(p.requests) && fits32(p.columns) && fits32(p.words),
        "attention: a size is negative or beyond 2^31 - 1");
+  // the join has a block of 512 threads for each, and 2^32 threads a dimension
+  layout(p.requests < (int64_t{1} << 23) - 1, "attention: more than 2^23 - 2 requests");
   const int64_t kv = p.cache.kv_heads, dim = p.cache.dim;
   need(p.heads >= 1 && kv >= 1 && p.heads % kv == 0, "attention: query heads are a multiple of the key heads");
   layout(p.heads <= 65535, "attention: more than 65535 heads");
@@ -340,6 +347,7 @@ int relx_norm_rotate(relx_ctx *ctx, const relx_rotation *rot, const relx_heads *
     relx::need(rot != nullptr, "null arguments");
     int type;
     relx::RotateArgs a = relx::rotate_args(*rot, type);
+    relx::fits_launch(a);
     const bool uq = a.rows && a.heads[0], uk = a.rows && a.heads[1];
     a.x[0] = relx::heads_of(q, uq, "norm and rotation: null queries");
     a.x[1] = relx::heads_of(k, uk, "norm and rotation: null keys");
@@ -372,6 +380,7 @@ int relx_norm_rotate_backward(relx_ctx *ctx, const relx_rotation *rot, const rel
     relx::need(rot != nullptr, "null arguments");
     int type;
     relx::RotateArgs a = relx::rotate_args(*rot, type);
+    relx::fits_launch(a);
     const bool uq = a.rows && a.heads[0], uk = a.rows && a.heads[1];
     a.x[0] = relx::heads_of(q, uq, "norm and rotation: null queries");
     a.x[1] = relx::heads_of(k, uk, "norm and rotation: null keys");
@@ -427,6 +436,7 @@ int relx_norm_rotate_append(relx_ctx *ctx, const relx_rotation *rot, const relx_
     a.y[0] = relx::heads_of(q_out, uq, "append: null query result");
     relx::need(!uk || slots, "append: null slots");
     a.chunks[2] = a.chunks[1];
+    relx::fits_launch(a);
     a.slots = slots;
     a.page = relx::make_div(cache->page);
     a.pages_slots = cache->pages * cache->page;

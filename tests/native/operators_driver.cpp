@@ -123,6 +123,40 @@ std::string append(int64_t page, int64_t slot, int64_t head) {
   return relx_norm_rotate_append(g_ctx, &r, nullptr, &x, &x, nullptr, g_long, &c, 0, &err) == RELX_OK ? "ok" : err.code;
 }
 
+// heads of 512 of each kind
+std::string rotate_wide(int64_t heads, bool cache) {
+  relx_rotation r{};
+  r.positions = g_int;
+  r.rows = 1;
+  r.heads = r.kv_heads = heads;
+  r.dim = 512;
+  r.bits = 16;
+  relx_heads x{g_long, heads * 512, 512};
+  relx_cache c{g_long, heads * 512, heads * 512, 512, g_long, heads * 512, heads * 512, 512, nullptr, nullptr, 1, 1,
+               heads,  512,         0,           16};
+  relx_err err;
+  const int rc = cache ? relx_norm_rotate_append(g_ctx, &r, &x, &x, &x, &x, g_long, &c, 0, &err)
+                       : relx_norm_rotate(g_ctx, &r, &x, &x, &x, &x, 0, &err);
+  return rc == RELX_OK ? "ok" : err.code;
+}
+
+// one row of `requests` requests
+std::string attend_many(int64_t requests) {
+  relx_tree_attention_args a{};
+  a.q = a.out = {g_long, 8, 8};
+  a.cache = {g_long, 8, 8, 8, g_long, 8, 8, 8, nullptr, nullptr, 1, 1, 1, 8, 0, 16};
+  a.rows = a.heads = 1;
+  a.requests = requests;
+  a.cached = a.starts = g_int;
+  alignas(16) static char room[16];
+  a.workspace = room;
+  a.workspace_bytes = INT64_MAX;
+  a.bits = 16;
+  a.scale = 1.0;
+  relx_err err;
+  return relx_tree_attention(g_ctx, &a, 0, &err) == RELX_OK ? "ok" : err.code;
+}
+
 std::string attend(int64_t rows, int64_t row, int64_t heads, int64_t head) {
   relx_tree_attention_args a{};
   a.q = {g_long, heads * 8, 8};
@@ -158,6 +192,12 @@ int main() {
   say("attend", attend(5, 16, 2, 8));
   say("attend, one row for all", attend(5, 0, 2, 8));
   say("attend, one head for all", attend(5, 16, 2, 0));
+  say("65534 blocks of heads", rotate_wide(65534, false));
+  say("65536 blocks of heads", rotate_wide(65535, false));
+  say("65535 blocks of heads and values", rotate_wide(43690, true));
+  say("65538 blocks of heads and values", rotate_wide(43691, true));
+  say("2^23 - 2 requests", attend_many((int64_t{1} << 23) - 2));
+  say("2^23 - 1 requests", attend_many((int64_t{1} << 23) - 1));
   g_ctx->ctx->quarantined = true;
   say("tables of a quarantined context", tables());
   g_ctx->ctx->quarantined = false;

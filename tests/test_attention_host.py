@@ -50,6 +50,14 @@ def test_results_that_share_elements_are_refused(results):
         assert results[what] == "invalid_argument", what
 
 
+def test_sizes_that_no_launch_holds_are_refused(results):
+    """Rather than launched, which fails and leaves its error to the next call."""
+    for what in ("65534 blocks of heads", "65535 blocks of heads and values", "2^23 - 2 requests"):
+        assert results[what] == "ok", what
+    for what in ("65536 blocks of heads", "65538 blocks of heads and values", "2^23 - 1 requests"):
+        assert results[what] == "unsupported_layout", what
+
+
 def test_workspace_sizes_while_others_clear_them(monkeypatch):
     """Every size of the backward's workspace is found, also where it is cleared
     between a thread's look and its answer."""
