@@ -313,8 +313,13 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
   return p;
 }
 
+size_t attend_part_rows(const AttendPlan &p) {
+  // 256 rows always run half of the workgroups; 16 may, by the cache's addresses
+  return static_cast<size_t>(p.rows == 256 ? kMostWorkgroups / 2 : kMostWorkgroups) * 2 * static_cast<size_t>(p.rows);
+}
+
 size_t attend_workspace(const AttendPlan &p, int64_t requests) {
-  const size_t rows = static_cast<size_t>(kMostWorkgroups) * 2 * static_cast<size_t>(p.rows);
+  const size_t rows = attend_part_rows(p);
   return rows * static_cast<size_t>(p.width + 2) * sizeof(float) +
          (static_cast<size_t>(requests) + 1) * sizeof(int64_t);
 }
@@ -488,7 +493,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
       if (args->workspace_bytes < 0 || static_cast<size_t>(args->workspace_bytes) < want || !args->workspace)
         throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(args->workspace_bytes) +
                                                        " bytes, the call takes " + std::to_string(want));
-      const size_t rows = static_cast<size_t>(relx::kMostWorkgroups) * 2 * static_cast<size_t>(plan.rows);
+      const size_t rows = relx::attend_part_rows(plan);
       relx::need(reinterpret_cast<uintptr_t>(args->workspace) % 16 == 0, "attention: workspace alignment");
       a.partial = static_cast<float *>(args->workspace);
       a.stats = a.partial + rows * static_cast<size_t>(plan.width);

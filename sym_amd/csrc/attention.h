@@ -117,7 +117,9 @@ constexpr int turn_workgroups(int width, bool i8, bool async) {
 }
 AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
                        int64_t page);
-// Bytes of a call's workspace, whatever its cache's addresses.
+// Rows of partial sums that a call's workspace holds, and its bytes, whatever its
+// cache's addresses.
+size_t attend_part_rows(const AttendPlan &p);
 size_t attend_workspace(const AttendPlan &p, int64_t requests);
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8,
                          hipStream_t s);

@@ -94,3 +94,16 @@ def test_workspace_sizes_while_others_clear_them(monkeypatch):
     rot = A._ROTATION.pack(N.ctypes.addressof(positions), 0, 0, 0, 0, 0, 32, 4, 6, 2, 64, 0, 0, 0, 0, 16, 1e-6)
     sizes = [A._rotate_room(rot, torch.Size((4, 6, 64)), torch.Size((4, 2, 64)), torch.float16) for _ in range(3)]
     assert sizes[0] > 0 and len(set(sizes)) == 1
+
+
+def test_a_workspace_holds_what_the_workgroups_leave():
+    """Two parts a workgroup of an item's rows, each a sum of the head's width, a
+    maximum and a sum of weights, and the schedule: 256 workgroups at 256 rows, 512
+    below."""
+    pytest.importorskip("torch")
+    from sym_amd import attention as A
+    for rows, item, groups in ((1, 16, 512), (16, 64, 512), (32, 128, 512), (64, 256, 256), (500, 256, 256)):
+        for dim, width in ((64, 64), (72, 128), (128, 128)):
+            want = groups * 2 * item * (width + 2) * 4 + 8 * 3
+            assert A.tree_attention_workspace(2 * rows, 2, 32, 8, dim, 16) == want, (rows, dim)
+    assert A.tree_attention_workspace(1000, 2, 32, 8, 256, 16) == 512 * 2 * 64 * 258 * 4 + 8 * 3

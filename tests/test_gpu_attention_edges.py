@@ -216,3 +216,26 @@ def test_expanded_results_are_refused(ctx):
     A.tree_attention(ctx, s["q"], s["cache_k"][:1].expand(4, 16, 2, 64), s["cache_v"][:1].expand(4, 16, 2, 64), s["table"],
                      s["cached"], s["starts"])
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fresh,dim,cache", [(1, 128, F16), (3, 256, I8), (12, 128, F16), (12, 136, I8), (30, 64, F16), (64, 128, F16),
+                                             (64, 64, I8), (100, 128, I8)])
+def test_nothing_is_written_past_the_workspace(ctx, fresh, dim, cache):
+    """Contexts so long that every workgroup leaves partial sums."""
+    say("workspace", fresh, dim, cache)
+    cached, page, heads, kv = 70_000, 64, 8, 2
+    gen = torch.Generator().manual_seed(dim + fresh)
+    made = [torch.randint(-9, 10, (40, page, kv, dim), generator=gen, dtype=I8).to(cache).to(DEV) for _ in range(2)]
+    scale = torch.full((kv,), 0.1, device=DEV) if cache == I8 else None
+    i32 = dict(dtype=torch.int32, device=DEV)
+    table = torch.randint(0, 40, (1, -(-(cached + fresh) // page)), generator=gen).to(**i32)
+    args = (torch.randn((fresh, heads, dim), generator=gen).to(F16).to(DEV), *made, table, torch.tensor([cached], **i32),
+            torch.tensor([0, fresh], **i32))
+    size = A.tree_attention_workspace(fresh, 1, heads, kv, dim, page)
+    room = torch.full((size + (1 << 20),), 0xa5, dtype=torch.uint8, device=DEV)
+    out = A.tree_attention(ctx, *args, k_scale=scale, v_scale=scale, workspace=room[:size])
+    want = A.tree_attention(ctx, *args, k_scale=scale, v_scale=scale)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and (room[size:] == 0xa5).all() and not (room[:size] == 0xa5).all()
+    with pytest.raises(P.TransferError, match="insufficient_capacity"):
+        A.tree_attention(ctx, *args, k_scale=scale, v_scale=scale, workspace=room[:size - 1])
