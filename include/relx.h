@@ -705,6 +705,9 @@ typedef struct relx_tree_attention_args {
 } relx_tree_attention_args;
 int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uint64_t stream,
                         relx_err *err);
+/* The workspace's bytes go by rows / requests: fewer rows of fewer requests may
+ * take more. The bytes of the same rows in one request, and eight a request, are
+ * enough for any step of at most so many of both. */
 int relx_tree_attention_workspace(const relx_tree_attention_args *args, size_t *bytes,
                                   relx_err *err);
 

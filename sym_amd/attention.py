@@ -393,7 +393,9 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
 @lru_cache(maxsize=4096)
 def tree_attention_workspace(rows, requests, heads, kv_heads, dim, page):
     """Bytes of device memory that a `tree_attention` call of these sizes
-    works in."""
+    works in. They go by rows / requests, so fewer rows may take more: the bytes
+    of all rows in one request, and eight a request, are enough for every call of
+    at most so many rows and requests."""
     size, err = ctypes.c_size_t(), N.relx_err()
     args = N.relx_tree_attention_args()
     args.rows, args.requests, args.heads = rows, requests, heads
