@@ -270,31 +270,30 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   a.columns = static_cast<int32_t>(p.columns);
   a.words = static_cast<int32_t>(p.words);
   a.scale = scale;
-  plan = attend_plan(p.rows, p.requests, kv, p.heads / kv, dim, p.cache.page);
+  plan = attend_plan(p.rows, p.requests, p.heads / kv, dim, p.cache.page);
   // a lane's distance inside a tile of 16 tokens is held in 32 bits
   if (a.key_slot > INT32_MAX / 32 || a.value_slot > INT32_MAX / 32)
     plan.even = false;
   const int64_t at = reinterpret_cast<int64_t>(a.keys) | reinterpret_cast<int64_t>(a.values) | a.key_page | a.key_slot |
                      a.key_head | a.value_page | a.value_slot | a.value_head;
   // Tiles that go to shared memory by themselves against tiles through registers:
-  // 8 requests of 256 rows over up to 32768 tokens 314 us against 366, one of 52
-  // rows over 131072 97 against 166, 64 int8 requests of one 250 against 434.
+  // 8 requests of 256 rows over up to 32768 tokens 276 us against 357, one of 52
+  // rows over 131072 106 against 172, 64 int8 requests of one 259 against 431.
   plan.async = plan.even && (at | dim * (i8 ? 1 : 2)) % 16 == 0;
   if (plan.rows == 16)
     plan.workgroups = turn_workgroups(plan.width, i8, plan.async);
   a.workgroups = plan.workgroups;
-  // Then keys and values go past the caches: 52 rows over 131072 tokens 97 us
-  // against 108, 128 rows of 8 requests over up to 32768 170 against 198, 64 int8
-  // requests of one row, whose kernel always does, 247 against 278. Where other
-  // tiles read them too: 528 against 480 (512 tokens of 8 requests, up to 8192).
+  // Then keys and values go past the caches: 52 rows over 131072 tokens 106 us
+  // against 120, 128 rows of 8 requests over up to 32768 182 to 189 against 209, 64
+  // int8 requests of one row, whose kernel always does, 247 against 278. Where other
+  // tiles read them too: 461 against 434 (512 tokens of 8 requests, up to 8192).
   a.once = p.requests > 0 && (p.rows + p.requests - 1) / p.requests * (p.heads / kv) <= plan.rows;
   return a;
 }
 
 } // namespace
 
-AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
-                       int64_t page) {
+AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t group, int64_t dim, int64_t page) {
   AttendPlan p{};
   p.width = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
   p.even = page % 16 == 0;
@@ -302,14 +301,13 @@ AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t
   // tile less often and leave fewer waves to read ahead; a row that is not there
   // costs what one that is does. 8 requests of up to 32768 tokens, 8 key heads
   // of 128, bf16, us by rows of an item:
-  //   256 rows each   64: 586   128: 349   256: 314
-  //   128 rows        64: 333   128: 170   256: 193
-  //   64 rows         16: 445   64: 159
-  //   16 rows         16: 166   64: 171; 64 int8 requests of one row: 16: 250, 64: 434
+  //   256 rows each   64: 598   128: 367   256: 270
+  //   128 rows        64: 340   128: 173   256: 195
+  //   64 rows         16: 440   64: 169   128: 174
+  //   16 rows         16: 171   64: 176; 64 int8 requests of one row: 16: 254, 64: 423
   const int64_t q = requests > 0 ? (rows + requests - 1) / requests * group : 0;
   p.rows = q <= 16 ? 16 : q <= 64 || p.width == 256 ? 64 : q <= 128 ? 128 : 256;
   p.workgroups = p.rows == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;
-  (void)kv_heads;
   return p;
 }
 
@@ -474,8 +472,8 @@ int relx_tree_attention_workspace(const relx_tree_attention_args *args, size_t *
     relx::need(relx::fits32(p.rows) && relx::fits32(p.requests) && p.heads >= 1 && p.cache.kv_heads >= 1 &&
                    p.cache.page >= 1,
                "attention: sizes");
-    *bytes = relx::attend_workspace(relx::attend_plan(p.rows, p.requests, p.cache.kv_heads,
-                                                      p.heads / p.cache.kv_heads, p.cache.dim, p.cache.page),
+    *bytes = relx::attend_workspace(relx::attend_plan(p.rows, p.requests, p.heads / p.cache.kv_heads, p.cache.dim,
+                                                      p.cache.page),
                                     p.requests);
   });
 }

@@ -107,16 +107,15 @@ constexpr int kMostWorkgroups = 512; // two to a compute unit
 // Waves that take turns, and workgroups of them that the card holds at once: a
 // ring of two tiles a wave, in 64 KiB (int8 heads of 128, say) or 128 KiB of a
 // compute unit's 160. Where two fit, two: 64 requests of 512 int8 tokens at most
-// with 32 key heads take 53 us with 512 workgroups, 74 with 256; up to 4096 tokens
-// 250 and 290. Rings of four tiles in 256 workgroups were slower still.
+// with 32 key heads take 58 us with 512 workgroups, 78 with 256; up to 4096 tokens
+// 248 to 258 and 246.
 constexpr int turn_waves(int width) { return width == 256 ? 2 : 4; }
 constexpr int turn_workgroups(int width, bool i8, bool async) {
   const int ring = 2 * 2 * 32 * width * (i8 ? 1 : 2) * turn_waves(width);
   return async ? (ring > 64 * 1024 ? kMostWorkgroups / 2 : kMostWorkgroups)
                : width == 256 ? kMostWorkgroups / 2 : kMostWorkgroups;
 }
-AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t kv_heads, int64_t group, int64_t dim,
-                       int64_t page);
+AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t group, int64_t dim, int64_t page);
 // Rows of partial sums that a call's workspace holds, and its bytes, whatever its
 // cache's addresses.
 size_t attend_part_rows(const AttendPlan &p);

@@ -1,5 +1,6 @@
 // k_attend.h - attention of a step's query rows over a paged cache (device
-// templates; instantiated in k_attend_f16.hip and k_attend_bf16.hip).
+// templates; instantiated in k_attend_f16.hip, k_attend_bf16.hip and, over int8
+// caches, k_attend_f16_i8.hip and k_attend_bf16_i8.hip).
 //
 // One pass over the keys and values with the running maximum and sum of the
 // softmax. The query rows of a request that share a key head (its new tokens
@@ -37,13 +38,15 @@
 // lengths cost nothing.
 //
 // Measured, with the join (8 key heads of 128 each, unless said):
-//   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 250 to 265
-//     us, 5.9 to 6.3 TB/s of cache. Bound by the reads.
-//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 103 us, 5.2 TB/s. Bound
-//     by the reads, but for the join's 6.
-//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 77 us, 456 TFLOP/s; up to
-//     32768: 323 us, 560 TFLOP/s. Bound by the waves' own instructions: an
-//     earlier form of 90 us took 57 for the reads alone, 70 without the softmax.
+//   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 246 to 250
+//     us, 6.3 TB/s of cache. Bound by the reads.
+//   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 100 to 101 us, 5.3 TB/s.
+//     Bound by the reads, but for the join's 6.
+//   8 requests of 64 rows x 4 heads, up to 8192 tokens: 77 to 78 us, 455 TFLOP/s; up
+//     to 32768: 274 to 315 us by the card's clock, 575 to 660 TFLOP/s. No unit is busy most of the time: the matrix
+//     units for 0.27 of it, shared memory 0.21 (a third of that in bank conflicts),
+//     the vector units a quarter by their count of instructions. The waves' steps
+//     wait for one another (products, softmax, products) more than they overlap.
 #pragma once
 
 #include <algorithm>
@@ -1177,8 +1180,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
   // A tile's values are read ahead of the softmax, where the registers hold them:
   // 77 us against 81 for 8 requests of 256 rows over up to 8192 tokens of 8 key
-  // heads of 128, 314 against 341 up to 32768. The same for the next tile's keys
-  // was slower (81).
+  // heads of 128, 280 against 287 up to 32768 (the fastest of 40). The same for the
+  // next tile's keys was slower (81).
   constexpr bool EARLY = DP <= 128 && (I8 || SRC == kAsync);
   Rows<T, DP, RT, false, EARLY> r;
   if (tid < 2)
@@ -1501,8 +1504,8 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
   if (e != hipSuccess)
     return e;
   // A wave for every piece of an even batch, within 2^16 blocks a request; eight
-  // where an item lies in more than eight runs, on average: 8.1 us against 11.8
-  // for 64 parts of 64 rows (14 MB), but 27 against 8.8 for five of 256 (31 MB).
+  // where an item lies in more than eight runs, on average: 6.7 us against 10.0
+  // for 64 parts of 64 rows (14 MB), but 28 against 8.9 for five of 256 (31 MB).
   const int64_t requests = std::max(a.requests, 1);
   const int64_t rows = (a.rows + requests - 1) / requests * a.group.d;
   const int64_t n = ROWS > 16 ? 16 : 256 / DP;

@@ -17,10 +17,10 @@
 // Bound by bytes: everything is read once and written once, past the caches.
 // What decides is how much is on its way, so a wave loads its next row before
 // it works on this one. 32768 rows of 32 + 8 heads of 128 in bf16, from views
-// of a fused projection: forward 119 to 125 us (5.4 to 5.7 TB/s; 177 without the next
-// row ahead, 155 with stores through the caches), backward with the weights'
-// gradients 182 to 186 us (5.5 TB/s; 310 before). 8192 rows into a cache 76 us
-// (5.3 TB/s; 113 before). The sums of the weights' gradients are added block
+// of a fused projection: forward 125 us (5.4 TB/s; 119 now and then; 177 without
+// the next row ahead, 155 with stores through the caches), backward with the
+// weights' gradients 185 to 188 us (5.4 TB/s; 310 before). 8192 rows into a cache
+// 78 us (5.2 TB/s; 113 before). The sums of the weights' gradients are added block
 // by block in a fixed order by a second launch (4 us): no atomics.
 #include "attention.h"
 #include "index.h"
