@@ -711,6 +711,53 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
 int relx_tree_attention_workspace(const relx_tree_attention_args *args, size_t *bytes,
                                   relx_err *err);
 
+/* The scales of an int8 cache whose blocks of `block` tokens have one each for
+ * every head: [pages, page / block, kv_heads] of any strides, the same for keys
+ * and values. A block is a multiple of 16 tokens and divides the page. */
+typedef struct relx_block_scales {
+  float *key_scale, *value_scale;
+  int64_t page, block_stride, head; /* strides */
+  int64_t block;
+} relx_block_scales;
+
+/* What attention sees of a cache. A row at position p (cached + j, or cached +
+ * its depth in the tree that its mask says) sees the cached tokens x with
+ * x < sinks or p - x < window, and of the request's own those that it would see
+ * without a window, with the same rule where there is no mask. window 0: of
+ * everything. With a mask the window holds the tree: at least 64 words.
+ * `scales`: of an int8 cache, instead of the cache's scales a head, which are
+ * then not read (block 0: none). Any other argument and the workspace are
+ * relx_tree_attention's. */
+typedef struct relx_cache_view {
+  int64_t window, sinks;
+  relx_block_scales scales;
+} relx_cache_view;
+int relx_tree_attention_view(relx_ctx *ctx, const relx_tree_attention_args *args,
+                             const relx_cache_view *view, uint64_t stream, relx_err *err);
+
+/* Quantizes a step's keys and values into an int8 cache with a scale a block.
+ * Request b's rows [starts[b], starts[b + 1]) go to the places cached[b], ... of
+ * its table row. A block's scale becomes the largest of its new tokens' largest
+ * finite magnitude / 127, 2^-126, and, where it holds tokens of the request
+ * already, its scale so far; if it grows, those are rounded anew to q * old /
+ * new. Codes are round(x * (1 / scale)) to even, clamped as the plans' quantize
+ * stage clamps (NaN: -128). Rows whose page is not in the cache or not in the
+ * table are skipped; no two requests share a block that both write to. k and v
+ * are f32, f16 or bf16 [rows, kv_heads, dim]; the cache's scales a head are not
+ * read. */
+typedef struct relx_block_append_args {
+  relx_heads k, v;
+  relx_cache cache;
+  relx_block_scales scales;
+  const int32_t *table; /* [requests, columns] */
+  int64_t table_row;
+  const int32_t *cached; /* [requests] */
+  const int32_t *starts; /* [requests + 1] */
+  int64_t rows, requests, columns, kind, bits;
+} relx_block_append_args;
+int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_t stream,
+                      relx_err *err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -130,6 +130,12 @@ relx_tree_attention_args = _record(
     "relx_tree_attention_args", relx_heads, "q out", relx_cache, "cache", _P8, "table",
     _I8, "table_row", _P8, "cached starts mask lse workspace",
     _I8, "workspace_bytes rows requests heads columns words kind bits", _D8, "scale")
+relx_block_scales = _record(
+    "relx_block_scales", _P8, "key_scale value_scale", _I8, "page block_stride head block")
+relx_cache_view = _record("relx_cache_view", _I8, "window sinks", relx_block_scales, "scales")
+relx_block_append_args = _record(
+    "relx_block_append_args", relx_heads, "k v", relx_cache, "cache", relx_block_scales, "scales",
+    _P8, "table", _I8, "table_row", _P8, "cached starts", _I8, "rows requests columns kind bits")
 
 # every entry point include/relx.h declares, with its ctypes signature
 _VP, _SZ, _I, _I64, _U64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64
@@ -201,6 +207,8 @@ SIGNATURES = {
     "relx_norm_rotate_append": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _U64, _E]),
     "relx_tree_attention": (_I, [_VP, _VP, _U64, _E]),
     "relx_tree_attention_workspace": (_I, [_VP, ctypes.POINTER(_SZ), _E]),
+    "relx_tree_attention_view": (_I, [_VP, _VP, _VP, _U64, _E]),
+    "relx_block_append": (_I, [_VP, _VP, _U64, _E]),
     "relx_ctx_synchronize": (_I, [_VP, _E]),
     "relx_ctx_time_kernels": (_I, [_VP, _I, _E]),
     "relx_ctx_kernel_times": (_I, [_VP, ctypes.POINTER(relx_kernel_times), _E]),

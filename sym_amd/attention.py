@@ -54,6 +54,9 @@ _CACHE = struct.Struct(_format(N.relx_cache))
 _TABLES = struct.Struct(_format(N.relx_block_tables_args))
 _ROTATION = struct.Struct(_format(N.relx_rotation))
 _ATTENTION = struct.Struct(_format(N.relx_tree_attention_args)[6:])  # after its two relx_heads
+_SCALES = struct.Struct(_format(N.relx_block_scales))
+_VIEW = struct.Struct(_format(N.relx_cache_view)[:2])  # before its scales
+_APPEND = struct.Struct(_format(N.relx_block_append_args)[6 + 16 + 6:])  # after its heads, cache and scales
 
 
 def _bad(message):
@@ -124,8 +127,24 @@ def _table(t, device):
     return requests, columns, t.data_ptr(), t.stride(0)
 
 
-def _cache(keys, values, k_scale, v_scale, device):
-    """The cache's record fields: keys and values [pages, page, kv_heads, dim]."""
+def _block_scales(k_scale, v_scale, shape, device):
+    """The record of an int8 cache's scales [pages, page / block, kv_heads]."""
+    kss = k_scale.shape
+    if v_scale is None or v_scale.shape != kss or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or \
+            k_scale.get_device() != device or v_scale.get_device() != device or len(shape) != 4 or len(kss) != 3 or \
+            kss[0] != shape[0] or kss[2] != shape[2] or kss[1] < 1 or shape[1] % kss[1] or k_scale.stride() != v_scale.stride():
+        _bad("scales of blocks: float32 [pages, page / block, kv_heads] on device %d, alike in both; got %s %s and %s for a cache %s"
+             % (device, k_scale.dtype, list(kss), "none" if v_scale is None else "%s %s" % (v_scale.dtype, list(v_scale.shape)),
+                list(shape)))
+    return _SCALES.pack(k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), shape[1] // kss[1])
+
+
+_NO_SCALES = _SCALES.pack(*(0,) * 6)
+
+
+def _cache(keys, values, k_scale, v_scale, device, blocks=False):
+    """The cache's record fields: keys and values [pages, page, kv_heads, dim].
+    `blocks`: its scales are of blocks, in a record of their own."""
     shape, dtype = keys.shape, keys.dtype
     kind = _KINDS.get(dtype)
     if len(shape) != 4 or values.shape != shape or values.dtype is not dtype or kind is None or \
@@ -137,7 +156,11 @@ def _cache(keys, values, k_scale, v_scale, device):
     if (ko != 1 or vo != 1) and shape[3] > 1 and keys.numel():
         _bad("cache: the last dimension must be contiguous")
     k_ptr = v_ptr = 0
-    if dtype is torch.int8:
+    if blocks:
+        if dtype is not torch.int8:
+            _bad("scales go with an int8 cache")
+        k_ptr, v_ptr = k_scale.data_ptr(), v_scale.data_ptr()
+    elif dtype is torch.int8:
         if k_scale is None or v_scale is None:
             _bad("an int8 cache takes k_scale and v_scale")
         k_ptr = _row(k_scale, "k_scale", torch.float32, shape[2], device)
@@ -388,6 +411,39 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     return out
 
 
+# ------------------------------------------------------------ blocks of a cache
+
+def block_append(ctx, k, v, cache_k, cache_v, k_scale, v_scale, table, cached, starts):
+    """Quantizes a step's keys and values [rows, kv_heads, dim] (f32, f16 or bf16,
+    any row and head strides) into an int8 cache [pages, page, kv_heads, dim] whose
+    blocks of tokens have a scale each for every head: `k_scale` and `v_scale`,
+    float32 [pages, page / block, kv_heads] of any strides, the same in both, with
+    blocks of a multiple of 16 tokens.
+
+    Request b's rows [starts[b], starts[b + 1]) become the tokens cached[b], ... of
+    its row of `table` (int32 [requests, columns]). A block's scale is the largest
+    finite magnitude of its tokens / 127: where it grows, the codes of the tokens
+    that the request already has in the block are rounded anew. Infinities become
+    the largest codes, NaN -128, as in the package's plans. Tokens whose page is
+    not in the cache are left out; a block is of one request that writes to it.
+    Caches and scales are updated in place; there is no gradient."""
+    device = _device(ctx, k)
+    shape, dtype = k.shape, k.dtype
+    kind = _KINDS.get(dtype)
+    if len(shape) != 3 or kind is None or kind[1] == 8 or cache_k.dim() != 4 or cache_k.dtype is not torch.int8 or \
+            cache_k.shape[2:] != shape[1:]:
+        _bad("keys: a floating type [rows, kv_heads, dim], into an int8 cache of the same heads; got %s %s and %s %s"
+             % (dtype, list(shape), cache_k.dtype, list(cache_k.shape)))
+    scales = _block_scales(k_scale, v_scale, cache_k.shape, device)
+    requests, columns, t_ptr, t_row = _table(table, device)
+    _call("relx_block_append", ctx,
+          _heads(k, "keys", shape, dtype, device) + _heads(v, "values", shape, dtype, device) +
+          _CACHE.pack(*_cache(cache_k, cache_v, k_scale, v_scale, device, True)) + scales +
+          _APPEND.pack(t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
+                       _row(starts, "starts", torch.int32, requests + 1, device), shape[0], requests, columns, *kind),
+          _stream(device))
+
+
 # ------------------------------------------------------------ attention
 
 @lru_cache(maxsize=4096)
@@ -406,7 +462,7 @@ def tree_attention_workspace(rows, requests, heads, kv_heads, dim, page):
 
 
 def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None, scale=None, k_scale=None,
-                   v_scale=None, out=None, lse=None, workspace=None):
+                   v_scale=None, window=None, sinks=0, out=None, lse=None, workspace=None):
     """Attention of a step's rows q [rows, heads, dim] (f16, bf16) over a paged
     cache [pages, page, kv_heads, dim] of any strides, of the same type or
     int8 with scales [kv_heads].
@@ -418,6 +474,13 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     itself (one row a request: plain decoding). Head h reads key head
     h // (heads // kv_heads). A row that sees nothing, or of no request, is 0.
 
+    `window`: a row at position p sees of the tokens x only those with
+    p - x < window, and the first `sinks` ones; p is cached + j, or with a mask
+    cached + the token's depth in its tree, of which it sees what its mask says
+    (the window has to hold the tree: 64 * words at least). An int8 cache
+    with a scale a block of tokens, as `block_append` fills it, has scales
+    [pages, page / block, kv_heads] (float32, any strides, the same in both).
+
     `scale`: of the scores, by default dim ** -0.5. `lse`: float32 [rows,
     heads] for the logarithm of each row's sum of exponentials. `workspace`: a
     uint8 tensor of `tree_attention_workspace` bytes, for programs that keep
@@ -427,14 +490,17 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
         return _NoGradient.apply(
             "tree_attention",
             partial(tree_attention, ctx, q, cache_k, cache_v, table, cached, starts, mask=mask, scale=scale, k_scale=k_scale,
-                    v_scale=v_scale, lse=lse, workspace=workspace), q, cache_k, cache_v, k_scale, v_scale)
+                    v_scale=v_scale, window=window, sinks=sinks, lse=lse, workspace=workspace), q, cache_k, cache_v, k_scale,
+            v_scale)
     device = _device(ctx, q)
     shape, dtype = q.shape, q.dtype
     kind = _KINDS.get(dtype)
     if len(shape) != 3 or kind is None or kind[1] != 16:
         _bad("queries: f16 or bf16 [rows, heads, dim]; got %s %s" % (dtype, list(shape)))
     rows, heads, dim = shape
-    cache = _cache(cache_k, cache_v, k_scale, v_scale, device)
+    blocks = k_scale is not None and k_scale.dim() == 3
+    scales = _block_scales(k_scale, v_scale, cache_k.shape, device) if blocks else _NO_SCALES
+    cache = _cache(cache_k, cache_v, k_scale, v_scale, device, blocks)
     kv_heads = cache[12]
     if cache[13] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads or \
             (cache_k.dtype is not dtype and cache_k.dtype is not torch.int8):
@@ -462,10 +528,22 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
                                 dtype=torch.uint8)
     elif workspace.dtype is not torch.uint8 or workspace.get_device() != device or not workspace.is_contiguous():
         _bad("workspace: contiguous uint8 on device %d" % device)
-    _call("relx_tree_attention", ctx,
-          _heads(q, "queries", shape, dtype, device) + result +
-          _ATTENTION.pack(*cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
-                          _row(starts, "starts", torch.int32, requests + 1, device), m_ptr, l_ptr,
-                          workspace.data_ptr(), workspace.numel(), rows, requests, heads, columns, words, *kind,
-                          dim ** -0.5 if scale is None else float(scale)), _stream(device))
+    args = _heads(q, "queries", shape, dtype, device) + result + \
+        _ATTENTION.pack(*cache, t_ptr, t_row, _row(cached, "cached", torch.int32, requests, device),
+                        _row(starts, "starts", torch.int32, requests + 1, device), m_ptr, l_ptr,
+                        workspace.data_ptr(), workspace.numel(), rows, requests, heads, columns, words, *kind,
+                        dim ** -0.5 if scale is None else float(scale))
+    if window is None and not blocks:
+        if sinks:
+            _bad("first tokens that stay go with a window")
+        _call("relx_tree_attention", ctx, args, _stream(device))
+    else:
+        _call("relx_tree_attention_view", ctx, args, _view(window, sinks) + scales, _stream(device))
     return out
+
+
+def _view(window, sinks):
+    window, sinks = 0 if window is None else int(window), int(sinks)
+    if window < 0 or sinks < 0 or (window == 0 and sinks):
+        _bad("a window of %d tokens with %d first ones" % (window, sinks))
+    return _VIEW.pack(window, sinks)

@@ -4,85 +4,11 @@
 
 #include <climits>
 #include <cmath>
-#include <cstdlib>
-#include <utility>
 
-#include "capi.h"
-#include "runtime.h"
+#include "operators.h"
 
 namespace relx {
 namespace {
-
-void need(bool ok, const char *what) {
-  if (!ok)
-    throw Error("invalid_argument", what);
-}
-
-void layout(bool ok, const char *what) {
-  if (!ok)
-    throw Error("unsupported_layout", what);
-}
-
-int element_type(int64_t kind, int64_t bits) {
-  if (kind == 0 && bits == 32)
-    return kF32;
-  if (kind == 0 && bits == 16)
-    return kF16;
-  if (kind == 1 && bits == 16)
-    return kBF16;
-  if (kind == 2 && bits == 8)
-    return kI8;
-  throw Error("unsupported_layout", "element type (kind " + std::to_string(kind) + ", " +
-                                        std::to_string(bits) + " bits)");
-}
-
-bool fits32(int64_t v) { return v >= 0 && v <= INT32_MAX; }
-
-void launched(hipError_t e, const char *what) {
-  if (e != hipSuccess)
-    throw Error("backend_failure", std::string(what) + ": " + hipGetErrorString(e));
-}
-
-// Runs `fn` with the context's device current, if the context takes calls.
-// Not under its mutex, which transfers hold until the GPU has done them: these
-// calls use nothing that it guards.
-template <class F> void on_context(relx_ctx *ctx, F &&fn) {
-  need(ctx != nullptr, "null context");
-  if (ctx->ctx->closed || ctx->ctx->quarantined)
-    throw Error("resources_closed", "context is closed or quarantined");
-  DeviceScope scope(ctx->ctx->device);
-  fn();
-}
-
-hipStream_t stream_of(uint64_t s) { return reinterpret_cast<hipStream_t>(s); }
-
-// Whether elements of [n1, n2, dim] with these strides share a place.
-bool overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t dim) {
-  using Wide = __int128;
-  s1 = n1 > 1 ? std::abs(s1) : 0;
-  s2 = n2 > 1 ? std::abs(s2) : 0;
-  if (s1 > s2) {
-    std::swap(n1, n2);
-    std::swap(s1, s2);
-  }
-  if ((n1 > 1 && s1 < dim) || (n2 > 1 && s2 < dim))
-    return true;
-  if (n1 <= 1 || n2 <= 1)
-    return false;
-  // the larger steps that end inside the smaller ones' reach: hardly ever any
-  const Wide reach = static_cast<Wide>(n1 - 1) * s1;
-  for (int64_t i = 1; i < n2 && static_cast<Wide>(i) * s2 < reach + dim; ++i) {
-    const Wide at = static_cast<Wide>(i) * s2, below = at / s1; // the steps next to it
-    if ((below < n1 && at - below * s1 < dim) || (below + 1 < n1 && (below + 1) * s1 - at < dim))
-      return true;
-  }
-  return false;
-}
-
-// A result that several threads would write in one place is refused.
-void writable(const relx_heads *h, int64_t rows, int64_t heads, int64_t dim) {
-  need(!h || rows == 0 || heads == 0 || !overlap(rows, h->row, heads, h->head, dim), "a result's elements overlap");
-}
 
 // ------------------------------------------------------------ block tables
 
@@ -171,11 +97,6 @@ void fits_launch(const RotateArgs &a) {
   layout(a.chunks[0] + a.chunks[1] + a.chunks[2] <= 65535, "norm and rotation: more than 65535 blocks of heads");
 }
 
-Heads heads_of(const relx_heads *h, bool used, const char *what) {
-  need(!used || (h && h->data), what);
-  return used ? Heads{static_cast<char *>(h->data), h->row, h->head} : Heads{};
-}
-
 size_t rotate_partial(const RotateArgs &a) {
   const int64_t chunks = a.chunks[0] + a.chunks[1];
   if (a.rows == 0 || chunks == 0)
@@ -184,32 +105,7 @@ size_t rotate_partial(const RotateArgs &a) {
          sizeof(float);
 }
 
-// ------------------------------------------------------------ paged caches
-
-struct CacheBytes {
-  int64_t key_page, key_slot, key_head, value_page, value_slot, value_head;
-  int type;
-};
-
-CacheBytes cache_bytes(const relx_cache &c) {
-  CacheBytes b;
-  b.type = element_type(c.kind, c.bits);
-  need(c.pages >= 0 && fits32(c.pages) && c.page >= 1 && fits32(c.page) && c.kv_heads >= 0, "cache: sizes");
-  layout(c.page * c.pages <= INT32_MAX, "cache: more than 2^31 - 1 slots");
-  need(c.pages == 0 || c.kv_heads == 0 || (c.keys && c.values), "cache: null keys or values");
-  need(b.type != kI8 || c.kv_heads == 0 || (c.key_scale && c.value_scale), "cache: an int8 cache has a scale a head");
-  need(c.key_page >= 0 && c.key_slot >= 0 && c.key_head >= 0 && c.value_page >= 0 && c.value_slot >= 0 &&
-           c.value_head >= 0,
-       "cache: negative strides");
-  const int64_t w = b.type == kI8 ? 1 : b.type == kF32 ? 4 : 2;
-  b.key_page = c.key_page * w;
-  b.key_slot = c.key_slot * w;
-  b.key_head = c.key_head * w;
-  b.value_page = c.value_page * w;
-  b.value_slot = c.value_slot * w;
-  b.value_head = c.value_head * w;
-  return b;
-}
+} // namespace
 
 // ------------------------------------------------------------ attention
 
@@ -291,8 +187,6 @@ AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int 
   return a;
 }
 
-} // namespace
-
 AttendPlan attend_plan(int64_t rows, int64_t requests, int64_t group, int64_t dim, int64_t page) {
   AttendPlan p{};
   p.width = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
@@ -320,6 +214,20 @@ size_t attend_workspace(const AttendPlan &p, int64_t requests) {
   const size_t rows = attend_part_rows(p);
   return rows * static_cast<size_t>(p.width + 2) * sizeof(float) +
          (static_cast<size_t>(requests) + 1) * sizeof(int64_t);
+}
+
+void attend_room(AttendArgs &a, const AttendPlan &plan, const relx_tree_attention_args &p) {
+  if (a.rows <= 0 || a.requests <= 0)
+    return;
+  const size_t want = attend_workspace(plan, a.requests);
+  if (p.workspace_bytes < 0 || static_cast<size_t>(p.workspace_bytes) < want || !p.workspace)
+    throw Error("insufficient_capacity", "workspace holds " + std::to_string(p.workspace_bytes) +
+                                             " bytes, the call takes " + std::to_string(want));
+  const size_t rows = attend_part_rows(plan);
+  need(reinterpret_cast<uintptr_t>(p.workspace) % 16 == 0, "attention: workspace alignment");
+  a.partial = static_cast<float *>(p.workspace);
+  a.stats = a.partial + rows * static_cast<size_t>(plan.width);
+  a.schedule = reinterpret_cast<int64_t *>(a.stats + rows * 2);
 }
 
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8, hipStream_t s) {
@@ -486,17 +394,7 @@ int relx_tree_attention(relx_ctx *ctx, const relx_tree_attention_args *args, uin
     int type;
     bool i8;
     relx::AttendArgs a = relx::attend_args(*args, plan, type, i8);
-    if (a.rows > 0 && a.requests > 0) {
-      const size_t want = relx::attend_workspace(plan, a.requests);
-      if (args->workspace_bytes < 0 || static_cast<size_t>(args->workspace_bytes) < want || !args->workspace)
-        throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(args->workspace_bytes) +
-                                                       " bytes, the call takes " + std::to_string(want));
-      const size_t rows = relx::attend_part_rows(plan);
-      relx::need(reinterpret_cast<uintptr_t>(args->workspace) % 16 == 0, "attention: workspace alignment");
-      a.partial = static_cast<float *>(args->workspace);
-      a.stats = a.partial + rows * static_cast<size_t>(plan.width);
-      a.schedule = reinterpret_cast<int64_t *>(a.stats + rows * 2);
-    }
+    relx::attend_room(a, plan, *args);
     relx::on_context(ctx, [&] {
       if (a.rows > 0)
         relx::launched(relx::attend_launch(a, plan, type, i8, relx::stream_of(stream)), "attention");

@@ -7,6 +7,8 @@
 
 #include <cstdint>
 
+#include "../../include/relx.h"
+
 #include "program.h"
 
 namespace relx {
@@ -92,6 +94,11 @@ struct AttendArgs {
   int32_t workgroups;
   float scale; // of a score, times log2 e
   bool once;   // in an even batch, one tile of query rows reads a key head
+  // with a window (2^30: of everything) or a scale a block
+  int32_t window, sinks;
+  uint32_t scale_page, scale_block; // bytes
+  int64_t scale_head;
+  FastDiv block;
 };
 
 // How a call runs.
@@ -122,9 +129,33 @@ size_t attend_part_rows(const AttendPlan &p);
 size_t attend_workspace(const AttendPlan &p, int64_t requests);
 hipError_t attend_launch(const AttendArgs &a, const AttendPlan &p, int type, bool i8,
                          hipStream_t s);
+// The arguments of a call without a window, and how it runs; the workspace's place.
+AttendArgs attend_args(const relx_tree_attention_args &p, AttendPlan &plan, int &type, bool &i8);
+void attend_room(AttendArgs &a, const AttendPlan &plan, const relx_tree_attention_args &p);
 hipError_t attend_launch_f16(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
 hipError_t attend_launch_f16_i8(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
 hipError_t attend_launch_bf16(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
 hipError_t attend_launch_bf16_i8(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+// with a window; of int8 with a scale a block and a window
+hipError_t attend_launch_f16_window(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_f16_blocks(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_bf16_window(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+hipError_t attend_launch_bf16_blocks(const AttendArgs &a, const AttendPlan &p, hipStream_t s);
+
+// ------------------------------------------------------------ blocks of a cache
+
+struct BlockArgs {
+  Heads x[2];       // keys, values
+  char *cache[2];   // [pages, page, kv_heads, dim] int8
+  int64_t page_stride[2], slot_stride[2], head_stride[2]; // bytes
+  float *scale[2];
+  int64_t scale_page, scale_block, scale_head;
+  const int32_t *table;
+  int64_t table_row;
+  const int32_t *cached, *starts;
+  FastDiv page, block;
+  int32_t rows, requests, columns, pages, kv_heads, dim;
+};
+hipError_t blocks_launch(const BlockArgs &a, int type, hipStream_t s);
 
 } // namespace relx

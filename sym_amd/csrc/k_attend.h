@@ -75,6 +75,14 @@ constexpr int kSharedUnit = 64;
 constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
 
 enum Source : int { kAsync, kStaged, kStagedEven };
+// What a call's rows see, and how a cache's codes are scaled:
+//   kWhole    all of the context; int8 by a scale a head
+//   kWindow   the last `window` tokens and the first `sinks` ones; no int8
+//   kBlocks   the same of an int8 cache with a scale a block of tokens and head
+// With a window, an item's tiles of tokens are numbered without the ones that
+// none of its rows sees: up to `edge`, the end of the tiles with first tokens,
+// a place is the token's own, and from there on `jump` tokens before it.
+enum Form : int { kWhole, kWindow, kBlocks };
 // Where a row's reference maximum starts: finite, so that a difference with a
 // masked score's -inf stays -inf.
 constexpr float kNone = -3.402823466e38f;
@@ -94,6 +102,10 @@ template <class T> __device__ __forceinline__ void store(char *p, const T &v) {
 // do not queue behind the vector loads in flight.
 __device__ __forceinline__ int32_t scalar_load(const int32_t *p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uint64_t>(p));
+}
+
+__device__ __forceinline__ float scalar_load(const float *p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) float *>(reinterpret_cast<uint64_t>(p));
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -189,6 +201,12 @@ __device__ __forceinline__ int64_t divide(int64_t n, int d) {
 
 // ------------------------------------------------------------ the schedule
 
+// The end of the tiles with first tokens. Sizes are 2^30 at most, so that sums
+// of three stay within 32 bits.
+__device__ __forceinline__ int edge_of(const AttendArgs &a, int length) {
+  return (min(a.sinks, length) + kTile - 1) & ~(kTile - 1);
+}
+
 struct Request {
   int cached, length; // tokens in the cache before the step, and with it: at most 2^30
   int start, fresh;   // its rows
@@ -197,7 +215,7 @@ struct Request {
 };
 
 // ROWS: query rows of an item, UNIT: tokens of a unit.
-template <int ROWS, int UNIT>
+template <int FORM, int ROWS, int UNIT>
 __device__ __forceinline__ Request attend_request(const AttendArgs &a, int b) {
   Request r;
   const int s = min(max(a.starts[b], 0), a.rows), e = min(max(a.starts[b + 1], s), a.rows);
@@ -208,13 +226,22 @@ __device__ __forceinline__ Request attend_request(const AttendArgs &a, int b) {
   r.length = r.fresh < room - r.cached ? r.cached + r.fresh : room;
   const int64_t q = static_cast<int64_t>(r.fresh) * a.group.d;
   r.tiles = static_cast<int>((q + ROWS - 1) / ROWS);
-  r.units = max((r.length + UNIT - 1) / UNIT, 1);
+  int reach = r.length;
+  if constexpr (FORM != kWhole) {
+    // as many tokens as any of its items has: first ones, those that the windows
+    // of an item's rows span, and the rest of the tile in which the span begins
+    const uint32_t g = a.group.d;
+    const uint32_t span = a.mask ? r.fresh : min(static_cast<uint32_t>(r.fresh), (ROWS - 1) / g + 2);
+    const uint32_t most = static_cast<uint32_t>(edge_of(a, r.length)) + kTile - 1 + static_cast<uint32_t>(a.window) + span;
+    reach = static_cast<int>(min(static_cast<uint32_t>(reach), most));
+  }
+  r.units = max((reach + UNIT - 1) / UNIT, 1);
   return r;
 }
 
-template <int ROWS, int UNIT>
+template <int FORM, int ROWS, int UNIT>
 __device__ __forceinline__ int64_t request_units(const AttendArgs &a, int b) {
-  const Request r = attend_request<ROWS, UNIT>(a, b);
+  const Request r = attend_request<FORM, ROWS, UNIT>(a, b);
   return static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
 }
 
@@ -225,7 +252,7 @@ struct Schedule {
   int64_t waves[kScan / 64];
 };
 
-template <int ROWS, int UNIT>
+template <int FORM, int ROWS, int UNIT>
 __device__ __forceinline__ void add_up(const AttendArgs &a, Schedule &sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (a.requests + kScan - 1) / kScan;
@@ -234,7 +261,7 @@ __device__ __forceinline__ void add_up(const AttendArgs &a, Schedule &sh) {
   int64_t mine = 0, upto = 0;
   if (in) {
     for (int b = b0; b < b1; ++b)
-      mine += request_units<ROWS, UNIT>(a, b);
+      mine += request_units<FORM, ROWS, UNIT>(a, b);
     upto = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -257,7 +284,7 @@ __device__ __forceinline__ void add_up(const AttendArgs &a, Schedule &sh) {
       int64_t at = first;
       for (int b = b0; b < b1; ++b) {
         a.schedule[b] = at;
-        at += request_units<ROWS, UNIT>(a, b);
+        at += request_units<FORM, ROWS, UNIT>(a, b);
       }
       if (tid == kScan - 1)
         a.schedule[a.requests] = first + mine;
@@ -299,8 +326,39 @@ template <int DP, int ROWS> __device__ __forceinline__ int part_at(int i, int d)
 // The part of an item that lies in a run: the units [s0, s1) of its `units`.
 struct Item {
   int b, start, fresh, head, tile, cached, length, s0, s1, units;
+  int reach;      // places of tokens: of the request, or those that its rows may see
+  int edge, jump; // where places and tokens part, and by how much
+  int all_see;    // every row's window holds the tokens from here on
+  template <int FORM> __device__ __forceinline__ int token(int place) const {
+    return FORM == kWhole ? place : place < edge ? place : place + jump;
+  }
+  // Whether some rows' windows begin after the 32 tokens from x do.
+  template <int FORM> __device__ __forceinline__ bool windowed(int x, int sinks) const {
+    return FORM != kWhole && x < all_see && x + kTile > sinks;
+  }
 };
-template <int ROWS, int UNIT>
+// Where the window of the j-th new token, at the d-th place after the cached ones, begins.
+__device__ __forceinline__ int window_from(const AttendArgs &a, int cached, int d) {
+  const int64_t from = static_cast<int64_t>(cached) + d - a.window + 1;
+  return static_cast<int>(max(min(from, int64_t{1} << 30), int64_t{0}));
+}
+// The d of a row: the token's depth in its tree, or j.
+__device__ __forceinline__ int row_depth(const AttendArgs &a, int start, int j) {
+  if (!a.mask)
+    return j;
+  int n = 0;
+  for (int w = 0; w < a.words; ++w)
+    n += __builtin_popcountll(static_cast<uint64_t>(a.mask[(start + static_cast<int64_t>(j)) * a.words + w]));
+  return max(n - 1, 0);
+}
+// Of the 32 tokens from x: the first ones, and those from `from` on.
+__device__ __forceinline__ uint32_t window_sees(int x, int from, int sinks) {
+  const int first = sinks - x, before = from - x;
+  return (first >= 32 ? 0xffffffffu : first > 0 ? (1u << first) - 1u : 0u) |
+         (before >= 32 ? 0u : before > 0 ? 0xffffffffu << before : 0xffffffffu);
+}
+
+template <int FORM, int ROWS, int UNIT>
 __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Run &run) {
   int lo = 0, hi = kScan;
   while (hi - lo > 1) {
@@ -312,13 +370,13 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   }
   int b = lo * ((a.requests + kScan - 1) / kScan);
   int64_t at = uniform64(sh.before[lo]);
-  Request r = attend_request<ROWS, UNIT>(a, b);
+  Request r = attend_request<FORM, ROWS, UNIT>(a, b);
   for (;;) {
     const int64_t n = static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
     if (run.unit < at + n)
       break;
     at += n;
-    r = attend_request<ROWS, UNIT>(a, ++b);
+    r = attend_request<FORM, ROWS, UNIT>(a, ++b);
   }
   Item i;
   i.b = uniform(b);
@@ -335,6 +393,23 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   i.head = uniform(static_cast<int>(divide(item, tiles)));
   i.tile = static_cast<int>(item - static_cast<int64_t>(i.head) * tiles);
   run.unit = uniform64(run.unit + i.s1 - i.s0);
+  i.reach = i.length;
+  i.edge = i.jump = i.all_see = 0;
+  if constexpr (FORM != kWhole) {
+    // the places of its first and last rows' tokens
+    const int row0 = i.tile * ROWS;
+    const int j0 = a.mask ? 0 : static_cast<int>(fdiv(static_cast<uint32_t>(row0), a.group));
+    const int j1 = a.mask ? i.fresh - 1
+                          : min(i.fresh - 1, static_cast<int>(fdiv(static_cast<uint32_t>(row0 + ROWS - 1), a.group)));
+    if (j1 + 1 < i.length - i.cached)
+      i.length = i.cached + j1 + 1;
+    i.length = uniform(i.length);
+    const int from = min(window_from(a, i.cached, j0), i.length);
+    i.all_see = uniform(min(window_from(a, i.cached, j1), i.length));
+    i.edge = uniform(edge_of(a, i.length));
+    i.jump = uniform(max((from & ~(kTile - 1)) - i.edge, 0));
+    i.reach = i.length - i.jump;
+  }
   return i;
 }
 
@@ -553,8 +628,13 @@ __device__ __forceinline__ bool clean(char *tv, int first, uint32_t seen, bool m
   return __any(odd);
 }
 
+// kBlocks: the scales of a tile's keys and values, of sixteen tokens each.
+struct Scales {
+  float key[2], value[2];
+};
+
 // A wave's query rows and their sums.
-template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
+template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   static constexpr int E = DP / 16, QS = DP / 32;
   u32x4 q[RT][QS];
   float top[RT];     // reference maximum of a row's scaled scores
@@ -564,6 +644,13 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   uint64_t mask[RT]; // of one word
   float scale;       // above zero: its sign is the queries'
   int words;         // of a mask; 0: none
+  int from[FORM == kWhole ? 1 : RT]; // where a row's window begins
+  int sinks;
+  // kBlocks: the values' scales go into the weights of the second product. In f16
+  // they go there over the largest so far, a power of two, which the sums are of:
+  // else weights of up to 2^14 times a scale of four would be none.
+  static constexpr bool kOver = FORM == kBlocks && T == kF16;
+  float over;
 
   __device__ __forceinline__ void start(const AttendArgs &a, const Item &it, int row0, int rows, float score_scale,
                                         int lane) {
@@ -575,6 +662,8 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     const uint32_t sign = score_scale < 0.0f ? 0x80008000u : 0u;
     scale = fabsf(score_scale) < kLeast ? kLeast : fabsf(score_scale);
     words = a.mask ? a.words : 0;
+    sinks = FORM == kWhole ? 0 : a.sinks;
+    over = 0.0f;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
@@ -583,6 +672,8 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       mask[t] = 0u;
       if (words == 1 && place[t] < it.fresh)
         mask[t] = static_cast<uint64_t>(a.mask[it.start + static_cast<int64_t>(j)]);
+      if constexpr (FORM != kWhole)
+        from[t] = place[t] < it.fresh ? window_from(a, it.cached, row_depth(a, it.start, place[t])) : 0;
       const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
                                (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma unroll
@@ -646,15 +737,21 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   }
 
   // The weights of a row, and their sum over the lane's tokens.
-  __device__ __forceinline__ float weigh(int t) {
+  __device__ __forceinline__ float weigh(int t, const float *value_scale) {
     float p[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         p[n][i] = __builtin_amdgcn_exp2f(s[t][n][i] * scale - top[t]);
-      weights[t][n * 2] = pack16<T>(p[n][0], p[n][1]);
-      weights[t][n * 2 + 1] = pack16<T>(p[n][2], p[n][3]);
+      if constexpr (FORM == kBlocks) {
+        const float f = value_scale[n];
+        weights[t][n * 2] = pack16<T>(p[n][0] * f, p[n][1] * f);
+        weights[t][n * 2 + 1] = pack16<T>(p[n][2] * f, p[n][3] * f);
+      } else {
+        weights[t][n * 2] = pack16<T>(p[n][0], p[n][1]);
+        weights[t][n * 2 + 1] = pack16<T>(p[n][2], p[n][3]);
+      }
     }
     return ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
   }
@@ -662,14 +759,54 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   // Weights go by the reference maximum, which moves only where some lane has
   // seen a score far above it: in a row's first tile and a few later ones. So
   // lanes compare theirs then and not at every tile.
-  __device__ __forceinline__ void soften(const Item &it, int row0, int x, uint32_t seen, bool cut, int lane_) {
+  // kBlocks: the scales of the tile's keys and values, of sixteen tokens each.
+  __device__ __forceinline__ void soften(const Item &it, int row0, int x, uint32_t seen, bool cut, int lane_,
+                                         const Scales &tile) {
     constexpr float kBias = weight_bias<T>();
+    float values[RT][2];
+    if constexpr (FORM == kBlocks) {
+      float v[2] = {tile.value[0], tile.value[1]};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        if (!(seen >> (16 * n) & 0xffffu))
+          v[n] = 0.0f; // of no token: may be anything
+      if constexpr (kOver) {
+        const float most = fmaxf(fabsf(v[0]), fabsf(v[1]));
+        if (__builtin_expect(most > over, 0)) {
+          const float next = __uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u);
+          const float shrink = over / next;
+          over = next;
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              acc[t][e] *= shrink;
+        }
+        const float back = over > 0.0f ? 1.0f / over : 0.0f; // over: a power of two
+        v[0] *= back;
+        v[1] *= back;
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        values[t][0] = v[0];
+        values[t][1] = v[1];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          s[t][n] *= tile.key[n];
+      }
+    }
     if (__builtin_expect(cut, 0)) {
       const int lane = anew(lane_), c = lane & 15, g = lane >> 4;
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const uint32_t bits = seen & (words > 1 ? row_sees(args_again(), it, row0 + t * 16 + c, x)
-                                                : sees(it, words == 1, place[t], mask[t], x));
+        uint32_t bits = seen & (words > 1 ? row_sees(args_again(), it, row0 + t * 16 + c, x)
+                                          : sees(it, words == 1, place[t], mask[t], x));
+        if constexpr (FORM != kWhole)
+          bits &= window_sees(x, from[t], sinks);
+        if constexpr (FORM == kBlocks)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            values[t][n] = bits >> (16 * n) & 0xffffu ? values[t][n] : 0.0f;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -705,7 +842,7 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t)
-      sum[t] += weigh(t);
+      sum[t] += weigh(t, values[t]);
   }
 
   __device__ __forceinline__ void add(const Values<T, DP, RAW, EARLY> &v) {
@@ -720,10 +857,10 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 
   // tk, tv: the places of the tile's keys and values.
   __device__ __forceinline__ void step(const Item &it, int row0, int x, uint32_t seen, bool cut, uint32_t tk, uint32_t tv,
-                                       const Reads<DP, RAW> &reads, int lane) {
+                                       const Reads<DP, RAW> &reads, int lane, const Scales &tile) {
     scores(tk + reads.key);
     const Values<T, DP, RAW, EARLY> v(tv + reads.value); // EARLY: they arrive during the softmax
-    soften(it, row0, x, seen, cut, lane);
+    soften(it, row0, x, seen, cut, lane, tile);
     add(v);
   }
 
@@ -751,10 +888,13 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       const char *q = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
                              (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma clang loop unroll(disable)
-      for (int x = x0; x < x_end; x += pace) {
-        if (x + kTile <= it.cached)
+      for (int at0 = x0; at0 < x_end; at0 += pace) {
+        const int x = it.token<FORM>(at0);
+        if (x + kTile <= it.cached && !it.windowed<FORM>(x, sinks))
           continue;
-        const uint32_t sees = row_sees(a, it, p, x);
+        uint32_t sees = row_sees(a, it, p, x);
+        if constexpr (FORM != kWhole)
+          sees &= window_sees(x, from[t], sinks);
 #pragma clang loop unroll(disable)
         for (int y = x; y < min(x + kTile, it.length); ++y) {
           const uint32_t at = fdiv(static_cast<uint32_t>(y), a.page), off = static_cast<uint32_t>(y) - at * a.page.d;
@@ -782,7 +922,7 @@ template <int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
 
 // How a wave brings its tokens of a tile into shared memory: NT tokens from
 // `first`, of every tile. Its tiles are PACE tokens apart.
-template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Loader {
+template <int FORM, int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Loader {
   static constexpr int CELL = I8 ? 1 : 2;
   using Lanes = Share<DP, CELL, NT>;
   static constexpr int LB = Lanes::LB, TL = Lanes::TL, TPI = Lanes::TPI, LOADS = Lanes::LOADS;
@@ -794,6 +934,10 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   int64_t key_page, value_page;
   uint32_t key_slot, value_slot;
   int64_t key_slot64, value_slot64; // kStaged: of any size
+  int edge, jump; // see Item
+  const char *key_scale, *value_scale; // kBlocks: the head's
+  uint32_t scale_page, scale_block;    // bytes
+  FastDiv block;
   int length, pages, first, token, dim, cell_at, head_dims;
   uint32_t key_token, value_token; // kStagedEven: where the lane's token lies after the load's first
   bool full; // the head fills the tile's rows
@@ -803,6 +947,7 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   bool whole;  // all of them
   u32x4 stage[2][SRC == kAsync ? 1 : LOADS];
   uint32_t there; // loads that are a token's, by bit
+  Scales fetched; // with them
   // kAsync: the lane's token of the first load in its group of sixteen, and its piece
   uint32_t key_lane, value_lane, place16;
 
@@ -821,6 +966,11 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     once = a.once;
     pages = a.pages;
     page = a.page;
+    if constexpr (FORM == kBlocks) {
+      scale_page = a.scale_page;
+      scale_block = a.scale_block;
+      block = a.block;
+    }
     has = dim < a.dim && Lanes::brings(lane);
     whole = dim + LB <= a.dim;
     cell_at = has ? dim * CELL : 0;
@@ -836,6 +986,15 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     values = a.values + it.head * a.value_head;
     table = a.table + it.b * a.table_row;
     length = it.length;
+    edge = it.edge;
+    jump = it.jump;
+    if constexpr (FORM == kBlocks) {
+      key_scale = reinterpret_cast<const char *>(a.key_scale) + static_cast<uint64_t>(static_cast<uint32_t>(it.head)) * a.scale_head;
+      value_scale = reinterpret_cast<const char *>(a.value_scale) + static_cast<uint64_t>(static_cast<uint32_t>(it.head)) * a.scale_head;
+    }
+  }
+  __device__ __forceinline__ int token_of(int place) const {
+    return FORM == kWhole ? place : place < edge ? place : place + jump;
   }
 
   __device__ __forceinline__ bool is_page(int id) const {
@@ -860,13 +1019,18 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   int64_t key_at, value_at;
   uint64_t paged; // the groups that lie on a page
   uint32_t room;  // [2][64] of this wave
-  __device__ __forceinline__ int group_at(int x, int lane) const { return x + (lane >> 1) * PACE + (lane & 1) * 16; }
+  uint32_t scale_room; // kBlocks: [2][2][64], keys' and values' scales of the same groups
+  __device__ __forceinline__ int group_at(int x, int lane) const {
+    return token_of(x + (lane >> 1) * PACE) + (lane & 1) * 16;
+  }
   __device__ __forceinline__ uint32_t entry_at(int x, int lane) const {
     return fdiv(static_cast<uint32_t>(min(group_at(x, lane), length - 1)), page);
   }
   // Past the length: the last page's first tokens; of no page: the first one's,
   // which nothing will see.
-  __device__ __forceinline__ void take_entries(int id, int x, int lane) {
+  // kBlocks: the groups' scales go on their way to shared memory, ahead of all of
+  // the tiles that they are of, whose arrival is waited for: in this order.
+  __device__ __forceinline__ void take_entries(int id, int x, int lane, uint32_t half) {
     const bool is = is_page(id);
     const int x0 = group_at(x, lane);
     const uint32_t off = is && x0 < length ? static_cast<uint32_t>(x0) - fdiv(static_cast<uint32_t>(x0), page) * page.d : 0u;
@@ -874,19 +1038,35 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
     key_at = static_cast<int64_t>(at * key_page + static_cast<uint64_t>(off) * key_slot);
     value_at = static_cast<int64_t>(at * value_page + static_cast<uint64_t>(off) * value_slot);
     paged = __ballot(is);
+    if constexpr (FORM == kBlocks) {
+      const uint32_t scale_at = static_cast<uint32_t>(at) * scale_page + fdiv(off, block) * scale_block;
+      load_async4(key_scale, scale_at, scale_room + half * 2);
+      load_async4(value_scale, scale_at, scale_room + half * 2 + 256);
+    }
+  }
+  // kBlocks: the n-th tile's scales, once it has arrived.
+  __device__ __forceinline__ Scales scales(int n) const {
+    Scales t = {};
+    if constexpr (FORM == kBlocks) {
+      typedef const __attribute__((address_space(3))) f32x2 *Pair;
+      const uint32_t from = scale_room + (n / kAhead % 2) * 512 + (n % kAhead) * 8;
+      const f32x2 k = *reinterpret_cast<Pair>(from), v = *reinterpret_cast<Pair>(from + 256);
+      t.key[0] = k.x, t.key[1] = k.y, t.value[0] = v.x, t.value[1] = v.y;
+    }
+    return t;
   }
   // The first entries, and the next on their way.
   __device__ __forceinline__ void first_entries(int x, int count, int lane) {
     const int id = table[entry_at(x, lane)];
     if (count > kAhead)
       load_async4(table, entry_at(x + kAhead * PACE, lane) * 4u, room + 256);
-    take_entries(id, x, lane);
+    take_entries(id, x, lane, 0);
   }
   // The n-th tile, at x; called for one after the other.
   __device__ __forceinline__ Next look(int n, int x, int lane) {
     if (n > 0 && n % kAhead == 0) {
       const uint32_t half = n / kAhead % 2 * 256;
-      take_entries(*reinterpret_cast<const __attribute__((address_space(3))) int *>(room + half + lane * 4), x, lane);
+      take_entries(*reinterpret_cast<const __attribute__((address_space(3))) int *>(room + half + lane * 4), x, lane, half);
       load_async4(table, entry_at(x + kAhead * PACE, lane) * 4u, room + (half ^ 256));
     }
     const int g = n % kAhead * 2;
@@ -927,8 +1107,19 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
   }
 
   // Through registers: the wave's tokens of the tile at x.
-  __device__ __forceinline__ void fetch(int x) {
+  __device__ __forceinline__ void fetch(int place) {
+    const int x = token_of(place);
     there = 0u;
+    if constexpr (FORM == kBlocks) { // pages are of whole blocks, and blocks of sixteen tokens
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int x0 = uniform(x + 16 * h), id = entry(x0);
+        const uint32_t off = static_cast<uint32_t>(x0) - fdiv(static_cast<uint32_t>(x0), page) * page.d;
+        const uint32_t at = is_page(id) ? static_cast<uint32_t>(id) * scale_page + fdiv(off, block) * scale_block : 0u;
+        fetched.key[h] = scalar_load(reinterpret_cast<const float *>(key_scale + at));
+        fetched.value[h] = scalar_load(reinterpret_cast<const float *>(value_scale + at));
+      }
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int t0 = first + i * TPI;
@@ -997,14 +1188,15 @@ template <int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE> struct Lo
 
 // ---------------------------------------------------------- up to 16 rows
 
-template <int T, bool I8, int DP, int SRC>
+template <int FORM, int T, bool I8, int DP, int SRC>
 __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC == kAsync) == kMostWorkgroups ? 2 : 1)
 void k_attend_turns(AttendArgs a) {
   constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
   constexpr int TILE = kTile * DP * (I8 ? 1 : 2);
   constexpr int RING = SRC == kAsync ? 2 : 1; // tiles of a wave
-  using Load = Loader<T, I8, DP, SRC, kTile, I8, UNIT>;
+  using Load = Loader<FORM, T, I8, DP, SRC, kTile, I8, UNIT>;
   __shared__ int entries[SRC == kAsync ? W : 1][2][64];
+  __shared__ float block_scales[FORM == kBlocks && SRC == kAsync ? W : 1][2][2][64];
 
   __shared__ Schedule schedule;
   constexpr int SUMS = W * 16 * (DP + 4) * sizeof(float); // the waves', at the end
@@ -1016,28 +1208,30 @@ void k_attend_turns(AttendArgs a) {
   const int c = lane & 15, g = lane >> 4;
   Load load(a, lane, 0);
   load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
-  Rows<T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
+  if constexpr (FORM == kBlocks)
+    load.scale_room = place(reinterpret_cast<const char *>(&block_scales[SRC == kAsync ? wave : 0][0][0][0]));
+  Rows<FORM, T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
   const Reads<DP, I8> reads(lane);
-  add_up<ROWS, UNIT>(a, schedule);
+  add_up<FORM, ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
 
   while (run.unit < run.end) {
-    const Item it = take<ROWS, UNIT>(args_again(), schedule, run);
+    const Item it = take<FORM, ROWS, UNIT>(args_again(), schedule, run);
     const int row0 = it.tile * ROWS;
     const int rows = it.fresh * static_cast<int>(args_again().group.d) - row0; // of this tile and later ones
     load.item(args_again(), it);
-    const int x_end = min(it.s1 * UNIT, it.length), x0 = it.s0 * UNIT + wave * kTile;
+    const int x_end = min(it.s1 * UNIT, it.reach), x0 = it.s0 * UNIT + wave * kTile;
     const int count = x0 < x_end ? (x_end - x0 + UNIT - 1) / UNIT : 0; // this wave's tiles
     bool odd = false;
     auto start = [&] {
       const AttendArgs &b = args_again();
-      r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
+      r.start(b, it, row0, rows, I8 && FORM != kBlocks ? b.scale * b.key_scale[it.head] : b.scale, lane);
     };
     const uint32_t at = place(tiles[wave][0][0]);
-    auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
+    auto take_in = [&](int x, uint32_t seen, bool cut, int slot, const Scales &tile) {
       if (!I8 && __builtin_expect(cut, 0)) // what int8 holds is finite
-        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, x + kTile > it.cached, lane);
-      r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
+        odd |= clean<T, DP, kTile>(tiles[wave][slot][1], 0, seen, x + kTile > it.cached || it.windowed<FORM>(x, r.sinks), lane);
+      r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane, tile);
     };
 
     if constexpr (SRC == kAsync) {
@@ -1067,8 +1261,9 @@ void k_attend_turns(AttendArgs a) {
           arrived<(RING - 1) * 2 * Load::LOADS>();
         else
           arrived<0>();
-        const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
-        take_in(x, cut ? load.seen(x, on) : 0xffffffffu, cut, slot);
+        const int xt = it.token<FORM>(x);
+        const bool cut = (on & 3u) != 3u || xt + kTile > it.cached || it.windowed<FORM>(xt, r.sinks);
+        take_in(xt, cut ? load.seen(xt, on) : 0xffffffffu, cut, slot, load.scales(n));
         shared_done(); // its place is free
         on >>= 2;
         if (n + RING < count)
@@ -1086,9 +1281,11 @@ void k_attend_turns(AttendArgs a) {
       for (int n = 0; n < count; ++n, x += UNIT) {
         load.put(tk, tv);
         const uint32_t seen = load.tokens_there();
+        const Scales tile = load.fetched;
         if (n + 1 < count)
           load.fetch(x + UNIT);
-        take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, 0);
+        const int xt = it.token<FORM>(x);
+        take_in(xt, seen, seen != 0xffffffffu || xt + kTile > it.cached || it.windowed<FORM>(xt, r.sinks), 0, tile);
       }
     }
 
@@ -1105,7 +1302,7 @@ void k_attend_turns(AttendArgs a) {
 #pragma unroll
       for (int w = 0; w < W; ++w)
         most = fmaxf(most, row_max[w][c]);
-      const float f = __builtin_amdgcn_exp2f(r.top[0] - most);
+      const float f = __builtin_amdgcn_exp2f(r.top[0] - most) * (r.kOver ? r.over : 1.0f);
       if (c < rows)
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -1131,7 +1328,7 @@ void k_attend_turns(AttendArgs a) {
       const int64_t row = it.start + static_cast<int64_t>(j);
       const int64_t qh = static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d);
       const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * ROWS + i;
-      const float f = finish(l, I8 ? a.value_scale[it.head] : 1.0f);
+      const float f = finish(l, I8 && FORM != kBlocks ? a.value_scale[it.head] : 1.0f);
 #pragma unroll
       for (int d = 0; d < DIMS; d += 4) {
         f32x4 o = *reinterpret_cast<const f32x4 *>(&sums[0][i][d0 + d]);
@@ -1161,13 +1358,13 @@ void k_attend_turns(AttendArgs a) {
 
 // ---------------------------------------------------------- more rows
 
-template <int T, bool I8, int DP, int RT, int W, int SRC>
+template <int FORM, int T, bool I8, int DP, int RT, int W, int SRC>
 __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   constexpr int ROWS = 16 * RT * W, E = DP / 16, UNIT = kSharedUnit;
   constexpr int TILE = kTile * DP * 2;
   // tiles at a time: 64 KiB for each four waves
   constexpr int RING = SRC != kAsync ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
-  using Load = Loader<T, I8, DP, SRC, kTile / W, false, kTile>;
+  using Load = Loader<FORM, T, I8, DP, SRC, kTile / W, false, kTile>;
   __shared__ int entries[SRC == kAsync ? W : 1][2][64];
 
   __shared__ Schedule schedule;
@@ -1183,10 +1380,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   // heads of 128, 280 against 287 up to 32768 (the fastest of 40). The same for the
   // next tile's keys was slower (81).
   constexpr bool EARLY = DP <= 128 && (I8 || SRC == kAsync);
-  Rows<T, DP, RT, false, EARLY> r;
+  Rows<FORM, T, DP, RT, false, EARLY> r;
   if (tid < 2)
     odd_of[tid] = 0;
-  add_up<ROWS, UNIT>(a, schedule);
+  add_up<FORM, ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
   const Reads<DP, false> reads(lane);
   if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
@@ -1194,17 +1391,19 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
       *reinterpret_cast<u32x4 *>(&tiles[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
 
   for (int turn = 0; run.unit < run.end; turn ^= 1) {
-    const Item it = take<ROWS, UNIT>(args_again(), schedule, run);
+    const Item it = take<FORM, ROWS, UNIT>(args_again(), schedule, run);
     int &odd = odd_of[turn];
     const int row0 = (it.tile * W + wave) * 16 * RT;                // the wave's first
     const int rows = it.fresh * static_cast<int>(args_again().group.d) - row0; // and how many from there
     load.item(args_again(), it);
-    const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.length);
+    const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.reach);
     const int count = x0 < x_end ? (x_end - x0 + kTile - 1) / kTile : 0;
     // this wave's tokens of a tile that it has brought, before the others may read them
     auto clean_own = [&](int x, uint32_t seen, bool cut, int slot) {
       if (!I8 && __builtin_expect(cut, 0) &&
-          clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen, x + kTile > it.cached, lane) && lane == 0)
+          clean<T, DP, kTile / W>(tiles[slot][1], wave * (kTile / W), seen,
+                                  x + kTile > it.cached || it.windowed<FORM>(x, args_again().sinks), lane) &&
+          lane == 0)
         odd = 1;
     };
     const uint32_t at = place(tiles[0][0]);
@@ -1216,13 +1415,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
     // that in none the sums meet a way round them.
     auto work = [&](auto busy) {
       constexpr bool BUSY = decltype(busy)::value;
-      auto take_in = [&](int x, uint32_t seen, bool cut, int slot) {
+      auto take_in = [&](int x, uint32_t seen, bool cut, int slot, const Scales &tile) {
         if constexpr (BUSY)
-          r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane);
+          r.step(it, row0, x, seen, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads, lane, tile);
       };
       auto start = [&] {
         const AttendArgs &b = args_again();
-        r.start(b, it, row0, rows, I8 ? b.scale * b.key_scale[it.head] : b.scale, lane);
+        r.start(b, it, row0, rows, I8 && FORM != kBlocks ? b.scale * b.key_scale[it.head] : b.scale, lane);
       };
 
       if constexpr (SRC == kAsync) {
@@ -1255,14 +1454,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
             arrived<(RING - 2) * 2 * Load::LOADS>();
           else
             arrived<0>();
-          const bool cut = (on & 3u) != 3u || x + kTile > it.cached;
-          const uint32_t seen = cut ? load.seen(x, on) : 0xffffffffu;
-          clean_own(x, seen, cut, slot);
+          const int xt = it.token<FORM>(x);
+          const bool cut = (on & 3u) != 3u || xt + kTile > it.cached || (FORM != kWhole && it.windowed<FORM>(xt, args_again().sinks));
+          const uint32_t seen = cut ? load.seen(xt, on) : 0xffffffffu;
+          clean_own(xt, seen, cut, slot);
           meet();
           on >>= 2;
           if (x + (RING - 1) * kTile <= last)
             send(then, slot == 0 ? RING - 1 : slot - 1, RING - 2);
-          take_in(x, seen, cut, slot);
+          take_in(xt, seen, cut, slot, Scales{});
           then = load.look(n + RING, x + RING * kTile, lane);
           slot = slot + 1 == RING ? 0 : slot + 1;
         }
@@ -1276,12 +1476,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           const uint32_t t = load.tokens_there();
           if (lane == 0)
             tokens[slot][wave] = static_cast<uint8_t>(t);
-          const int xp = x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile); // the tile put: this one or the next
+          // the tile put: this one or the next
+          const int xp = it.token<FORM>(x + (slot == ((x - x0) / kTile & 1) ? 0 : kTile));
           const uint32_t seen = t << (wave * (kTile / W)) | ~(((1u << (kTile / W)) - 1u) << (wave * (kTile / W)));
-          clean_own(xp, seen, seen != 0xffffffffu || xp + kTile > it.cached, slot);
+          clean_own(xp, seen, seen != 0xffffffffu || xp + kTile > it.cached || it.windowed<FORM>(xp, args_again().sinks), slot);
         };
+        Scales tile = {}, next_tile = {}; // of this tile and of the next, which has been put
         if (count > 0) {
           load.fetch(x);
+          next_tile = load.fetched;
           put(0);
         }
         if (count > 1)
@@ -1294,11 +1497,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           for (int w = 0; w < W; ++w)
             seen |= static_cast<uint32_t>(tokens[slot][w]) << (w * (kTile / W));
           seen = static_cast<uint32_t>(uniform(static_cast<int>(seen)));
-          if (n + 1 < count)
+          tile = next_tile;
+          if (n + 1 < count) {
+            next_tile = load.fetched;
             put(slot ^ 1);
+          }
           if (n + 2 < count)
             load.fetch(x + 2 * kTile);
-          take_in(x, seen, seen != 0xffffffffu || x + kTile > it.cached, slot);
+          const int xt = it.token<FORM>(x);
+          take_in(xt, seen, seen != 0xffffffffu || xt + kTile > it.cached || it.windowed<FORM>(xt, args_again().sinks), slot, tile);
         }
       }
 
@@ -1320,7 +1527,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           const uint32_t j = fdiv(p, b.group);
           const int64_t row = it.start + static_cast<int64_t>(j);
           const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
-          const float f = finish(sum, I8 ? b.value_scale[it.head] : 1.0f);
+          const float f = finish(sum, I8 && FORM != kBlocks ? b.value_scale[it.head] : 1.0f) * (r.kOver ? r.over : 1.0f);
           char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
 #pragma unroll
           for (int e = 0; e < E; ++e)
@@ -1335,7 +1542,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           float *dst = b.partial + (part - c) * DP + part_at<DP, ROWS>(c, 4 * g);
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            *reinterpret_cast<f32x4 *>(dst + e * 256) = r.acc[t][e];
+            *reinterpret_cast<f32x4 *>(dst + e * 256) = r.kOver ? r.acc[t][e] * r.over : r.acc[t][e];
           if (g == 0) {
             b.stats[part * 2] = r.top[t];
             b.stats[part * 2 + 1] = sum;
@@ -1371,7 +1578,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
 // rows of a request, PHASES waves a piece of 64 times four dims at a time. It is
 // bound by how long a read takes of what other dies have written: so all parts
 // are on their way at once, where there are many by sharing them among waves.
-template <int T, bool I8, int DP, int ROWS, int UNIT, int PHASES>
+template <int FORM, int T, bool I8, int DP, int ROWS, int UNIT, int PHASES>
 __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join(AttendArgs a) {
   constexpr bool LANED = ROWS > 16;                   // see part_at
   constexpr int N = LANED ? 16 : 256 / DP;            // rows of a piece
@@ -1401,7 +1608,7 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
     }
     return;
   }
-  const Request r = attend_request<ROWS, UNIT>(a, b);
+  const Request r = attend_request<FORM, ROWS, UNIT>(a, b);
   const int64_t total = a.schedule[a.requests], first = a.schedule[b];
   const int64_t per = units_of_run(total, a.workgroups);
   const int64_t rows = static_cast<int64_t>(r.fresh) * a.group.d;
@@ -1481,7 +1688,7 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
       const uint32_t j = fdiv(p, a.group);
       const int64_t row = r.start + static_cast<int64_t>(j);
       const int64_t qh = static_cast<int64_t>(head) * a.group.d + (p - j * a.group.d);
-      acc *= finish(sum, I8 ? a.value_scale[head] : 1.0f);
+      acc *= finish(sum, I8 && FORM != kBlocks ? a.value_scale[head] : 1.0f);
       if (d < a.dim)
         store(a.out + (row * a.out_row + qh * a.out_head + d) * 2,
               u32x2{pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3])});
@@ -1493,7 +1700,7 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
   }
 }
 
-template <int T, bool I8, int DP, int ROWS, int UNIT>
+template <int FORM, int T, bool I8, int DP, int ROWS, int UNIT>
 hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args, const AttendPlan &p,
                         hipStream_t s) {
   AttendArgs a = args;
@@ -1512,53 +1719,53 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
   const int64_t pieces = (rows + n - 1) / n * a.kv_heads * (ROWS > 16 ? DP / 16 : 1);
   const int64_t items = (rows + ROWS - 1) / ROWS * a.kv_heads * requests;
   const bool many = p.workgroups > 8 * items;
-  return hipLaunchKernel(many ? reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 8>)
-                              : reinterpret_cast<const void *>(k_attend_join<T, I8, DP, ROWS, UNIT, 1>),
+  return hipLaunchKernel(many ? reinterpret_cast<const void *>(k_attend_join<FORM, T, I8, DP, ROWS, UNIT, 8>)
+                              : reinterpret_cast<const void *>(k_attend_join<FORM, T, I8, DP, ROWS, UNIT, 1>),
                          dim3(static_cast<uint32_t>(a.requests) + 1,
                               static_cast<uint32_t>(std::min<int64_t>(many ? pieces : (pieces + 3) / 4, 65535))),
                          dim3(many ? 512 : 256), pa, 0, s);
 }
 
-template <int T, bool I8, int DP, int RT, int W, int SRC>
+template <int FORM, int T, bool I8, int DP, int RT, int W, int SRC>
 hipError_t attend_start_shared(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  return attend_start<T, I8, DP, 16 * RT * W, kSharedUnit>(
-      reinterpret_cast<const void *>(k_attend_shared<T, I8, DP, RT, W, SRC>), 64 * W, a, p, s);
+  return attend_start<FORM, T, I8, DP, 16 * RT * W, kSharedUnit>(
+      reinterpret_cast<const void *>(k_attend_shared<FORM, T, I8, DP, RT, W, SRC>), 64 * W, a, p, s);
 }
 
-template <int T, bool I8, int DP, int SRC>
+template <int FORM, int T, bool I8, int DP, int SRC>
 hipError_t attend_shared(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   if constexpr (DP < 256) { // 32 rows of a wave with a head of 256 would not fit its registers
     if (p.rows == 128)
-      return attend_start_shared<T, I8, DP, 2, 4, SRC>(a, p, s);
+      return attend_start_shared<FORM, T, I8, DP, 2, 4, SRC>(a, p, s);
     if (p.rows == 256)
-      return attend_start_shared<T, I8, DP, 2, 8, SRC>(a, p, s);
+      return attend_start_shared<FORM, T, I8, DP, 2, 8, SRC>(a, p, s);
   }
-  return attend_start_shared<T, I8, DP, 1, 4, SRC>(a, p, s);
+  return attend_start_shared<FORM, T, I8, DP, 1, 4, SRC>(a, p, s);
 }
 
-template <int T, bool I8, int DP>
+template <int FORM, int T, bool I8, int DP>
 hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   if (p.rows == 16)
-    return attend_start<T, I8, DP, 16, turn_unit(DP)>(
-        p.async ? reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, kAsync>)
-                : reinterpret_cast<const void *>(k_attend_turns<T, I8, DP, kStaged>),
+    return attend_start<FORM, T, I8, DP, 16, turn_unit(DP)>(
+        p.async ? reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kAsync>)
+                : reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kStaged>),
         64 * turn_waves(DP), a, p, s);
   // int8 is widened once for all waves, on its way through registers
   if constexpr (I8)
-    return p.even ? attend_shared<T, I8, DP, kStagedEven>(a, p, s) : attend_shared<T, I8, DP, kStaged>(a, p, s);
+    return p.even ? attend_shared<FORM, T, I8, DP, kStagedEven>(a, p, s) : attend_shared<FORM, T, I8, DP, kStaged>(a, p, s);
   else
-    return p.async ? attend_shared<T, I8, DP, kAsync>(a, p, s) : attend_shared<T, I8, DP, kStaged>(a, p, s);
+    return p.async ? attend_shared<FORM, T, I8, DP, kAsync>(a, p, s) : attend_shared<FORM, T, I8, DP, kStaged>(a, p, s);
 }
 
-template <int T, bool I8>
+template <int FORM, int T, bool I8>
 hipError_t attend_width(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   switch (p.width) {
   case 64:
-    return attend_source<T, I8, 64>(a, p, s);
+    return attend_source<FORM, T, I8, 64>(a, p, s);
   case 128:
-    return attend_source<T, I8, 128>(a, p, s);
+    return attend_source<FORM, T, I8, 128>(a, p, s);
   default:
-    return attend_source<T, I8, 256>(a, p, s);
+    return attend_source<FORM, T, I8, 256>(a, p, s);
   }
 }
 

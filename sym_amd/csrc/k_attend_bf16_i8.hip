@@ -4,7 +4,7 @@
 namespace relx {
 
 hipError_t attend_launch_bf16_i8(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  return attend_width<kBF16, true>(a, p, s);
+  return attend_width<kWhole, kBF16, true>(a, p, s);
 }
 
 } // namespace relx

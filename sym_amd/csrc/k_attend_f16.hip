@@ -4,7 +4,7 @@
 namespace relx {
 
 hipError_t attend_launch_f16(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  return attend_width<kF16, false>(a, p, s);
+  return attend_width<kWhole, kF16, false>(a, p, s);
 }
 
 } // namespace relx

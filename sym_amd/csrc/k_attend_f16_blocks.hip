@@ -1,0 +1,10 @@
+// k_attend_f16_blocks.hip - tree attention with f16 queries over a cache of int8 with a scale a block.
+#include "k_attend.h"
+
+namespace relx {
+
+hipError_t attend_launch_f16_blocks(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  return attend_width<kBlocks, kF16, true>(a, p, s);
+}
+
+} // namespace relx
