@@ -758,6 +758,31 @@ typedef struct relx_block_append_args {
 int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_t stream,
                       relx_err *err);
 
+/* Attention over packed sequences, for training and for prompts: sequence b has
+ * the rows [starts[b], starts[b + 1]) of q and out [rows, heads, dim] and of k and
+ * v [rows, kv_heads, dim]. A row at place p of its sequence sees the places x <= p
+ * with p - x < window (0: any) or x < sinks (256 at most). lse, where it is
+ * wanted, is [heads, rows], natural logarithms. Rows of no sequence are 0 with
+ * lse -inf, and nothing of one sequence reaches another; what is not finite may
+ * reach any row of its own. f16 or bf16, head sizes of multiples of 8 up to 128,
+ * rows and heads at 16-byte addresses, rows at most 2^24 elements apart. */
+typedef struct relx_window_args {
+  relx_heads q, k, v, out;
+  const int32_t *starts; /* [sequences + 1] */
+  float *lse;
+  int64_t rows, sequences, heads, kv_heads, dim, window, sinks, kind, bits;
+  double scale;
+} relx_window_args;
+int relx_window_attention(relx_ctx *ctx, const relx_window_args *args, uint64_t stream, relx_err *err);
+/* The gradients of relx_window_attention's operands for its result's, of the same
+ * arguments with the result and lse that it gave. Those of k and v are sums over
+ * a key head's query heads. No atomics: the same bits every time. `workspace`: at
+ * least the bytes that relx_window_attention_workspace says, any contents. */
+int relx_window_attention_backward(relx_ctx *ctx, const relx_window_args *args, const relx_heads *out_grad,
+                                   const relx_heads *q_grad, const relx_heads *k_grad, const relx_heads *v_grad,
+                                   void *workspace, size_t workspace_bytes, uint64_t stream, relx_err *err);
+int relx_window_attention_workspace(const relx_window_args *args, size_t *bytes, relx_err *err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,6 +136,9 @@ relx_cache_view = _record("relx_cache_view", _I8, "window sinks", relx_block_sca
 relx_block_append_args = _record(
     "relx_block_append_args", relx_heads, "k v", relx_cache, "cache", relx_block_scales, "scales",
     _P8, "table", _I8, "table_row", _P8, "cached starts", _I8, "rows requests columns kind bits")
+relx_window_args = _record(
+    "relx_window_args", relx_heads, "q k v out", _P8, "starts lse",
+    _I8, "rows sequences heads kv_heads dim window sinks kind bits", _D8, "scale")
 
 # every entry point include/relx.h declares, with its ctypes signature
 _VP, _SZ, _I, _I64, _U64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64
@@ -209,6 +212,9 @@ SIGNATURES = {
     "relx_tree_attention_workspace": (_I, [_VP, ctypes.POINTER(_SZ), _E]),
     "relx_tree_attention_view": (_I, [_VP, _VP, _VP, _U64, _E]),
     "relx_block_append": (_I, [_VP, _VP, _U64, _E]),
+    "relx_window_attention": (_I, [_VP, _VP, _U64, _E]),
+    "relx_window_attention_backward": (_I, [_VP] * 7 + [_SZ, _U64, _E]),
+    "relx_window_attention_workspace": (_I, [_VP, ctypes.POINTER(_SZ), _E]),
     "relx_ctx_synchronize": (_I, [_VP, _E]),
     "relx_ctx_time_kernels": (_I, [_VP, _I, _E]),
     "relx_ctx_kernel_times": (_I, [_VP, ctypes.POINTER(relx_kernel_times), _E]),

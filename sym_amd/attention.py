@@ -56,6 +56,7 @@ _ROTATION = struct.Struct(_format(N.relx_rotation))
 _ATTENTION = struct.Struct(_format(N.relx_tree_attention_args)[6:])  # after its two relx_heads
 _SCALES = struct.Struct(_format(N.relx_block_scales))
 _VIEW = struct.Struct(_format(N.relx_cache_view)[:2])  # before its scales
+_WINDOW = struct.Struct(_format(N.relx_window_args)[12:])  # after its four relx_heads
 _APPEND = struct.Struct(_format(N.relx_block_append_args)[6 + 16 + 6:])  # after its heads, cache and scales
 
 
@@ -547,3 +548,111 @@ def _view(window, sinks):
     if window < 0 or sinks < 0 or (window == 0 and sinks):
         _bad("a window of %d tokens with %d first ones" % (window, sinks))
     return _VIEW.pack(window, sinks)
+
+
+# ------------------------------------------------------------ packed sequences
+
+class _Window(torch.autograd.Function):
+    @staticmethod
+    def forward(fn, q, k, v, ctx, starts, window, sinks, scale, lse):
+        if lse is None:
+            lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+        out = _window_attention(ctx, q, k, v, starts, window, sinks, scale, None, lse)
+        fn.save_for_backward(q, k, v, out, lse, starts)
+        fn.rest = ctx, window, sinks, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(fn, dout):
+        q, k, v, out, lse, starts = fn.saved_tensors
+        ctx, window, sinks, scale = fn.rest
+        dq, dk, dv = window_attention_backward(ctx, _packed(dout), q, k, v, out, lse, starts, window=window, sinks=sinks, scale=scale)
+        wants = fn.needs_input_grad
+        return dq if wants[0] else None, dk if wants[1] else None, dv if wants[2] else None, None, None, None, None, None, None
+
+
+def _packed(t):
+    """A gradient as it lies, if its rows do as the kernels want them."""
+    row, head, one = t.stride()
+    return t if one == 1 and row % 8 == 0 and head % 8 == 0 and row and head and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale):
+    device = _device(ctx, q)
+    shape, ks, dtype = q.shape, k.shape, q.dtype
+    kind = _KINDS.get(dtype)
+    if len(shape) != 3 or len(ks) != 3 or kind is None or kind[1] != 16 or ks[0] != shape[0] or ks[2] != shape[2] or \
+            ks[1] < 1 or shape[1] < 1 or shape[1] % ks[1]:
+        _bad("queries and keys: f16 or bf16 [rows, heads, dim] and [rows, kv_heads, dim], kv_heads dividing heads; got %s %s and %s %s"
+             % (dtype, list(shape), k.dtype, list(ks)))
+    window, sinks = 0 if window is None else int(window), int(sinks)
+    if window < 0 or sinks < 0 or (window == 0 and sinks):
+        _bad("a window of %d tokens with %d first ones" % (window, sinks))
+    l_ptr = 0
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != (shape[1], shape[0]) or lse.get_device() != device or \
+                not lse.is_contiguous():
+            _bad("lse: contiguous float32 [%d, %d]" % (shape[1], shape[0]))
+        l_ptr = lse.data_ptr()
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        _bad("starts: int32 [sequences + 1]")
+    return (_heads(q, "queries", shape, dtype, device) + _heads(k, "keys", ks, dtype, device) +
+            _heads(v, "values", ks, dtype, device) + _heads(out, "result", shape, dtype, device) +
+            _WINDOW.pack(_row(starts, "starts", torch.int32, None, device), l_ptr, shape[0], starts.shape[0] - 1, shape[1], ks[1],
+                         shape[2], window, sinks, *kind, shape[2] ** -0.5 if scale is None else float(scale))), device
+
+
+def window_attention(ctx, q, k, v, starts, *, window=None, sinks=0, scale=None, out=None, lse=None):
+    """Attention over packed sequences, for training and prompts: sequence b has the
+    rows [starts[b], starts[b + 1]) (int32 [sequences + 1]) of the queries
+    [rows, heads, dim] and of the keys and values [rows, kv_heads, dim] (f16 or bf16;
+    strides of multiples of eight elements, so views of a fused projection do). Head h
+    reads key head h // (heads // kv_heads).
+
+    A row at place p of its sequence sees the places x <= p with p - x < `window`
+    (None: any), and the first `sinks` ones (256 at most). Rows of no sequence are
+    0, and nothing of one sequence reaches another. `scale`: of the scores, by
+    default dim ** -0.5. `lse`: float32 [heads, rows] for the logarithm of each row's
+    sum of exponentials. Differentiable in q, k and v, once (without `out`)."""
+    if out is None and _in_graph(q, k, v):
+        return _Window.apply(q, k, v, ctx, starts, window, sinks, scale, lse)
+    return _window_attention(ctx, q, k, v, starts, window, sinks, scale, out, lse)
+
+
+def _window_attention(ctx, q, k, v, starts, window, sinks, scale, out, lse):
+    if out is None:
+        out = q.new_empty(q.shape)
+    args, device = _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale)
+    _call("relx_window_attention", ctx, args, _stream(device))
+    return out
+
+
+def window_attention_backward(ctx, dout, q, k, v, out, lse, starts, *, window=None, sinks=0, scale=None):
+    """Gradients of `window_attention` for its result's gradient `dout`, from its
+    result and its `lse`: (queries', keys', values'), of the operands' type; those of
+    keys and values are summed over a key head's query heads. The same bits every time."""
+    args, device = _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale)
+    if lse is None:
+        _bad("the backward takes the forward's lse")
+    shape, ks = q.shape, k.shape
+    dq, dk, dv = q.new_empty(shape), q.new_empty(ks), q.new_empty(ks)
+    size = _window_room(args, shape, ks, q.dtype, starts.shape[0], window, sinks)
+    room = q.new_empty(size, dtype=torch.uint8)
+    _call("relx_window_attention_backward", ctx, args, _heads(dout, "result's gradient", shape, q.dtype, device),
+          _made(dq, shape), _made(dk, ks), _made(dv, ks), room.data_ptr(), size, _stream(device))
+    return dq, dk, dv
+
+
+def _window_room(args, shape, ks, dtype, starts, window, sinks):
+    key = (shape, ks[1], dtype, starts, window, sinks)
+    room = _rooms.get(key)
+    if room is None:
+        size, err = ctypes.c_size_t(), N.relx_err()
+        if N.lib().relx_window_attention_workspace(args, ctypes.byref(size), ctypes.byref(err)):
+            _fail(err)
+        room = size.value
+        if len(_rooms) >= 1024:
+            _rooms.clear()
+        _rooms[key] = room
+    return room

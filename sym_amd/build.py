@@ -30,7 +30,7 @@ SOURCES = ["plan.cpp", "program.cpp", "runtime.cpp", "workers.cpp", "indexed.cpp
            "k_interleave_generic.hip", "k_interleave_ragged.hip", "k_permute.hip", "k_gather.hip", "k_copy.hip", "noalloc.hip",
            "attention.cpp", "k_tables.hip", "k_rotate.hip",
            "k_attend_f16.hip", "k_attend_f16_i8.hip", "k_attend_bf16.hip", "k_attend_bf16_i8.hip",
-           "window.cpp", "k_blocks.hip",
+           "window.cpp", "k_blocks.hip", "k_window_f16.hip", "k_window_bf16.hip",
            "k_attend_f16_window.hip", "k_attend_f16_blocks.hip", "k_attend_bf16_window.hip", "k_attend_bf16_blocks.hip"]
 
 
@@ -43,6 +43,8 @@ EXTRA = {"k_interleave.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
          "k_attend_f16_i8.hip": ["-ffp-contract=fast"],
          "k_attend_bf16.hip": ["-ffp-contract=fast"],
          "k_attend_bf16_i8.hip": ["-ffp-contract=fast"],
+         "k_window_f16.hip": ["-ffp-contract=fast"],
+         "k_window_bf16.hip": ["-ffp-contract=fast"],
          "k_attend_f16_window.hip": ["-ffp-contract=fast"],
          "k_attend_f16_blocks.hip": ["-ffp-contract=fast"],
          "k_attend_bf16_window.hip": ["-ffp-contract=fast"],

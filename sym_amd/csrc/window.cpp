@@ -5,6 +5,7 @@
 
 #include "attention.h"
 #include "operators.h"
+#include "window.h"
 
 namespace relx {
 namespace {
@@ -84,10 +85,146 @@ BlockArgs block_args(const relx_block_append_args &p, int &type) {
   return a;
 }
 
+// ------------------------------------------------------------ packed sequences
+
+constexpr int kTileRows = 128, kTileKeys = 128, kMostSinks = 256;
+
+// Rows that are read in pieces of 16 bytes, tiles of them from one address.
+Heads rows_of(const relx_heads *h, bool used, int64_t rows, int64_t heads, const char *what) {
+  const Heads x = heads_of(h, used, what);
+  if (!used)
+    return x;
+  need(x.row >= 0 && x.head >= 0, "window attention: negative strides");
+  layout((rows <= 1 || (x.row % 8 == 0 && x.row <= (int64_t{1} << 24))) && (heads <= 1 || x.head % 8 == 0) &&
+             reinterpret_cast<uintptr_t>(x.data) % 16 == 0,
+         "window attention: rows and heads at 16-byte addresses, rows at most 2^24 elements apart");
+  return x;
+}
+
+WindowArgs window_args(const relx_window_args &p, int &type) {
+  type = element_type(p.kind, p.bits);
+  layout(type == kF16 || type == kBF16, "window attention: f16 or bf16 heads");
+  need(fits32(p.rows) && fits32(p.sequences), "window attention: a size is negative or beyond 2^31 - 1");
+  need(p.heads >= 1 && p.kv_heads >= 1 && p.heads % p.kv_heads == 0,
+       "window attention: query heads are a multiple of the key heads");
+  layout(p.heads <= 65535, "window attention: more than 65535 heads");
+  layout(p.dim >= 8 && p.dim <= 128 && p.dim % 8 == 0, "window attention: head sizes are multiples of 8 up to 128");
+  layout(p.rows <= kMost, "window attention: more than 2^30 rows");
+  need(p.window >= 0 && p.sinks >= 0, "window attention: a negative window or number of first tokens");
+  layout(p.sinks <= kMostSinks, "window attention: more than 256 first tokens");
+  const float scale = static_cast<float>(p.scale * 1.4426950408889634);
+  need(std::isfinite(scale), "window attention: scale");
+  need(p.rows == 0 || p.starts, "window attention: null starts");
+  WindowArgs a{};
+  a.starts = p.starts;
+  a.lse = p.lse;
+  a.rows = static_cast<int32_t>(p.rows);
+  a.sequences = static_cast<int32_t>(p.sequences);
+  a.heads = static_cast<int32_t>(p.heads);
+  a.kv_heads = static_cast<int32_t>(p.kv_heads);
+  a.dim = static_cast<int32_t>(p.dim);
+  a.window = static_cast<int32_t>(p.window == 0 ? kMost : std::min(p.window, kMost));
+  a.sinks = static_cast<int32_t>(a.window >= a.rows ? 0 : p.sinks); // a window that no row leaves
+  a.scale = scale;
+  a.plain_scale = static_cast<float>(p.scale);
+  const int64_t group = p.heads / p.kv_heads, parts = (group + 15) / 16, heads = (group + parts - 1) / parts;
+  a.parts = static_cast<int32_t>((group + heads - 1) / heads);
+  a.tile_heads = make_div(heads);
+  a.tile_tokens = make_div(kTileRows / heads);
+  a.key_tokens = make_div(kTileKeys);
+  a.first_blocks = (a.sinks + 31) / 32;
+  // as many workgroups as run at a time and half as many again
+  const int64_t first = p.rows * p.kv_heads * std::max(a.first_blocks, 1) / 768;
+  a.first_tokens = make_div(std::min<int64_t>(std::max<int64_t>((first + 31) / 32 * 32, 128), 4096));
+  const auto pieces = [&](const FastDiv &size, int64_t heads_of_piece) {
+    const int64_t n = p.rows / size.d + p.sequences + 2;
+    // a workgroup of 256 threads for each, and 2^32 threads a dimension
+    layout(n * heads_of_piece < (int64_t{1} << 24) - 8, "window attention: more than 2^24 - 8 tiles of rows and heads");
+    return static_cast<int32_t>(n);
+  };
+  a.row_pieces = pieces(a.tile_tokens, p.kv_heads * a.parts);
+  a.key_pieces = pieces(a.key_tokens, p.kv_heads);
+  a.first_pieces = pieces(a.first_tokens, p.kv_heads * std::max(a.first_blocks, 1));
+  return a;
+}
+
+int64_t window_width(const WindowArgs &a) { return a.dim <= 64 ? 64 : 128; }
+size_t stats_floats(const WindowArgs &a) { return (static_cast<size_t>(a.heads) * a.rows * 2 + 3) / 4 * 4; }
+size_t window_workspace(const WindowArgs &a) {
+  const size_t first = a.sinks ? static_cast<size_t>(a.first_pieces) * a.kv_heads * a.sinks * 2 * window_width(a) : 0;
+  return (stats_floats(a) + first) * sizeof(float);
+}
+
+hipError_t window_launch(const WindowArgs &a, bool back, int type, hipStream_t s) {
+  return type == kF16 ? window_launch_f16(a, back, s) : window_launch_bf16(a, back, s);
+}
+
 } // namespace
 } // namespace relx
 
 extern "C" {
+
+int relx_window_attention(relx_ctx *ctx, const relx_window_args *args, uint64_t stream, relx_err *err) {
+  return guarded(err, [&] {
+    relx::need(args != nullptr, "null arguments");
+    int type;
+    relx::WindowArgs a = relx::window_args(*args, type);
+    const bool used = a.rows > 0;
+    a.q = relx::rows_of(&args->q, used, a.rows, a.heads, "window attention: null queries");
+    a.k = relx::rows_of(&args->k, used, a.rows, a.kv_heads, "window attention: null keys");
+    a.v = relx::rows_of(&args->v, used, a.rows, a.kv_heads, "window attention: null values");
+    a.o = relx::rows_of(&args->out, used, a.rows, a.heads, "window attention: null result");
+    relx::writable(&args->out, a.rows, a.heads, a.dim);
+    relx::on_context(ctx, [&] {
+      if (used)
+        relx::launched(relx::window_launch(a, false, type, relx::stream_of(stream)), "window attention");
+    });
+  });
+}
+
+int relx_window_attention_workspace(const relx_window_args *args, size_t *bytes, relx_err *err) {
+  return guarded(err, [&] {
+    relx::need(args && bytes, "null arguments");
+    relx_window_args p = *args;
+    p.starts = reinterpret_cast<const int32_t *>(&p); // not read: only sizes count
+    int type;
+    *bytes = relx::window_workspace(relx::window_args(p, type));
+  });
+}
+
+int relx_window_attention_backward(relx_ctx *ctx, const relx_window_args *args, const relx_heads *out_grad,
+                                   const relx_heads *q_grad, const relx_heads *k_grad, const relx_heads *v_grad,
+                                   void *workspace, size_t workspace_bytes, uint64_t stream, relx_err *err) {
+  return guarded(err, [&] {
+    relx::need(args != nullptr, "null arguments");
+    int type;
+    relx::WindowArgs a = relx::window_args(*args, type);
+    const bool used = a.rows > 0;
+    a.q = relx::rows_of(&args->q, used, a.rows, a.heads, "window attention: null queries");
+    a.k = relx::rows_of(&args->k, used, a.rows, a.kv_heads, "window attention: null keys");
+    a.v = relx::rows_of(&args->v, used, a.rows, a.kv_heads, "window attention: null values");
+    a.o = relx::rows_of(&args->out, used, a.rows, a.heads, "window attention: null result");
+    a.dout = relx::rows_of(out_grad, used, a.rows, a.heads, "window attention: null result's gradient");
+    a.dq = relx::rows_of(q_grad, used, a.rows, a.heads, "window attention: null query gradient");
+    a.dk = relx::rows_of(k_grad, used, a.rows, a.kv_heads, "window attention: null key gradient");
+    a.dv = relx::rows_of(v_grad, used, a.rows, a.kv_heads, "window attention: null value gradient");
+    relx::writable(q_grad, a.rows, a.heads, a.dim);
+    relx::writable(k_grad, a.rows, a.kv_heads, a.dim);
+    relx::writable(v_grad, a.rows, a.kv_heads, a.dim);
+    relx::need(!used || a.lse, "window attention: the backward takes lse");
+    const size_t want = relx::window_workspace(a);
+    if (used && (workspace_bytes < want || !workspace))
+      throw relx::Error("insufficient_capacity", "workspace holds " + std::to_string(workspace_bytes) +
+                                                     " bytes, the call takes " + std::to_string(want));
+    relx::need(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "window attention: workspace alignment");
+    a.stats = static_cast<float *>(workspace);
+    a.first_sums = a.stats + relx::stats_floats(a);
+    relx::on_context(ctx, [&] {
+      if (used)
+        relx::launched(relx::window_launch(a, true, type, relx::stream_of(stream)), "window attention, backward");
+    });
+  });
+}
 
 int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_t stream, relx_err *err) {
   return guarded(err, [&] {
