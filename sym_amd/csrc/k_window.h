@@ -565,13 +565,15 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
 // Otherwise from the rows in whose windows a tile of 128 keys is.
 template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2) void k_window_dkv(WindowArgs a) {
   constexpr int RB = DP * 2, TILE = 32 * RB, E = DP / 32, KS = DP / 16, KEYS = 32 * kWaves;
-  constexpr int RING = FIRST ? 1 : 4;          // tiles at a time; FIRST: of each wave
-  constexpr int SLOTS = FIRST ? kWaves : RING;
+  constexpr bool SHARED = DP == 128;           // values in shared memory: registers do not hold them beside the sums
+  constexpr int RING = FIRST || SHARED ? 2 : 4; // tiles at a time; FIRST: of each wave
+  constexpr int SLOTS = FIRST ? kWaves * RING : RING;
   constexpr int NT = FIRST ? 32 : 32 / kWaves; // tokens that a wave brings
   using Loads = Bring<DP, NT>;
   constexpr int ROOM = SLOTS * 2 * TILE;
   __shared__ __attribute__((aligned(256))) char tiles[ROOM];
   __shared__ __attribute__((aligned(16))) float stats[SLOTS][32][2];
+  __shared__ __attribute__((aligned(256))) char values[SHARED ? (FIRST ? 32 : KEYS) * RB : 16];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int group = a.heads / a.kv_heads;
   const Work w = my_work(FIRST ? a.first_pieces : a.key_pieces, FIRST ? a.kv_heads * a.first_blocks : a.kv_heads);
@@ -625,15 +627,21 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
   u32x4 k[KS], v[KS];
   take_row<DP>(k, a.k.data + (key_row * a.k.row + kv * a.k.head) * 2, a.dim, lane);
   take_row<DP>(v, a.v.data + (key_row * a.v.row + kv * a.v.head) * 2, a.dim, lane);
+  const uint32_t direct = direct_at<RB>(lane), turn0 = turned_at<RB>(lane, 0), turn1 = turned_at<RB>(lane, 1);
+  const uint32_t values_at = place(values) + (FIRST ? 0 : wave * 32 * RB) + direct;
 #pragma unroll
-  for (int s = 0; s < KS; ++s)
-    asm volatile("" : "+v"(k[s]), "+v"(v[s]));
+  for (int s = 0; s < KS; ++s) {
+    if constexpr (SHARED) // FIRST: the same by all waves
+      *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>(values_at ^ (s * 32)) = v[s];
+    asm volatile("" : "+v"(k[s]));
+    if constexpr (!SHARED)
+      asm volatile("" : "+v"(v[s]));
+  }
   Over<T, E> over;
   f32x16 dk[E], dv[E];
 #pragma unroll
   for (int m = 0; m < E; ++m)
     dk[m] = dv[m] = zero16();
-  const uint32_t direct = direct_at<RB>(lane), turn0 = turned_at<RB>(lane, 0), turn1 = turned_at<RB>(lane, 1);
 
   auto take_in = [&](int p, int slot) {
     const uint32_t tq = at + slot * 2 * TILE, tg = tq + TILE;
@@ -643,7 +651,7 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
       s = mfma32<T>(read16(tq + direct ^ (i * 32)), k[i], s);
 #pragma unroll
     for (int i = 0; i < KS; ++i)
-      dp = mfma32<T>(read16(tg + direct ^ (i * 32)), v[i], dp);
+      dp = mfma32<T>(read16(tg + direct ^ (i * 32)), SHARED ? read16(values_at ^ (i * 32)) : v[i], dp);
     const uint32_t st = stats_at + slot * 256 + (lane >> 5) * 32;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -687,12 +695,19 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
   };
 
   if constexpr (FIRST) {
-    for (int n = wave; n < count; n += kWaves) { // tiles of its own
-      send(n, wave);
-      arrived<0>();
-      const int p = p0 + n % per * 32;
-      take_in(p, wave);
-      shared_done();
+    int slot = wave * RING;
+    if (wave < count)
+      send(wave, slot);
+#pragma clang loop unroll(disable)
+    for (int n = wave; n < count; n += kWaves, slot ^= 1) { // tiles of its own
+      if (n + kWaves < count) {
+        send(n + kWaves, slot ^ 1);
+        arrived<SENT>();
+      } else {
+        arrived<0>();
+      }
+      take_in(p0 + n % per * 32, slot);
+      shared_done(); // its place is free
     }
   } else {
     for (int n = 0; n < min(count, RING - 1); ++n)
