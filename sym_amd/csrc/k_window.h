@@ -45,7 +45,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 4;
-constexpr int kKeys = 64; // tokens of a tile of keys
+constexpr int kAhead = 4; // reads of shared memory ahead of their product
 
 template <int T> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (T == kF16)
@@ -93,10 +93,10 @@ __device__ __forceinline__ Piece find(const WindowArgs &a, FastDiv size, int num
     hi = min(hi, lo + step);
   }
   Piece p;
-  p.begin = st;
-  p.n = max(en - st, 0);
-  p.number = lo;
-  p.index = number - static_cast<int>(fdiv(static_cast<uint32_t>(st), size)) - lo;
+  p.begin = uniform(st);
+  p.n = uniform(max(en - st, 0));
+  p.number = uniform(lo);
+  p.index = uniform(number - static_cast<int>(fdiv(static_cast<uint32_t>(st), size)) - lo);
   p.real = lo > 0 && lo < many - 1;
   if (p.index < 0 || static_cast<int64_t>(p.index) * size.d >= p.n)
     p.n = 0;
@@ -216,7 +216,7 @@ __device__ __forceinline__ void put_row(char *row, const f32x16 (&acc)[DP / 32],
 // f16 has few bits for small numbers: P is taken 2^10 times as large (it is at
 // most one), and dS over a power of two that holds the largest so far, of which
 // the sums then are.
-template <int T> constexpr float kMore() { return T == kF16 ? 10.0f : 0.0f; }
+constexpr float kMore = 10.0f;
 template <int T> __device__ __forceinline__ constexpr float less() { return T == kF16 ? 0.0009765625f : 1.0f; }
 template <int T, int E> struct Over {
   int e = 1; // exponent of the power of two, as a float holds it
@@ -272,15 +272,15 @@ struct MyRow {
 
 // The tiles of keys that a tile of rows reads: those with first tokens, then those
 // of its rows' windows.
-struct KeyTiles {
+template <int KEYS> struct KeyTiles {
   int first, jump, count;
   __device__ __forceinline__ KeyTiles(const WindowArgs &a, int from_row, int to_row) {
-    const int from = max(from_row - a.window + 1, 0) / kKeys;
-    first = min((a.sinks + kKeys - 1) / kKeys, from);
+    const int from = max(from_row - a.window + 1, 0) / KEYS;
+    first = min((a.sinks + KEYS - 1) / KEYS, from);
     jump = from - first;
-    count = to_row / kKeys - jump + 1;
+    count = to_row / KEYS - jump + 1;
   }
-  __device__ __forceinline__ int token(int n) const { return (n < first ? n : n + jump) * kKeys; }
+  __device__ __forceinline__ int token(int n) const { return (n < first ? n : n + jump) * KEYS; }
 };
 // Whether rows from p0 to p1 see none, or all, of the tokens from x0 to x1.
 __device__ __forceinline__ bool see_none(const WindowArgs &a, int p0, int p1, int x0, int x1) {
@@ -288,6 +288,25 @@ __device__ __forceinline__ bool see_none(const WindowArgs &a, int p0, int p1, in
 }
 __device__ __forceinline__ bool see_all(const WindowArgs &a, int p0, int p1, int x0, int x1) {
   return x1 <= p0 && (p1 - x0 < a.window || x1 < a.sinks);
+}
+
+// Puts `none` in the place of what a lane's row does not see of the 32 tokens from
+// x. Compares and selects only: as branches, which the compiler makes of conditions
+// that are read one after the other, a tile with an edge took three times as long.
+__device__ __forceinline__ void hide(const WindowArgs &a, f32x16 &s, int row, int x, int first_row, int last_row, int lane, float none) {
+  const int at = x + 4 * (lane >> 5);
+  if (x + 31 > first_row) {
+    const int most = row - at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = row_of(i, 0) > most ? none : s[i];
+  }
+  if (x <= last_row - a.window) {
+    const int upto = row - a.window - at, stay = a.sinks - at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = (row_of(i, 0) <= upto) & (row_of(i, 0) >= stay) ? none : s[i];
+  }
 }
 
 // Rows of no sequence: zeros.
@@ -302,8 +321,12 @@ __device__ __forceinline__ void zero_rows(const WindowArgs &a, const Heads &h, i
 
 // ------------------------------------------------------------ forward
 
-template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_window_forward(WindowArgs a) {
-  constexpr int RB = DP * 2, TILE = kKeys * RB, E = DP / 32, KS = DP / 16, RING = 2;
+// Three waves a SIMD, for which a head of 128 takes 32 tokens at a time: 497 us
+// against 536 with 64 and two waves (24.6k rows of 32 + 8 heads, window 1024).
+template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 3) void k_window_forward(WindowArgs a) {
+  constexpr int KEYS = DP == 128 ? 32 : 64, B = KEYS / 32; // tokens of a tile
+  constexpr int RB = DP * 2, TILE = KEYS * RB, E = DP / 32, KS = DP / 16, RING = DP == 128 ? 3 : 2;
+  using Loads = Bring<DP, KEYS / kWaves>;
   __shared__ __attribute__((aligned(256))) char tiles[RING][2][TILE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const Work w = my_work(a.row_pieces, a.kv_heads * a.parts);
@@ -326,19 +349,20 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
     __syncthreads();
   }
   const int last = rows.first + rows.tokens - 1;
-  const KeyTiles keys(a, rows.first, last);
+  const KeyTiles<KEYS> keys(a, rows.first, last);
   const int kv = w.head / a.parts;
   const char *k0 = a.k.data + (static_cast<int64_t>(piece.begin) * a.k.row + kv * a.k.head) * 2;
   const char *v0 = a.v.data + (static_cast<int64_t>(piece.begin) * a.v.row + kv * a.v.head) * 2;
   const uint32_t krow = static_cast<uint32_t>(a.k.row) * 2, vrow = static_cast<uint32_t>(a.v.row) * 2;
-  const Bring<DP, kKeys / kWaves> bring(lane, wave * (kKeys / kWaves), a.dim);
+  const Loads bring(lane, wave * (KEYS / kWaves), a.dim);
   const uint32_t at = place(&tiles[0][0][0]);
   auto send = [&](int n, int slot) {
     const int x = keys.token(n);
     bring.send(k0 + static_cast<int64_t>(x) * krow, krow, piece.n - x, at + slot * 2 * TILE);
     bring.send(v0 + static_cast<int64_t>(x) * vrow, vrow, piece.n - x, at + slot * 2 * TILE + TILE);
   };
-  send(0, 0);
+  for (int n = 0; n < min(keys.count, RING - 1); ++n)
+    send(n, n);
 
   const MyRow row(a, rows, wave * 32 + (lane & 31));
   const int first_row = uniform(MyRow(a, rows, wave * 32).token), last_row = uniform(MyRow(a, rows, wave * 32 + 31).token);
@@ -362,37 +386,49 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
   const uint32_t direct = direct_at<RB>(lane), turn0 = turned_at<RB>(lane, 0), turn1 = turned_at<RB>(lane, 1);
 
 #pragma clang loop unroll(disable)
-  for (int n = 0; n < keys.count; ++n) {
-    const int slot = n & 1, x = keys.token(n);
-    arrived<0>();
+  for (int n = 0, next = 0; n < keys.count; ++n) {
+    const int slot = next, x = keys.token(n);
+    next = slot + 1 == RING ? 0 : slot + 1;
+    if (n + RING - 2 < keys.count)
+      arrived<(RING - 2) * 2 * Loads::LOADS>();
+    else
+      arrived<0>();
     meet(); // the tile is there, and everybody has read the one before
-    if (n + 1 < keys.count)
-      send(n + 1, slot ^ 1);
-    if (!busy || see_none(a, first_row, last_row, x, x + kKeys - 1))
+    if (n + RING - 1 < keys.count)
+      send(n + RING - 1, slot == 0 ? RING - 1 : slot - 1);
+    if (!busy || see_none(a, first_row, last_row, x, x + KEYS - 1))
       continue;
     const uint32_t tk = at + slot * 2 * TILE + direct, tv = at + slot * 2 * TILE + TILE;
-    f32x16 s[2];
+    f32x16 s[B];
+    // reads go out ahead of their products, in this order: see dK and dV
+    auto operand = [&](int n) {
+      const int b = n / KS % B, i = n % KS, m = i / 2 * 64, tokens = (b * 32 + i % 2 * 16) * RB;
+      return n < B * KS ? read16((tk ^ (i * 32)) + b * 32 * RB)
+                        : turned((tv + turn0 ^ m) + tokens, (tv + turn1 ^ m) + tokens);
+    };
+    u32x4 ahead[kAhead];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int n = 0; n < kAhead; ++n)
+      ahead[n] = operand(n);
+    keep_order();
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
       s[b] = zero16();
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        s[b] = mfma32<T>(read16((tk ^ (i * 32)) + b * 32 * RB), q[i], s[b]);
+      for (int i = 0; i < KS; ++i) {
+        s[b] = mfma32<T>(ahead[i % kAhead], q[i], s[b]);
+        ahead[i % kAhead] = operand(b * KS + i + kAhead);
+        keep_order();
+      }
     }
-    if (!see_all(a, first_row, last_row, x, x + kKeys - 1)) {
-      const int from = row.token - a.window;
+    if (!see_all(a, first_row, last_row, x, x + KEYS - 1)) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int y = x + 32 * b + row_of(i, lane);
-          if (y > row.token || (y <= from && y >= a.sinks))
-            s[b][i] = -__builtin_inff();
-        }
+      for (int b = 0; b < B; ++b)
+        hide(a, s[b], row.token, x + 32 * b, first_row, last_row, lane, -__builtin_inff());
     }
     float most = s[0][0];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < B; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         most = fmaxf(most, s[b][i]);
@@ -408,7 +444,7 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
         acc[m] *= shrink;
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < B; ++b) {
       float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -419,12 +455,11 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
       u32x4 p[2];
       pack_operands<T>(s[b], p);
 #pragma unroll
-      for (int m = 0; m < E; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tokens = (b * 32 + h * 16) * RB;
-          acc[m] = mfma32<T>(turned((tv + turn0 ^ (m * 64)) + tokens, (tv + turn1 ^ (m * 64)) + tokens), p[h], acc[m]);
-        }
+      for (int i = 0; i < 2 * E; ++i) {
+        acc[i / 2] = mfma32<T>(ahead[i % kAhead], p[i % 2], acc[i / 2]);
+        if (b * KS + i + kAhead < B * KS)
+          ahead[i % kAhead] = operand((B + b) * KS + i + kAhead);
+      }
     }
   }
   arrived<0>();
@@ -440,6 +475,7 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
 // ------------------------------------------------------------ dQ
 
 template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_window_dq(WindowArgs a) {
+  constexpr int kKeys = 64; // tokens of a tile
   constexpr int RB = DP * 2, TILE = kKeys * RB, E = DP / 32, KS = DP / 16, RING = 2;
   __shared__ __attribute__((aligned(256))) char tiles[RING][2][TILE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -459,7 +495,7 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
     __syncthreads();
   }
   const int last = rows.first + rows.tokens - 1;
-  const KeyTiles keys(a, rows.first, last);
+  const KeyTiles<kKeys> keys(a, rows.first, last);
   const int kv = w.head / a.parts;
   const char *k0 = a.k.data + (static_cast<int64_t>(piece.begin) * a.k.row + kv * a.k.head) * 2;
   const char *v0 = a.v.data + (static_cast<int64_t>(piece.begin) * a.v.row + kv * a.v.head) * 2;
@@ -494,9 +530,9 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
   d += __shfl_xor(d, 32);
   const float lse = a.lse[static_cast<int64_t>(row.head) * a.rows + at_row] * 1.44269504088896341f;
   if (row.there && lane < 32) {
-    float *to = a.stats + (static_cast<int64_t>(row.head) * a.rows + at_row) * 2;
-    to[0] = lse;
-    to[1] = d;
+    float *to = a.stats + static_cast<int64_t>(row.head) * a.rows + at_row;
+    to[0] = -lse / a.scale;
+    to[static_cast<int64_t>(a.heads) * a.rows] = -d;
   }
 #pragma unroll
   for (int s = 0; s < KS; ++s)
@@ -521,37 +557,51 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
     const bool cut = !see_all(a, first_row, last_row, x, x + kKeys - 1);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      if (DP == 128 && see_none(a, first_row, last_row, x + 32 * b, x + 32 * b + 31))
+        continue; // heads of 64 have too little to gain
       f32x16 s = zero16(), dp = zero16();
+      auto operand = [&](int n) {
+        const int i = n % KS, m = i / 2 * 64, tokens = (b * 32 + i % 2 * 16) * RB;
+        return n < KS       ? read16((tk + direct ^ (i * 32)) + b * 32 * RB)
+               : n < 2 * KS ? read16((tv + direct ^ (i * 32)) + b * 32 * RB)
+                            : turned((tk + turn0 ^ m) + tokens, (tk + turn1 ^ m) + tokens);
+      };
+      u32x4 ahead[kAhead];
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        s = mfma32<T>(read16((tk + direct ^ (i * 32)) + b * 32 * RB), q[i], s);
+      for (int n = 0; n < kAhead; ++n)
+        ahead[n] = operand(n);
+      keep_order();
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        dp = mfma32<T>(read16((tv + direct ^ (i * 32)) + b * 32 * RB), g[i], dp);
+      for (int i = 0; i < KS; ++i) {
+        s = mfma32<T>(ahead[i % kAhead], q[i], s);
+        ahead[i % kAhead] = operand(i + kAhead);
+        keep_order();
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        dp = mfma32<T>(ahead[i % kAhead], g[i], dp);
+        ahead[i % kAhead] = operand(KS + i + kAhead);
+#pragma unroll
+        for (int n = 16 / KS * i; n < 16 / KS * (i + 1); ++n)
+          s[n] = __builtin_amdgcn_exp2f(s[n] * a.scale - lse);
+        keep_order();
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale - lse) * (dp[i] - d);
-      if (cut) {
-        const int from = row.token - a.window;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int y = x + 32 * b + row_of(i, lane);
-          if (y > row.token || (y <= from && y >= a.sinks))
-            s[i] = 0.0f;
-        }
-      }
+        s[i] *= dp[i] - d;
+      if (cut)
+        hide(a, s, row.token, x + 32 * b, first_row, last_row, lane, 0.0f);
       over.hold(s, acc);
       if constexpr (T == kF16)
         s *= over.down();
       u32x4 p[2];
       pack_operands<T>(s, p);
 #pragma unroll
-      for (int m = 0; m < E; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int tokens = (b * 32 + h * 16) * RB;
-          acc[m] = mfma32<T>(turned((tk + turn0 ^ (m * 64)) + tokens, (tk + turn1 ^ (m * 64)) + tokens), p[h], acc[m]);
-        }
+      for (int i = 0; i < 2 * E; ++i) {
+        acc[i / 2] = mfma32<T>(ahead[i % kAhead], p[i % 2], acc[i / 2]);
+        if (i + kAhead < KS)
+          ahead[i % kAhead] = operand(2 * KS + i + kAhead);
+      }
     }
   }
   arrived<0>();
@@ -561,19 +611,21 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
 
 // ------------------------------------------------------------ dK and dV
 
+// A wave's keys stay in registers with their gradients' sums, its values in shared
+// memory: both in registers left too few (1842 us against 1396 with heads of 128;
+// 1422 against 1378 for a step with heads of 64, which three waves a SIMD fit so).
 // FIRST: the first tokens' gradients from the rows whose window has left them.
 // Otherwise from the rows in whose windows a tile of 128 keys is.
-template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2) void k_window_dkv(WindowArgs a) {
+template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(WindowArgs a) {
   constexpr int RB = DP * 2, TILE = 32 * RB, E = DP / 32, KS = DP / 16, KEYS = 32 * kWaves;
-  constexpr bool SHARED = DP == 128;           // values in shared memory: registers do not hold them beside the sums
-  constexpr int RING = FIRST || SHARED ? 2 : 4; // tiles at a time; FIRST: of each wave
+  constexpr int RING = FIRST || DP == 128 ? 2 : 3; // tiles at a time; FIRST: of each wave
   constexpr int SLOTS = FIRST ? kWaves * RING : RING;
   constexpr int NT = FIRST ? 32 : 32 / kWaves; // tokens that a wave brings
   using Loads = Bring<DP, NT>;
   constexpr int ROOM = SLOTS * 2 * TILE;
   __shared__ __attribute__((aligned(256))) char tiles[ROOM];
-  __shared__ __attribute__((aligned(16))) float stats[SLOTS][32][2];
-  __shared__ __attribute__((aligned(256))) char values[SHARED ? (FIRST ? 32 : KEYS) * RB : 16];
+  __shared__ __attribute__((aligned(16))) float stats[SLOTS][2][32];
+  __shared__ __attribute__((aligned(256))) char values[(FIRST ? 32 : KEYS) * RB];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int group = a.heads / a.kv_heads;
   const Work w = my_work(FIRST ? a.first_pieces : a.key_pieces, FIRST ? a.kv_heads * a.first_blocks : a.kv_heads);
@@ -610,15 +662,18 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
   const Loads bring(lane, FIRST ? 0 : wave * NT, a.dim);
   const uint32_t at = place(tiles), stats_at = place(reinterpret_cast<const char *>(&stats[0][0][0]));
   const uint32_t qrow = static_cast<uint32_t>(a.q.row) * 2, grow = static_cast<uint32_t>(a.dout.row) * 2;
+  const uint32_t stats_apart = static_cast<uint32_t>(a.heads) * static_cast<uint32_t>(a.rows); // -lse / scale, then -D
   auto send = [&](int n, int slot) {
     const int h = n / per, p = p0 + (n - h * per) * 32, head = kv * group + h;
     const int64_t row = static_cast<int64_t>(piece.begin) + p;
     bring.send(a.q.data + (row * a.q.row + head * a.q.head) * 2, qrow, piece.n - p, at + slot * 2 * TILE);
     bring.send(a.dout.data + (row * a.dout.row + head * a.dout.head) * 2, grow, piece.n - p, at + slot * 2 * TILE + TILE);
-    const int t = (FIRST ? 0 : wave * NT) + (lane >> 1);
-    if (lane < 2 * NT)
-      load_async4(a.stats + (static_cast<int64_t>(head) * a.rows + row) * 2, (min(t, piece.n - p - 1) * 2 + (lane & 1)) * 4,
-                  stats_at + slot * 256 + (FIRST ? 0 : wave * NT) * 8);
+    // 64 numbers of the tile's rows: each wave a quarter, FIRST: all
+    const int number = FIRST ? lane : wave * 16 + lane;
+    if (FIRST || lane < 16)
+      load_async4(a.stats + static_cast<int64_t>(head) * a.rows + row,
+                  (static_cast<uint32_t>(min(number & 31, piece.n - p - 1)) + (number < 32 ? 0u : stats_apart)) * 4,
+                  stats_at + slot * 256 + (FIRST ? 0 : wave * 64));
   };
   constexpr int SENT = 2 * Loads::LOADS + 1;
 
@@ -631,11 +686,9 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
   const uint32_t values_at = place(values) + (FIRST ? 0 : wave * 32 * RB) + direct;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    if constexpr (SHARED) // FIRST: the same by all waves
-      *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>(values_at ^ (s * 32)) = v[s];
+    // FIRST: the same by all waves
+    *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>(values_at ^ (s * 32)) = v[s];
     asm volatile("" : "+v"(k[s]));
-    if constexpr (!SHARED)
-      asm volatile("" : "+v"(v[s]));
   }
   Over<T, E> over;
   f32x16 dk[E], dv[E];
@@ -643,55 +696,95 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
   for (int m = 0; m < E; ++m)
     dk[m] = dv[m] = zero16();
 
+  // Reads of shared memory go out a product or more ahead of their use, each where
+  // the product before has freed its registers, and the order is kept: left to
+  // itself the compiler, short of registers, waits for each read where it uses it.
   auto take_in = [&](int p, int slot) {
-    const uint32_t tq = at + slot * 2 * TILE, tg = tq + TILE;
-    f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-      s = mfma32<T>(read16(tq + direct ^ (i * 32)), k[i], s);
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-      dp = mfma32<T>(read16(tg + direct ^ (i * 32)), SHARED ? read16(values_at ^ (i * 32)) : v[i], dp);
-    const uint32_t st = stats_at + slot * 256 + (lane >> 5) * 32;
+    const uint32_t tq = at + slot * 2 * TILE, tg = tq + TILE, st = stats_at + slot * 256 + (lane >> 5) * 16;
+    // S and dP begin with -lse / scale and -D of their rows
+    f32x16 s, dp;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const u32x4 one = read16(st + i * 64), two = read16(st + i * 64 + 16);
+      const u32x4 x = read16(st + i * 32);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float lse = __uint_as_float(r < 2 ? one[2 * r] : two[2 * r - 4]);
-        const float d = __uint_as_float(r < 2 ? one[2 * r + 1] : two[2 * r - 3]);
-        s[4 * i + r] = __builtin_amdgcn_exp2f(s[4 * i + r] * a.scale - lse + kMore<T>());
-        dp[4 * i + r] -= d;
-      }
+      for (int r = 0; r < 4; ++r)
+        s[4 * i + r] = __uint_as_float(x[r]);
+    }
+    auto operand = [&](int n) {
+      const int i = n % KS, m = i / 2 * 64, tokens = i % 2 * 16 * RB;
+      return n < KS       ? read16(tq + direct ^ (i * 32))
+             : n < 2 * KS ? read16(tg + direct ^ (i * 32))
+             : n < 3 * KS ? turned((tg + turn0 ^ m) + tokens, (tg + turn1 ^ m) + tokens)
+                          : turned((tq + turn0 ^ m) + tokens, (tq + turn1 ^ m) + tokens);
+    };
+    u32x4 ahead[kAhead], w[2];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n)
+      ahead[n] = operand(n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const u32x4 x = read16(st + 128 + i * 32);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        dp[4 * i + r] = __uint_as_float(x[r]);
+    }
+    keep_order();
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      s = mfma32<T>(ahead[i % kAhead], k[i], s);
+      ahead[i % kAhead] = operand(i + kAhead);
+      if (i >= KS - 2)
+        w[i - KS + 2] = read16(values_at ^ ((i - KS + 2) * 32));
+      keep_order();
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      dp = mfma32<T>(ahead[i % kAhead], w[i % 2], dp);
+      ahead[i % kAhead] = operand(KS + i + kAhead);
+      if (i + 2 < KS)
+        w[i % 2] = read16(values_at ^ ((i + 2) * 32));
+#pragma unroll
+      for (int n = 16 / KS * i; n < 16 / KS * (i + 1); ++n)
+        s[n] = __builtin_amdgcn_exp2f(T == kF16 ? s[n] * a.scale + kMore : s[n] * a.scale);
+      keep_order();
     }
     const bool whole = p + 31 < p1 && (FIRST ? x_last < a.sinks && p - x_last >= a.window
                                              : x_last <= p && p + 31 - x_first < a.window);
     if (!whole) {
+      // the rows from `low` on and before `high` see the lane's key
+      const int at_row = p + 4 * (lane >> 5);
+      const int low = (FIRST ? key < a.sinks ? key + a.window : p1 : key) - at_row;
+      const int high = (FIRST ? p1 : static_cast<int>(min(static_cast<int64_t>(p1), static_cast<int64_t>(key) + a.window))) - at_row;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int y = p + row_of(i, lane);
-        const bool sees = FIRST ? key < a.sinks && y - key >= a.window : key <= y && y - key < a.window;
-        if (!sees || y >= p1)
-          s[i] = 0.0f, dp[i] = 0.0f;
+        const bool sees = (row_of(i, 0) >= low) & (row_of(i, 0) < high);
+        s[i] = sees ? s[i] : 0.0f;
+        dp[i] = sees ? dp[i] : 0.0f;
       }
     }
-    u32x4 w2[2];
-    pack_operands<T>(s, w2);
+    u32x4 p2[2];
+    pack_operands<T>(s, p2);
+    keep_order();
 #pragma unroll
-    for (int m = 0; m < E; ++m)
+    for (int i = 0; i < 2 * E; ++i) {
+      dv[i / 2] = mfma32<T>(ahead[i % kAhead], p2[i % 2], dv[i / 2]);
+      ahead[i % kAhead] = operand(2 * KS + i + kAhead);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        dv[m] = mfma32<T>(turned((tg + turn0 ^ (m * 64)) + h * 16 * RB, (tg + turn1 ^ (m * 64)) + h * 16 * RB), w2[h], dv[m]);
-    s *= dp;
+      for (int n = 16 / KS * i; n < 16 / KS * (i + 1); ++n)
+        s[n] *= dp[n];
+      keep_order();
+    }
     over.hold(s, dk);
     if constexpr (T == kF16)
       s *= over.down();
-    pack_operands<T>(s, w2);
+    pack_operands<T>(s, p2);
 #pragma unroll
-    for (int m = 0; m < E; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        dk[m] = mfma32<T>(turned((tq + turn0 ^ (m * 64)) + h * 16 * RB, (tq + turn1 ^ (m * 64)) + h * 16 * RB), w2[h], dk[m]);
+    for (int i = 0; i < 2 * E; ++i) {
+      dk[i / 2] = mfma32<T>(ahead[i % kAhead], p2[i % 2], dk[i / 2]);
+      if (i + kAhead < KS)
+        ahead[i % kAhead] = operand(3 * KS + i + kAhead);
+      keep_order();
+    }
   };
 
   if constexpr (FIRST) {
@@ -723,7 +816,7 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, 2
       if (n + RING - 1 < count)
         send(n + RING - 1, slot == 0 ? RING - 1 : slot - 1);
       const int p = p0 + in_head * 32;
-      if (!(p + 31 < x_first || p - x_last >= a.window))
+      if (p + 31 >= x_first && p - x_last < a.window)
         take_in(p, slot);
       slot = slot + 1 == RING ? 0 : slot + 1;
       in_head = in_head + 1 == per ? 0 : in_head + 1;

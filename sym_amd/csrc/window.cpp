@@ -125,7 +125,9 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   a.dim = static_cast<int32_t>(p.dim);
   a.window = static_cast<int32_t>(p.window == 0 ? kMost : std::min(p.window, kMost));
   a.sinks = static_cast<int32_t>(a.window >= a.rows ? 0 : p.sinks); // a window that no row leaves
-  a.scale = scale;
+  // By a scale below 2^-64 no score within f16's and bf16's usual range reaches a
+  // bit of a weight: then 2^-64, by which the kernels divide.
+  a.scale = std::fabs(scale) < 0x1p-64f ? std::copysign(0x1p-64f, scale) : scale;
   a.plain_scale = static_cast<float>(p.scale);
   const int64_t group = p.heads / p.kv_heads, parts = (group + 15) / 16, heads = (group + parts - 1) / parts;
   a.parts = static_cast<int32_t>((group + heads - 1) / heads);
