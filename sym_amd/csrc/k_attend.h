@@ -954,6 +954,37 @@ template <int FORM, int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE>
     }
   }
 
+  // The wave's tokens of an int8 tile, keys and values; and as T in another tile.
+  // Lanes that bring none read another place of the tile.
+  struct Codes {
+    u32x4 part[2][LOADS];
+  };
+  __device__ __forceinline__ Codes codes(uint32_t from, int lane) const {
+    Codes c;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        c.part[kv][i] = read16(from + kv * kTile * DP + piece<RB>((first + i * TPI + token) % kTile, lane % TL));
+    return c;
+  }
+  __device__ __forceinline__ void widen(const Codes &c, uint32_t to, int lane) const {
+    constexpr int WB = DP * 2;
+    typedef __attribute__((address_space(3))) u32x4 *Place;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int t = first + i * TPI + token, n = lane % TL;
+      if (NT >= TPI || token < NT)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const u32x4 b = c.part[kv][i];
+          const uint32_t at = to + kv * kTile * WB;
+          *reinterpret_cast<Place>(at + piece<WB>(t, 2 * n)) = widen8<T>(b.x, b.y);
+          *reinterpret_cast<Place>(at + piece<WB>(t, 2 * n + 1)) = widen8<T>(b.z, b.w);
+        }
+    }
+  }
+
   // Through registers: the wave's tokens of the tile at x.
   __device__ __forceinline__ void fetch(int place) {
     const int x = token_of(place);
@@ -1210,10 +1241,16 @@ template <int FORM, int T, bool I8, int DP, int RT, int W, int SRC>
 __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   constexpr int ROWS = 16 * RT * W, E = DP / 16, UNIT = kSharedUnit;
   constexpr int TILE = kTile * DP * 2;
+  // int8 on its way by itself: a ring of tiles as they lie in the cache, of which a
+  // wave widens the tokens that it has brought, into the other of two tiles
+  constexpr bool WIDEN = I8 && SRC == kAsync;
   // tiles at a time: 64 KiB for each four waves
-  constexpr int RING = SRC != kAsync ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
-  using Load = Loader<FORM, T, I8, DP, SRC, kTile / W, false, kTile>;
+  constexpr int RING = SRC != kAsync || WIDEN ? 2 : 16 * 1024 * W / (2 * TILE) < 8 ? 16 * 1024 * W / (2 * TILE) : 8;
+  constexpr int RAW = WIDEN ? (DP <= 128 ? 5 : 2) : 1; // tiles of int8
+  using Load = Loader<FORM, T, I8, DP, SRC, kTile / W, WIDEN, kTile>;
   __shared__ int entries[SRC == kAsync ? W : 1][2][64];
+  __shared__ float block_scales[FORM == kBlocks && SRC == kAsync ? W : 1][2][2][64];
+  __shared__ __attribute__((aligned(16))) char raw[RAW][2][WIDEN ? kTile * DP : 16];
 
   __shared__ Schedule schedule;
   __shared__ __attribute__((aligned(16))) char tiles[RING][2][TILE];
@@ -1223,6 +1260,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   Load load(a, lane, wave * (kTile / W));
   load.room = place(reinterpret_cast<const char *>(&entries[SRC == kAsync ? wave : 0][0][0]));
+  if constexpr (FORM == kBlocks)
+    load.scale_room = place(reinterpret_cast<const char *>(&block_scales[SRC == kAsync ? wave : 0][0][0][0]));
   // A tile's values are read ahead of the softmax, where the registers hold them:
   // 77 us against 81 for 8 requests of 256 rows over up to 8192 tokens of 8 key
   // heads of 128, 280 against 287 up to 32768 (the fastest of 40). The same for the
@@ -1237,6 +1276,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
   if (SRC == kAsync && a.dim < DP) // places past the head's dims: no load writes them
     for (int i = tid * 16; i < RING * 2 * TILE; i += 64 * W * 16)
       *reinterpret_cast<u32x4 *>(&tiles[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
+  if (WIDEN && a.dim < DP)
+    for (int i = tid * 16; i < static_cast<int>(sizeof(raw)); i += 64 * W * 16)
+      *reinterpret_cast<u32x4 *>(&raw[0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
 
   for (int turn = 0; run.unit < run.end; turn ^= 1) {
     const Item it = take<FORM, ROWS, UNIT>(args_again(), schedule, run);
@@ -1272,7 +1314,60 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
         r.start(b, it, row0, rows, I8 && FORM != kBlocks ? b.scale * b.key_scale[it.head] : b.scale, lane);
       };
 
-      if constexpr (SRC == kAsync) {
+      if constexpr (WIDEN) {
+        uint32_t on = 0u; // of this tile and those on their way: their halves on a page
+        const uint32_t raw_at = place(raw[0][0]);
+        auto send = [&](const typename Load::Next &next, int slot, int place) {
+          const uint32_t to = raw_at + slot * 2 * (kTile * DP);
+          if (load.once)
+            load.template send<true>(next, to, to + kTile * DP);
+          else
+            load.template send<false>(next, to, to + kTile * DP);
+          on |= next.on << (2 * place);
+        };
+        if (count > 0)
+          load.first_entries(x0, count, lane);
+        if constexpr (BUSY)
+          start();
+#pragma clang loop unroll(disable)
+        for (int i = 0; i < min(count, RAW); ++i)
+          send(load.look(i, x0 + i * kTile, lane), i, i);
+        typename Load::Next then = {}; // the next tile to send
+        if (count > 0)
+          then = load.look(RAW, x0 + RAW * kTile, lane);
+        int slot = 0; // of the tile that is widened next, the n-th
+        auto read = [&](int n) {
+          if (n + RAW - 1 < count)
+            arrived<(RAW - 1) * 2 * Load::LOADS>();
+          else
+            arrived<0>();
+          return load.codes(raw_at + slot * 2 * (kTile * DP), lane);
+        };
+        auto widen = [&](const typename Load::Codes &codes, int n) {
+          load.widen(codes, at + (n & 1) * 2 * TILE, lane); // which have been read: their place is free
+          if (n + RAW < count)
+            send(then, slot, RAW);
+          then = load.look(n + RAW + 1, x0 + (n + RAW + 1) * kTile, lane);
+          slot = slot + 1 == RAW ? 0 : slot + 1;
+        };
+        if (count > 0)
+          widen(read(0), 0);
+#pragma clang loop unroll(disable)
+        for (int n = 0; n < count; ++n) {
+          const int xt = it.token<FORM>(x0 + n * kTile);
+          const bool cut = (on & 3u) != 3u || xt + kTile > it.cached || it.windowed<FORM>(xt, args_again().sinks);
+          const uint32_t seen = cut ? load.seen(xt, on) : 0xffffffffu;
+          on >>= 2;
+          meet(); // the tile is whole, and everybody has read the one before
+          typename Load::Codes codes;
+          if (n + 1 < count)
+            codes = read(n + 1); // on their way while this tile is worked on
+          take_in(xt, seen, cut, n & 1, load.scales(n));
+          if (n + 1 < count)
+            widen(codes, n + 1);
+        }
+        arrived<0>(); // the last entries, wanted or not
+      } else if constexpr (SRC == kAsync) {
         uint32_t on = 0u; // of the tiles on their way: their halves on a page
         auto send = [&](const typename Load::Next &next, int slot, int place) {
           const uint32_t to = at + slot * 2 * TILE;
@@ -1599,6 +1694,9 @@ hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s
                 : reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kStaged>),
         64 * turn_waves(DP), a, p, s);
   // int8 is widened once for all waves, on its way through registers
+  if constexpr (FORM == kBlocks)
+    if (p.async)
+      return attend_shared<FORM, T, I8, DP, kAsync>(a, p, s);
   if constexpr (I8)
     return p.even ? attend_shared<FORM, T, I8, DP, kStagedEven>(a, p, s) : attend_shared<FORM, T, I8, DP, kStaged>(a, p, s);
   else
