@@ -663,8 +663,8 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
   const uint32_t at = place(tiles), stats_at = place(reinterpret_cast<const char *>(&stats[0][0][0]));
   const uint32_t qrow = static_cast<uint32_t>(a.q.row) * 2, grow = static_cast<uint32_t>(a.dout.row) * 2;
   const uint32_t stats_apart = static_cast<uint32_t>(a.heads) * static_cast<uint32_t>(a.rows); // -lse / scale, then -D
-  auto send = [&](int n, int slot) {
-    const int h = n / per, p = p0 + (n - h * per) * 32, head = kv * group + h;
+  auto send = [&](int h, int i, int slot) { // the i-th tile of a head of the group
+    const int p = p0 + i * 32, head = kv * group + h;
     const int64_t row = static_cast<int64_t>(piece.begin) + p;
     bring.send(a.q.data + (row * a.q.row + head * a.q.head) * 2, qrow, piece.n - p, at + slot * 2 * TILE);
     bring.send(a.dout.data + (row * a.dout.row + head * a.dout.head) * 2, grow, piece.n - p, at + slot * 2 * TILE + TILE);
@@ -790,11 +790,11 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
   if constexpr (FIRST) {
     int slot = wave * RING;
     if (wave < count)
-      send(wave, slot);
+      send(wave / per, wave % per, slot);
 #pragma clang loop unroll(disable)
     for (int n = wave; n < count; n += kWaves, slot ^= 1) { // tiles of its own
       if (n + kWaves < count) {
-        send(n + kWaves, slot ^ 1);
+        send((n + kWaves) / per, (n + kWaves) % per, slot ^ 1);
         arrived<SENT>();
       } else {
         arrived<0>();
@@ -803,9 +803,15 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
       shared_done(); // its place is free
     }
   } else {
+    int slot = 0, in_head = 0, next_head = 0, next_in = 0; // of this tile, and the next to send
+    auto send_next = [&](int to) {
+      send(next_head, next_in, to);
+      const bool end = next_in + 1 == per;
+      next_head += end;
+      next_in = end ? 0 : next_in + 1;
+    };
     for (int n = 0; n < min(count, RING - 1); ++n)
-      send(n, n);
-    int slot = 0, in_head = 0;
+      send_next(n);
 #pragma clang loop unroll(disable)
     for (int n = 0; n < count; ++n) {
       if (n + RING - 2 < count)
@@ -814,7 +820,7 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
         arrived<0>();
       meet();
       if (n + RING - 1 < count)
-        send(n + RING - 1, slot == 0 ? RING - 1 : slot - 1);
+        send_next(slot == 0 ? RING - 1 : slot - 1);
       const int p = p0 + in_head * 32;
       if (p + 31 >= x_first && p - x_last < a.window)
         take_in(p, slot);
