@@ -614,18 +614,23 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 2) void k_win
 // A wave's keys stay in registers with their gradients' sums, its values in shared
 // memory: both in registers left too few (1842 us against 1396 with heads of 128;
 // 1422 against 1378 for a step with heads of 64, which three waves a SIMD fit so).
-// FIRST: the first tokens' gradients from the rows whose window has left them.
-// Otherwise from the rows in whose windows a tile of 128 keys is.
-template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(WindowArgs a) {
-  constexpr int RB = DP * 2, TILE = 32 * RB, E = DP / 32, KS = DP / 16, KEYS = 32 * kWaves;
-  constexpr int RING = FIRST || DP == 128 ? 2 : 3; // tiles at a time; FIRST: of each wave
-  constexpr int SLOTS = FIRST ? kWaves * RING : RING;
-  constexpr int NT = FIRST ? 32 : 32 / kWaves; // tokens that a wave brings
+//   kWide    128 keys a workgroup, 32 a wave, over the rows in whose windows they are
+//   kNarrow  32 keys a workgroup, whose waves take turns at the tiles of rows and add
+//            up at the end: where there are few keys, four times the workgroups
+//   kFirst   the same, of first tokens over the rows whose window has left them
+enum KeyMode : int { kWide, kNarrow, kFirst };
+template <int T, int DP, int MODE>
+__global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(WindowArgs a) {
+  constexpr bool FIRST = MODE == kFirst, TURNS = MODE != kWide;
+  constexpr int RB = DP * 2, TILE = 32 * RB, E = DP / 32, KS = DP / 16, KEYS = TURNS ? 32 : 32 * kWaves;
+  constexpr int RING = TURNS || DP == 128 ? 2 : 3; // tiles at a time; TURNS: of each wave
+  constexpr int SLOTS = TURNS ? kWaves * RING : RING;
+  constexpr int NT = TURNS ? 32 : 32 / kWaves; // tokens that a wave brings
   using Loads = Bring<DP, NT>;
   constexpr int ROOM = SLOTS * 2 * TILE;
   __shared__ __attribute__((aligned(256))) char tiles[ROOM];
   __shared__ __attribute__((aligned(16))) float stats[SLOTS][2][32];
-  __shared__ __attribute__((aligned(256))) char values[(FIRST ? 32 : KEYS) * RB];
+  __shared__ __attribute__((aligned(256))) char values[KEYS * RB];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int group = a.heads / a.kv_heads;
   const Work w = my_work(FIRST ? a.first_pieces : a.key_pieces, FIRST ? a.kv_heads * a.first_blocks : a.kv_heads);
@@ -659,7 +664,7 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
   }
   const int per = (p1 - p0 + 31) >> 5; // tiles of a head
   const int count = per * group;
-  const Loads bring(lane, FIRST ? 0 : wave * NT, a.dim);
+  const Loads bring(lane, TURNS ? 0 : wave * NT, a.dim);
   const uint32_t at = place(tiles), stats_at = place(reinterpret_cast<const char *>(&stats[0][0][0]));
   const uint32_t qrow = static_cast<uint32_t>(a.q.row) * 2, grow = static_cast<uint32_t>(a.dout.row) * 2;
   const uint32_t stats_apart = static_cast<uint32_t>(a.heads) * static_cast<uint32_t>(a.rows); // -lse / scale, then -D
@@ -668,25 +673,25 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
     const int64_t row = static_cast<int64_t>(piece.begin) + p;
     bring.send(a.q.data + (row * a.q.row + head * a.q.head) * 2, qrow, piece.n - p, at + slot * 2 * TILE);
     bring.send(a.dout.data + (row * a.dout.row + head * a.dout.head) * 2, grow, piece.n - p, at + slot * 2 * TILE + TILE);
-    // 64 numbers of the tile's rows: each wave a quarter, FIRST: all
-    const int number = FIRST ? lane : wave * 16 + lane;
-    if (FIRST || lane < 16)
+    // 64 numbers of the tile's rows: each wave a quarter, TURNS: all
+    const int number = TURNS ? lane : wave * 16 + lane;
+    if (TURNS || lane < 16)
       load_async4(a.stats + static_cast<int64_t>(head) * a.rows + row,
                   (static_cast<uint32_t>(min(number & 31, piece.n - p - 1)) + (number < 32 ? 0u : stats_apart)) * 4,
-                  stats_at + slot * 256 + (FIRST ? 0 : wave * 64));
+                  stats_at + slot * 256 + (TURNS ? 0 : wave * 64));
   };
   constexpr int SENT = 2 * Loads::LOADS + 1;
 
-  const int x_first = x0 + (FIRST ? 0 : wave * 32), x_last = x_first + 31, key = x_first + (lane & 31);
+  const int x_first = x0 + (TURNS ? 0 : wave * 32), x_last = x_first + 31, key = x_first + (lane & 31);
   const int64_t key_row = static_cast<int64_t>(piece.begin) + min(key, piece.n - 1);
   u32x4 k[KS], v[KS];
   take_row<DP>(k, a.k.data + (key_row * a.k.row + kv * a.k.head) * 2, a.dim, lane);
   take_row<DP>(v, a.v.data + (key_row * a.v.row + kv * a.v.head) * 2, a.dim, lane);
   const uint32_t direct = direct_at<RB>(lane), turn0 = turned_at<RB>(lane, 0), turn1 = turned_at<RB>(lane, 1);
-  const uint32_t values_at = place(values) + (FIRST ? 0 : wave * 32 * RB) + direct;
+  const uint32_t values_at = place(values) + (TURNS ? 0 : wave * 32 * RB) + direct;
 #pragma unroll
   for (int s = 0; s < KS; ++s) {
-    // FIRST: the same by all waves
+    // TURNS: the same by all waves
     *reinterpret_cast<__attribute__((address_space(3))) u32x4 *>(values_at ^ (s * 32)) = v[s];
     asm volatile("" : "+v"(k[s]));
   }
@@ -787,7 +792,7 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
     }
   };
 
-  if constexpr (FIRST) {
+  if constexpr (TURNS) {
     int slot = wave * RING;
     if (wave < count)
       send(wave / per, wave % per, slot);
@@ -831,10 +836,19 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
   }
 
   const float fk = a.plain_scale * over.up() * less<T>(), fv = less<T>();
-  if constexpr (FIRST) {
+  const int sinks = min(a.sinks, piece.n);
+  // what the later rows, whose windows have left them, add to first tokens from
+  // x_first on: `add` takes the place of each sum
+  const int size = static_cast<int>(a.first_tokens.d);
+  const bool more = !FIRST && x_first < sinks && a.window + x_first < piece.n;
+  auto add_first = [&](auto add) {
+    const int64_t base = static_cast<int64_t>(fdiv(static_cast<uint32_t>(piece.begin), a.first_tokens)) + piece.number;
+    for (int c = (a.window + x_first) / size; static_cast<int64_t>(c) * size < piece.n; ++c)
+      add(a.first_sums + ((base + c) * a.kv_heads + kv) * a.sinks * 2 * DP);
+  };
+  if constexpr (TURNS) {
     // the waves' sums, in order, keys' then values'
     float *room = reinterpret_cast<float *>(tiles);
-    float *to = a.first_sums + ((static_cast<int64_t>(w.number) * a.kv_heads + kv) * a.sinks + x0) * 2 * DP;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
@@ -848,12 +862,22 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
               f32x4{x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f};
         }
       __syncthreads();
-      for (int i = threadIdx.x * 4; i < min(32, a.sinks - x0) * DP; i += 64 * kWaves * 4) {
+      for (int i = threadIdx.x * 4; i < min(32, (FIRST ? a.sinks : piece.n) - x0) * DP; i += 64 * kWaves * 4) {
         f32x4 sum = *reinterpret_cast<const f32x4 *>(room + i);
 #pragma unroll
         for (int o = 1; o < kWaves; ++o)
           sum += *reinterpret_cast<const f32x4 *>(room + o * 32 * DP + i);
-        *reinterpret_cast<f32x4 *>(to + (i / DP * 2 + which) * DP + i % DP) = sum;
+        const int x = x0 + i / DP, d = i % DP, at_sum = (x * 2 + which) * DP + d;
+        if constexpr (FIRST) {
+          *reinterpret_cast<f32x4 *>(a.first_sums + (static_cast<int64_t>(w.number) * a.kv_heads + kv) * a.sinks * 2 * DP + at_sum) = sum;
+        } else {
+          if (more && x < sinks)
+            add_first([&](const float *from) { sum += *reinterpret_cast<const f32x4 *>(from + at_sum); });
+          const Heads &to = which ? a.dv : a.dk;
+          if (d < a.dim)
+            *reinterpret_cast<u32x2 *>(to.data + ((static_cast<int64_t>(piece.begin) + x) * to.row + kv * to.head + d) * 2) =
+                u32x2{pack16<T>(sum[0], sum[1]), pack16<T>(sum[2], sum[3])};
+        }
       }
     }
   } else {
@@ -862,27 +886,22 @@ template <int T, int DP, bool FIRST> __global__ __launch_bounds__(64 * kWaves, D
       dk[m] *= fk;
       dv[m] *= fv;
     }
-    if (x_first < a.sinks && a.window + x_first < piece.n) { // what the later rows add
-      if (key < min(a.sinks, piece.n)) {
-        const int size = static_cast<int>(a.first_tokens.d);
-        const int64_t base = static_cast<int64_t>(fdiv(static_cast<uint32_t>(piece.begin), a.first_tokens)) + piece.number;
-        for (int c = (a.window + x_first) / size; static_cast<int64_t>(c) * size < piece.n; ++c) {
-          const float *from = a.first_sums + (((base + c) * a.kv_heads + kv) * a.sinks + key) * 2 * DP + 4 * (lane >> 5);
+    if (more && key < sinks)
+      add_first([&](const float *from) {
+        from += key * 2 * DP + 4 * (lane >> 5);
 #pragma unroll
-          for (int m = 0; m < E; ++m)
+        for (int m = 0; m < E; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f32x4 x = *reinterpret_cast<const f32x4 *>(from + 32 * m + 8 * i);
-              const f32x4 y = *reinterpret_cast<const f32x4 *>(from + DP + 32 * m + 8 * i);
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(from + 32 * m + 8 * i);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(from + DP + 32 * m + 8 * i);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                dk[m][4 * i + r] += x[r];
-                dv[m][4 * i + r] += y[r];
-              }
+            for (int r = 0; r < 4; ++r) {
+              dk[m][4 * i + r] += x[r];
+              dv[m][4 * i + r] += y[r];
             }
-        }
-      }
-    }
+          }
+      });
     if (key < piece.n) {
       put_row<T, DP>(a.dk.data + (key_row * a.dk.row + kv * a.dk.head) * 2, dk, 1.0f, a.dim, lane);
       put_row<T, DP>(a.dv.data + (key_row * a.dv.row + kv * a.dv.head) * 2, dv, 1.0f, a.dim, lane);
@@ -906,10 +925,12 @@ template <int T, int DP> hipError_t window_backward(const WindowArgs &a, hipStre
   hipError_t e = window_start(reinterpret_cast<const void *>(k_window_dq<T, DP>), a,
                               static_cast<int64_t>(a.row_pieces) * a.kv_heads * a.parts, s);
   if (e == hipSuccess && a.sinks > 0)
-    e = window_start(reinterpret_cast<const void *>(k_window_dkv<T, DP, true>), a,
+    e = window_start(reinterpret_cast<const void *>(k_window_dkv<T, DP, kFirst>), a,
                      static_cast<int64_t>(a.first_pieces) * a.kv_heads * a.first_blocks, s);
   if (e == hipSuccess)
-    e = window_start(reinterpret_cast<const void *>(k_window_dkv<T, DP, false>), a,
+    e = window_start(a.key_tokens.d == 32 ? reinterpret_cast<const void *>(k_window_dkv<T, DP, kNarrow>)
+                                            : reinterpret_cast<const void *>(k_window_dkv<T, DP, kWide>),
+                     a,
                      static_cast<int64_t>(a.key_pieces) * a.kv_heads, s);
   return e;
 }

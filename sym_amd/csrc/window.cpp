@@ -87,7 +87,7 @@ BlockArgs block_args(const relx_block_append_args &p, int &type) {
 
 // ------------------------------------------------------------ packed sequences
 
-constexpr int kTileRows = 128, kTileKeys = 128, kMostSinks = 256;
+constexpr int kTileRows = 128, kMostSinks = 256;
 
 // Rows that are read in pieces of 16 bytes, tiles of them from one address.
 Heads rows_of(const relx_heads *h, bool used, int64_t rows, int64_t heads, const char *what) {
@@ -133,7 +133,15 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   a.parts = static_cast<int32_t>((group + heads - 1) / heads);
   a.tile_heads = make_div(heads);
   a.tile_tokens = make_div(kTileRows / heads);
-  a.key_tokens = make_div(kTileKeys);
+  // Keys of a workgroup in the backward pass: where there are few tiles of 128 of
+  // all heads, 32. us of the whole backward with 32 and with 128, four query heads a
+  // key head, window 512:
+  //   heads of 128    17 tiles: 83, 168    136: 136, 188    260: 288, 340    520: 498, 493
+  //   heads of 64     17 tiles: 58, 127    136: 76, 134     520: 252, 295
+  // and longer, eight query heads, window 2048: 130 tiles of 128: 893, 953, 260: 1328,
+  // 1158; four, window 1024: 1032 tiles of 64: 702, 706, 2056: 1425, 1358.
+  const int64_t tiles = (p.rows / 128 + p.sequences) * p.kv_heads;
+  a.key_tokens = make_div(tiles < (p.dim <= 64 ? 1024 : 256) ? 32 : 128);
   a.first_blocks = (a.sinks + 31) / 32;
   // as many workgroups as run at a time and half as many again
   const int64_t first = p.rows * p.kv_heads * std::max(a.first_blocks, 1) / 768;

@@ -90,6 +90,14 @@ def test_long_sequences(ctx):
     check(ctx, W.window_case(4, [1300], 1, 1, 128, F16), "long", 200, 40)
 
 
+@pytest.mark.parametrize("dtype,kv,lengths,dim", [(BF16, 43, [700], 128), (F16, 90, [300, 130], 128), (BF16, 86, [15] * 12, 64),
+                                                  (F16, 172, [200, 90, 130], 64)])
+def test_many_keys(ctx, dtype, kv, lengths, dim):
+    """Enough tiles of keys for the form of large batches."""
+    assert (sum(lengths) // 128 + len(lengths)) * kv >= (256 if dim > 64 else 1024)
+    check(ctx, W.window_case(15, lengths, kv, kv, dim, dtype), "many keys", 60, 5)
+
+
 def test_rows_of_no_sequence(ctx):
     s = W.window_case(5, [100, 50], 4, 2, 64, BF16, before=37, after=150)
     check(ctx, s, "padded", 40, 2)
