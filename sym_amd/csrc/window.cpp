@@ -146,6 +146,10 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   // as many workgroups as run at a time and half as many again
   const int64_t first = p.rows * p.kv_heads * std::max(a.first_blocks, 1) / 768;
   a.first_tokens = make_div(std::min<int64_t>(std::max<int64_t>((first + 31) / 32 * 32, 128), 4096));
+  // Where windows are of few tokens, or the first rows of sequences, which see few,
+  // are a good part of them: gradients of sequences of 600 rows on average are then
+  // 1.4 and not 1.5 times as far off as their rounding; of 4000 they are 1.45 without.
+  a.sums_d = p.rows / std::max<int64_t>(p.sequences, 1) <= 2048 || static_cast<int64_t>(a.window) + a.sinks <= 128;
   const auto pieces = [&](const FastDiv &size, int64_t heads_of_piece) {
     const int64_t n = p.rows / size.d + p.sequences + 2;
     // a workgroup of 256 threads for each, and 2^32 threads a dimension

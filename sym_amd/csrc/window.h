@@ -20,6 +20,7 @@ struct WindowArgs {
   int32_t first_blocks;                         // of 32 first tokens
   int32_t rows, sequences, heads, kv_heads, parts, dim, window, sinks;
   float scale, plain_scale; // of a score, times log2 e, and as it is
+  bool sums_d;              // the backward sums D from the weights
 };
 hipError_t window_launch_f16(const WindowArgs &a, bool back, hipStream_t s);
 hipError_t window_launch_bf16(const WindowArgs &a, bool back, hipStream_t s);
