@@ -56,7 +56,7 @@
 #include "attend_share.h"
 #include "attention.h"
 #include "index.h"
-#include "wave.h"
+#include "k_attend_wave.h"
 
 namespace relx {
 namespace {

@@ -1,4 +1,4 @@
-// wave.h - what the attention kernels share: vectors, a wave's scalars, matrix
+// k_attend_wave.h - what the attention kernels share: vectors, a wave's scalars, matrix
 // instructions, reads of shared memory and loads into it.
 #pragma once
 

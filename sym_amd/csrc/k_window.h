@@ -36,7 +36,7 @@
 
 #include "attention.h"
 #include "index.h"
-#include "wave.h"
+#include "k_attend_wave.h"
 #include "window.h"
 
 namespace relx {
