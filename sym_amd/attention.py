@@ -427,7 +427,10 @@ def block_append(ctx, k, v, cache_k, cache_v, k_scale, v_scale, table, cached, s
     that the request already has in the block are rounded anew. Infinities become
     the largest codes, NaN -128, as in the package's plans. Tokens whose page is
     not in the cache are left out; a block is of one request that writes to it.
-    Caches and scales are updated in place; there is no gradient."""
+    Caches and scales are updated in place; there is no gradient, so keys or values
+    that want one are refused (in a graph, detach them)."""
+    if _in_graph(k, v):
+        _bad("block_append has no gradient: it takes detached keys and values, or runs under torch.no_grad()")
     device = _device(ctx, k)
     shape, dtype = k.shape, k.dtype
     kind = _KINDS.get(dtype)
