@@ -120,8 +120,7 @@ __device__ __forceinline__ int64_t divide(int64_t n, int d) {
 
 // ------------------------------------------------------------ the schedule
 
-// The end of the tiles with first tokens. Sizes are 2^30 at most, so that sums
-// of three stay within 32 bits.
+// The end of the tiles with first tokens.
 __device__ __forceinline__ int edge_of(const AttendArgs &a, int length) {
   return (min(a.sinks, length) + kTile - 1) & ~(kTile - 1);
 }
@@ -151,8 +150,8 @@ __device__ __forceinline__ Request attend_request(const AttendArgs &a, int b) {
     // of an item's rows span, and the rest of the tile in which the span begins
     const uint32_t g = a.group.d;
     const uint32_t span = a.mask ? r.fresh : min(static_cast<uint32_t>(r.fresh), (ROWS - 1) / g + 2);
-    const uint32_t most = static_cast<uint32_t>(edge_of(a, r.length)) + kTile - 1 + static_cast<uint32_t>(a.window) + span;
-    reach = static_cast<int>(min(static_cast<uint32_t>(reach), most));
+    const int64_t most = static_cast<int64_t>(edge_of(a, r.length)) + kTile - 1 + a.window + span;
+    reach = static_cast<int>(min(static_cast<int64_t>(reach), most));
   }
   r.units = max((reach + UNIT - 1) / UNIT, 1);
   return r;

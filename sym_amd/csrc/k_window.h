@@ -525,8 +525,8 @@ template <int T, int DP, bool SUMS> __global__ __launch_bounds__(64 * kWaves, 2)
   u32x4 q[KS], g[KS];
   take_row<DP>(q, a.q.data + (at_row * a.q.row + row.head * a.q.head) * 2, a.dim, lane);
   take_row<DP>(g, a.dout.data + (at_row * a.dout.row + row.head * a.dout.head) * 2, a.dim, lane);
-  float *stats = a.stats + static_cast<int64_t>(row.head) * a.rows + at_row; // of the row: -lse / scale
-  float *stats_d = stats + static_cast<int64_t>(a.heads) * a.rows;           // and -D
+  float *stats = a.stats + static_cast<int64_t>(row.head) * 2 * a.rows + at_row; // of the row: -lse / scale
+  float *stats_d = stats + a.rows;                                               // and -D
   float d = 0.0f;
   if (!SUMS && few) {
     d = -*stats_d;
@@ -694,7 +694,6 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(Wi
   const Loads bring(lane, TURNS ? 0 : wave * NT, a.dim);
   const uint32_t at = place(tiles), stats_at = place(reinterpret_cast<const char *>(&stats[0][0][0]));
   const uint32_t qrow = static_cast<uint32_t>(a.q.row) * 2, grow = static_cast<uint32_t>(a.dout.row) * 2;
-  const uint32_t stats_apart = static_cast<uint32_t>(a.heads) * static_cast<uint32_t>(a.rows); // -lse / scale, then -D
   auto send = [&](int h, int i, int slot) { // the i-th tile of a head of the group
     const int p = p0 + i * 32, head = kv * group + h;
     const int64_t row = static_cast<int64_t>(piece.begin) + p;
@@ -703,8 +702,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(Wi
     // 64 numbers of the tile's rows: each wave a quarter, TURNS: all
     const int number = TURNS ? lane : wave * 16 + lane;
     if (TURNS || lane < 16)
-      load_async4(a.stats + static_cast<int64_t>(head) * a.rows + row,
-                  (static_cast<uint32_t>(min(number & 31, piece.n - p - 1)) + (number < 32 ? 0u : stats_apart)) * 4,
+      load_async4(a.stats + static_cast<int64_t>(head) * 2 * a.rows + row, // rows: 2^29 at most
+                  static_cast<uint32_t>(min(number & 31, piece.n - p - 1) + (number < 32 ? 0 : a.rows)) * 4,
                   stats_at + slot * 256 + (TURNS ? 0 : wave * 64));
   };
   constexpr int SENT = 2 * Loads::LOADS + 1;
@@ -894,7 +893,8 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(Wi
 #pragma unroll
         for (int o = 1; o < kWaves; ++o)
           sum += *reinterpret_cast<const f32x4 *>(room + o * 32 * DP + i);
-        const int x = x0 + i / DP, d = i % DP, at_sum = (x * 2 + which) * DP + d;
+        const int x = x0 + i / DP, d = i % DP;
+        const int64_t at_sum = (static_cast<int64_t>(x) * 2 + which) * DP + d;
         if constexpr (FIRST) {
           *reinterpret_cast<f32x4 *>(a.first_sums + (static_cast<int64_t>(w.number) * a.kv_heads + kv) * a.sinks * 2 * DP + at_sum) = sum;
         } else {

@@ -109,7 +109,7 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
        "window attention: query heads are a multiple of the key heads");
   layout(p.heads <= 65535, "window attention: more than 65535 heads");
   layout(p.dim >= 8 && p.dim <= 128 && p.dim % 8 == 0, "window attention: head sizes are multiples of 8 up to 128");
-  layout(p.rows <= kMost, "window attention: more than 2^30 rows");
+  layout(p.rows <= kMost / 2, "window attention: more than 2^29 rows");
   need(p.window >= 0 && p.sinks >= 0, "window attention: a negative window or number of first tokens");
   layout(p.sinks <= kMostSinks, "window attention: more than 256 first tokens");
   const float scale = static_cast<float>(p.scale * 1.4426950408889634);

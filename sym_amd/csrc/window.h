@@ -11,7 +11,7 @@ struct WindowArgs {
   Heads dout, dq, dk, dv;
   const int32_t *starts;
   float *lse;        // [heads, rows]
-  float *stats;      // [2, heads, rows]: -lse / scale (both in powers of two), and -D
+  float *stats;      // [heads, 2, rows]: -lse / scale (both in powers of two), and -D
   float *first_sums; // [pieces, kv_heads, sinks, 2, width]: what pieces of rows add to the first tokens' gradients
   // a workgroup's rows: tokens, times heads of a group (in `parts` where those are many)
   FastDiv tile_tokens, tile_heads;

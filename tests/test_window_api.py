@@ -61,7 +61,7 @@ BAD_WINDOWS = [
     ("invalid_argument", dict(kv_heads=3)), ("invalid_argument", dict(kv_heads=0)), ("invalid_argument", dict(heads=0)),
     ("invalid_argument", dict(window=-1)), ("invalid_argument", dict(sinks=-1)), ("invalid_argument", dict(scale=float("inf"))),
     ("invalid_argument", dict(scale=float("nan"))), ("invalid_argument", dict(starts=None)),
-    ("unsupported_layout", dict(rows=2 ** 30 + 1)), ("unsupported_layout", dict(dim=136)), ("unsupported_layout", dict(dim=4)),
+    ("unsupported_layout", dict(rows=2 ** 29 + 1, heads=1, kv_heads=1)), ("unsupported_layout", dict(dim=136)), ("unsupported_layout", dict(dim=4)),
     ("unsupported_layout", dict(dim=60)), ("unsupported_layout", dict(sinks=257)), ("unsupported_layout", dict(kind=0, bits=32)),
     ("unsupported_layout", dict(kind=2, bits=8)), ("unsupported_layout", dict(kind=7)),
     ("unsupported_layout", dict(heads=65536, kv_heads=1)), ("unsupported_layout", dict(rows=2 ** 28, heads=32, kv_heads=32)),
