@@ -108,6 +108,7 @@ struct AttendPlan {
   bool even;      // pages of whole tiles of 16 tokens
   bool async;     // and rows of whole 16-byte pieces at 16-byte addresses
   int workgroups;
+  bool quads;     // four heads of up to four rows at a time (int8 of a view)
 };
 constexpr int kMostWorkgroups = 512; // two to a compute unit
 

@@ -24,6 +24,8 @@
 //   kStaged  everything else: through registers, where what is no token
 //            becomes zero
 // and who works on them:
+//   up to 4 query rows, int8 heads side by side (a view's): a wave has a head of its
+//     own, so that four heads of a token are one piece of memory.
 //   up to 16 query rows share a key head (decoding): bound by the cache's
 //     bytes. The waves of a workgroup take turns at the tiles, each with a ring
 //     of its own and no barrier, and add up at the end. int8 is widened in the
@@ -65,6 +67,13 @@ constexpr int kScan = 128;    // runs of requests whose units a workgroup (of at
 constexpr int kTile = 32;     // tokens of a tile
 constexpr int kSharedUnit = 64;
 constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
+// Rows of an item of four heads at a time (k_attend_quads), which fit the places of
+// sixteen, and its unit.
+constexpr int kQuadRows = 4, kQuadUnit = 4 * kTile;
+// Heads' items of a request.
+template <int ROWS> __device__ __forceinline__ int head_items(const AttendArgs &a) {
+  return ROWS == kQuadRows ? a.kv_heads >> 2 : a.kv_heads;
+}
 
 enum Source : int { kAsync, kStaged, kStagedEven };
 // What a call's rows see, and how a cache's codes are scaled:
@@ -160,7 +169,7 @@ __device__ __forceinline__ Request attend_request(const AttendArgs &a, int b) {
 template <int FORM, int ROWS, int UNIT>
 __device__ __forceinline__ int64_t request_units(const AttendArgs &a, int b) {
   const Request r = attend_request<FORM, ROWS, UNIT>(a, b);
-  return static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
+  return static_cast<int64_t>(head_items<ROWS>(a)) * r.tiles * r.units;
 }
 
 // The units before each run of requests, which every workgroup adds up for
@@ -290,7 +299,7 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   int64_t at = uniform64(sh.before[lo]);
   Request r = attend_request<FORM, ROWS, UNIT>(a, b);
   for (;;) {
-    const int64_t n = static_cast<int64_t>(a.kv_heads) * r.tiles * r.units;
+    const int64_t n = static_cast<int64_t>(head_items<ROWS>(a)) * r.tiles * r.units;
     if (run.unit < at + n)
       break;
     at += n;
@@ -1234,6 +1243,107 @@ void k_attend_turns(AttendArgs a) {
   }
 }
 
+// ------------------------------------------- up to four rows, four heads at a time
+
+// The same where a token's heads lie side by side: each wave has a head of its own,
+// so that what the four read of a token is one piece of memory, 512 bytes for int8
+// heads of 128. Nothing is added up between waves.
+template <int T, int DP> __global__ __launch_bounds__(256, 2) void k_attend_quads(AttendArgs a) {
+  constexpr int W = 4, UNIT = kQuadUnit, ROWS = kQuadRows, E = DP / 16, TILE = kTile * DP, RING = 2;
+  using Load = Loader<kBlocks, T, true, DP, kAsync, kTile, true, kTile>;
+  __shared__ int entries[W][2][64];
+  __shared__ float block_scales[W][2][2][64];
+  __shared__ Schedule schedule;
+  __shared__ __attribute__((aligned(16))) char tiles[W][RING][2][TILE];
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  Load load(a, lane, 0);
+  load.room = place(reinterpret_cast<const char *>(&entries[wave][0][0]));
+  load.scale_room = place(reinterpret_cast<const char *>(&block_scales[wave][0][0][0]));
+  Rows<kBlocks, T, DP, 1, true, true> r;
+  const Reads<DP, true> reads(lane);
+  const uint32_t at = place(tiles[wave][0][0]);
+  if (!load.full) // places past the head's dims: no load writes them
+    for (int i = lane * 16; i < RING * 2 * TILE; i += 64 * 16)
+      *reinterpret_cast<u32x4 *>(&tiles[wave][0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
+  shared_done();
+  add_up<kBlocks, ROWS, UNIT>(a, schedule);
+  Run run = my_run(schedule);
+
+  while (run.unit < run.end) {
+    Item it = take<kBlocks, ROWS, UNIT>(args_again(), schedule, run);
+    it.head = it.head * 4 + wave;
+    const int row0 = it.tile * ROWS;
+    const int rows = min(it.fresh * static_cast<int>(args_again().group.d) - row0, ROWS);
+    load.item(args_again(), it);
+    const int x0 = it.s0 * UNIT, x_end = min(it.s1 * UNIT, it.reach);
+    const int count = x0 < x_end ? (x_end - x0 + kTile - 1) / kTile : 0;
+    uint32_t on = 0u; // of the tiles on their way: their halves on a page
+    auto send = [&](const typename Load::Next &next, int slot, int place) {
+      load.template send<true>(next, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE);
+      on |= next.on << (2 * place);
+    };
+    if (count > 0)
+      load.first_entries(x0, count, lane);
+    r.start(args_again(), it, row0, rows, args_again().scale, lane); // the queries arrive while the table does
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < min(count, RING); ++i)
+      send(load.look(i, x0 + i * kTile, lane), i, i);
+    typename Load::Next then = {}; // the next tile to send
+    if (count > 0)
+      then = load.look(RING, x0 + RING * kTile, lane);
+    int x = x0, slot = 0;
+#pragma clang loop unroll(disable)
+    for (int n = 0; n < count; ++n, x += kTile) {
+      if (n + RING <= count)
+        arrived<(RING - 1) * 2 * Load::LOADS>();
+      else
+        arrived<0>();
+      const int xt = it.token<kBlocks>(x);
+      const bool cut = (on & 3u) != 3u || xt + kTile > it.cached || it.windowed<kBlocks>(xt, r.sinks);
+      r.step(it, row0, xt, cut ? load.seen(xt, on) : 0xffffffffu, cut, at + slot * 2 * TILE, at + slot * 2 * TILE + TILE, reads,
+             lane, load.scales(n));
+      shared_done(); // its place is free
+      on >>= 2;
+      if (n + RING < count)
+        send(then, slot, RING - 1);
+      then = load.look(n + RING + 1, x + (RING + 1) * kTile, lane);
+      slot = slot + 1 == RING ? 0 : slot + 1;
+    }
+    arrived<0>(); // the last entries, wanted or not
+
+    const AttendArgs &b = args_again();
+    const float sum = r.total(0), over = r.kOver ? r.over : 1.0f;
+    if (c < rows) {
+      if (it.s0 == 0 && it.s1 == it.units) {
+        const uint32_t p = static_cast<uint32_t>(row0 + c);
+        const uint32_t j = fdiv(p, b.group);
+        const int64_t row = it.start + static_cast<int64_t>(j);
+        const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
+        const float f = finish(sum, 1.0f) * over;
+        char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (e * 16 + 4 * g < b.dim) {
+            const f32x4 o = r.acc[0][e] * f;
+            store(dst + e * 32, u32x2{pack16<T>(o[0], o[1]), pack16<T>(o[2], o[3])});
+          }
+        if (b.lse && g == 0)
+          b.lse[row * b.heads + qh] = log_sum(r.top[0], sum);
+      } else {
+        const int64_t part = (run.wg * 2 + (it.s0 == 0 ? 1 : 0)) * 16 + wave * ROWS + c;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          *reinterpret_cast<f32x4 *>(b.partial + part * DP + e * 16 + 4 * g) = r.acc[0][e] * over;
+        if (g == 0) {
+          b.stats[part * 2] = r.top[0];
+          b.stats[part * 2 + 1] = sum;
+        }
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------- more rows
 
 template <int FORM, int T, bool I8, int DP, int RT, int W, int SRC>
@@ -1561,7 +1671,7 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
     const int e = static_cast<int>(i % E), head = static_cast<int>(divide(i / E, groups));
     const int row0 = static_cast<int>(i / E - static_cast<int64_t>(head) * groups) * N;
     const int d = LANED ? e * 16 + (lane >> 4) * 4 : lane % (DP / 4) * 4;
-    const int64_t u0 = first + (static_cast<int64_t>(head) * r.tiles + row0 / ROWS) * r.units;
+    const int64_t u0 = first + (static_cast<int64_t>(ROWS == kQuadRows ? head >> 2 : head) * r.tiles + row0 / ROWS) * r.units;
     const int64_t w0 = uniform64(divide(u0, static_cast<int>(per)));
     const int64_t w1 = uniform64(divide(u0 + r.units - 1, static_cast<int>(per)));
     if (w0 == w1)
@@ -1579,7 +1689,9 @@ __global__ __launch_bounds__(PHASES == 1 ? 256 : 64 * PHASES) void k_attend_join
       for (int k = 0; k < MANY; ++k) {
         // a run that begins inside the item left its part in its first place,
         // the run in which the item begins in its second
-        const int64_t wk = min(w + k * PHASES, w1), at = (wk * 2 + (wk == w0 ? 1 : 0)) * ROWS + row0 % ROWS;
+        const int64_t wk = min(w + k * PHASES, w1);
+        const int64_t at = ROWS == kQuadRows ? (wk * 2 + (wk == w0 ? 1 : 0)) * 16 + head % 4 * ROWS + row0 % ROWS
+                                             : (wk * 2 + (wk == w0 ? 1 : 0)) * ROWS + row0 % ROWS;
         ml[k] = *reinterpret_cast<const f32x2 *>(a.stats + (at + c) * 2);
         o[k] = *reinterpret_cast<const f32x4 *>(a.partial + at * DP + (e * 64 + lane) * 4);
       }
@@ -1687,6 +1799,10 @@ hipError_t attend_shared(const AttendArgs &a, const AttendPlan &p, hipStream_t s
 
 template <int FORM, int T, bool I8, int DP>
 hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  if constexpr (FORM == kBlocks && DP <= 128)
+    if (p.quads)
+      return attend_start<FORM, T, I8, DP, kQuadRows, kQuadUnit>(reinterpret_cast<const void *>(k_attend_quads<T, DP>), 256, a,
+                                                                 p, s);
   if (p.rows == 16)
     return attend_start<FORM, T, I8, DP, 16, turn_unit(DP)>(
         p.async ? reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kAsync>)

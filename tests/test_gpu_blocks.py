@@ -144,6 +144,25 @@ def test_blocks(ctx, dtype, cached, fresh, heads, kv, dim, page, block, order):
     check_view(ctx, W.view_case(5, cached, fresh, heads, kv, dim, dtype, I8, page, block, order), "blocks %s" % [cached, fresh, dim])
 
 
+@pytest.mark.parametrize("cached,fresh,heads,kv,dim,page,block,window,sinks", [
+    ([700, 3, 129], [1, 1, 1], 16, 4, 128, 64, 32, None, 0),
+    ([700, 0, 129], [2, 1, 1], 8, 8, 80, 64, 16, None, 0),
+    ([5000, 31, 300], [1, 1, 1], 8, 4, 64, 48, 16, 1000, 3),
+    ([300, 260, 900], [1, 2, 1], 12, 4, 128, 128, 64, 70, 40),
+    ([90, 1000, 64], [9, 1, 0], 8, 8, 16, 64, 64, 33, 0),  # more rows of one request than fit at a time
+    ([400, 200, 100], [1, 1, 1], 16, 16, 128, 64, None, 200, 1),  # a scale a head
+])
+def test_four_heads_at_a_time(ctx, cached, fresh, heads, kv, dim, page, block, window, sinks):
+    """Decoding over many tokens whose heads lie side by side."""
+    columns = (1 << 17) // (3 * page * kv) + 1
+    for dtype in (F16, BF16):
+        s = W.view_case(14, cached, fresh, heads, kv, dim, dtype, I8, page, block, columns=max(columns, 5100 // page + 1))
+        got = check_view(ctx, s, "four heads %s" % [cached, fresh, dim, window], window, sinks)
+        narrow = dict(s, table=s["table"][:, :max(-(-(c + f) // page) for c, f in zip(cached, fresh))].contiguous())
+        other = check_view(ctx, narrow, "the same, one at a time", window, sinks)
+        assert float((got.float() - other.float()).abs().max()) < 0.05
+
+
 @pytest.mark.parametrize("cache", ["own", "int8", "blocks"])
 @pytest.mark.parametrize("cached,fresh,heads,kv,dim,page,window,sinks", [
     ([0], [1], 2, 1, 64, 16, 1, 0),
