@@ -7,10 +7,14 @@ then attends over them. The calls of its step, in order:
                         taken from the free list, masks of drafted trees
   norm_rotate_append    norm and rotation of the step's queries and keys; keys
                         and values into the cache (int8 by a scale a head)
-  tree_attention        attention of the step's rows over the cache
+  block_append          or, after `norm_rotate`, keys and values into an int8
+                        cache with a scale for each block of tokens and head
+  tree_attention        attention of the step's rows over the cache, all of it
+                        or a window with first tokens that stay
 
 and, in training, `norm_rotate` (a differentiable function of its queries, keys
-and weights) with `norm_rotate_backward` beneath it.
+and weights) and `window_attention` over packed sequences, with
+`norm_rotate_backward` and `window_attention_backward` beneath them.
 
 Calls take a `pyreloc.Context`, run on torch's current stream of its device,
 return at once and never wait for the GPU, so they can be captured into a
