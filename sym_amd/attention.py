@@ -550,11 +550,16 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     return out
 
 
-def _view(window, sinks):
+def _reach(window, sinks):
+    """Both as the library takes them: whole numbers of 63 bits, no window as 0."""
     window, sinks = 0 if window is None else int(window), int(sinks)
     if window < 0 or sinks < 0 or (window == 0 and sinks):
         _bad("a window of %d tokens with %d first ones" % (window, sinks))
-    return _VIEW.pack(window, sinks)
+    return min(window, 1 << 62), min(sinks, 1 << 62)
+
+
+def _view(window, sinks):
+    return _VIEW.pack(*_reach(window, sinks))
 
 
 # ------------------------------------------------------------ packed sequences
@@ -593,9 +598,7 @@ def _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale):
             ks[1] < 1 or shape[1] < 1 or shape[1] % ks[1]:
         _bad("queries and keys: f16 or bf16 [rows, heads, dim] and [rows, kv_heads, dim], kv_heads dividing heads; got %s %s and %s %s"
              % (dtype, list(shape), k.dtype, list(ks)))
-    window, sinks = 0 if window is None else int(window), int(sinks)
-    if window < 0 or sinks < 0 or (window == 0 and sinks):
-        _bad("a window of %d tokens with %d first ones" % (window, sinks))
+    window, sinks = _reach(window, sinks)
     l_ptr = 0
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != (shape[1], shape[0]) or lse.get_device() != device or \

@@ -254,6 +254,24 @@ def test_large_and_small_scales_in_f16(ctx):
     check_view(ctx, s, "scales far apart")
 
 
+@pytest.mark.parametrize("scale", [0.05, -0.05, 0.0])
+def test_scales_of_either_sign(ctx, scale):
+    """Of the scores, and of an int8 cache's keys and values, a head's or a block's."""
+    for block in (None, 16):
+        for fresh in ([1, 1], [30, 7]):
+            s = W.view_case(15, [200, 50], fresh, 4, 4, 64, BF16, I8, 32, block)
+            s["scale"] = scale
+            for z in (s["k_scale"], s["v_scale"]):
+                z[..., 1] *= -1
+                z[..., 2] = 0.0
+            check_view(ctx, s, "scales %s %s" % (scale, block), 64, 2)
+
+
+def test_windows_beyond_any_number(ctx):
+    s = W.view_case(16, [100], [1], 2, 1, 64, F16, F16, 16)
+    check_view(ctx, s, "all", 10 ** 30, 10 ** 30)
+
+
 def test_a_step_over_blocks(ctx):
     """Tables, norm and rotation, appending, attention: prompts, then single tokens, captured and replayed."""
     say("a step over blocks")

@@ -231,6 +231,34 @@ def test_other_streams_and_graphs(ctx):
             assert torch.equal(x, y)
 
 
+def test_a_captured_training_step(ctx):
+    """Forward and backward through torch's graph, replayed."""
+    s = W.window_case(17, [150, 60], 4, 2, 64, BF16)
+    starts = s["starts"].to(DEV)
+    leaves = [s[n].to(DEV).contiguous().requires_grad_() for n in "qkv"]
+    dout = s["dout"].to(DEV)
+
+    def step():
+        o = A.window_attention(ctx, *leaves, starts, window=50, sinks=2)
+        return [o.detach(), *torch.autograd.grad(o, leaves, dout)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t in (*leaves, dout):
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(i)).to(BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(made, step()):
+            assert torch.equal(x, y)
+
+
 def test_a_training_step(ctx):
     """Norm and rotation, then attention: gradients of a fused projection and both weights against 64 bits."""
     from tests import attention_cases as C

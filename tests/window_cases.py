@@ -69,7 +69,7 @@ def view_attention(q, keys, vals, table, cached, starts, mask, scale, k_scale, v
             k_scale, v_scale = (z[None, None].expand(pages, 1, kv) for z in (k_scale, v_scale))
         keys, vals = values(keys, k_scale), values(vals, v_scale)
         most_scale = float(v_scale.abs().max())
-    window = window or MANY
+    window, sinks = min(window or MANY, MANY), min(sinks, MANY)
     for b in range(table.shape[0]):
         r0, r1 = int(starts[b]), int(starts[b + 1])
         if r1 <= r0:
