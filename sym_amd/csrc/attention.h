@@ -109,6 +109,7 @@ struct AttendPlan {
   bool async;     // and rows of whole 16-byte pieces at 16-byte addresses
   int workgroups;
   bool quads;     // four heads of up to four rows at a time (int8 of a view)
+  bool whole;     // no item is cut (a view)
 };
 constexpr int kMostWorkgroups = 512; // two to a compute unit
 

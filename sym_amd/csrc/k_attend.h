@@ -40,7 +40,8 @@
 // head, tile of query rows), cut into equal runs, one per workgroup; an item
 // that lies in several runs leaves partial sums that k_attend_join adds up. So
 // one long context fills the card as well as many short ones do, and uneven
-// lengths cost nothing.
+// lengths cost nothing. A view's table of up to kWholeUnit tokens has units that hold
+// an item: there nothing is cut, and nothing joined.
 //
 // Measured, with the join (8 key heads of 128 each, unless said):
 //   64 requests of 1 row, 3000 int8 tokens on average, 32 key heads: 246 to 250
@@ -74,6 +75,9 @@ constexpr int kScan = 128;    // runs of requests whose units a workgroup (of at
 constexpr int kTile = 32;     // tokens of a tile
 constexpr int kSharedUnit = 64;
 constexpr int turn_unit(int dp) { return turn_waves(dp) * kTile; }
+// Unit of a call whose table holds no more tokens: no item is cut, so that no partial
+// sums are left, and no launch that joins them.
+constexpr int kWholeUnit = 512;
 // Rows of an item of four heads at a time (k_attend_quads), which fit the places of
 // sixteen, and its unit.
 constexpr int kQuadRows = 4, kQuadUnit = 4 * kTile;
@@ -132,6 +136,22 @@ __device__ __forceinline__ int64_t divide(int64_t n, int d) {
   if (__builtin_expect(n >> 32 == 0, 1))
     return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
   return n / d;
+}
+
+// Zeros for the rows of no request, where no join writes them.
+__device__ __forceinline__ void zero_unowned(const AttendArgs &a) {
+  const int r0 = min(max(a.starts[0], 0), a.rows), r1 = min(max(a.starts[a.requests], r0), a.rows);
+  const int64_t none = static_cast<int64_t>(r0 + a.rows - r1) * a.heads;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * waves + (threadIdx.x >> 6); i < none; i += static_cast<int64_t>(gridDim.x) * waves) {
+    int64_t row = i / a.heads;
+    const int64_t qh = i - row * a.heads;
+    row += row < r0 ? 0 : r1 - r0;
+    for (int d = lane; d < a.dim; d += 64)
+      store(a.out + (row * a.out_row + qh * a.out_head + d) * 2, static_cast<uint16_t>(0));
+    if (a.lse && lane == 0)
+      a.lse[row * a.heads + qh] = -__builtin_inff();
+  }
 }
 
 // ------------------------------------------------------------ the schedule
@@ -1082,13 +1102,13 @@ template <int FORM, int T, bool I8, int DP, int SRC, int NT, bool RAW, int PACE>
 
 // ---------------------------------------------------------- up to 16 rows
 
-template <int FORM, int T, bool I8, int DP, int SRC>
+template <int FORM, int T, bool I8, int DP, int SRC, int UNIT>
 __global__ __launch_bounds__(64 * turn_waves(DP), turn_workgroups(DP, I8, SRC == kAsync) == kMostWorkgroups ? 2 : 1)
 void k_attend_turns(AttendArgs a) {
-  constexpr int W = turn_waves(DP), UNIT = turn_unit(DP), ROWS = 16, E = DP / 16;
+  constexpr int W = turn_waves(DP), STEP = turn_unit(DP), ROWS = 16, E = DP / 16;
   constexpr int TILE = kTile * DP * (I8 ? 1 : 2);
   constexpr int RING = SRC == kAsync ? 2 : 1; // tiles of a wave
-  using Load = Loader<FORM, T, I8, DP, SRC, kTile, I8, UNIT>;
+  using Load = Loader<FORM, T, I8, DP, SRC, kTile, I8, STEP>;
   __shared__ int entries[SRC == kAsync ? W : 1][2][64];
   __shared__ float block_scales[FORM == kBlocks && SRC == kAsync ? W : 1][2][2][64];
 
@@ -1106,6 +1126,8 @@ void k_attend_turns(AttendArgs a) {
     load.scale_room = place(reinterpret_cast<const char *>(&block_scales[SRC == kAsync ? wave : 0][0][0][0]));
   Rows<FORM, T, DP, 1, I8, DP <= 128 && (I8 || SRC == kAsync)> r;
   const Reads<DP, I8> reads(lane);
+  if (UNIT == kWholeUnit)
+    zero_unowned(a);
   add_up<FORM, ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
 
@@ -1115,7 +1137,7 @@ void k_attend_turns(AttendArgs a) {
     const int rows = it.fresh * static_cast<int>(args_again().group.d) - row0; // of this tile and later ones
     load.item(args_again(), it);
     const int x_end = min(it.s1 * UNIT, it.reach), x0 = it.s0 * UNIT + wave * kTile;
-    const int count = x0 < x_end ? (x_end - x0 + UNIT - 1) / UNIT : 0; // this wave's tiles
+    const int count = x0 < x_end ? (x_end - x0 + STEP - 1) / STEP : 0; // this wave's tiles
     bool odd = false;
     auto start = [&] {
       const AttendArgs &b = args_again();
@@ -1143,14 +1165,14 @@ void k_attend_turns(AttendArgs a) {
       start(); // the queries arrive while the table does
 #pragma clang loop unroll(disable)
       for (int i = 0; i < min(count, RING); ++i)
-        send(load.look(i, x0 + i * UNIT, lane), i, i);
+        send(load.look(i, x0 + i * STEP, lane), i, i);
       typename Load::Next then = {}; // the next tile to send
       if (count > 0)
-        then = load.look(RING, x0 + RING * UNIT, lane);
+        then = load.look(RING, x0 + RING * STEP, lane);
       int x = x0;
       int slot = 0;
 #pragma clang loop unroll(disable)
-      for (int n = 0; n < count; ++n, x += UNIT) {
+      for (int n = 0; n < count; ++n, x += STEP) {
         if (n + RING <= count)
           arrived<(RING - 1) * 2 * Load::LOADS>();
         else
@@ -1162,7 +1184,7 @@ void k_attend_turns(AttendArgs a) {
         on >>= 2;
         if (n + RING < count)
           send(then, slot, RING - 1);
-        then = load.look(n + RING + 1, x + (RING + 1) * UNIT, lane);
+        then = load.look(n + RING + 1, x + (RING + 1) * STEP, lane);
         slot = slot + 1 == RING ? 0 : slot + 1;
       }
       arrived<0>(); // the last entries, wanted or not
@@ -1172,12 +1194,12 @@ void k_attend_turns(AttendArgs a) {
       int x = x0;
       if (count > 0)
         load.fetch(x);
-      for (int n = 0; n < count; ++n, x += UNIT) {
+      for (int n = 0; n < count; ++n, x += STEP) {
         load.put(tk, tv);
         const uint32_t seen = load.tokens_there();
         const Scales tile = load.fetched;
         if (n + 1 < count)
-          load.fetch(x + UNIT);
+          load.fetch(x + STEP);
         const int xt = it.token<FORM>(x);
         take_in(xt, seen, seen != 0xffffffffu || xt + kTile > it.cached || it.windowed<FORM>(xt, r.sinks), 0, tile);
       }
@@ -1202,7 +1224,7 @@ void k_attend_turns(AttendArgs a) {
         for (int e = 0; e < E; ++e)
           *reinterpret_cast<f32x4 *>(&sums[wave][c][e * 16 + 4 * g]) = r.acc[0][e] * f;
       if (!I8 && __builtin_expect(odd, 0))
-        r.add_odd(it, row0, rows, x0, x_end, UNIT, lane, [&](int, int d, float v) { sums[wave][c][d] += v * f; });
+        r.add_odd(it, row0, rows, x0, x_end, STEP, lane, [&](int, int d, float v) { sums[wave][c][d] += v * f; });
     }
     __syncthreads();
     constexpr int DIMS = 16 * DP / (64 * W); // of a thread: sixteen rows over the workgroup
@@ -1255,8 +1277,8 @@ void k_attend_turns(AttendArgs a) {
 // The same where a token's heads lie side by side: each wave has a head of its own,
 // so that what the four read of a token is one piece of memory, 512 bytes for int8
 // heads of 128. Nothing is added up between waves.
-template <int T, int DP> __global__ __launch_bounds__(256, 2) void k_attend_quads(AttendArgs a) {
-  constexpr int W = 4, UNIT = kQuadUnit, ROWS = kQuadRows, E = DP / 16, TILE = kTile * DP, RING = 2;
+template <int T, int DP, int UNIT> __global__ __launch_bounds__(256, 2) void k_attend_quads(AttendArgs a) {
+  constexpr int W = 4, ROWS = kQuadRows, E = DP / 16, TILE = kTile * DP, RING = 2;
   using Load = Loader<kBlocks, T, true, DP, kAsync, kTile, true, kTile>;
   __shared__ int entries[W][2][64];
   __shared__ float block_scales[W][2][2][64];
@@ -1274,6 +1296,8 @@ template <int T, int DP> __global__ __launch_bounds__(256, 2) void k_attend_quad
     for (int i = lane * 16; i < RING * 2 * TILE; i += 64 * 16)
       *reinterpret_cast<u32x4 *>(&tiles[wave][0][0][0] + i) = u32x4{0u, 0u, 0u, 0u};
   shared_done();
+  if (UNIT == kWholeUnit)
+    zero_unowned(a);
   add_up<kBlocks, ROWS, UNIT>(a, schedule);
   Run run = my_run(schedule);
 
@@ -1769,7 +1793,7 @@ hipError_t attend_start(const void *kernel, int threads, const AttendArgs &args,
   hipError_t e = hipSuccess;
   if (a.requests > 0)
     e = hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(p.workgroups)), dim3(static_cast<uint32_t>(threads)), pa, 0, s);
-  if (e != hipSuccess)
+  if (e != hipSuccess || (UNIT == kWholeUnit && a.requests > 0))
     return e;
   // A wave for every piece of an even batch, within 2^16 blocks a request; eight
   // where an item lies in more than eight runs, on average: 6.7 us against 10.0
@@ -1808,12 +1832,18 @@ template <int FORM, int T, bool I8, int DP>
 hipError_t attend_source(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   if constexpr (FORM == kBlocks && DP <= 128)
     if (p.quads)
-      return attend_start<FORM, T, I8, DP, kQuadRows, kQuadUnit>(reinterpret_cast<const void *>(k_attend_quads<T, DP>), 256, a,
-                                                                 p, s);
+      return p.whole ? attend_start<FORM, T, I8, DP, kQuadRows, kWholeUnit>(
+                           reinterpret_cast<const void *>(k_attend_quads<T, DP, kWholeUnit>), 256, a, p, s)
+                     : attend_start<FORM, T, I8, DP, kQuadRows, kQuadUnit>(
+                           reinterpret_cast<const void *>(k_attend_quads<T, DP, kQuadUnit>), 256, a, p, s);
+  if constexpr (FORM != kWhole)
+    if (p.whole)
+      return attend_start<FORM, T, I8, DP, 16, kWholeUnit>(
+          reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kAsync, kWholeUnit>), 64 * turn_waves(DP), a, p, s);
   if (p.rows == 16)
     return attend_start<FORM, T, I8, DP, 16, turn_unit(DP)>(
-        p.async ? reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kAsync>)
-                : reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kStaged>),
+        p.async ? reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kAsync, turn_unit(DP)>)
+                : reinterpret_cast<const void *>(k_attend_turns<FORM, T, I8, DP, kStaged, turn_unit(DP)>),
         64 * turn_waves(DP), a, p, s);
   // int8 is widened once for all waves, on its way through registers
   if constexpr (FORM == kBlocks)

@@ -153,7 +153,7 @@ template <int DP, int NT> struct Bring {
   __device__ __forceinline__ void send(const char *base, uint32_t row, int left, uint32_t to) const {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      // LOADS tokens on: the low bits of the token's swap are the lane's
+      // TPI tokens on: of the swap's bits, those that the lane's token has stay
       const int n = piece0 ^ (swap_of<RB>(i * TPI));
       const int t = min(first + i * TPI + token, left - 1);
       if (n * 8 < dims)
@@ -254,12 +254,10 @@ template <int T, int E> struct Over {
 
 // A workgroup's query rows: (token, head of the group) in this order, 128 at most.
 struct RowsOf {
-  int begin, n, real, first, tokens, head, heads; // of the sequence; of this tile
+  int first, tokens, head, heads;
   __device__ __forceinline__ RowsOf(const WindowArgs &a, const Piece &p, int which) {
-    begin = p.begin;
-    n = p.n;
     first = p.index * static_cast<int>(a.tile_tokens.d);
-    tokens = min(static_cast<int>(a.tile_tokens.d), n - first);
+    tokens = min(static_cast<int>(a.tile_tokens.d), p.n - first);
     const int parts = a.parts, kv = which / parts, part = which - kv * parts;
     const int group = a.heads / a.kv_heads;
     head = kv * group + part * static_cast<int>(a.tile_heads.d);

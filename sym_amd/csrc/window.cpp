@@ -294,14 +294,23 @@ int relx_tree_attention_view(relx_ctx *ctx, const relx_tree_attention_args *args
       plan.workgroups = a.workgroups = relx::kMostWorkgroups;
       a.once = false;
     }
+    // A table of up to 512 tokens: items are not cut, and nothing is left to join. us in
+    // a graph, whole and cut, 8 key heads of 128, four rows each:
+    //   bf16   1 request of 60 tokens 9.6, 11.5   of 440 13.1, 12.7   64 of up to 440 26.3, 40.3   256: 94, 120
+    //   int8   7.9, 9.8   10.9, 10.8   15.9, 19.3   256: 42.5, 48.5 (four heads at a time)
+    // and calls from Python 2 less than that, which the second launch took.
+    plan.whole = plan.rows == 16 && plan.async && p.columns * p.cache.page <= 512;
     // Four int8 heads at a time, a wave each, where a token's heads lie closer together
     // than a head's tokens: 64 requests of up to 8192 tokens of 8 key heads, four rows
     // each, us with heads of 128: 135 against 153, of 80: 153 against 202, of 64: 97
     // against 131; of up to 512: 19.4 against 23.4; one of 100000: 48 against 51. Eight
     // of up to 1000 have too little for it (18.4 against 15.7): so not where the table
-    // holds less than 2^17 tokens of all heads.
-    plan.quads = i8 && p.requests * p.columns * p.cache.page >= (1 << 17) / p.cache.kv_heads && plan.async && plan.rows == 16 && plan.width <= 128 && p.cache.kv_heads % 4 == 0 &&
-                 (p.rows + p.requests - 1) / std::max<int64_t>(p.requests, 1) * (p.heads / p.cache.kv_heads) <= 4 &&
+    // holds less than 2^17 tokens of all heads, nor for whole items that the card holds
+    // at once (64 requests of up to 250 tokens: 21.0 against 11.7; 256: 25.5, 37.9).
+    const int64_t kv = p.cache.kv_heads, tokens = p.columns * p.cache.page;
+    const bool much = plan.whole ? p.requests * kv > relx::kMostWorkgroups : p.requests * tokens >= (1 << 17) / kv;
+    plan.quads = i8 && much && plan.async && plan.rows == 16 && plan.width <= 128 && kv % 4 == 0 &&
+                 (p.rows + p.requests - 1) / std::max<int64_t>(p.requests, 1) * (p.heads / kv) <= 4 &&
                  p.cache.key_head < p.cache.key_slot && p.cache.value_head < p.cache.value_slot;
     relx::attend_room(a, plan, p);
     relx::on_context(ctx, [&] {

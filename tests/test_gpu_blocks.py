@@ -163,6 +163,28 @@ def test_four_heads_at_a_time(ctx, cached, fresh, heads, kv, dim, page, block, w
         assert float((got.float() - other.float()).abs().max()) < 0.05
 
 
+@pytest.mark.parametrize("kv,requests", [(8, 70), (4, 3)])
+def test_small_tables(ctx, kv, requests):
+    """Nothing is cut or joined; with many heads of many requests four at a time."""
+    cached = [(i * 37) % 200 for i in range(requests)]
+    fresh = [1 + (i == 2) for i in range(requests)]
+    s = W.view_case(18, cached, fresh, kv, kv, 16, BF16, I8, 64, 16)
+    check_view(ctx, s, "small tables", 90, 3)
+    wide = on_gpu(s)
+    rows = s["q"].shape[0]
+    q = torch.cat([wide["q"], wide["q"], wide["q"]])  # rows of no request before and after
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=DEV)
+    A.tree_attention(ctx, q, wide["cache_k"], wide["cache_v"], wide["table"], wide["cached"], wide["starts"] + rows,
+                     scale=wide["scale"], k_scale=wide["k_scale"], v_scale=wide["v_scale"], window=90, sinks=3, out=out, lse=lse)
+    assert not out[:rows].any() and not out[2 * rows:].any() and out[rows:2 * rows].any()
+    assert (lse[:rows] == -float("inf")).all() and (lse[2 * rows:] == -float("inf")).all()
+    none = torch.zeros((0, s["table"].shape[1]), dtype=torch.int32, device=DEV)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = A.tree_attention(ctx, q, wide["cache_k"], wide["cache_v"], none, zero[:0], zero, k_scale=wide["k_scale"],
+                           v_scale=wide["v_scale"])
+    assert not got.any()
+
+
 @pytest.mark.parametrize("cache", ["own", "int8", "blocks"])
 @pytest.mark.parametrize("cached,fresh,heads,kv,dim,page,window,sinks", [
     ([0], [1], 2, 1, 64, 16, 1, 0),
