@@ -765,7 +765,8 @@ int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_
  * wanted, is [heads, rows], natural logarithms. Rows of no sequence are 0 with
  * lse -inf, and nothing of one sequence reaches another; what is not finite may
  * reach any row of its own. f16 or bf16, head sizes of multiples of 8 up to 128,
- * rows and heads at 16-byte addresses, rows at most 2^24 elements apart. */
+ * rows and heads at 16-byte addresses, rows at most 2^24 elements apart and 2^29 of
+ * them. `scale` may have either sign or be zero. */
 typedef struct relx_window_args {
   relx_heads q, k, v, out;
   const int32_t *starts; /* [sequences + 1] */
