@@ -530,10 +530,12 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
   int from[FORM == kWhole ? 1 : RT]; // where a row's window begins
   int sinks;
   // kBlocks: the values' scales go into the weights of the second product. In f16
-  // they go there over the largest so far, a power of two, which the sums are of:
-  // else weights of up to 2^14 times a scale of four would be none.
+  // they go there over the largest that the row has seen so far, a power of two, of
+  // which its sums are: else weights of up to 2^14 times a scale of four would be none.
+  // For each row, since a page that it does not see may hold anything.
   static constexpr bool kOver = FORM == kBlocks && T == kF16;
-  float over;
+  float back[kOver ? RT : 1]; // one over it: from 2^126, of the least normal number, to 2^-127
+  __device__ __forceinline__ float whole(int t) const { return kOver ? 1.0f / back[kOver ? t : 0] : 1.0f; }
 
   __device__ __forceinline__ void start(const AttendArgs &a, const Item &it, int row0, int rows, float score_scale,
                                         int lane) {
@@ -546,9 +548,10 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
     scale = fabsf(score_scale) < kLeast ? kLeast : fabsf(score_scale);
     words = a.mask ? a.words : 0;
     sinks = FORM == kWhole ? 0 : a.sinks;
-    over = 0.0f;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
+      if constexpr (kOver)
+        back[t] = 0x1p126f;
       const uint32_t p = static_cast<uint32_t>(row0 + t * 16 + c);
       const uint32_t j = fdiv(p, a.group);
       place[t] = static_cast<int>(j);
@@ -653,22 +656,6 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       for (int n = 0; n < 2; ++n)
         if (!(seen >> (16 * n) & 0xffffu))
           v[n] = 0.0f; // of no token: may be anything
-      if constexpr (kOver) {
-        const float most = fmaxf(fabsf(v[0]), fabsf(v[1]));
-        if (__builtin_expect(most > over, 0)) {
-          const float next = __uint_as_float((__float_as_uint(most) & 0x7f800000u) + 0x00800000u);
-          const float shrink = over / next;
-          over = next;
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-              acc[t][e] *= shrink;
-        }
-        const float back = over > 0.0f ? 1.0f / over : 0.0f; // over: a power of two
-        v[0] *= back;
-        v[1] *= back;
-      }
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         values[t][0] = v[0];
@@ -697,6 +684,32 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
             if (!(bits >> (n * 16 + 4 * g + i) & 1u))
               s[t][n][i] = -__builtin_inff();
       }
+    }
+
+    if constexpr (kOver) {
+      bool larger = false;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        larger |= fmaxf(fabsf(values[t][0]), fabsf(values[t][1])) * back[t] > 1.0f;
+      if (__builtin_expect(__any(larger), 0)) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          // below 2^n, and at least half of it; 0: of no token that the row sees
+          const float size = fmaxf(fabsf(values[t][0]), fabsf(values[t][1]));
+          const int n = min(__builtin_amdgcn_frexp_expf(size), 127);
+          const float next = size > 0.0f ? fminf(back[t], __builtin_amdgcn_ldexpf(1.0f, -n)) : back[t];
+          const float shrink = next / back[t];
+          back[t] = next;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            acc[t][e] *= shrink;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          values[t][n] *= back[t];
     }
 
     float most[RT];
@@ -1218,7 +1231,7 @@ void k_attend_turns(AttendArgs a) {
 #pragma unroll
       for (int w = 0; w < W; ++w)
         most = fmaxf(most, row_max[w][c]);
-      const float f = __builtin_amdgcn_exp2f(r.top[0] - most) * (r.kOver ? r.over : 1.0f);
+      const float f = __builtin_amdgcn_exp2f(r.top[0] - most) * r.whole(0);
       if (c < rows)
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -1344,7 +1357,7 @@ template <int T, int DP, int UNIT> __global__ __launch_bounds__(256, 2) void k_a
     arrived<0>(); // the last entries, wanted or not
 
     const AttendArgs &b = args_again();
-    const float sum = r.total(0), over = r.kOver ? r.over : 1.0f;
+    const float sum = r.total(0), over = r.whole(0);
     if (c < rows) {
       if (it.s0 == 0 && it.s1 == it.units) {
         const uint32_t p = static_cast<uint32_t>(row0 + c);
@@ -1610,7 +1623,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           const uint32_t j = fdiv(p, b.group);
           const int64_t row = it.start + static_cast<int64_t>(j);
           const int64_t qh = static_cast<int64_t>(it.head) * b.group.d + (p - j * b.group.d);
-          const float f = finish(sum, I8 && FORM != kBlocks ? b.value_scale[it.head] : 1.0f) * (r.kOver ? r.over : 1.0f);
+          const float f = finish(sum, I8 && FORM != kBlocks ? b.value_scale[it.head] : 1.0f) * r.whole(t);
           char *dst = b.out + (row * b.out_row + qh * b.out_head + 4 * g) * 2;
 #pragma unroll
           for (int e = 0; e < E; ++e)
@@ -1625,7 +1638,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_shared(AttendArgs a) {
           float *dst = b.partial + (part - c) * DP + part_at<DP, ROWS>(c, 4 * g);
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            *reinterpret_cast<f32x4 *>(dst + e * 256) = r.kOver ? r.acc[t][e] * r.over : r.acc[t][e];
+            *reinterpret_cast<f32x4 *>(dst + e * 256) = r.kOver ? r.acc[t][e] * r.whole(t) : r.acc[t][e];
           if (g == 0) {
             b.stats[part * 2] = r.top[t];
             b.stats[part * 2 + 1] = sum;
