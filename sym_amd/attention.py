@@ -567,10 +567,10 @@ def _view(window, sinks):
 class _Window(torch.autograd.Function):
     @staticmethod
     def forward(fn, q, k, v, ctx, starts, window, sinks, scale, lse):
-        if lse is None:
-            lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
-        out = _window_attention(ctx, q, k, v, starts, window, sinks, scale, None, lse)
-        fn.save_for_backward(q, k, v, out, lse, starts)
+        # the backward's own: the caller's buffer may be another call's before that runs
+        own = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32) if lse is None else lse
+        out = _window_attention(ctx, q, k, v, starts, window, sinks, scale, None, own)
+        fn.save_for_backward(q, k, v, out, own if lse is None else lse.clone(), starts)
         fn.rest = ctx, window, sinks, scale
         return out
 
