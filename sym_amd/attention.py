@@ -31,6 +31,7 @@ from collections import namedtuple
 from functools import lru_cache, partial
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -184,6 +185,15 @@ def _in_graph(*operands):
     return False
 
 
+def _no_tangent(name, *operands):
+    """Refuses what carries a forward-mode derivative: the result would have none,
+    which says that it is zero."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in operands:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("sym_amd.attention.%s has no forward-mode derivative" % name)
+
+
 class _NoGradient(torch.autograd.Function):
     """A call that has no gradient, of operands that want one: its result says so
     when a gradient reaches it, rather than end it in silence."""
@@ -320,7 +330,8 @@ def norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, *, pair
     (i, i + rotary / 2), or neighbours (2 i, 2 i + 1) with `pairs`. A position
     outside the table gives NaN. Returns (queries, keys); `out`: a pair of
     tensors to write into. Differentiable in q, k and the weights, once (without
-    `out`; a second derivative, or one by cos and sin, raises)."""
+    `out`; a second derivative, one by cos and sin, or one of forward mode raises)."""
+    _no_tangent("norm_rotate", q, k, q_weight, k_weight, cos, sin)
     if out is None and _in_graph(q, k, q_weight, k_weight, cos, sin):
         return _NormRotate.apply(q, k, q_weight, k_weight, ctx, positions, cos, sin, eps, pairs)
     return _norm_rotate(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs, out)
@@ -347,6 +358,7 @@ def norm_rotate_backward(ctx, dq, dk, q, k, positions, cos, sin, q_weight, k_wei
     [dim], summed over rows and heads in a fixed order (None where the weight
     is, or where `weight_grads` says that it is not wanted); the others have the
     operands' type."""
+    _no_tangent("norm_rotate_backward", dq, dk, q, k, q_weight, k_weight, cos, sin)
     rot, qs, ks, device = _rotation(ctx, q, k, positions, cos, sin, q_weight, k_weight, eps, pairs)
     dtype = q.dtype
     gq, gk = q.new_empty(qs), k.new_empty(ks)
@@ -396,6 +408,7 @@ def norm_rotate_append(ctx, q, k, v, slots, cache_k, cache_v, positions, cos, si
     int8 with a scale a head (float32 [kv_heads] each), quantized as the
     package's plans quantize. There is no gradient: one that reaches the result
     (without `out`) raises."""
+    _no_tangent("norm_rotate_append", q, k, v, cos, sin, q_weight, k_weight)
     if out is None and _in_graph(q, k, v, cos, sin, q_weight, k_weight):
         return _NoGradient.apply(
             "norm_rotate_append",
@@ -433,6 +446,7 @@ def block_append(ctx, k, v, cache_k, cache_v, k_scale, v_scale, table, cached, s
     not in the cache are left out; a block is of one request that writes to it.
     Caches and scales are updated in place; there is no gradient, so keys or values
     that want one are refused (in a graph, detach them)."""
+    _no_tangent("block_append", k, v)
     if _in_graph(k, v):
         _bad("block_append has no gradient: it takes detached keys and values, or runs under torch.no_grad()")
     device = _device(ctx, k)
@@ -494,6 +508,7 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     uint8 tensor of `tree_attention_workspace` bytes, for programs that keep
     one a stream; by default torch's allocator gives it. There is no gradient:
     one that reaches the result (without `out`) raises."""
+    _no_tangent("tree_attention", q, cache_k, cache_v, k_scale, v_scale)
     if out is None and _in_graph(q, cache_k, cache_v, k_scale, v_scale):
         return _NoGradient.apply(
             "tree_attention",
@@ -624,7 +639,9 @@ def window_attention(ctx, q, k, v, starts, *, window=None, sinks=0, scale=None, 
     (None: any), and the first `sinks` ones (256 at most). Rows of no sequence are
     0, and nothing of one sequence reaches another. `scale`: of the scores, by
     default dim ** -0.5. `lse`: float32 [heads, rows] for the logarithm of each row's
-    sum of exponentials. Differentiable in q, k and v, once (without `out`)."""
+    sum of exponentials. Differentiable in q, k and v, once (without `out`; a second
+    derivative, or one of forward mode, raises)."""
+    _no_tangent("window_attention", q, k, v)
     if out is None and _in_graph(q, k, v):
         return _Window.apply(q, k, v, ctx, starts, window, sinks, scale, lse)
     return _window_attention(ctx, q, k, v, starts, window, sinks, scale, out, lse)
@@ -642,6 +659,7 @@ def window_attention_backward(ctx, dout, q, k, v, out, lse, starts, *, window=No
     """Gradients of `window_attention` for its result's gradient `dout`, from its
     result and its `lse`: (queries', keys', values'), of the operands' type; those of
     keys and values are summed over a key head's query heads. The same bits every time."""
+    _no_tangent("window_attention_backward", dout, q, k, v, out, lse)
     args, device = _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale)
     if lse is None:
         _bad("the backward takes the forward's lse")

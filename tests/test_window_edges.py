@@ -4,6 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 from sym_amd import attention as A  # noqa: E402
+from torch.autograd import forward_ad as F  # noqa: E402
 
 
 class Ctx:
@@ -32,3 +33,61 @@ def test_one_lse_buffer_for_two_calls(sums):
     for q, out in zip(leaves, outs):
         out.sum().backward()
     assert (leaves[0].grad == 48.0).all() and (leaves[1].grad == 96.0).all()
+
+
+# ------------------------------------------------------------ forward mode
+
+def calls():
+    """Each call by name, with the operands that may carry a derivative."""
+    h = [torch.zeros((2, n, 8), dtype=torch.float16) for n in (4, 2, 2)]
+    cache = [torch.zeros((3, 16, 2, 8), dtype=torch.float16) for _ in range(2)]
+    codes = [torch.zeros((3, 16, 2, 8), dtype=torch.int8) for _ in range(2)]
+    scales = [torch.ones((3, 1, 2)) for _ in range(2)]
+    i32 = torch.zeros(3, dtype=torch.int32)
+    w, cos, sin = torch.ones(8, dtype=torch.float16), torch.ones((1, 4)), torch.ones((1, 4))
+    step = i32[:2, None], i32[:2], i32
+    return {
+        "norm_rotate": (lambda q, k, w, c, s: A.norm_rotate(Ctx, q, k, i32[:2], c, s, w, None, 1e-6), [*h[:2], w, cos, sin]),
+        "norm_rotate_backward": (lambda dq, dk, q, w: A.norm_rotate_backward(Ctx, dq, dk, q, h[1], i32[:2], cos, sin, w, None, 1e-6),
+                                 [*h[:2], h[0], w]),
+        "norm_rotate_append": (lambda q, k, v, w, c: A.norm_rotate_append(Ctx, q, k, v, torch.zeros(2, dtype=torch.int64), *cache,
+                                                                          i32[:2], c, sin, w, None, 1e-6), [*h, w, cos]),
+        "block_append": (lambda k, v: A.block_append(Ctx, k, v, *codes, *scales, *step), h[1:]),
+        "tree_attention": (lambda q, k, v: A.tree_attention(Ctx, q, k, v, *step), [h[0], *cache]),
+        "window_attention": (lambda q, k, v: A.window_attention(Ctx, q, k, v, i32), h),
+        "window_attention_backward": (lambda d, q, k, v: A.window_attention_backward(Ctx, d, q, k, v, h[0], torch.zeros((4, 2)), i32),
+                                      [h[0], *h]),
+    }
+
+
+@pytest.mark.parametrize("name", list(calls()))
+def test_a_forward_mode_derivative_raises(monkeypatch, name):
+    """It does not end in a result that says zero; without one the call runs, in such a block too."""
+    made = []
+    monkeypatch.setattr(A, "_call", lambda name, ctx, *args: made.append(name))
+    monkeypatch.setattr(A, "_device", lambda ctx, like: like.get_device())
+    monkeypatch.setattr(A, "_stream", lambda device: 0)
+    monkeypatch.setattr(A, "_rotate_room", lambda *sizes: 64)
+    monkeypatch.setattr(A, "_window_room", lambda *sizes: 64)
+    call, operands = calls()[name]
+    call(*operands)
+    with F.dual_level():
+        call(*operands)
+        assert made == ["relx_" + name] * 2
+        for i, t in enumerate(operands):
+            dual = [F.make_dual(t, torch.ones_like(t)) if k == i else x for k, x in enumerate(operands)]
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(RuntimeError, match="sym_amd.attention.%s has no forward-mode derivative" % name):
+                    call(*dual)
+        call(*operands)
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda q: call(q, *operands[1:]), (operands[0],), (operands[0],))
+    assert made == ["relx_" + name] * 3
+
+
+def test_a_forward_mode_derivative_of_a_gradient_raises(monkeypatch):
+    monkeypatch.setattr(A, "_window_attention", lambda ctx, q, k, v, starts, window, sinks, scale, out, lse: q + k + v)
+    q = torch.ones((3, 2, 8)).requires_grad_()
+    out = A.window_attention(Ctx, q, q.detach(), q.detach(), torch.zeros(2, dtype=torch.int32))
+    with F.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.autograd.grad(out, q, F.make_dual(torch.ones_like(out), torch.ones_like(out)))
