@@ -761,7 +761,8 @@ int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_
 /* Attention over packed sequences, for training and for prompts: sequence b has
  * the rows [starts[b], starts[b + 1]) of q and out [rows, heads, dim] and of k and
  * v [rows, kv_heads, dim]. A row at place p of its sequence sees the places x <= p
- * with p - x < window (0: any) or x < sinks (256 at most). lse, where it is
+ * with p - x < window (0: any) or x < sinks (256 at most, unless no row leaves the
+ * window). lse, where it is
  * wanted, is [heads, rows], natural logarithms. Rows of no sequence are 0 with
  * lse -inf, and nothing of one sequence reaches another; what is not finite may
  * reach any row of its own. f16 or bf16, head sizes of multiples of 8 up to 128,

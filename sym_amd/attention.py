@@ -636,7 +636,8 @@ def window_attention(ctx, q, k, v, starts, *, window=None, sinks=0, scale=None, 
     reads key head h // (heads // kv_heads).
 
     A row at place p of its sequence sees the places x <= p with p - x < `window`
-    (None: any), and the first `sinks` ones (256 at most). Rows of no sequence are
+    (None: any), and the first `sinks` ones (256 at most, unless no row leaves the
+    window). Rows of no sequence are
     0, and nothing of one sequence reaches another. `scale`: of the scores, by
     default dim ** -0.5. `lse`: float32 [heads, rows] for the logarithm of each row's
     sum of exponentials. Differentiable in q, k and v, once (without `out`; a second

@@ -111,7 +111,9 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   layout(p.dim >= 8 && p.dim <= 128 && p.dim % 8 == 0, "window attention: head sizes are multiples of 8 up to 128");
   layout(p.rows <= kMost / 2, "window attention: more than 2^29 rows");
   need(p.window >= 0 && p.sinks >= 0, "window attention: a negative window or number of first tokens");
-  layout(p.sinks <= kMostSinks, "window attention: more than 256 first tokens");
+  const int64_t window = p.window == 0 ? kMost : std::min(p.window, kMost);
+  const int64_t sinks = window >= p.rows ? 0 : p.sinks; // of a window that no row leaves: none apart
+  layout(sinks <= kMostSinks, "window attention: more than 256 first tokens");
   const float scale = static_cast<float>(p.scale * 1.4426950408889634);
   need(std::isfinite(scale), "window attention: scale");
   need(p.rows == 0 || p.starts, "window attention: null starts");
@@ -123,8 +125,8 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   a.heads = static_cast<int32_t>(p.heads);
   a.kv_heads = static_cast<int32_t>(p.kv_heads);
   a.dim = static_cast<int32_t>(p.dim);
-  a.window = static_cast<int32_t>(p.window == 0 ? kMost : std::min(p.window, kMost));
-  a.sinks = static_cast<int32_t>(a.window >= a.rows ? 0 : p.sinks); // a window that no row leaves
+  a.window = static_cast<int32_t>(window);
+  a.sinks = static_cast<int32_t>(sinks);
   // By a scale below 2^-64 no score within f16's and bf16's usual range reaches a
   // bit of a weight: then 2^-64, by which the kernels divide.
   a.scale = std::fabs(scale) < 0x1p-64f ? std::copysign(0x1p-64f, scale) : scale;

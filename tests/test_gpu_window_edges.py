@@ -1,8 +1,9 @@
 """Attention over packed sequences and its gradients, on the GPU: buffers that calls
-share."""
+share, numbers of first tokens."""
 import pytest
 
 from tests import window_cases as W
+from tests.test_gpu_window import check
 
 torch = pytest.importorskip("torch")
 from sym_amd import attention as A  # noqa: E402
@@ -46,3 +47,9 @@ def test_one_lse_buffer_for_two_calls(ctx):
     for out, own, leaves, dout in outs:
         for x, y in zip(torch.autograd.grad(out, leaves, dout), torch.autograd.grad(own, leaves, dout)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("sinks", [257, 1000])
+def test_first_tokens_that_every_window_holds(ctx, sinks):
+    """However many, where no row leaves the window."""
+    check(ctx, W.window_case(34, [90, 40], 2, 1, 64, BF16), "first tokens", 130, sinks)

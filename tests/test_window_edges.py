@@ -1,10 +1,14 @@
 """What torch's graph and the C boundary make of window attention's calls that other
 tests do not make, without a GPU."""
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
-from sym_amd import attention as A  # noqa: E402
 from torch.autograd import forward_ad as F  # noqa: E402
+from sym_amd import _native as N  # noqa: E402
+from sym_amd import attention as A  # noqa: E402
+from tests.test_window_api import refused, window_args  # noqa: E402
 
 
 class Ctx:
@@ -91,3 +95,23 @@ def test_a_forward_mode_derivative_of_a_gradient_raises(monkeypatch):
     out = A.window_attention(Ctx, q, q.detach(), q.detach(), torch.zeros(2, dtype=torch.int32))
     with F.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         torch.autograd.grad(out, q, F.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+# ------------------------------------------------------------ sizes
+
+def workspace(**more):
+    n, err = ctypes.c_size_t(), N.relx_err()
+    assert N.lib().relx_window_attention_workspace(bytes(window_args(**more)), ctypes.byref(n), ctypes.byref(err)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("window", [0, 100, 2 ** 62])
+def test_first_tokens_of_a_window_that_no_row_leaves(window):
+    """However many: every row sees them without."""
+    for sinks in (257, 2 ** 40):
+        args = window_args(rows=100, window=window, sinks=sinks)
+        assert "null context" in refused(N.lib().relx_window_attention, None, bytes(args), 0)[1]
+        assert workspace(rows=100, window=window, sinks=sinks) == workspace(rows=100, window=0, sinks=0)
+    if window:
+        more = window_args(rows=101, window=min(window, 100), sinks=257)
+        assert refused(N.lib().relx_window_attention, None, bytes(more), 0)[0] == "unsupported_layout"
