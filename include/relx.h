@@ -762,10 +762,9 @@ int relx_block_append(relx_ctx *ctx, const relx_block_append_args *args, uint64_
  * the rows [starts[b], starts[b + 1]) of q and out [rows, heads, dim] and of k and
  * v [rows, kv_heads, dim]. A row at place p of its sequence sees the places x <= p
  * with p - x < window (0: any) or x < sinks (256 at most, unless no row leaves the
- * window). lse, where it is
- * wanted, is [heads, rows], natural logarithms. Rows of no sequence are 0 with
- * lse -inf, and nothing of one sequence reaches another; what is not finite may
- * reach any row of its own. f16 or bf16, head sizes of multiples of 8 up to 128,
+ * window). lse, where it is wanted, is [heads, rows], natural logarithms. Rows of no
+ * sequence are 0 with lse -inf, and nothing of one sequence reaches another; what is
+ * not finite may reach any row of its own. f16 or bf16, head sizes of multiples of 8 up to 128,
  * rows and heads at 16-byte addresses, rows at most 2^24 elements apart and 2^29 of
  * them. `scale` may have either sign or be zero. */
 typedef struct relx_window_args {

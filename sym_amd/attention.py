@@ -496,8 +496,8 @@ def tree_attention(ctx, q, cache_k, cache_v, table, cached, starts, *, mask=None
     itself (one row a request: plain decoding). Head h reads key head
     h // (heads // kv_heads). A row that sees nothing, or of no request, is 0.
 
-    `window`: a row at position p sees of the tokens x only those with
-    p - x < window, and the first `sinks` ones; p is cached + j, or with a mask
+    `window` (None or 0: of everything): a row at position p sees of the tokens x
+    only those with p - x < window, and the first `sinks` ones; p is cached + j, or with a mask
     cached + the token's depth in its tree, of which it sees what its mask says
     (the window has to hold the tree: 64 * words at least). An int8 cache
     with a scale a block of tokens, as `block_append` fills it, has scales
@@ -636,7 +636,7 @@ def window_attention(ctx, q, k, v, starts, *, window=None, sinks=0, scale=None, 
     reads key head h // (heads // kv_heads).
 
     A row at place p of its sequence sees the places x <= p with p - x < `window`
-    (None: any), and the first `sinks` ones (256 at most, unless no row leaves the
+    (None or 0: any), and the first `sinks` ones (256 at most, unless no row leaves the
     window). Rows of no sequence are
     0, and nothing of one sequence reaches another. `scale`: of the scores, by
     default dim ** -0.5. `lse`: float32 [heads, rows] for the logarithm of each row's

@@ -115,3 +115,10 @@ def test_first_tokens_of_a_window_that_no_row_leaves(window):
     if window:
         more = window_args(rows=101, window=min(window, 100), sinks=257)
         assert refused(N.lib().relx_window_attention, None, bytes(more), 0)[0] == "unsupported_layout"
+
+
+def test_no_window_is_none_or_zero():
+    assert A._reach(None, 0) == A._reach(0, 0) == (0, 0) and A._reach(10 ** 30, 3) == (2 ** 62, 3)
+    for window in (None, 0):
+        with pytest.raises(ValueError, match="first ones"):
+            A._reach(window, 2)
