@@ -721,10 +721,11 @@ typedef struct relx_block_scales {
 } relx_block_scales;
 
 /* What attention sees of a cache. A row at position p (cached + j, or cached +
- * its depth in the tree that its mask says) sees the cached tokens x with
- * x < sinks or p - x < window, and of the request's own those that it would see
- * without a window, with the same rule where there is no mask. window 0: of
- * everything. With a mask the window holds the tree: at least 64 words.
+ * its depth in the tree that its mask says, whose bits beyond the request's rows
+ * say nothing) sees the cached tokens x with x < sinks or p - x < window, and of
+ * the request's own those that it would see without a window, with the same rule
+ * where there is no mask. window 0: of everything. With a mask the window holds
+ * the tree: at least 64 words.
  * `scales`: of an int8 cache, instead of the cache's scales a head, which are
  * then not read (block 0: none). Any other argument and the workspace are
  * relx_tree_attention's. */

@@ -296,13 +296,17 @@ __device__ __forceinline__ int window_from(const AttendArgs &a, int cached, int 
   const int64_t from = static_cast<int64_t>(cached) + d - a.window + 1;
   return static_cast<int>(max(min(from, int64_t{1} << 30), int64_t{0}));
 }
-// The d of a row: the token's depth in its tree, or j.
-__device__ __forceinline__ int row_depth(const AttendArgs &a, int start, int j) {
+// The d of a row: the token's depth in its tree, or j. Of a mask's bits those of the
+// request's `fresh` tokens count: the others are no tokens, and items are laid out
+// for depths below fresh.
+__device__ __forceinline__ int row_depth(const AttendArgs &a, int start, int fresh, int j) {
   if (!a.mask)
     return j;
   int n = 0;
-  for (int w = 0; w < a.words; ++w)
-    n += __builtin_popcountll(static_cast<uint64_t>(a.mask[(start + static_cast<int64_t>(j)) * a.words + w]));
+  for (int w = 0, left = fresh; w < a.words && left > 0; ++w, left -= 64) {
+    const uint64_t word = static_cast<uint64_t>(a.mask[(start + static_cast<int64_t>(j)) * a.words + w]);
+    n += __builtin_popcountll(left >= 64 ? word : word & ((uint64_t{1} << left) - 1));
+  }
   return max(n - 1, 0);
 }
 // Of the 32 tokens from x: the first ones, and those from `from` on.
@@ -559,7 +563,7 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       if (words == 1 && place[t] < it.fresh)
         mask[t] = static_cast<uint64_t>(a.mask[it.start + static_cast<int64_t>(j)]);
       if constexpr (FORM != kWhole)
-        from[t] = place[t] < it.fresh ? window_from(a, it.cached, row_depth(a, it.start, place[t])) : 0;
+        from[t] = place[t] < it.fresh ? window_from(a, it.cached, row_depth(a, it.start, it.fresh, place[t])) : 0;
       const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
                                (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma unroll

@@ -1,5 +1,5 @@
 """What reaches a result of attention over a cache with a window, and what must not:
-scales of blocks that a row does not see."""
+scales of blocks that a row does not see, bits of a mask beyond a request's rows."""
 import pytest
 
 from tests import window_cases as W
@@ -94,3 +94,22 @@ def test_scales_that_other_rows_see(ctx, dtype, fresh, words):
             t = dict(s, v_scale=s["v_scale"].clone())
             t["v_scale"][at[0], at[1]] = bad
             assert torch.equal(attend(ctx, t, window, sinks)[~rows], want[~rows]), (at, bad)
+
+
+# ------------------------------------------------------------ masks
+
+@pytest.mark.parametrize("cache", ["own", "blocks"])
+@pytest.mark.parametrize("fresh,words", [([1, 5, 2], 1), ([3, 70, 1], 2)])
+def test_bits_beyond_a_requests_rows(ctx, cache, fresh, words):
+    """A mask's bits of tokens that a request does not add say nothing, of depths neither."""
+    window = 64 * words
+    s = W.view_case(23, [500, 90, 333], fresh, 4, 2, 64, BF16, BF16 if cache == "own" else I8, 32, 16 if cache == "blocks" else None,
+                    tree_words=words)
+    want = check_view(ctx, s, "bits %s" % fresh, window, 3).cpu()
+    mask = s["mask"].clone()
+    for b, n in enumerate(fresh):
+        for w in range(words):
+            beyond = (2 ** 64 - 1) ^ (2 ** min(max(n - 64 * w, 0), 64) - 1)
+            mask[int(s["starts"][b]):int(s["starts"][b + 1]), w] |= beyond - (2 ** 64 if beyond >> 63 else 0)
+    assert not torch.equal(mask, s["mask"])
+    assert torch.equal(attend(ctx, dict(s, mask=mask), window, 3), want)
