@@ -600,9 +600,12 @@ class _Window(torch.autograd.Function):
 
 
 def _packed(t):
-    """A gradient as it lies, if its rows do as the kernels want them."""
+    """A gradient as it lies, if its rows do as the kernels want them, or a copy: one
+    whose elements lie in order may begin at any address."""
     row, head, one = t.stride()
-    return t if one == 1 and row % 8 == 0 and head % 8 == 0 and row and head and t.data_ptr() % 16 == 0 else t.contiguous()
+    if one == 1 and row % 8 == 0 and head % 8 == 0 and 0 < row <= 1 << 24 and head > 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _window_record(ctx, q, k, v, out, lse, starts, window, sinks, scale):

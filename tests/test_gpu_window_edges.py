@@ -1,5 +1,5 @@
 """Attention over packed sequences and its gradients, on the GPU: buffers that calls
-share, numbers of first tokens."""
+share, numbers of first tokens, gradients that lie anyhow."""
 import pytest
 
 from tests import window_cases as W
@@ -53,3 +53,25 @@ def test_one_lse_buffer_for_two_calls(ctx):
 def test_first_tokens_that_every_window_holds(ctx, sinks):
     """However many, where no row leaves the window."""
     check(ctx, W.window_case(34, [90, 40], 2, 1, 64, BF16), "first tokens", 130, sinks)
+
+
+def test_gradients_that_lie_anyhow(ctx):
+    """A result's gradient at an address of no 16 bytes, or with rows that no kernel steps over."""
+    say("gradients that lie anyhow")
+    qkv, starts, dout = packed(33, [70, 33], 4, 2, 64, F16)
+    leaves = [t.requires_grad_() for t in qkv]
+    out = A.window_attention(ctx, *leaves, starts, window=25, sinks=1)
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    room = torch.zeros(dout.numel() + 1, dtype=F16, device=DEV)
+    room[1:] = dout.flatten()
+    wide = torch.zeros((103, 4, 65), dtype=F16, device=DEV)
+    wide[..., :64] = dout
+    for given in (room[1:].view(dout.shape), wide[..., :64], dout.transpose(0, 2).contiguous().transpose(0, 2)):
+        assert torch.equal(given, dout)
+        for x, y in zip(torch.autograd.grad(out, leaves, given, retain_graph=True), want):
+            assert torch.equal(x, y)
+    # as it comes about: a result beside another tensor of an odd length
+    both = torch.cat([torch.zeros(1, dtype=F16, device=DEV), out.flatten()])
+    weights = torch.cat([torch.zeros(1, dtype=F16, device=DEV), dout.flatten()])
+    for x, y in zip(torch.autograd.grad(both, leaves, weights), want):
+        assert torch.equal(x, y)

@@ -122,3 +122,19 @@ def test_no_window_is_none_or_zero():
     for window in (None, 0):
         with pytest.raises(ValueError, match="first ones"):
             A._reach(window, 2)
+
+
+def test_gradients_are_laid_out_for_the_kernels():
+    """As they lie where the kernels take them so, else as a copy of the same numbers."""
+    x = torch.randn((5, 4, 16)).half()
+    room = torch.zeros(x.numel() + 1, dtype=torch.float16)
+    room[1:] = x.flatten()
+    wide = torch.zeros((5, 4, 20), dtype=torch.float16)
+    wide[..., :16] = x
+    far = torch.empty_strided((1, 4, 16), ((1 << 24) + 8, 16, 1), dtype=torch.float16).copy_(x[:1])
+    assert A._packed(x) is x and A._packed(x[:, 1:3]).data_ptr() == x[:, 1:3].data_ptr()
+    one = torch.tensor(2.0, dtype=torch.float16).expand(5, 4, 16)
+    for t in (room[1:].view(5, 4, 16), room.new_zeros(x.numel() + 3)[3:].view(5, 4, 16), wide[..., :16], one, x[:1].expand(5, 4, 16),
+              x.transpose(1, 2).contiguous().transpose(1, 2), far):
+        p = A._packed(t)
+        assert torch.equal(p, t) and p.is_contiguous() and p.data_ptr() % 16 == 0 and p.data_ptr() != t.data_ptr()
