@@ -75,10 +75,18 @@ struct Piece {
   bool real;
 };
 
-// Piece `number`: those of sequence b (of all, with the two) are numbered from
-// begin / size + b on, since n rows are at most n / size + 1 pieces. Lanes
-// compare 64 sequences at a time. n = 0: there is no such piece.
-__device__ __forceinline__ Piece find(const WindowArgs &a, FastDiv size, int number) {
+// The number of a sequence's first piece: begin / size and one for each sequence
+// before, since n rows are at most n / size + 1 pieces. LONG: of sequences of more
+// rows than the window has, of which no two begin in the same span of so many rows;
+// others have no pieces.
+template <bool LONG> __device__ __forceinline__ int first_piece(const WindowArgs &a, FastDiv size, int begin, int sequence) {
+  const int before = LONG ? min(sequence, static_cast<int>(fdiv(static_cast<uint32_t>(begin), a.longer))) : sequence;
+  return static_cast<int>(fdiv(static_cast<uint32_t>(begin), size)) + before;
+}
+
+// Piece `number`, of all sequences, with the two. Lanes compare 64 of them at a time.
+// n = 0: there is no such piece.
+template <bool LONG> __device__ __forceinline__ Piece find(const WindowArgs &a, FastDiv size, int number) {
   const int lane = threadIdx.x & 63, many = a.sequences + 2;
   int lo = 0, hi = many, st = 0, en = 0;
   for (;;) {
@@ -88,7 +96,7 @@ __device__ __forceinline__ Piece find(const WindowArgs &a, FastDiv size, int num
       st = b == 0 ? 0 : min(max(a.starts[b - 1], 0), a.rows);
       if (step == 1)
         en = b == many - 1 ? a.rows : min(max(a.starts[b], 0), a.rows);
-      upto = static_cast<int>(fdiv(static_cast<uint32_t>(st), size)) + b <= number;
+      upto = first_piece<LONG>(a, size, st, b) <= number;
     }
     const uint64_t not_yet = ~__ballot(upto);
     const int n = max(not_yet ? __builtin_ctzll(not_yet) : 64, 1) - 1;
@@ -104,7 +112,7 @@ __device__ __forceinline__ Piece find(const WindowArgs &a, FastDiv size, int num
   p.begin = uniform(st);
   p.n = uniform(max(en - st, 0));
   p.number = uniform(lo);
-  p.index = uniform(number - static_cast<int>(fdiv(static_cast<uint32_t>(st), size)) - lo);
+  p.index = uniform(number - first_piece<LONG>(a, size, st, lo));
   p.real = lo > 0 && lo < many - 1;
   if (p.index < 0 || static_cast<int64_t>(p.index) * size.d >= p.n)
     p.n = 0;
@@ -338,7 +346,7 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 3) void k_win
   const Work w = my_work(a.row_pieces, a.kv_heads * a.parts);
   if (w.none)
     return;
-  const Piece piece = find(a, a.tile_tokens, w.number);
+  const Piece piece = find<false>(a, a.tile_tokens, w.number);
   if (piece.n == 0)
     return;
   const RowsOf rows(a, piece, w.head);
@@ -493,7 +501,7 @@ template <int T, int DP, bool SUMS> __global__ __launch_bounds__(64 * kWaves, 2)
   const Work w = my_work(a.row_pieces, a.kv_heads * a.parts);
   if (w.none)
     return;
-  const Piece piece = find(a, a.tile_tokens, w.number);
+  const Piece piece = find<false>(a, a.tile_tokens, w.number);
   if (piece.n == 0)
     return;
   const RowsOf rows(a, piece, w.head);
@@ -669,7 +677,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(Wi
   const Work w = my_work(FIRST ? a.first_pieces : a.key_pieces, FIRST ? a.kv_heads * a.first_blocks : a.kv_heads);
   if (w.none)
     return;
-  const Piece piece = find(a, FIRST ? a.first_tokens : a.key_tokens, w.number);
+  const Piece piece = find<FIRST>(a, FIRST ? a.first_tokens : a.key_tokens, w.number);
   if (piece.n == 0)
     return;
   const int kv = FIRST ? w.head / a.first_blocks : w.head;
@@ -874,7 +882,7 @@ __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(Wi
   const int size = static_cast<int>(a.first_tokens.d);
   const bool more = !FIRST && x_first < sinks && a.window + x_first < piece.n;
   auto add_first = [&](auto add) {
-    const int64_t base = static_cast<int64_t>(fdiv(static_cast<uint32_t>(piece.begin), a.first_tokens)) + piece.number;
+    const int64_t base = first_piece<true>(a, a.first_tokens, piece.begin, piece.number);
     for (int c = (a.window + x_first) / size; static_cast<int64_t>(c) * size < piece.n; ++c)
       add(a.first_sums + ((base + c) * a.kv_heads + kv) * a.sinks * 2 * DP);
   };

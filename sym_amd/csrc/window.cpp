@@ -152,15 +152,18 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   // are a good part of them: gradients of sequences of 600 rows on average are then
   // 1.4 and not 1.5 times as far off as their rounding; of 4000 they are 1.45 without.
   a.sums_d = p.rows / std::max<int64_t>(p.sequences, 1) <= 2048 || static_cast<int64_t>(a.window) + a.sinks <= 128;
-  const auto pieces = [&](const FastDiv &size, int64_t heads_of_piece) {
-    const int64_t n = p.rows / size.d + p.sequences + 2;
+  // Of rows that add to first tokens from outside their windows: only sequences
+  // longer than the window have any, and there may be fewer of those than sequences.
+  a.longer = make_div(std::min(window, p.rows) + 1);
+  const auto pieces = [&](const FastDiv &size, int64_t sequences, int64_t heads_of_piece) {
+    const int64_t n = p.rows / size.d + sequences + 2;
     // a workgroup of 256 threads for each, and 2^32 threads a dimension
     layout(n * heads_of_piece < (int64_t{1} << 24) - 8, "window attention: more than 2^24 - 8 tiles of rows and heads");
     return static_cast<int32_t>(n);
   };
-  a.row_pieces = pieces(a.tile_tokens, p.kv_heads * a.parts);
-  a.key_pieces = pieces(a.key_tokens, p.kv_heads);
-  a.first_pieces = pieces(a.first_tokens, p.kv_heads * std::max(a.first_blocks, 1));
+  a.row_pieces = pieces(a.tile_tokens, p.sequences, p.kv_heads * a.parts);
+  a.key_pieces = pieces(a.key_tokens, p.sequences, p.kv_heads);
+  a.first_pieces = pieces(a.first_tokens, std::min<int64_t>(p.sequences, p.rows / a.longer.d), p.kv_heads * std::max(a.first_blocks, 1));
   return a;
 }
 

@@ -16,6 +16,7 @@ struct WindowArgs {
   // a workgroup's rows: tokens, times heads of a group (in `parts` where those are many)
   FastDiv tile_tokens, tile_heads;
   FastDiv key_tokens, first_tokens; // tokens of its keys; rows that share sums of the first tokens
+  FastDiv longer;                   // the fewest rows of a sequence that some window leaves
   int32_t row_pieces, key_pieces, first_pieces; // numbers of such pieces, at most
   int32_t first_blocks;                         // of 32 first tokens
   int32_t rows, sequences, heads, kv_heads, parts, dim, window, sinks;

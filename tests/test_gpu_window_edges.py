@@ -1,5 +1,6 @@
 """Attention over packed sequences and its gradients, on the GPU: buffers that calls
-share, numbers of first tokens, gradients that lie anyhow."""
+share, numbers of first tokens, gradients that lie anyhow,
+sequences shorter and longer than the window."""
 import pytest
 
 from tests import window_cases as W
@@ -75,3 +76,11 @@ def test_gradients_that_lie_anyhow(ctx):
     weights = torch.cat([torch.zeros(1, dtype=F16, device=DEV), dout.flatten()])
     for x, y in zip(torch.autograd.grad(both, leaves, weights), want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16)])
+def test_short_and_long_sequences_with_first_tokens(ctx, dim, dtype):
+    """Those that no window leaves have no sums of first tokens; the others keep theirs apart."""
+    lengths = [30, 0, 41, 200, 12, 40, 42, 170, 1, 300, 39, 43, 500, 5, 45, 45, 45]
+    check(ctx, W.window_case(36, lengths, 4, 2, dim, dtype, before=50, after=70), "short and long", 40, 33)
+    check(ctx, W.window_case(37, lengths, 2, 2, dim, dtype, before=3), "a narrow window", 2, 5)

@@ -1,6 +1,7 @@
 """What torch's graph and the C boundary make of window attention's calls that other
 tests do not make, without a GPU."""
 import ctypes
+import random
 
 import pytest
 
@@ -115,6 +116,33 @@ def test_first_tokens_of_a_window_that_no_row_leaves(window):
     if window:
         more = window_args(rows=101, window=min(window, 100), sinks=257)
         assert refused(N.lib().relx_window_attention, None, bytes(more), 0)[0] == "unsupported_layout"
+
+
+def test_a_workspace_of_short_sequences():
+    """First tokens' sums are of sequences that some window leaves: 4096 of 32 rows, within a
+    window of 1024, have room for as many as could be longer, and not for all of them."""
+    a_piece = 8 * 256 * 2 * 128 * 4
+    stats = 32 * 2 ** 17 * 2 * 4
+    sizes = dict(rows=2 ** 17, heads=32, kv_heads=8, dim=128, sinks=256, window=1024)
+    assert workspace(sequences=4096, **sizes) <= stats + (2 ** 17 // 4096 + 2 ** 17 // 1025 + 2) * a_piece
+    assert workspace(sequences=5, **sizes) == stats + (2 ** 17 // 4096 + 5 + 2) * a_piece  # all of a few
+
+    # the numbers of pieces: each of its own, in order, and within the room
+    rng = random.Random(1)
+    for _ in range(300):
+        window, size = rng.randint(1, 60), rng.choice([32, 96, 128])
+        lengths = [rng.choice([0, 1, window, window + 1, rng.randint(0, 400)]) for _ in range(rng.randint(0, 40))]
+        before, after = rng.randint(0, 90), rng.randint(0, 90)
+        rows, at, taken = before + sum(lengths) + after, before, -1
+        for b, n in enumerate(lengths, 1):
+            first = at // size + min(b, at // (window + 1))
+            if n > window:
+                assert first > taken
+                taken = first + -(-n // size) - 1
+            at += n
+            if b < len(lengths):  # the next sequence's is beyond: a search for the last that is not ends here
+                assert at // size + min(b + 1, at // (window + 1)) > taken
+        assert taken < rows // size + min(len(lengths), rows // (window + 1)) + 2
 
 
 def test_no_window_is_none_or_zero():
