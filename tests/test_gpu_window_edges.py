@@ -1,18 +1,22 @@
 """Attention over packed sequences and its gradients, on the GPU: buffers that calls
-share, numbers of first tokens, gradients that lie anyhow,
-sequences shorter and longer than the window."""
+share, numbers of first tokens, gradients that lie anyhow, sequences shorter and longer
+than the window, forms of large batches, places around operands and results."""
+import ctypes
+
 import pytest
 
 from tests import window_cases as W
-from tests.test_gpu_window import check
+from tests.test_gpu_window import check, within
 
 torch = pytest.importorskip("torch")
+from sym_amd import _native as N  # noqa: E402
 from sym_amd import attention as A  # noqa: E402
 from sym_amd import pyreloc as P  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 F16, BF16 = torch.float16, torch.bfloat16
+NAN = float("nan")
 
 
 @pytest.fixture(scope="module")
@@ -84,3 +88,47 @@ def test_short_and_long_sequences_with_first_tokens(ctx, dim, dtype):
     lengths = [30, 0, 41, 200, 12, 40, 42, 170, 1, 300, 39, 43, 500, 5, 45, 45, 45]
     check(ctx, W.window_case(36, lengths, 4, 2, dim, dtype, before=50, after=70), "short and long", 40, 33)
     check(ctx, W.window_case(37, lengths, 2, 2, dim, dtype, before=3), "a narrow window", 2, 5)
+
+
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 8, 64, F16), (16, 16, 128, BF16)])
+def test_a_long_sequence_of_many_first_tokens(ctx, heads, kv, dim, dtype):
+    """Pieces of rows longer than the least, and no power of two; D of the result alone."""
+    blocks = 8
+    assert 2100 * kv * blocks // 768 > 128 and (2100 * kv * blocks // 768 + 31) // 32 in (6, 11)
+    check(ctx, W.window_case(35, [2100], heads, kv, dim, dtype), "long, many first tokens", 300, 256)
+
+
+@pytest.mark.parametrize("starts", [[-5, 100, 10 ** 9], [50, 20, 160], [160, 0], [2 ** 31 - 1, -2 ** 31], [0, 60, 160]])
+def test_nothing_outside_the_operands(ctx, starts):
+    """Starts out of order or out of range: what lies around results and workspace stays, and
+    what lies around operands reaches nothing."""
+    say("nothing outside", starts)
+    rows, heads, kv, dim, pad = 160, 4, 2, 64, 4096
+    s = W.window_case(38, [100, 60], heads, kv, dim, BF16, fused=False)
+
+    def put(t, around):  # inside a larger buffer
+        room = torch.full((t.numel() + 2 * pad,), around, dtype=t.dtype, device=DEV)
+        room[pad:-pad] = t.to(DEV).flatten()
+        return room, room[pad:-pad].view(t.shape)
+    q, k, v, dout = (put(s[n], NAN)[1] for n in ("q", "k", "v", "dout"))
+    made = {n: put(t, 7.0) for n, t in dict(out=torch.zeros_like(s["q"]), lse=torch.zeros((heads, rows)), dq=torch.zeros_like(s["q"]),
+                                            dk=torch.zeros_like(s["k"]), dv=torch.zeros_like(s["v"])).items()}
+    z = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out, lse = made["out"][1], made["lse"][1]
+    A.window_attention(ctx, q, k, v, z, window=30, sinks=40, out=out, lse=lse)
+    args, device = A._window_record(ctx, q, k, v, out, lse, z, 30, 40, None)
+    size, err = ctypes.c_size_t(), N.relx_err()
+    assert N.lib().relx_window_attention_workspace(args, ctypes.byref(size), ctypes.byref(err)) == 0
+    room, workspace = put(torch.zeros(size.value // 4), 7.0)
+    A._call("relx_window_attention_backward", ctx, args, A._heads(dout, "", dout.shape, BF16, device),
+            *(A._heads(made[n][1], "", made[n][1].shape, BF16, device) for n in ("dq", "dk", "dv")), workspace.data_ptr(),
+            size.value, A._stream(device))
+    torch.cuda.synchronize()
+    for name, (whole, inside) in dict(made, workspace=(room, workspace)).items():
+        assert (whole[:pad] == 7.0).all() and (whole[-pad:] == 7.0).all(), name
+    for name in ("out", "dq", "dk", "dv"):
+        assert torch.isfinite(made[name][1]).all(), name
+    if starts == [0, 60, 160]:
+        want = W.window_attention(s["q"], s["k"], s["v"], torch.tensor(starts), 30, 40, dim ** -0.5, s["dout"])
+        for name, x in (("out", "o"), ("dq", "dq"), ("dk", "dk"), ("dv", "dv")):
+            within(made[name][1], want[x], want["b" + x], name)
