@@ -119,6 +119,21 @@ template <bool LONG> __device__ __forceinline__ Piece find(const WindowArgs &a, 
   return p;
 }
 
+// The first pieces alone, `few_pieces` of each sequence.
+__device__ __forceinline__ Piece first_of(const WindowArgs &a, FastDiv size, int number) {
+  const int sequence = number / a.few_pieces;
+  const int st = min(max(a.starts[sequence], 0), a.rows), en = min(max(a.starts[sequence + 1], 0), a.rows);
+  Piece p;
+  p.begin = uniform(st);
+  p.number = sequence + 1;
+  p.index = number - sequence * a.few_pieces;
+  p.n = uniform(max(en - st, 0));
+  p.real = true;
+  if (p.index * static_cast<int>(size.d) >= p.n)
+    p.n = 0;
+  return p;
+}
+
 // A workgroup's piece and key head: neighbours share a die, whose cache serves the
 // tiles that they both read. Later pieces, which in a sequence read more, first.
 struct Work {
@@ -492,16 +507,18 @@ template <int T, int DP> __global__ __launch_bounds__(64 * kWaves, 3) void k_win
 // rounded weight is, over the root of the number of tokens that a row sees, and in
 // all of them alike: with a few tokens gradients are 1.7 times as far off as their own
 // rounding is, and 1.4 times with this D (with 128 tokens 1.5 and 1.4). So it is for
-// tiles of rows that see up to 128.
+// tiles of rows that see up to kFew, in long sequences too: their first tokens'
+// gradients are the largest, and mostly of rows that see few.
 template <int T, int DP, bool SUMS> __global__ __launch_bounds__(64 * kWaves, 2) void k_window_dq(WindowArgs a) {
   constexpr int kKeys = 64; // tokens of a tile
   constexpr int RB = DP * 2, TILE = kKeys * RB, E = DP / 32, KS = DP / 16, RING = 2;
   __shared__ __attribute__((aligned(256))) char tiles[RING][2][TILE];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const Work w = my_work(a.row_pieces, a.kv_heads * a.parts);
+  const bool of_few = SUMS && a.few_pieces > 0;
+  const Work w = my_work(of_few ? a.sequences * a.few_pieces : a.row_pieces, a.kv_heads * a.parts);
   if (w.none)
     return;
-  const Piece piece = find<false>(a, a.tile_tokens, w.number);
+  const Piece piece = of_few ? first_of(a, a.tile_tokens, w.number) : find<false>(a, a.tile_tokens, w.number);
   if (piece.n == 0)
     return;
   const RowsOf rows(a, piece, w.head);
@@ -515,7 +532,7 @@ template <int T, int DP, bool SUMS> __global__ __launch_bounds__(64 * kWaves, 2)
     __syncthreads();
   }
   const int last = rows.first + rows.tokens - 1;
-  const bool few = a.sums_d && min(last + 1, a.window + a.sinks) <= 128;
+  const bool few = min(last + 1, a.window + a.sinks) <= kFew;
   if (SUMS && !few)
     return;
   const KeyTiles<kKeys> keys(a, rows.first, last);
@@ -965,8 +982,9 @@ template <int T, int DP> hipError_t window_forward(const WindowArgs &a, hipStrea
 template <int T, int DP> hipError_t window_backward(const WindowArgs &a, hipStream_t s) {
   const int64_t tiles = static_cast<int64_t>(a.row_pieces) * a.kv_heads * a.parts;
   hipError_t e = hipSuccess;
-  if (a.sums_d)
-    e = window_start(reinterpret_cast<const void *>(k_window_dq<T, DP, true>), a, tiles, s);
+  const int64_t few = a.few_pieces ? static_cast<int64_t>(a.sequences) * a.few_pieces * a.kv_heads * a.parts : tiles;
+  if (few > 0)
+    e = window_start(reinterpret_cast<const void *>(k_window_dq<T, DP, true>), a, few, s);
   if (e == hipSuccess)
     e = window_start(reinterpret_cast<const void *>(k_window_dq<T, DP, false>), a, tiles, s);
   if (e == hipSuccess && a.sinks > 0)

@@ -148,10 +148,6 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   // as many workgroups as run at a time and half as many again
   const int64_t first = p.rows * p.kv_heads * std::max(a.first_blocks, 1) / 768;
   a.first_tokens = make_div(std::min<int64_t>(std::max<int64_t>((first + 31) / 32 * 32, 128), 4096));
-  // Where windows are of few tokens, or the first rows of sequences, which see few,
-  // are a good part of them: gradients of sequences of 600 rows on average are then
-  // 1.4 and not 1.5 times as far off as their rounding; of 4000 they are 1.45 without.
-  a.sums_d = p.rows / std::max<int64_t>(p.sequences, 1) <= 2048 || static_cast<int64_t>(a.window) + a.sinks <= 128;
   // Of rows that add to first tokens from outside their windows: only sequences
   // longer than the window have any, and there may be fewer of those than sequences.
   a.longer = make_div(std::min(window, p.rows) + 1);
@@ -162,6 +158,9 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
     return static_cast<int32_t>(n);
   };
   a.row_pieces = pieces(a.tile_tokens, p.sequences, p.kv_heads * a.parts);
+  // Unless windows are as narrow, it is the first rows of a sequence that see few.
+  const int64_t few = (kFew + a.tile_tokens.d - 1) / a.tile_tokens.d;
+  a.few_pieces = window + sinks > kFew && p.sequences * few < a.row_pieces ? static_cast<int32_t>(few) : 0;
   a.key_pieces = pieces(a.key_tokens, p.sequences, p.kv_heads);
   a.first_pieces = pieces(a.first_tokens, std::min<int64_t>(p.sequences, p.rows / a.longer.d), p.kv_heads * std::max(a.first_blocks, 1));
   return a;

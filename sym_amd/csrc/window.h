@@ -6,6 +6,8 @@
 
 namespace relx {
 
+constexpr int kFew = 128; // tokens of a row whose D the backward sums from its weights
+
 struct WindowArgs {
   Heads q, k, v, o;
   Heads dout, dq, dk, dv;
@@ -21,7 +23,7 @@ struct WindowArgs {
   int32_t first_blocks;                         // of 32 first tokens
   int32_t rows, sequences, heads, kv_heads, parts, dim, window, sinks;
   float scale, plain_scale; // of a score, times log2 e, and as it is
-  bool sums_d;              // the backward sums D from the weights
+  int32_t few_pieces;       // of a sequence's rows, at most, that see up to kFew tokens; 0: any may
 };
 hipError_t window_launch_f16(const WindowArgs &a, bool back, hipStream_t s);
 hipError_t window_launch_bf16(const WindowArgs &a, bool back, hipStream_t s);

@@ -132,3 +132,37 @@ def test_nothing_outside_the_operands(ctx, starts):
         want = W.window_attention(s["q"], s["k"], s["v"], torch.tensor(starts), 30, 40, dim ** -0.5, s["dout"])
         for name, x in (("out", "o"), ("dq", "dq"), ("dk", "dk"), ("dv", "dv")):
             within(made[name][1], want[x], want["b" + x], name)
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("lengths,window,sinks", [([2100], None, 0), ([30, 2500, 2100], 1000, 4)])
+def test_rows_that_see_few_tokens(ctx, dtype, dim, lengths, window, sinks):
+    """In long sequences too their D is summed in 32 bits: where values have much in common,
+    dP and D are large beside their difference, and D of the rounded result would be off by
+    more than all of the bound."""
+    say("few tokens", lengths)
+    heads, kv, scale = 2, 1, dim ** -0.5
+    s = W.window_case(39, lengths, heads, kv, dim, dtype, fused=False, std=0.25)
+    s["v"] = (8 + s["v"].float()).to(dtype)
+    s["dout"] = (1 + s["dout"].float()).to(dtype)
+    leaves = [s[n].to(DEV).requires_grad_() for n in "qkv"]
+    out = A.window_attention(ctx, *leaves, s["starts"].to(DEV), window=window, sinks=sinks)
+    dq = torch.autograd.grad(out, leaves[0], s["dout"].to(DEV))[0].cpu().double()
+    u, f32 = W.ROUND[dtype], W.F32
+    for a, b in zip(s["starts"].tolist(), s["starts"].tolist()[1:]):
+        n = min(b - a, 128)  # rows that see up to so many
+        see = W.sees(n, window, sinks)
+        for h in range(heads):
+            q, k, v, do = (s[x][a:a + n, y].double() for x, y in (("q", h), ("k", 0), ("v", 0), ("dout", h)))
+            p = torch.softmax(torch.where(see, q @ k.T * scale, -float("inf")), 1)
+            dp, size = do @ v.T, do.abs() @ v.abs().T
+            g = p * (dp - (p * dp).sum(1, keepdim=True)) * scale
+            # scores and lse in 32 bits: weights off by 2 ds; dP, its products with them and
+            # their sum: in 32 bits; dS rounded to u of itself (f16: or 2^-30 of the largest)
+            ds = (dim + 4) * f32 * (q.abs() @ k.abs().T * see).amax(1, keepdim=True) * scale + 8 * f32 * (1 + n) ** 0.5
+            d_off = (2 * ds + (dim + n + 8) * f32) * (p * size).sum(1, keepdim=True)
+            off = u * g.abs() + p * scale * ((2 * ds + (dim + 8) * f32) * size + d_off) + see * 2.0 ** -30 * scale * float(size.max())
+            want = g @ k
+            bound = (off + (n / 32 + 16) * f32 * g.abs()) @ k.abs() + u * want.abs() + W.STEP[dtype]
+            far = (dq[a:a + n, h] - want).abs() - bound
+            assert float(far.max()) <= 0, (a, h, float(far.max()))
