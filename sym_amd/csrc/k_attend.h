@@ -49,9 +49,9 @@
 //   1 request of 13 rows x 4 heads, 131072 bf16 tokens: 100 to 101 us, 5.3 TB/s.
 //     Bound by the reads, but for the join's 6.
 //   64 requests of 1 row x 4 heads, 6100 int8 tokens with a scale a block on average, a
-//     token's heads side by side: 134 us, 5.8 TB/s (a head at a time 153).
-//   64 requests of 1 row x 4 heads, window of 2048 bf16 tokens: 96 us, 5.6 TB/s.
-//   8 requests of 48 rows x 4 heads, up to 8192 int8 tokens, a scale a block: 86 us.
+//     token's heads side by side: 136 us, 5.7 TB/s (a head at a time 153).
+//   64 requests of 1 row x 4 heads, window of 2048 bf16 tokens: 98 us, 5.5 TB/s.
+//   8 requests of 48 rows x 4 heads, up to 8192 int8 tokens, a scale a block: 88 us.
 //   8 requests of 64 rows x 4 heads, up to 8192 tokens: 77 to 78 us, 455 TFLOP/s; up
 //     to 32768: 274 to 315 us by the card's clock, 575 to 660 TFLOP/s. No unit is busy most of the time: the matrix
 //     units for 0.27 of it, shared memory 0.21 (a third of that in bank conflicts),

@@ -31,12 +31,14 @@
 // their own that leaves sums in 32 bits; they are added in order at the end.
 //
 // Measured, 24.6k rows of 32 + 8 heads of 128 in bf16, window 1024, 4 first tokens:
-// forward 490 us (850 TFLOP/s), dQ 690, dK and dV 970, the first tokens' 97; 16384
-// rows of 16 heads of 64 in f16, window 4096: 310, 420, 640 and 24. Matrix units are
+// forward 490 us (850 TFLOP/s), dQ 695, dK and dV 974, the first tokens' 95, D of rows
+// that see few 11; 16384 rows of 16 heads of 64 in f16, window 4096: 307, 424, 632, 25
+// and 7 (each at least, in traces; steps in a row take 2250 and 1369). Matrix units are
 // busy for 0.47 to 0.49 of the cycles (at 1.7 to 1.8 GHz under this load), vector
 // units for 0.56 (forward), 0.41 and 0.32, shared memory for 0.23, 0.24 and 0.37,
 // without bank conflicts: products and softmax of one wave follow one another, and
-// only the two or three waves of a SIMD overlap them.
+// only the two or three waves of a SIMD overlap them. (Where 32 keys are a workgroup's,
+// shared memory holds two with heads of 64, and one, of a wave a SIMD, with wider.)
 #pragma once
 
 #include <algorithm>
@@ -676,6 +678,8 @@ template <int T, int DP, bool SUMS> __global__ __launch_bounds__(64 * kWaves, 2)
 //   kNarrow  32 keys a workgroup, whose waves take turns at the tiles of rows and add
 //            up at the end: where there are few keys, four times the workgroups
 //   kFirst   the same, of first tokens over the rows whose window has left them
+// The last two take 70 KiB of shared memory with heads of 64 and 138 KiB with wider
+// ones: that, and not their 126 and 164 registers, says how many run on a compute unit.
 enum KeyMode : int { kWide, kNarrow, kFirst };
 template <int T, int DP, int MODE>
 __global__ __launch_bounds__(64 * kWaves, DP == 64 ? 3 : 2) void k_window_dkv(WindowArgs a) {

@@ -145,7 +145,8 @@ WindowArgs window_args(const relx_window_args &p, int &type) {
   const int64_t tiles = (p.rows / 128 + p.sequences) * p.kv_heads;
   a.key_tokens = make_div(tiles < (p.dim <= 64 ? 1024 : 256) ? 32 : 128);
   a.first_blocks = (a.sinks + 31) / 32;
-  // as many workgroups as run at a time and half as many again
+  // half as many workgroups again as run at a time with heads of 64, three times as
+  // many as run with wider ones, by shared memory
   const int64_t first = p.rows * p.kv_heads * std::max(a.first_blocks, 1) / 768;
   a.first_tokens = make_div(std::min<int64_t>(std::max<int64_t>((first + 31) / 32 * 32, 128), 4096));
   // Of rows that add to first tokens from outside their windows: only sequences
