@@ -282,6 +282,7 @@ struct Item {
   int b, start, fresh, head, tile, cached, length, s0, s1, units;
   int reach;      // places of tokens: of the request, or those that its rows may see
   int edge, jump; // where places and tokens part, and by how much
+  int position;   // of the first new token: the cached ones, of which the table may hold fewer
   int all_see;    // every row's window holds the tokens from here on
   template <int FORM> __device__ __forceinline__ int token(int place) const {
     return FORM == kWhole ? place : place < edge ? place : place + jump;
@@ -292,8 +293,8 @@ struct Item {
   }
 };
 // Where the window of the j-th new token, at the d-th place after the cached ones, begins.
-__device__ __forceinline__ int window_from(const AttendArgs &a, int cached, int d) {
-  const int64_t from = static_cast<int64_t>(cached) + d - a.window + 1;
+__device__ __forceinline__ int window_from(const AttendArgs &a, int position, int d) {
+  const int64_t from = static_cast<int64_t>(position) + d - a.window + 1;
   return static_cast<int>(max(min(from, int64_t{1} << 30), int64_t{0}));
 }
 // The d of a row: the token's depth in its tree, or j. Of a mask's bits those of the
@@ -352,7 +353,7 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
   i.tile = static_cast<int>(item - static_cast<int64_t>(i.head) * tiles);
   run.unit = uniform64(run.unit + i.s1 - i.s0);
   i.reach = i.length;
-  i.edge = i.jump = i.all_see = 0;
+  i.edge = i.jump = i.all_see = i.position = 0;
   if constexpr (FORM != kWhole) {
     // the places of its first and last rows' tokens
     const int row0 = i.tile * ROWS;
@@ -362,8 +363,9 @@ __device__ __forceinline__ Item take(const AttendArgs &a, const Schedule &sh, Ru
     if (j1 + 1 < i.length - i.cached)
       i.length = i.cached + j1 + 1;
     i.length = uniform(i.length);
-    const int from = min(window_from(a, i.cached, j0), i.length);
-    i.all_see = uniform(min(window_from(a, i.cached, j1), i.length));
+    i.position = uniform(max(a.cached[b], 0));
+    const int from = min(window_from(a, i.position, j0), i.length);
+    i.all_see = uniform(min(window_from(a, i.position, j1), i.length));
     i.edge = uniform(edge_of(a, i.length));
     i.jump = uniform(max((from & ~(kTile - 1)) - i.edge, 0));
     i.reach = i.length - i.jump;
@@ -563,7 +565,7 @@ template <int FORM, int T, int DP, int RT, bool RAW, bool EARLY> struct Rows {
       if (words == 1 && place[t] < it.fresh)
         mask[t] = static_cast<uint64_t>(a.mask[it.start + static_cast<int64_t>(j)]);
       if constexpr (FORM != kWhole)
-        from[t] = place[t] < it.fresh ? window_from(a, it.cached, row_depth(a, it.start, it.fresh, place[t])) : 0;
+        from[t] = place[t] < it.fresh ? window_from(a, it.position, row_depth(a, it.start, it.fresh, place[t])) : 0;
       const char *src = a.q + ((it.start + static_cast<int64_t>(j)) * a.q_row +
                                (static_cast<int64_t>(it.head) * a.group.d + (p - j * a.group.d)) * a.q_head) * 2;
 #pragma unroll

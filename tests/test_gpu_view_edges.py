@@ -1,5 +1,6 @@
 """What reaches a result of attention over a cache with a window, and what must not:
-scales of blocks that a row does not see, bits of a mask beyond a request's rows."""
+scales of blocks that a row does not see, bits of a mask beyond a request's rows, tokens
+beyond a table."""
 import pytest
 
 from tests import window_cases as W
@@ -113,3 +114,21 @@ def test_bits_beyond_a_requests_rows(ctx, cache, fresh, words):
             mask[int(s["starts"][b]):int(s["starts"][b + 1]), w] |= beyond - (2 ** 64 if beyond >> 63 else 0)
     assert not torch.equal(mask, s["mask"])
     assert torch.equal(attend(ctx, dict(s, mask=mask), window, 3), want)
+
+
+# ------------------------------------------------------------ tables
+
+@pytest.mark.parametrize("cache", ["own", "int8", "blocks"])
+@pytest.mark.parametrize("cached,fresh,dim,page,columns,window,sinks,words", [
+    ([63, 5], [2, 1], 64, 32, 1, 20, 1, 0),
+    ([700, 40], [1, 1], 128, 64, 9, 300, 33, 0),
+    ([700, 640], [40, 9], 64, 64, 10, 130, 3, 0),
+    ([500, 90], [3, 30], 64, 32, 7, 300, 0, 2),
+    ([500], [1], 64, 16, 10, 100, 0, 0),  # nothing of the window is left
+])
+def test_a_table_that_holds_fewer_than_the_cached_tokens(ctx, cache, cached, fresh, dim, page, columns, window, sinks, words):
+    """Positions go by the cached tokens, those in the table or not."""
+    for dtype in (F16, BF16):
+        s = W.view_case(24, cached, fresh, 4, 2, dim, dtype, dtype if cache == "own" else I8, page, 16 if cache == "blocks" else None,
+                        tree_words=words, columns=columns)
+        check_view(ctx, s, "short table %s" % [cached, columns], window, sinks)
